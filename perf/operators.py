@@ -108,8 +108,9 @@ def draw(rng):
         heads = kvh * group
         new = 1 if rng.random() < 0.5 else _log(rng, 2, 2048)
         kv = _log(rng, max(new, 16), 16384)
-        new = min(new, (1 << 31) // (heads * kv))
-        most = min((1 << 31) // (heads * new * kv), (1 << 29) // (kv * kvh * hd), 64)
+        pairs = (1 << 37) // (heads * hd)        # of the prompt of 8192, half of them seen
+        new = min(new, pairs // kv)
+        most = min(pairs // (new * kv), (1 << 29) // (kv * kvh * hd), 64)
         seqs = _log(rng, 1, max(1, most))
         causal = rng.random() < 0.8
         return {"kind": kind, "type": typ, "seqs": seqs, "new": new, "kv": kv, "heads": heads,
