@@ -312,6 +312,175 @@ int qc_hip_qgemm_w8a8(const int8_t* w, const int8_t* x, const float* ws, const f
                       float* y, long long m, long long n, long long k, int* dev_status,
                       void* stream);
 
+/* ---- Between the projections: rotary positions, 8-bit cache, MXFP4 -----
+ * Operators that a decoder needs beside its quantized products; no
+ * counterpart in the reference's quantized path.  `type` arguments are
+ * QC_STORAGE_*; 16-bit values are decoded exactly, arithmetic is f32 and every
+ * output is rounded once (nearest even).  Data-dependent errors follow the
+ * dev_status convention above: with a device int the call is asynchronous, sets
+ * it to 3 and leaves the outputs that the entry names as they were; with NULL the
+ * call looks the device data over first, blocks, and returns 3 with nothing
+ * written (not while the stream is being captured). */
+
+/* Layout of the rotated pairs: elements (i, i + rotary_dim / 2) or (2 i, 2 i + 1). */
+#define QC_ROPE_HALF 0
+#define QC_ROPE_INTERLEAVED 1
+
+/* Pair i of rotary_dim / 2 turns by w_i radians a position; unscaled w_i =
+ * base^(-2 i / rotary_dim).  With factor s >= 1 and L = original_positions:
+ *   LINEAR  w_i / s
+ *   NTK     the base becomes base * s^(rotary_dim / (rotary_dim - 2)) (rotary_dim > 2)
+ *   TURNS   t = L w_i / 2 pi turns over the original context, g = (t - low_turns) /
+ *           (high_turns - low_turns) clamped to [0, 1]: g w_i + (1 - g) w_i / s
+ *   YARN    the same blend with g = 1 - (i - low) / (high - low) clamped, where low and
+ *           high are the pair indexes (floor, ceil, within [0, rotary_dim - 1], at least
+ *           0.001 apart) of the frequencies that make high_turns and low_turns turns
+ * Every cosine and sine is multiplied by `magnitude` (1 for none; 0.1 ln s + 1 is
+ * usual with YARN). */
+#define QC_ROPE_SCALE_NONE 0
+#define QC_ROPE_SCALE_LINEAR 1
+#define QC_ROPE_SCALE_NTK 2
+#define QC_ROPE_SCALE_TURNS 3
+#define QC_ROPE_SCALE_YARN 4
+typedef struct qc_rope_scaling {
+  int kind;                    /* QC_ROPE_SCALE_* */
+  double factor;
+  double original_positions;   /* TURNS, YARN */
+  double low_turns;
+  double high_turns;
+  double magnitude;
+} qc_rope_scaling;
+
+/* cosine, sine f32 [positions][rotary_dim / 2]: the rows of positions
+ * first_position, first_position + 1, ... (the tables qc_hip_rope,
+ * qc_hip_qgemv_qkv_rope_kv and, row by row, qc_hip_cint8_project take).  Angles,
+ * cosines and sines are computed in 64 bits and rounded once.  scaling NULL:
+ * none.  Status: 1 when positions is not positive, first_position negative, their
+ * sum beyond 2^31, rotary_dim odd or not in 2..512; 3 for NULL tables, a base that is
+ * not finite and above 1, or a scaling out of range (its kind unknown; factor not finite
+ * or below 1; magnitude not finite and above 0; TURNS / YARN: original_positions or
+ * low_turns not above 0, or high_turns not above low_turns; NTK: rotary_dim 2). */
+int qc_hip_rope_table(float* cosine, float* sine, long long first_position, long long positions,
+                      long long rotary_dim, double base, const qc_rope_scaling* scaling,
+                      void* stream);
+
+/* y = x with the first rotary_dim elements of every head rotated by the token's
+ * position: out_a = a c - b s, out_b = b c + a s (each product and sum rounded to
+ * f32), c and s from row positions[token] of the tables [max_position][rotary_dim / 2].
+ * Element (t, h, d) of x is x[t * x_token_stride + h * x_head_stride + d], of y
+ * likewise, so Q and K heads that lie side by side in one projection's rows are one
+ * call.  y may be x (same strides): the elements past rotary_dim are then not
+ * touched, else they are copied.  Other overlaps of x and y are not allowed.  A token
+ * at position -1 is padding and left as it was; a position below -1 or from
+ * max_position on is an error and its token left as it was.  Status: 1 for sizes
+ * that are not positive, rotary_dim odd or above head_dim, strides shorter than what
+ * they step over (a stride of one element's count 1 is not read), 2 for an unknown
+ * type, 3 for NULL pointers or a bad layout. */
+int qc_hip_rope(const void* x, void* y, int type, long long tokens, long long heads,
+                long long head_dim, long long rotary_dim, long long x_token_stride,
+                long long x_head_stride, long long y_token_stride, long long y_head_stride,
+                const float* cosine, const float* sine, const int* positions,
+                long long max_position, int layout, int* dev_status, void* stream);
+
+/* An int8 key/value cache in pages of tokens.  codes [pages][kv_heads]
+ * [page_tokens][head_dim] and scales [pages][kv_heads], for K and V each; element =
+ * code * scale.  page_tokens: a power of two in 16..256; head_dim: a multiple of 16
+ * in 16..256; codes 16-byte aligned. */
+typedef struct qc_kv8_cache {
+  int8_t* k_codes;
+  int8_t* v_codes;
+  float* k_scales;
+  float* v_scales;
+  long long pages;
+  long long kv_heads;
+  long long page_tokens;
+  long long head_dim;
+} qc_kv8_cache;
+
+/* A ragged batch, described on the device.  Rows [seq_start[s], seq_start[s + 1]) of
+ * the batch's `tokens` token rows are sequence s's new tokens (none is allowed);
+ * kv_len[s] counts its tokens in the cache, the new ones last.  Position p of it
+ * lies in page block_table[s * columns + p / page_tokens], slot p % page_tokens.
+ * Host bounds: no sequence has more than max_new new tokens or max_kv tokens;
+ * rows from seq_start[seqs] on belong to no one and are neither read nor written.
+ * A sequence whose figures break these bounds, or a page id that a call needs and
+ * that is not in [0, pages), is an error: the sequence is left out (append,
+ * gather: that page of it; attention: its rows see the other pages). */
+typedef struct qc_kv8_batch {
+  const int* block_table;   /* [seqs][columns] */
+  const int* seq_start;     /* [seqs + 1] */
+  const int* kv_len;        /* [seqs] */
+  long long seqs;
+  long long columns;
+  long long tokens;
+  long long max_new;
+  long long max_kv;
+} qc_kv8_batch;
+
+/* Writes the new tokens' keys and values (k, v: [tokens][kv_heads * head_dim],
+ * token rows k_stride / v_stride elements apart) into the cache at positions
+ * kv_len - n .. kv_len - 1 of their sequences.  Per page and head, with t the new
+ * tokens' largest magnitude there and s the scale held (0 where the page has no
+ * token before the new ones): s' = max(s, t / 127), or 0 below 2^-126; codes held
+ * become rint(code * (s / s')), new ones clamp(rint(x * (1 / s')), +-127), each
+ * step rounded to f32.  A page written by a call must belong to one sequence.
+ * A page and head with a non-finite new value, and a sequence of more new tokens than
+ * kv_len, are errors and left as they were.  Status: 1 for sizes out of range, 2 for an
+ * unknown type, 3 for NULL or misaligned pointers. */
+int qc_hip_kv8_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* k,
+                      long long k_stride, const void* v, long long v_stride, int type,
+                      int* dev_status, void* stream);
+
+/* The same places read back: k and v rows of the batch's tokens receive the
+ * values held at positions kv_len - n .. kv_len - 1 (a seq_start that spans whole
+ * sequences reads all of them).  Status and errors as for qc_hip_kv8_append. */
+int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void* k,
+                      long long k_stride, void* v, long long v_stride, int type, int* dev_status,
+                      void* stream);
+
+/* out = softmax(scale * q k^T + mask) v over the cache, for the new tokens of
+ * every sequence (which the cache holds already).  q and out: [tokens][heads *
+ * head_dim], rows q_stride / out_stride elements apart, `heads` a multiple of
+ * kv_heads, query heads h * heads / kv_heads .. sharing key head h.  Token i of n
+ * stands at p = kv_len - n + i and sees the positions j < kv_len; with causal != 0
+ * j <= p, and with window > 0 (causal only) j > p - window.  A row that sees nothing
+ * (n > kv_len, or kv_len 0) is zeros.  Pages that no row sees are not looked at.
+ * 16-bit q: the probabilities enter the product with the values in 11 bits, f32 q: in
+ * 22; sums and statistics are f32.  Status: 1 for sizes out of range, 2 for an
+ * unknown type, 3 for NULL or misaligned pointers, a scale that is not finite, or a
+ * window without causal. */
+int qc_hip_kv8_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* q,
+                         long long q_stride, void* out, long long out_stride, int type,
+                         long long heads, float scale, int causal, long long window,
+                         int* dev_status, void* stream);
+
+/* MXFP4: blocks of 32 values of a row as 4-bit floats (sign, 2 exponent bits, 1
+ * mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6) under a power of two.  codes
+ * [rows][dim / 2], the even element in a byte's low half; scales [rows][dim / 32],
+ * exponent + 127.  dim is a multiple of 32, codes are 16-byte aligned.
+ *
+ * Of a block: e = clamp(floor(log2 max|x|) - 2, -127, 127) (-127 when all are
+ * zero), code = x * 2^-e rounded to nearest, ties to even, at most 6.  x: [rows][dim]
+ * of `type`, rows x_stride elements apart.  A block with a non-finite value is an
+ * error and left as it was.  Status: 1 for sizes out of range, 2 for an unknown
+ * type, 3 for NULL or misaligned pointers. */
+int qc_hip_quantize_mxfp4(const void* x, int type, long long x_stride, uint8_t* codes,
+                          uint8_t* scales, long long rows, long long dim, int* dev_status,
+                          void* stream);
+
+/* out[rows][dim] of `type` = the values codes and scales stand for (a scale byte of
+ * 255: NaN). */
+int qc_hip_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, void* out, int type,
+                            long long rows, long long dim, void* stream);
+
+/* y[m][n] = x . w^T of two MXFP4 matrices, w [n][k] and x [m][k]: products exact,
+ * sums f32, y of y_type.  A scale byte of 255 makes the outputs of its row NaN.
+ * Status: 1 for sizes that are not positive or k not a multiple of 32, 2 for an
+ * unknown type, 3 for NULL pointers or codes that are not 16-byte aligned. */
+int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* x_codes,
+                      const uint8_t* x_scales, void* y, int y_type, long long m, long long n,
+                      long long k, void* stream);
+
 /* Measurement seam with no reference counterpart: reads `bytes` (a multiple
  * of 16) of device memory with 16-byte loads as fast as the chip allows and
  * stores one XOR word per thread into out (grid * 256 words).  bench.py times

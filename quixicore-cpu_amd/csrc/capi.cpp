@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <cmath>
@@ -167,6 +168,49 @@ int all_finite(const float* x, long long count, hipStream_t s, bool* finite) {
 }
 
 int finish(hipError_t e) { return e == hipSuccess ? QC_OK : device_error(e); }
+
+bool known_storage(int type) {
+  return type == QC_STORAGE_F32 || type == QC_STORAGE_F16 || type == QC_STORAGE_BF16;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// dev_status set: launch(dev_status), asynchronous.  NULL: check(flag) first,
+// 3 and nothing written if it set the flag, then launch and wait.
+template <class Check, class Launch>
+int checked(int* dev_status, hipStream_t s, Check&& check, Launch&& launch) {
+  if (dev_status != nullptr) return finish(launch(dev_status));
+  int bad = 0;
+  int st = with_flag(s, &bad, check);
+  if (st != QC_OK) return st;
+  if (bad) return QC_INVALID_ARGUMENT;
+  st = with_flag(s, &bad, launch);
+  return st == QC_OK && bad ? QC_INVALID_ARGUMENT : st;
+}
+
+// Sizes of a cache and a batch; 64-bit element offsets, int counts.
+bool kv8_shapes(const qc_kv8_cache& c, const qc_kv8_batch& b) {
+  if (!valid_product({c.pages, c.kv_heads, c.page_tokens, c.head_dim})) return false;
+  if (c.page_tokens < 16 || c.page_tokens > 256 || (c.page_tokens & (c.page_tokens - 1)) != 0)
+    return false;
+  if (c.head_dim > 256 || c.head_dim % 16 != 0) return false;
+  if (!valid_product({b.seqs, b.columns, c.page_tokens}) || b.tokens <= 0 || b.max_new <= 0 ||
+      b.max_kv <= 0)
+    return false;
+  if (c.pages > INT_MAX || c.kv_heads > INT_MAX / 256 || b.seqs > INT_MAX - 1 || b.tokens > INT_MAX ||
+      b.columns * c.page_tokens > INT_MAX - 512)
+    return false;
+  if (b.max_new > b.tokens || b.max_kv > b.columns * c.page_tokens) return false;
+  // a workgroup per sequence, touched page and head
+  const long long slots = (b.max_new + c.page_tokens - 2) / c.page_tokens + 1;
+  return valid_product({2, c.kv_heads, slots, b.seqs}) && 2 * c.kv_heads * slots * b.seqs <= INT_MAX;
+}
+
+bool kv8_pointers(const qc_kv8_cache& c, const qc_kv8_batch& b) {
+  return c.k_codes != nullptr && c.v_codes != nullptr && c.k_scales != nullptr &&
+         c.v_scales != nullptr && b.block_table != nullptr && b.seq_start != nullptr &&
+         b.kv_len != nullptr && aligned16(c.k_codes) && aligned16(c.v_codes);
+}
 
 }  // namespace
 
@@ -709,6 +753,233 @@ int qc_hip_dequantize_int8_asymmetric(const int8_t* codes, const float* scales,
   if (!codes || !scales || !zero_points || !out) return QC_INVALID_ARGUMENT;
   return finish(qc::launch_dequantize_int8_asymmetric(codes, scales, zero_points, out, rows,
                                                       dim, as_stream(stream)));
+}
+
+// ---- Rotary positions, 8-bit cache, MXFP4 (no reference counterpart) -------
+
+int qc_hip_rope_table(float* cosine, float* sine, long long first_position, long long positions,
+                      long long rotary_dim, double base, const qc_rope_scaling* scaling,
+                      void* stream) {
+  if (positions <= 0 || first_position < 0 || positions > (1LL << 31) ||
+      first_position > (1LL << 31) - positions)
+    return QC_INVALID_SHAPE;
+  if (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > 2 * qc::kRopeMaxHalf)
+    return QC_INVALID_SHAPE;
+  if (cosine == nullptr || sine == nullptr) return QC_INVALID_ARGUMENT;
+  if (!std::isfinite(base) || base <= 1.0) return QC_INVALID_ARGUMENT;
+  constexpr double kPi = 3.14159265358979323846;
+  const int half = static_cast<int>(rotary_dim / 2);
+  const double d = static_cast<double>(rotary_dim);
+  const int kind = scaling != nullptr ? scaling->kind : QC_ROPE_SCALE_NONE;
+  const bool blend = kind == QC_ROPE_SCALE_TURNS || kind == QC_ROPE_SCALE_YARN;
+  double factor = 1.0, magnitude = 1.0;
+  if (scaling != nullptr) {
+    if (kind < QC_ROPE_SCALE_NONE || kind > QC_ROPE_SCALE_YARN) return QC_INVALID_ARGUMENT;
+    factor = scaling->factor;
+    magnitude = scaling->magnitude;
+    if (!std::isfinite(magnitude) || magnitude <= 0.0) return QC_INVALID_ARGUMENT;
+    if (kind != QC_ROPE_SCALE_NONE && (!std::isfinite(factor) || factor < 1.0))
+      return QC_INVALID_ARGUMENT;
+    if (kind == QC_ROPE_SCALE_NTK && rotary_dim == 2) return QC_INVALID_ARGUMENT;
+    if (blend && !(scaling->original_positions > 0.0 && std::isfinite(scaling->original_positions) &&
+                   scaling->low_turns > 0.0 && scaling->high_turns > scaling->low_turns &&
+                   std::isfinite(scaling->high_turns)))
+      return QC_INVALID_ARGUMENT;
+  }
+  const double b = kind == QC_ROPE_SCALE_NTK ? base * std::pow(factor, d / (d - 2.0)) : base;
+  double low = 0.0, high = 0.0;
+  if (kind == QC_ROPE_SCALE_YARN) {
+    // the pair index whose frequency makes t turns over the original context
+    const auto index = [&](double t) {
+      return d * std::log(scaling->original_positions / (2.0 * kPi * t)) / (2.0 * std::log(base));
+    };
+    low = std::max(std::floor(index(scaling->high_turns)), 0.0);
+    high = std::min(std::ceil(index(scaling->low_turns)), d - 1.0);
+    high = low + std::max(high - low, 0.001);
+  }
+  qc::RopeFrequencies f = {};
+  f.magnitude = magnitude;
+  for (int i = 0; i < half; ++i) {
+    const double w = std::pow(b, -2.0 * i / d);
+    double keep = 1.0;
+    if (kind == QC_ROPE_SCALE_LINEAR) {
+      keep = 0.0;
+    } else if (kind == QC_ROPE_SCALE_TURNS) {
+      const double turns = scaling->original_positions * w / (2.0 * kPi);
+      keep = (turns - scaling->low_turns) / (scaling->high_turns - scaling->low_turns);
+    } else if (kind == QC_ROPE_SCALE_YARN) {
+      keep = 1.0 - (i - low) / (high - low);
+    }
+    keep = std::min(std::max(keep, 0.0), 1.0);
+    f.w[i] = keep * w + (1.0 - keep) * w / factor;
+  }
+  return finish(qc::launch_rope_table(cosine, sine, first_position, positions, half, f,
+                                      as_stream(stream)));
+}
+
+int qc_hip_rope(const void* x, void* y, int type, long long tokens, long long heads,
+                long long head_dim, long long rotary_dim, long long x_token_stride,
+                long long x_head_stride, long long y_token_stride, long long y_head_stride,
+                const float* cosine, const float* sine, const int* positions,
+                long long max_position, int layout, int* dev_status, void* stream) {
+  if (!valid_product({tokens, heads, head_dim}) || tokens > INT_MAX || heads > INT_MAX / 256 ||
+      head_dim > 65536 || heads * head_dim > (1LL << 30))
+    return QC_INVALID_SHAPE;
+  if (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > head_dim) return QC_INVALID_SHAPE;
+  if (max_position <= 0 || max_position > INT_MAX) return QC_INVALID_SHAPE;
+  // heads do not overlap within a token, nor tokens each other
+  const long long strides[2][2] = {{x_token_stride, x_head_stride}, {y_token_stride, y_head_stride}};
+  for (const auto& st : strides) {
+    const long long token = st[0], head = heads > 1 ? st[1] : head_dim;
+    if (head < head_dim || head > LLONG_MAX / heads / 8) return QC_INVALID_SHAPE;
+    if (tokens > 1 && token < (heads - 1) * head + head_dim) return QC_INVALID_SHAPE;
+    if (tokens > 1 && token > LLONG_MAX / tokens / 8) return QC_INVALID_SHAPE;
+  }
+  if (!known_storage(type)) return QC_UNSUPPORTED_FORMAT;
+  if (layout != QC_ROPE_HALF && layout != QC_ROPE_INTERLEAVED) return QC_INVALID_ARGUMENT;
+  if (x == nullptr || y == nullptr || cosine == nullptr || sine == nullptr || positions == nullptr)
+    return QC_INVALID_ARGUMENT;
+  qc::RopeLaunch r;
+  r.x = x;
+  r.y = y;
+  r.type = type;
+  r.tokens = tokens;
+  r.heads = heads;
+  r.head_dim = head_dim;
+  r.rotary = rotary_dim;
+  r.x_token = tokens > 1 ? x_token_stride : 0;
+  r.x_head = heads > 1 ? x_head_stride : 0;
+  r.y_token = tokens > 1 ? y_token_stride : 0;
+  r.y_head = heads > 1 ? y_head_stride : 0;
+  if (x == y && (r.x_token != r.y_token || r.x_head != r.y_head)) return QC_INVALID_ARGUMENT;
+  r.cosine = cosine;
+  r.sine = sine;
+  r.positions = positions;
+  r.max_position = max_position;
+  r.interleaved = layout == QC_ROPE_INTERLEAVED;
+  const hipStream_t s = as_stream(stream);
+  return checked(
+      dev_status, s,
+      [&](int* flag) { return qc::launch_rope_check(positions, tokens, max_position, flag, s); },
+      [&](int* flag) { return qc::launch_rope(r, flag, s); });
+}
+
+int qc_hip_kv8_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* k,
+                      long long k_stride, const void* v, long long v_stride, int type,
+                      int* dev_status, void* stream) {
+  if (cache == nullptr || batch == nullptr) return QC_INVALID_ARGUMENT;
+  if (!kv8_shapes(*cache, *batch)) return QC_INVALID_SHAPE;
+  const long long row = cache->kv_heads * cache->head_dim, most = LLONG_MAX / 8 / batch->tokens;
+  if (k_stride < row || v_stride < row || k_stride > most || v_stride > most) return QC_INVALID_SHAPE;
+  if (!known_storage(type)) return QC_UNSUPPORTED_FORMAT;
+  if (!kv8_pointers(*cache, *batch) || k == nullptr || v == nullptr) return QC_INVALID_ARGUMENT;
+  const hipStream_t s = as_stream(stream);
+  return checked(
+      dev_status, s,
+      [&](int* flag) {
+        hipError_t e = qc::launch_kv8_check(*cache, *batch, true, 0, flag, s);
+        if (e == hipSuccess) e = qc::launch_kv8_nonfinite(*cache, *batch, k, k_stride, v, v_stride, type, flag, s);
+        return e;
+      },
+      [&](int* flag) {
+        return qc::launch_kv8_append(*cache, *batch, k, k_stride, v, v_stride, type, flag, s);
+      });
+}
+
+int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void* k,
+                      long long k_stride, void* v, long long v_stride, int type, int* dev_status,
+                      void* stream) {
+  if (cache == nullptr || batch == nullptr) return QC_INVALID_ARGUMENT;
+  if (!kv8_shapes(*cache, *batch)) return QC_INVALID_SHAPE;
+  const long long row = cache->kv_heads * cache->head_dim, most = LLONG_MAX / 8 / batch->tokens;
+  if (k_stride < row || v_stride < row || k_stride > most || v_stride > most) return QC_INVALID_SHAPE;
+  if (!known_storage(type)) return QC_UNSUPPORTED_FORMAT;
+  if (!kv8_pointers(*cache, *batch) || k == nullptr || v == nullptr) return QC_INVALID_ARGUMENT;
+  const hipStream_t s = as_stream(stream);
+  return checked(
+      dev_status, s,
+      [&](int* flag) { return qc::launch_kv8_check(*cache, *batch, true, 0, flag, s); },
+      [&](int* flag) {
+        return qc::launch_kv8_gather(*cache, *batch, k, k_stride, v, v_stride, type, flag, s);
+      });
+}
+
+int qc_hip_kv8_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* q,
+                         long long q_stride, void* out, long long out_stride, int type,
+                         long long heads, float scale, int causal, long long window,
+                         int* dev_status, void* stream) {
+  if (cache == nullptr || batch == nullptr) return QC_INVALID_ARGUMENT;
+  if (!kv8_shapes(*cache, *batch)) return QC_INVALID_SHAPE;
+  if (heads <= 0 || heads % cache->kv_heads != 0 || heads > INT_MAX / 256 || window < 0)
+    return QC_INVALID_SHAPE;
+  // rows of a sequence and key head are counted in an int
+  if (batch->max_new * (heads / cache->kv_heads) > INT_MAX / 2) return QC_INVALID_SHAPE;
+  const long long row = heads * cache->head_dim, most = LLONG_MAX / 8 / batch->tokens;
+  if (q_stride < row || out_stride < row || q_stride > most || out_stride > most)
+    return QC_INVALID_SHAPE;
+  if (!known_storage(type)) return QC_UNSUPPORTED_FORMAT;
+  if (!kv8_pointers(*cache, *batch) || q == nullptr || out == nullptr) return QC_INVALID_ARGUMENT;
+  if (!std::isfinite(scale) || (window > 0 && !causal)) return QC_INVALID_ARGUMENT;
+  qc::Kv8Attention r;
+  r.cache = cache;
+  r.batch = batch;
+  r.q = q;
+  r.out = out;
+  r.q_stride = q_stride;
+  r.out_stride = out_stride;
+  r.type = type;
+  r.heads = heads;
+  r.window = std::min<long long>(window, INT_MAX / 2);
+  r.scale = scale;
+  r.causal = causal != 0;
+  const hipStream_t s = as_stream(stream);
+  return checked(
+      dev_status, s,
+      [&](int* flag) {
+        return qc::launch_kv8_check(*cache, *batch, false, static_cast<int>(r.window), flag, s);
+      },
+      [&](int* flag) { return qc::launch_kv8_attention(r, flag, s); });
+}
+
+int qc_hip_quantize_mxfp4(const void* x, int type, long long x_stride, uint8_t* codes,
+                          uint8_t* scales, long long rows, long long dim, int* dev_status,
+                          void* stream) {
+  if (!valid_product({rows, dim, 4}) || dim % 32 != 0) return QC_INVALID_SHAPE;
+  if (rows > 1 && (x_stride < dim || x_stride > LLONG_MAX / 8 / rows)) return QC_INVALID_SHAPE;
+  if (!known_storage(type)) return QC_UNSUPPORTED_FORMAT;
+  if (x == nullptr || codes == nullptr || scales == nullptr || !aligned16(codes))
+    return QC_INVALID_ARGUMENT;
+  const long long stride = rows > 1 ? x_stride : dim;
+  const hipStream_t s = as_stream(stream);
+  return checked(
+      dev_status, s,
+      [&](int* flag) { return qc::launch_mxfp4_nonfinite(x, type, stride, rows, dim, flag, s); },
+      [&](int* flag) {
+        return qc::launch_quantize_mxfp4(x, type, stride, codes, scales, rows, dim, flag, s);
+      });
+}
+
+int qc_hip_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, void* out, int type,
+                            long long rows, long long dim, void* stream) {
+  if (!valid_product({rows, dim, 4}) || dim % 32 != 0) return QC_INVALID_SHAPE;
+  if (!known_storage(type)) return QC_UNSUPPORTED_FORMAT;
+  if (codes == nullptr || scales == nullptr || out == nullptr || !aligned16(codes))
+    return QC_INVALID_ARGUMENT;
+  return finish(qc::launch_dequantize_mxfp4(codes, scales, out, type, rows, dim, as_stream(stream)));
+}
+
+int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* x_codes,
+                      const uint8_t* x_scales, void* y, int y_type, long long m, long long n,
+                      long long k, void* stream) {
+  if (!valid_product({m, n, 4}) || !valid_product({m, k}) || !valid_product({n, k}) || k % 32 != 0)
+    return QC_INVALID_SHAPE;
+  if (m > INT_MAX / 2 || n > INT_MAX / 2 || k > INT_MAX / 2) return QC_INVALID_SHAPE;
+  if (!known_storage(y_type)) return QC_UNSUPPORTED_FORMAT;
+  if (w_codes == nullptr || w_scales == nullptr || x_codes == nullptr || x_scales == nullptr ||
+      y == nullptr || !aligned16(w_codes) || !aligned16(x_codes))
+    return QC_INVALID_ARGUMENT;
+  return finish(qc::launch_mxfp4_gemm(w_codes, w_scales, x_codes, x_scales, y, y_type, m, n, k,
+                                      as_stream(stream)));
 }
 
 int qc_hip_set_qgemm_panel(int mode) {

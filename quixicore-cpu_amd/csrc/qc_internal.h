@@ -251,4 +251,73 @@ hipError_t launch_pack(int fmt, const float* w, void* packed, long long n, long 
 hipError_t launch_unpack(int fmt, const void* packed, float* w, long long n, long long k,
                          hipStream_t s);
 
+// Rotation of `tokens` tokens' heads by their positions (qc_hip_rope); all
+// checks done by the caller.  Strides in elements.  *status = 3 where a position
+// is outside [-1, max_position).
+struct RopeLaunch {
+  const void* x = nullptr;
+  void* y = nullptr;
+  int type = QC_STORAGE_F32;
+  long long tokens = 0, heads = 0, head_dim = 0, rotary = 0;
+  long long x_token = 0, x_head = 0, y_token = 0, y_head = 0;
+  const float* cosine = nullptr;
+  const float* sine = nullptr;
+  const int* positions = nullptr;
+  long long max_position = 0;
+  bool interleaved = false;
+};
+hipError_t launch_rope(const RopeLaunch& r, int* status, hipStream_t s);
+hipError_t launch_rope_check(const int* positions, long long tokens, long long max_position,
+                             int* flag, hipStream_t s);
+
+// Cosine and sine rows [count][half] of positions first, first + 1, ...; the
+// frequencies travel as a kernel argument.
+constexpr int kRopeMaxHalf = 256;
+struct RopeFrequencies {
+  double magnitude;
+  double w[kRopeMaxHalf];
+};
+hipError_t launch_rope_table(float* cosine, float* sine, long long first, long long count,
+                             int half, const RopeFrequencies& f, hipStream_t s);
+
+// The 8-bit key/value cache (qc_hip_kv8_*); shapes and pointers checked by the
+// caller, the device's lengths and page ids by the kernels (*status = 3).
+hipError_t launch_kv8_check(const qc_kv8_cache& c, const qc_kv8_batch& b, bool from_new, int window,
+                            int* flag, hipStream_t s);
+hipError_t launch_kv8_nonfinite(const qc_kv8_cache& c, const qc_kv8_batch& b, const void* k,
+                                long long k_stride, const void* v, long long v_stride, int type,
+                                int* flag, hipStream_t s);
+hipError_t launch_kv8_append(const qc_kv8_cache& c, const qc_kv8_batch& b, const void* k,
+                             long long k_stride, const void* v, long long v_stride, int type,
+                             int* status, hipStream_t s);
+hipError_t launch_kv8_gather(const qc_kv8_cache& c, const qc_kv8_batch& b, void* k,
+                             long long k_stride, void* v, long long v_stride, int type, int* status,
+                             hipStream_t s);
+struct Kv8Attention {
+  const qc_kv8_cache* cache = nullptr;
+  const qc_kv8_batch* batch = nullptr;
+  const void* q = nullptr;
+  void* out = nullptr;
+  long long q_stride = 0, out_stride = 0;
+  int type = QC_STORAGE_F32;
+  long long heads = 0, window = 0;
+  float scale = 1.f;
+  int causal = 1;
+};
+hipError_t launch_kv8_attention(const Kv8Attention& r, int* status, hipStream_t s);
+
+// MXFP4 (qc_hip_*_mxfp4, qc_hip_mxfp4_gemm); dim and k multiples of 32, codes
+// 16-byte aligned.  Blocks with non-finite values are left unwritten and set
+// *status = 3.
+hipError_t launch_mxfp4_nonfinite(const void* x, int type, long long stride, long long rows,
+                                  long long dim, int* flag, hipStream_t s);
+hipError_t launch_quantize_mxfp4(const void* x, int type, long long stride, uint8_t* codes,
+                                 uint8_t* scales, long long rows, long long dim, int* status,
+                                 hipStream_t s);
+hipError_t launch_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, void* out, int type,
+                                   long long rows, long long dim, hipStream_t s);
+hipError_t launch_mxfp4_gemm(const uint8_t* w, const uint8_t* ws, const uint8_t* x,
+                             const uint8_t* xs, void* y, int type, long long m, long long n,
+                             long long k, hipStream_t s);
+
 }  // namespace qc

@@ -71,6 +71,16 @@ _SIGS = {
     "qc_hip_cint8_dequantize": ([_P, _P, _P, _P], _I),
     "qc_hip_cint8_quantized_gemm": ([_P, _P, _P, _P, _P], _I),
     "qc_hip_storage_to_f32": ([_P, _I, _LL, _P, _P], _I),
+    "qc_hip_rope_table": ([_P, _P, _LL, _LL, _LL, ctypes.c_double, _P, _P], _I),
+    "qc_hip_rope": ([_P, _P, _I, _LL, _LL, _LL, _LL, _LL, _LL, _LL, _LL, _P, _P, _P, _LL, _I, _P,
+                     _P], _I),
+    "qc_hip_kv8_append": ([_P, _P, _P, _LL, _P, _LL, _I, _P, _P], _I),
+    "qc_hip_kv8_gather": ([_P, _P, _P, _LL, _P, _LL, _I, _P, _P], _I),
+    "qc_hip_kv8_attention": ([_P, _P, _P, _LL, _P, _LL, _I, _LL, ctypes.c_float, _I, _LL, _P, _P],
+                             _I),
+    "qc_hip_quantize_mxfp4": ([_P, _I, _LL, _P, _P, _LL, _LL, _P, _P], _I),
+    "qc_hip_dequantize_mxfp4": ([_P, _P, _P, _I, _LL, _LL, _P], _I),
+    "qc_hip_mxfp4_gemm": ([_P, _P, _P, _P, _P, _I, _LL, _LL, _LL, _P], _I),
 }
 for _name, (_args, _res) in _SIGS.items():
     _fn = getattr(lib, _name)
@@ -330,6 +340,271 @@ def int8_gemm_i32(w, x):
     acc = torch.empty((m, n), dtype=torch.int32, device=x.device)
     _check(int8_gemm_i32_raw(w, x, acc, m, n, k), "int8_gemm_i32")
     return acc
+
+
+# Rotary positions, the 8-bit key/value cache and MXFP4 (include/quixicore_hip.h).
+# These helpers check what the C ABI cannot see: types, shapes, contiguity, and
+# that tensors lie on the current device, whose stream the call goes to.
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "turns": 3, "yarn": 4}
+
+
+class RopeScaling(ctypes.Structure):
+    """qc_rope_scaling (include/quixicore_hip.h)."""
+    _fields_ = [("kind", ctypes.c_int), ("factor", ctypes.c_double),
+                ("original_positions", ctypes.c_double), ("low_turns", ctypes.c_double),
+                ("high_turns", ctypes.c_double), ("magnitude", ctypes.c_double)]
+
+
+_storage_ids = None   # torch dtype -> STORAGE id
+_device = None        # index of the current device
+
+
+def _storage(t):
+    global _storage_ids, _device
+    if _storage_ids is None:
+        import torch
+        torch.cuda.current_stream()   # initialises the device
+        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        _storage_ids = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    st = _storage_ids.get(t.dtype)
+    if st is None:
+        raise TypeError(f"f32, f16 or bf16 tensors: got {t.dtype}")
+    _here(t)
+    return st
+
+
+def _here(*tensors):
+    global _device
+    if _device is None:
+        import torch
+        torch.cuda.current_stream()
+        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    now = _device()
+    for t in tensors:
+        if t is not None and (t.device.type != "cuda" or t.device.index != now):
+            raise ValueError(f"a tensor on {t.device}: the current device is cuda:{now}")
+
+
+def _flat(what, dtype, *tensors):
+    """Contiguous tensors of one type on the current device."""
+    _here(*tensors)
+    for t in tensors:
+        if t is not None and (t.dtype != dtype or not t.is_contiguous()):
+            raise ValueError(f"{what}: contiguous {dtype} tensors")
+
+
+def _status(dev_status):
+    import torch
+    if dev_status is not None:
+        _flat("dev_status", torch.int32, dev_status)
+    return _ptr(dev_status)
+
+
+def _rows(what, t, heads, head_dim):
+    """Row stride of token rows [tokens][heads * head_dim] or [tokens][heads][head_dim]."""
+    ok = (t.dim() == 2 and t.shape[1] == heads * head_dim and t.stride(1) == 1) or (
+        t.dim() == 3 and t.shape[1] == heads and t.shape[2] == head_dim and t.stride(2) == 1
+        and (heads == 1 or t.stride(1) == head_dim))
+    if not ok:
+        raise ValueError(f"{what}: rows of {heads} x {head_dim} elements side by side, got "
+                         f"{tuple(t.shape)} with strides {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else heads * head_dim
+
+
+def rope_table(positions, rotary_dim, base=10000.0, scaling="none", factor=1.0,
+               original_positions=0.0, low_turns=1.0, high_turns=32.0, magnitude=1.0,
+               first_position=0):
+    """(cosine, sine), f32 [positions][rotary_dim / 2], on the current device; scaling one of
+    ROPE_SCALING (see qc_rope_scaling)."""
+    import torch
+    cosine = torch.empty((positions, rotary_dim // 2), dtype=torch.float32, device="cuda")
+    sine = torch.empty_like(cosine)
+    sc = RopeScaling(ROPE_SCALING[scaling], factor, original_positions, low_turns, high_turns,
+                     magnitude)
+    _check(lib.qc_hip_rope_table(_ptr(cosine), _ptr(sine), first_position, positions, rotary_dim,
+                                 base, ctypes.addressof(sc), _stream(None)), "rope_table")
+    return cosine, sine
+
+
+def rope(x, cosine, sine, positions, interleaved=False, out=None, dev_status=None):
+    """x [tokens][heads][head_dim] (any token and head strides) with the first 2 *
+    cosine.shape[1] elements of every head rotated; out may be x."""
+    import torch
+    st = _storage(x)
+    if x.dim() != 3 or x.stride(2) != 1:
+        raise ValueError("rope: x is [tokens][heads][head_dim], elements side by side")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.stride(2) != 1 or out.dtype != x.dtype:
+        raise ValueError("rope: out is of x's shape and type")
+    _here(out)
+    _flat("rope tables", torch.float32, cosine, sine)
+    _flat("rope positions", torch.int32, positions)
+    tokens, heads, head_dim = x.shape
+    if cosine.dim() != 2 or sine.shape != cosine.shape or positions.numel() != tokens:
+        raise ValueError("rope: tables [max_position][rotary_dim / 2], a position for each token")
+    _check(lib.qc_hip_rope(_ptr(x), _ptr(out), st, tokens, heads, head_dim, 2 * cosine.shape[1],
+                           x.stride(0), x.stride(1), out.stride(0), out.stride(1), _ptr(cosine),
+                           _ptr(sine), _ptr(positions), cosine.shape[0], int(bool(interleaved)),
+                           _status(dev_status), _stream(None)), "rope")
+    return out
+
+
+class Kv8Cache(ctypes.Structure):
+    """qc_kv8_cache over int8 codes [pages][kv_heads][page_tokens][head_dim] and f32 scales
+    [pages][kv_heads]; keeps the tensors alive."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+                ("k_scales", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+                ("pages", ctypes.c_longlong), ("kv_heads", ctypes.c_longlong),
+                ("page_tokens", ctypes.c_longlong), ("head_dim", ctypes.c_longlong)]
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales):
+        import torch
+        _flat("cache codes", torch.int8, k_codes, v_codes)
+        _flat("cache scales", torch.float32, k_scales, v_scales)
+        if (k_codes.dim() != 4 or v_codes.shape != k_codes.shape
+                or k_scales.shape != k_codes.shape[:2] or v_scales.shape != k_codes.shape[:2]):
+            raise ValueError("codes [pages][kv_heads][page_tokens][head_dim], scales [pages][kv_heads]")
+        self.tensors = (k_codes, v_codes, k_scales, v_scales)
+        super().__init__(*[t.data_ptr() for t in self.tensors], *k_codes.shape)
+
+
+class Kv8Batch(ctypes.Structure):
+    """qc_kv8_batch over int32 block_table [seqs][columns], seq_start [seqs + 1] and
+    kv_len [seqs]; keeps the tensors alive."""
+    _fields_ = [("block_table", ctypes.c_void_p), ("seq_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("seqs", ctypes.c_longlong),
+                ("columns", ctypes.c_longlong), ("tokens", ctypes.c_longlong),
+                ("max_new", ctypes.c_longlong), ("max_kv", ctypes.c_longlong)]
+
+    def __init__(self, block_table, seq_start, kv_len, tokens, max_new, max_kv):
+        import torch
+        _flat("batch", torch.int32, block_table, seq_start, kv_len)
+        seqs, columns = block_table.shape
+        if seq_start.numel() != seqs + 1 or kv_len.numel() != seqs:
+            raise ValueError("block_table [seqs][columns], seq_start [seqs + 1], kv_len [seqs]")
+        self.tensors = (block_table, seq_start, kv_len)
+        super().__init__(*[t.data_ptr() for t in self.tensors], seqs, columns, tokens, max_new,
+                         max_kv)
+
+
+def _kv8_here(cache, batch):
+    _here(cache.tensors[0], batch.tensors[0])
+
+
+def kv8_cache(pages, kv_heads, page_tokens, head_dim):
+    """An empty cache (zeros) on the current device."""
+    import torch
+    shape = (pages, kv_heads, page_tokens, head_dim)
+    codes = [torch.zeros(shape, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros((pages, kv_heads), dtype=torch.float32, device="cuda") for _ in range(2)]
+    return Kv8Cache(*codes, *scales)
+
+
+def kv8_append(cache, batch, k, v, dev_status=None):
+    """Writes the batch's new tokens' k and v ([tokens][kv_heads][head_dim] or flat rows)."""
+    st = _storage(k)
+    _here(v)
+    _kv8_here(cache, batch)
+    if v.dtype != k.dtype or k.shape[0] != batch.tokens or v.shape[0] != batch.tokens:
+        raise ValueError("kv8_append: k and v of one type, a row for each of the batch's tokens")
+    _check(lib.qc_hip_kv8_append(ctypes.addressof(cache), ctypes.addressof(batch), _ptr(k),
+                                 _rows("k", k, cache.kv_heads, cache.head_dim), _ptr(v),
+                                 _rows("v", v, cache.kv_heads, cache.head_dim), st,
+                                 _status(dev_status), _stream(None)), "kv8_append")
+
+
+def kv8_gather(cache, batch, dtype=None, k=None, v=None, dev_status=None):
+    """(k, v) [tokens][kv_heads][head_dim]: the values the cache holds for the batch's
+    tokens.  Rows of no sequence are left as they were (zeros in new tensors)."""
+    import torch
+    shape = (batch.tokens, cache.kv_heads, cache.head_dim)
+    if k is None:
+        k = torch.zeros(shape, dtype=dtype or torch.float32, device=cache.tensors[0].device)
+    if v is None:
+        v = torch.zeros(shape, dtype=k.dtype, device=k.device)
+    st = _storage(k)
+    _here(v)
+    _kv8_here(cache, batch)
+    if v.dtype != k.dtype or k.shape[0] != batch.tokens or v.shape[0] != batch.tokens:
+        raise ValueError("kv8_gather: k and v of one type, a row for each of the batch's tokens")
+    _check(lib.qc_hip_kv8_gather(ctypes.addressof(cache), ctypes.addressof(batch), _ptr(k),
+                                 _rows("k", k, cache.kv_heads, cache.head_dim), _ptr(v),
+                                 _rows("v", v, cache.kv_heads, cache.head_dim), st,
+                                 _status(dev_status), _stream(None)), "kv8_gather")
+    return k, v
+
+
+def kv8_attention(cache, batch, q, scale=None, causal=True, window=0, out=None, dev_status=None):
+    """softmax(scale q k^T) v of the batch's tokens over the cache: q [tokens][heads][head_dim]
+    (rows may be strided), scale 1 / sqrt(head_dim) by default.  Rows of no sequence are left as
+    they were (zeros in a new tensor)."""
+    import torch
+    st = _storage(q)
+    _kv8_here(cache, batch)
+    if q.dim() != 3 or q.shape[0] != batch.tokens:
+        raise ValueError("kv8_attention: q is [tokens][heads][head_dim], a row for each of the batch's tokens")
+    heads = q.shape[1]
+    if out is None:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("kv8_attention: out is of q's shape and type")
+    _here(out)
+    if scale is None:
+        scale = cache.head_dim ** -0.5
+    _check(lib.qc_hip_kv8_attention(ctypes.addressof(cache), ctypes.addressof(batch), _ptr(q),
+                                    _rows("q", q, heads, cache.head_dim), _ptr(out),
+                                    _rows("out", out, heads, cache.head_dim), st, heads, scale,
+                                    int(bool(causal)), window, _status(dev_status), _stream(None)),
+           "kv8_attention")
+    return out
+
+
+def quantize_mxfp4(x, dev_status=None):
+    """(codes [rows][dim / 2], scales [rows][dim / 32]) uint8 of x [rows][dim] (rows may be
+    strided)."""
+    import torch
+    st = _storage(x)
+    if x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError("quantize_mxfp4: x is [rows][dim], elements side by side")
+    rows, dim = x.shape
+    codes = torch.empty((rows, dim // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((rows, dim // 32), dtype=torch.uint8, device=x.device)
+    _check(lib.qc_hip_quantize_mxfp4(_ptr(x), st, x.stride(0), _ptr(codes), _ptr(scales), rows,
+                                     dim, _status(dev_status), _stream(None)), "quantize_mxfp4")
+    return codes, scales
+
+
+def dequantize_mxfp4(codes, scales, dtype=None, out=None):
+    """The values [rows][dim] that MXFP4 codes and scales stand for."""
+    import torch
+    _flat("mxfp4", torch.uint8, codes, scales)
+    rows, dim = codes.shape[0], 2 * codes.shape[1]
+    if out is None:
+        out = torch.empty((rows, dim), dtype=dtype or torch.float32, device=codes.device)
+    if tuple(scales.shape) != (rows, dim // 32) or tuple(out.shape) != (rows, dim) or not out.is_contiguous():
+        raise ValueError("dequantize_mxfp4: codes [rows][dim / 2], scales [rows][dim / 32], out [rows][dim]")
+    _check(lib.qc_hip_dequantize_mxfp4(_ptr(codes), _ptr(scales), _ptr(out), _storage(out), rows,
+                                       dim, _stream(None)), "dequantize_mxfp4")
+    return out
+
+
+def mxfp4_gemm(w_codes, w_scales, x_codes, x_scales, dtype=None, y=None):
+    """y [m][n] = x . w^T of MXFP4 matrices w [n][k] and x [m][k]."""
+    import torch
+    _flat("mxfp4_gemm", torch.uint8, w_codes, w_scales, x_codes, x_scales)
+    (n, half), m = w_codes.shape, x_codes.shape[0]
+    k = 2 * half
+    if (x_codes.shape[1] != half or tuple(w_scales.shape) != (n, k // 32)
+            or tuple(x_scales.shape) != (m, k // 32)):
+        raise ValueError("mxfp4_gemm: codes [rows][k / 2], scales [rows][k / 32]")
+    if y is None:
+        y = torch.empty((m, n), dtype=dtype or torch.float32, device=x_codes.device)
+    elif tuple(y.shape) != (m, n) or not y.is_contiguous():
+        raise ValueError("mxfp4_gemm: y is [m][n], contiguous")
+    _check(lib.qc_hip_mxfp4_gemm(_ptr(w_codes), _ptr(w_scales), _ptr(x_codes), _ptr(x_scales),
+                                 _ptr(y), _storage(y), m, n, k, _stream(None)), "mxfp4_gemm")
+    return y
 
 
 def set_gemv_rows_per_wave(rows):
