@@ -421,7 +421,8 @@ typedef struct qc_kv8_batch {
  * token rows k_stride / v_stride elements apart) into the cache at positions
  * kv_len - n .. kv_len - 1 of their sequences.  Per page and head, with t the new
  * tokens' largest magnitude there and s the scale held (0 where the page has no
- * token before the new ones): s' = max(s, t / 127), or 0 below 2^-126; codes held
+ * token before the new ones): s' = max(s, t * c), c the f32
+ * nearest 1 / 127, or 0 below 2^-126; codes held
  * become rint(code * (s / s')), new ones clamp(rint(x * (1 / s')), +-127), each
  * step rounded to f32.  A page written by a call must belong to one sequence.
  * A page and head with a non-finite new value, and a sequence of more new tokens than

@@ -3,7 +3,7 @@
 // code * scale.
 //
 // Append.  A page's scale only grows while the page fills: with the new tokens'
-// largest magnitude t, s' = max(s, t / 127) (s = 0 where the page holds no
+// largest magnitude t, s' = max(s, t * c), c the f32 nearest 1 / 127 (s = 0 where the page holds no
 // tokens before the new ones; s' below 2^-126 counts as 0), the codes there
 // become rint(code * (s / s')) and the new ones clamp(rint(x * (1 / s')), -127,
 // 127), ties to even, each step rounded to f32.  So a call's codes are
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Kv8Args a, Rows k, Row
     return;
   }
   const float before = lo > p0 ? *scale_at : 0.f;
-  float scale = fmaxf(before, top / 127.0f);
+  float scale = fmaxf(before, top * (1.0f / 127.0f));
   if (scale < 1.17549435e-38f) scale = 0.f;
   const float inv = scale > 0.f ? 1.0f / scale : 0.f;
   const float ratio = scale > 0.f ? before / scale : 0.f;

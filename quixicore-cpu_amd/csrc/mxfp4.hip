@@ -113,28 +113,6 @@ __global__ __launch_bounds__(kThreads) void mxfp4_nonfinite(const void* __restri
   }
 }
 
-// y[m][n] = sum over blocks of 2^(ew + ex) sum_i w_i x_i: one thread an output.
-template <int TYPE>
-__global__ __launch_bounds__(kThreads) void product_simple(
-    const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws, const uint8_t* __restrict__ x,
-    const uint8_t* __restrict__ xs, void* __restrict__ y, long long m, long long n, long long blocks) {
-  typedef typename Storage<TYPE>::raw raw;
-  const long long o = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
-  if (o >= m * n) return;
-  const long long mi = o / n, ni = o - mi * n;
-  float acc = 0.f;
-  for (long long b = 0; b < blocks; ++b) {
-    const int ew = ws[ni * blocks + b], ex = xs[mi * blocks + b];
-    float sum = 0.f;
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t a = w[(ni * blocks + b) * 16 + j], c = x[(mi * blocks + b) * 16 + j];
-      sum += e2m1_value(a & 15) * e2m1_value(c & 15) + e2m1_value(a >> 4) * e2m1_value(c >> 4);
-    }
-    acc += ew == 255 || ex == 255 ? __uint_as_float(0x7FC00000u) : ldexpf(sum, ew + ex - 254);
-  }
-  static_cast<raw*>(y)[o] = encode<TYPE>(acc);
-}
-
 int grid_for(long long items) {
   return static_cast<int>(std::min<long long>((items + kThreads - 1) / kThreads, 1 << 20));
 }
@@ -187,23 +165,6 @@ hipError_t launch_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, 
       break;
     default:
       dequantize_kernel<QC_STORAGE_BF16><<<grid, kThreads, 0, s>>>(codes, scales, out, count);
-  }
-  return hipGetLastError();
-}
-
-hipError_t launch_mxfp4_gemm(const uint8_t* w, const uint8_t* ws, const uint8_t* x,
-                             const uint8_t* xs, void* y, int type, long long m, long long n,
-                             long long k, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>((m * n + kThreads - 1) / kThreads);
-  switch (type) {
-    case QC_STORAGE_F32:
-      product_simple<QC_STORAGE_F32><<<grid, kThreads, 0, s>>>(w, ws, x, xs, y, m, n, k / 32);
-      break;
-    case QC_STORAGE_F16:
-      product_simple<QC_STORAGE_F16><<<grid, kThreads, 0, s>>>(w, ws, x, xs, y, m, n, k / 32);
-      break;
-    default:
-      product_simple<QC_STORAGE_BF16><<<grid, kThreads, 0, s>>>(w, ws, x, xs, y, m, n, k / 32);
   }
   return hipGetLastError();
 }

@@ -1,0 +1,455 @@
+// Products of two MXFP4 matrices on gfx950's block-scaled 4-bit MFMA:
+// y[m][n] = sum_b 2^(ew[n][b] + ex[m][b]) sum_{i in b} w[n][b][i] x[m][b][i].
+//
+// v_mfma_scale_f32_{16x16x128,32x32x64}_f8f6f4 takes, per lane, 32 codes (16 bytes,
+// one block of one row) and that block's scale byte, so the stored bytes are the
+// operands: nothing is decoded.  Products are exact, sums f32.  Which blocks of a row
+// meet in one instruction is free as long as both operands agree.
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "qc_internal.h"
+#include "qc_lds_dma.h"
+#include "qc_storage.h"
+
+namespace qc {
+namespace {
+
+using namespace storage;
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ i32x8 fp4_operand(const i32x4& v) {
+  i32x8 o;
+  o[0] = v[0];
+  o[1] = v[1];
+  o[2] = v[2];
+  o[3] = v[3];
+  return o;
+}
+
+// Four consecutive columns of a row of y, those below n.
+template <int TYPE>
+__device__ __forceinline__ void store4(void* y, long long at, int left, const float* v, bool vec) {
+  if constexpr (TYPE == QC_STORAGE_F32) {
+    float* p = static_cast<float*>(y) + at;
+    if (vec) {
+      *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) p[e] = v[e];
+  } else {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    uint16_t* p = static_cast<uint16_t*>(y) + at;
+    const u32x2 w = {encode2<TYPE>(v[0], v[1]), encode2<TYPE>(v[2], v[3])};
+    if (vec) {
+      *reinterpret_cast<u32x2*>(p) = w;
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) p[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
+// ---- Few rows of x: weights straight from memory ------------------------------
+//
+// A workgroup owns 16 rows of w and MT tiles of 16 rows of x; its four waves take the
+// windows of 16 blocks (256 bytes of a row) in turn and add their sums in LDS.
+// In a window, instruction t multiplies blocks 4 t .. 4 t + 3: lane l holds block
+// 4 t + (l >> 4) of row l & 15, so a load covers 64 bytes of each row.
+constexpr int kDirectWaves = 4;
+
+// The scale bytes of blocks 4 t + g of a window, t = 0..3, in byte 0 of s[t].
+__device__ __forceinline__ void window_scales(const uint8_t* row, int g, int left, uint32_t (&s)[4]) {
+  if (left >= 16) {
+    uint32_t d[4];
+    __builtin_memcpy(d, row, 16);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) s[t] = d[t] >> (8 * g);
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) s[t] = 4 * t + g < left ? row[4 * t + g] : 0;
+  }
+}
+
+template <int MT, int TYPE>
+__global__ __launch_bounds__(64 * kDirectWaves) void mxfp4_direct(
+    const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws, const uint8_t* __restrict__ x,
+    const uint8_t* __restrict__ xs, void* __restrict__ y, int m, int n, int blocks) {
+  __shared__ f32x4 sums[kDirectWaves - 1][MT][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = lane & 15, g = lane >> 4;
+  const int n0 = 16 * blockIdx.x, m0 = 16 * MT * blockIdx.y;
+  const long long wr = min(n0 + row, n - 1);
+  const uint8_t* wp = w + wr * blocks * 16 + 16 * g;
+  const uint8_t* wsp = ws + wr * blocks;
+  const uint8_t* xp[MT];
+  const uint8_t* xsp[MT];
+  bool has[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int r = m0 + 16 * i + row;
+    has[i] = r < m;                              // lanes of rows past m load nothing
+    xp[i] = x + static_cast<long long>(has[i] ? r : 0) * blocks * 16 + 16 * g;
+    xsp[i] = xs + static_cast<long long>(has[i] ? r : 0) * blocks;
+  }
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int b0 = 16 * wave; b0 < blocks; b0 += 16 * kDirectWaves) {
+    const int left = blocks - b0;
+    uint32_t sw[4];
+    window_scales(wsp + b0, g, left, sw);
+    i32x4 a[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      a[t] = i32x4{0, 0, 0, 0};
+      if (4 * t + g < left)
+        a[t] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wp + 16LL * (b0 + 4 * t)));
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      uint32_t sx[4] = {0, 0, 0, 0};
+      i32x4 b[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) b[t] = i32x4{0, 0, 0, 0};
+      if (has[i]) {
+        window_scales(xsp[i] + b0, g, left, sx);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (4 * t + g < left) b[t] = *reinterpret_cast<const i32x4*>(xp[i] + 16LL * (b0 + 4 * t));
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            fp4_operand(a[t]), fp4_operand(b[t]), acc[i], 4, 4, 0, static_cast<int>(sw[t]), 0,
+            static_cast<int>(sx[t]));
+    }
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sums[wave - 1][i][lane] = acc[i];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+  // lane l: row l & 15 of x, rows 4 (l >> 4) .. + 3 of w
+  const int nc = n0 + 4 * g;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+#pragma unroll
+    for (int k = 0; k < kDirectWaves - 1; ++k) acc[i] += sums[k][i][lane];
+    if (!has[i] || nc >= n) continue;
+    const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+    store4<TYPE>(y, static_cast<long long>(m0 + 16 * i + row) * n + nc, n - nc, v,
+                 n % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0);
+  }
+}
+
+// ---- Many rows: both operands through an LDS ring ---------------------------
+//
+// A workgroup of WGN x WGM waves owns TN rows of w and TM rows of x.  A K step is
+// one 128-byte line of codes (8 blocks) of every row and its 8 scale bytes, copied to a
+// stage of an S-deep ring by global_load_lds: codes 8 rows an instruction, 16-byte chunk
+// c of row r at position c ^ ((r >> 1) & 7); scales 32 rows an instruction, lane l
+// the bytes 4 (l >> 5) .. + 3 of row l & 31.  Quarter q of a step multiplies, with
+// v_mfma_scale_f32_32x32x64, chunks q and 4 + q of the rows: lane l holds chunk
+// 4 (l >> 5) + q of row l & 31, whose scale is byte q of the dword that it holds for
+// the whole step.
+__device__ __forceinline__ void ring_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Workgroup b's tile: each XCD (b % 8) takes a contiguous range of an order of bands
+// of kBand tiles of x, so that it reads few panels of either operand.
+constexpr int kXcds = 8, kBand = 4;
+__device__ __forceinline__ void tile_at(int b, int total, int tiles_n, int tiles_m, int& tn, int& tm) {
+  const int q = total / kXcds, r = total % kXcds;
+  const int xcd = b % kXcds, idx = b / kXcds;
+  const int t = xcd * q + min(xcd, r) + idx;
+  const int band = t / (tiles_n * kBand);
+  const int rem = t - band * tiles_n * kBand;
+  const int gm = min(tiles_m - band * kBand, kBand);
+  tn = rem / gm;
+  tm = band * kBand + rem % gm;
+}
+
+template <int TN, int TM, int S, int WGN, int WGM, int TYPE>
+__global__ __launch_bounds__(64 * WGN * WGM, 1) void mxfp4_ring(
+    const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws, const uint8_t* __restrict__ x,
+    const uint8_t* __restrict__ xs, void* __restrict__ y, int m, int n, int blocks,
+    int scale_stride, int tiles_n, int tiles_m) {
+  constexpr int NW = WGN * WGM;
+  constexpr int FN = TN / WGN / 32, FM = TM / WGM / 32;
+  constexpr int R = TN + TM;                        // rows of a stage, w's first
+  constexpr int GC = R / 8 / NW, GS = (R / 32 + NW - 1) / NW;   // loads a wave and step
+  constexpr int G = GC + GS;
+  constexpr int kStage = R * 136;                   // codes, then scales
+  static_assert(R % (8 * NW) == 0 && FN >= 1 && FM >= 1 && S >= 2 && G * (S - 1) < 64, "tile");
+  static_assert(S * kStage <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S * kStage];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tn, tm;
+  tile_at(blockIdx.x, tiles_n * tiles_m, tiles_n, tiles_m, tn, tm);
+  const int n0 = tn * TN, m0 = tm * TM;
+  const int bytes = blocks * 16;                    // of a row's codes
+  const int nk = (blocks + 7) / 8;                  // steps
+
+  // Load j < GC of a wave: rows 8 (wave GC + j) + lane / 8 of the stage, lane writing
+  // position lane % 8.  Rows past the matrix repeat its last one.
+  const uint8_t* cbase[GC];
+  uint32_t cvo[GC];
+  int ccol[GC];
+#pragma unroll
+  for (int j = 0; j < GC; ++j) {
+    const int r8 = 8 * (wave * GC + j);             // uniform
+    const bool is_w = r8 < TN;
+    const int first = is_w ? n0 : m0, limit = is_w ? n : m, base = is_w ? r8 : r8 - TN;
+    cbase[j] = (is_w ? w : x) + static_cast<long long>(first) * bytes;
+    const int r = min(first + base + (lane >> 3), limit - 1) - first;
+    ccol[j] = ((lane & 7) ^ (((r8 >> 1) + (lane >> 4)) & 7)) * 16;
+    cvo[j] = static_cast<uint32_t>(r) * bytes;
+  }
+  const uint8_t* sbase[GS];
+  uint32_t svo[GS];
+#pragma unroll
+  for (int j = 0; j < GS; ++j) {
+    const int r32 = 32 * min(wave * GS + j, R / 32 - 1);
+    const bool is_w = r32 < TN;
+    const int first = is_w ? n0 : m0, limit = is_w ? n : m, base = is_w ? r32 : r32 - TN;
+    sbase[j] = (is_w ? ws : xs) + static_cast<long long>(first) * scale_stride;
+    svo[j] = static_cast<uint32_t>(min(first + base + (lane & 31), limit - 1) - first) * scale_stride;
+  }
+  auto issue = [&](int step, int stage, int from, int to) {
+    uint8_t* base = lds + stage * kStage;
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      if (j < from || j >= to) continue;
+      if (j < GC) {
+        const int col = min(128 * step + ccol[j < GC ? j : 0], bytes - 16);
+        dma16(cbase[j < GC ? j : 0], cvo[j < GC ? j : 0] + col, base + (wave * GC + j) * 1024);
+      } else {
+        const int i = j - GC;
+        const int col = min(8 * step + 4 * (lane >> 5), scale_stride - 4);
+        dma4(sbase[i < GS ? i : 0], svo[i < GS ? i : 0] + col,
+             base + R * 128 + min(wave * GS + i, R / 32 - 1) * 256);
+      }
+    }
+  };
+
+  const int wn = (wave / WGM) * FN * 32, wm = (wave % WGM) * FM * 32;
+  const int key = (lane >> 1) & 7;
+  i32x4 fa[2][FN], fb[2][FM];
+  int sa[2][FN], sb[2][FM];                         // scales of this step and the next
+  auto read_frags = [&](int stage, int q, int slot) {
+    const uint8_t* base = lds + stage * kStage + (lane & 31) * 128 + (((4 * (lane >> 5) + q) ^ key) * 16);
+#pragma unroll
+    for (int i = 0; i < FN; ++i) fa[slot][i] = *reinterpret_cast<const i32x4*>(base + (wn + 32 * i) * 128);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) fb[slot][j] = *reinterpret_cast<const i32x4*>(base + (TN + wm + 32 * j) * 128);
+  };
+  auto read_scales = [&](int stage, int slot) {
+    const uint8_t* base = lds + stage * kStage + R * 128 + 4 * lane;
+#pragma unroll
+    for (int i = 0; i < FN; ++i) sa[slot][i] = *reinterpret_cast<const int*>(base + (wn / 32 + i) * 256);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) sb[slot][j] = *reinterpret_cast<const int*>(base + ((TN + wm) / 32 + j) * 256);
+  };
+  f32x16 acc[FN][FM];
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  auto mfmas = [&](auto quarter, int slot, int ss) {
+    constexpr int Q = decltype(quarter)::value;
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+            fp4_operand(fa[slot][i]), fp4_operand(fb[slot][j]), acc[i][j], 4, 4, Q, sa[ss][i], Q,
+            sb[ss][j]);
+  };
+
+#pragma unroll
+  for (int st = 0; st < S; ++st) issue(min(st, nk - 1), st, 0, G);
+  wait_vmcnt<(S - 1) * G>();
+  ring_barrier();
+  read_scales(0, 0);
+  read_frags(0, 0, 0);
+  int stage = 0;
+  auto step = [&](int k, auto par) {
+    constexpr int P = decltype(par)::value;
+    read_frags(stage, 1, 1);
+    mfmas(std::integral_constant<int, 0>(), 0, P);
+    read_frags(stage, 2, 0);
+    mfmas(std::integral_constant<int, 1>(), 1, P);
+    read_frags(stage, 3, 1);
+    mfmas(std::integral_constant<int, 2>(), 0, P);
+    // step k + 1 is in; every wave has read all of stage
+    wait_vmcnt<(S - 2) * G>();
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));   // lgkmcnt(0)
+    ring_barrier();
+    issue(min(k + S, nk - 1), stage, 0, G);
+    stage = stage + 1 < S ? stage + 1 : 0;
+    read_scales(stage, P ^ 1);
+    read_frags(stage, 0, 0);
+    mfmas(std::integral_constant<int, 3>(), 1, P);
+  };
+  int k = 0;
+  for (; k + 2 < nk; k += 2) {
+    step(k, std::integral_constant<int, 0>());
+    step(k + 1, std::integral_constant<int, 1>());
+  }
+  int ss = 0;
+  if (k + 1 < nk) {
+    step(k, std::integral_constant<int, 0>());
+    ss = 1;
+  }
+  {
+    // the last step: blocks past the row's end count as zeros
+    const int left = blocks - 8 * (nk - 1);
+    int za[FN], zb[FM];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) za[i] = ss ? sa[1][i] : sa[0][i];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) zb[j] = ss ? sb[1][j] : sb[0][j];
+    auto last = [&](auto quarter) {
+      constexpr int Q = decltype(quarter)::value;
+      read_frags(stage, Q, 0);
+      const bool in = 4 * (lane >> 5) + Q < left;
+      const i32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < FN; ++i) {
+        fa[0][i] = in ? fa[0][i] : zero;
+        sa[0][i] = in ? za[i] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        fb[0][j] = in ? fb[0][j] : zero;
+        sb[0][j] = in ? zb[j] : 0;
+      }
+      mfmas(quarter, 0, 0);
+    };
+    last(std::integral_constant<int, 0>());
+    if (left > 1) last(std::integral_constant<int, 1>());
+    if (left > 2) last(std::integral_constant<int, 2>());
+    if (left > 3) last(std::integral_constant<int, 3>());
+  }
+  wait_vmcnt<0>();   // no load may land in LDS that is no longer this workgroup's
+
+  // lane l: row wm + 32 j + (l & 31) of x; register e: row 8 (e >> 2) + 4 (l >> 5) + (e & 3) of w
+  const bool vec = n % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    const int mr = m0 + wm + 32 * j + (lane & 31);
+    if (mr >= m) continue;
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int nc = n0 + wn + 32 * i + 2 * e + 4 * (lane >> 5);
+        if (nc >= n) continue;
+        const float v[4] = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+        store4<TYPE>(y, static_cast<long long>(mr) * n + nc, n - nc, v, vec);
+      }
+  }
+}
+
+// Scale rows at a stride that is a multiple of 4 bytes: the ring's loads are
+// dwords.  Bytes past a row's blocks are zero.
+__global__ __launch_bounds__(256) void pad_scales(const uint8_t* __restrict__ ws, long long n,
+                                                  const uint8_t* __restrict__ xs, long long m,
+                                                  int blocks, int stride, uint32_t* __restrict__ out) {
+  const int words = stride / 4;
+  const long long total = (n + m) * words;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += static_cast<long long>(gridDim.x) * 256) {
+    const long long r = i / words;
+    const int b = 4 * static_cast<int>(i - r * words);
+    const uint8_t* src = r < n ? ws + r * blocks : xs + (r - n) * blocks;
+    uint32_t v = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (b + e < blocks) v |= static_cast<uint32_t>(src[b + e]) << (8 * e);
+    out[i] = v;
+  }
+}
+
+struct Operands {
+  const uint8_t *w, *ws, *x, *xs;
+  void* y;
+  int m, n, blocks;
+};
+
+template <int MT, int TYPE>
+hipError_t run_direct(const Operands& o, hipStream_t s) {
+  const dim3 grid((o.n + 15) / 16, (o.m + 16 * MT - 1) / (16 * MT));
+  mxfp4_direct<MT, TYPE><<<grid, 64 * kDirectWaves, 0, s>>>(o.w, o.ws, o.x, o.xs, o.y, o.m, o.n, o.blocks);
+  return hipGetLastError();
+}
+
+template <int TN, int TM, int S, int WGN, int WGM, int TYPE>
+hipError_t run_ring(const Operands& o, int scale_stride, hipStream_t s) {
+  const int tiles_n = (o.n + TN - 1) / TN, tiles_m = (o.m + TM - 1) / TM;
+  mxfp4_ring<TN, TM, S, WGN, WGM, TYPE><<<static_cast<unsigned>(tiles_n) * tiles_m, 64 * WGN * WGM, 0, s>>>(
+      o.w, o.ws, o.x, o.xs, o.y, o.m, o.n, o.blocks, scale_stride, tiles_n, tiles_m);
+  return hipGetLastError();
+}
+
+template <int TYPE>
+hipError_t run_gemm(Operands o, hipStream_t s) {
+  if (o.m <= 16) return run_direct<1, TYPE>(o, s);
+  if (o.m <= 32) return run_direct<2, TYPE>(o, s);
+  if (o.m <= 64) return run_direct<4, TYPE>(o, s);
+  // the ring addresses a tile's codes with 32 bits
+  if (o.m <= 128 || o.blocks > (1 << 19)) return run_direct<8, TYPE>(o, s);
+  StreamWorkspace* ws = nullptr;
+  std::unique_lock<std::mutex> hold;
+  int stride = o.blocks;
+  if (o.blocks % 4 != 0) {
+    hipError_t e = stream_workspace(s, &ws);
+    if (e != hipSuccess) return e;
+    hold = std::unique_lock<std::mutex>(ws->call);
+    stride = (o.blocks + 3) / 4 * 4;
+    void* buf = nullptr;
+    const long long rows = static_cast<long long>(o.n) + o.m;
+    e = stream_buffer(ws, s, static_cast<size_t>(rows) * stride, 0, &buf);
+    if (e != hipSuccess) return e;
+    const long long words = rows * (stride / 4);
+    const int grid = static_cast<int>(std::min<long long>((words + 255) / 256, 4096));
+    pad_scales<<<grid, 256, 0, s>>>(o.ws, o.n, o.xs, o.m, o.blocks, stride, static_cast<uint32_t*>(buf));
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    o.ws = static_cast<const uint8_t*>(buf);
+    o.xs = o.ws + static_cast<long long>(o.n) * stride;
+  }
+  return run_ring<256, 256, 2, 4, 2, TYPE>(o, stride, s);
+}
+
+}  // namespace
+
+hipError_t launch_mxfp4_gemm(const uint8_t* w, const uint8_t* ws, const uint8_t* x,
+                             const uint8_t* xs, void* y, int type, long long m, long long n,
+                             long long k, hipStream_t s) {
+  const Operands o = {w, ws, x, xs, y, static_cast<int>(m), static_cast<int>(n), static_cast<int>(k / 32)};
+  switch (type) {
+    case QC_STORAGE_F32: return run_gemm<QC_STORAGE_F32>(o, s);
+    case QC_STORAGE_F16: return run_gemm<QC_STORAGE_F16>(o, s);
+    default: return run_gemm<QC_STORAGE_BF16>(o, s);
+  }
+}
+
+}  // namespace qc

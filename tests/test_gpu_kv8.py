@@ -73,7 +73,7 @@ def _append_reference(host, batch, k, v):
                     if not np.all(np.isfinite(r)):
                         continue
                     before = scales[pid, h] if a > 0 else f(0)
-                    scale = max(before, f(np.abs(r).max() / f(127)))
+                    scale = max(before, f(np.abs(r).max() * f(1 / 127)))
                     if scale < f(2.0 ** -126):
                         scale = f(0)
                     inv = f(1) / scale if scale > 0 else f(0)
