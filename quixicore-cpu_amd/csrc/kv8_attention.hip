@@ -6,6 +6,14 @@
 // the keys: running maximum m and sum l of the exponentials, both f32, and the
 // running sum of values, rescaled by exp(m_old - m_new) when m grows.  A row
 // that sees no key is zeros.
+//
+// Codes are exact in f16, so both products run on f16 MFMA with the codes themselves, and
+// the scales of a page stay outside: a page's key scale multiplies its scores, its value
+// scale the probabilities that meet its codes.
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
 #include "qc_kv8.h"
 #include "qc_storage.h"
 
@@ -14,92 +22,577 @@ namespace {
 
 using namespace storage;
 
-constexpr int kThreads = 256;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// One wavefront per query row and head; a lane holds head_dim / 64 elements
-// (rounded up), the wave walks over the keys.
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// The rows of one sequence and key head: row r is token r / group, head
+// kv_head * group + r % group.
+struct Unit {
+  int first, rows, kv;   // the sequence's first token row, new tokens, length
+  __device__ __forceinline__ int position(int token) const { return kv - rows + token; }
+};
+
+struct AttnArgs {
+  const void* q;
+  void* out;
+  long long q_stride, out_stride;
+  int heads, group;
+  float scale;
+  int causal, window;
+  int vec;              // q and out rows allow 16-byte accesses
+  float* part;          // [split][tokens * heads][head_dim], then statistics
+  float* stats;         // [split][tokens * heads][2]: maximum (log2 units), sum
+  int splits, chunk;    // key ranges of `chunk` tokens
+  int row_blocks;
+};
+
+// Keys [lo, hi) that rows of tokens t0..t1 (inclusive) see together.
+__device__ __forceinline__ void seen_range(const AttnArgs& p, const Unit& u, int t0, int t1, int& lo,
+                                           int& hi) {
+  hi = p.causal ? min(u.kv, u.position(t1) + 1) : u.kv;
+  lo = p.window > 0 ? max(0, u.position(t0) + 1 - p.window) : 0;
+}
+
+// Four signed bytes as f16: 0x6400 | u is 1024 + u for a byte u, and u = code + 128.
+__device__ __forceinline__ void bytes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;
+  const f16x2 bias = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+  lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias);
+  hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias);
+}
+
+// Rows r[0..3] of four bytes each -> t[c] = {r[0][c], r[1][c], r[2][c], r[3][c]}.
+__device__ __forceinline__ void transpose4(const uint32_t (&r)[4], uint32_t (&t)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(r[1], r[0], 0x05010400u), b = __builtin_amdgcn_perm(r[1], r[0], 0x07030602u);
+  const uint32_t c = __builtin_amdgcn_perm(r[3], r[2], 0x05010400u), d = __builtin_amdgcn_perm(r[3], r[2], 0x07030602u);
+  t[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+  t[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  t[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+  t[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+// Maximum / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float lanes16_max(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float lanes16_sum(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Power of two that takes a row whose largest magnitude is `top` to [2^14, 2^15):
+// elements down to 2^-28 of it keep their 11 bits in f16.  inverse: its inverse, NaN
+// for a row that is not finite.
+__device__ __forceinline__ float row_scale(float top, float& inverse) {
+  if (!(top <= 3.402823466e38f)) {
+    inverse = __uint_as_float(0x7FC00000u);
+    return 1.0f;
+  }
+  int e = -100;
+  if (top > 0.f) {
+    (void)frexpf(top, &e);
+    e = max(e, -100);
+  }
+  inverse = ldexpf(1.0f, e - 15);
+  return ldexpf(1.0f, 15 - e);
+}
+
+// Elements d, .., d + 7 of a q row (zeros at and past head_dim, a multiple of 16).
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void attention_simple(Kv8Args a, const void* qp,
-                                                             long long q_stride, void* out,
-                                                             long long out_stride, int heads,
-                                                             float scale, int causal, int window) {
+__device__ __forceinline__ void load8(const void* q, long long at, bool in, bool vec, float* v) {
   typedef typename Storage<TYPE>::raw raw;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  if (!in) return;
+  const raw* p = static_cast<const raw*>(q) + at;
+  if (vec) {
+    decode16<TYPE>(*reinterpret_cast<const u32x4*>(p), v);
+    if constexpr (TYPE == QC_STORAGE_F32) decode16<TYPE>(*reinterpret_cast<const u32x4*>(p + 4), v + 4);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = decode<TYPE>(p[j]);
+  }
+}
+
+// N consecutive elements of an out row.
+template <int TYPE, int N>
+__device__ __forceinline__ void store_n(void* out, long long at, bool vec, const float* v) {
+  typedef typename Storage<TYPE>::raw raw;
+  raw* p = static_cast<raw*>(out) + at;
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) p[j] = encode<TYPE>(v[j]);
+  } else if constexpr (TYPE == QC_STORAGE_F32) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) *reinterpret_cast<u32x4*>(p + j) = encode16<TYPE>(v + j);
+  } else if constexpr (N == 4) {
+    *reinterpret_cast<u32x2*>(p) = u32x2{encode2<TYPE>(v[0], v[1]), encode2<TYPE>(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 8) *reinterpret_cast<u32x4*>(p + j) = encode16<TYPE>(v + j);
+  }
+}
+
+// ---- Few rows a key head: the cache straight from memory -----------------------
+//
+// Workgroup = a range of keys, RT tiles of 16 rows of a key head, a sequence.  Its
+// waves take the range's steps of 32 keys in turn, each with statistics and sums of its
+// own, and join at the end through LDS; several ranges join in a second launch.
+//
+// S^T = K Q^T and O^T = V^T P^T with v_mfma_f32_16x16x32_f16, so that a lane's scores
+// and sums belong to one row (lane & 15): with g = lane >> 4, register e of key tile t is
+// key 16 t + 4 g + e, and the products' K order is free, so the lane's own eight
+// probabilities are its operand of the second product.  K: lane loads 16 bytes of key
+// lane & 15 at dimension 64 c + 16 g.  V: lane loads DP / 16 bytes of its eight
+// keys at dimension (DP / 16) (lane & 15), transposed in registers.
+constexpr int kWaves = 4;
+constexpr int kMaxGroups = 512;   // 16-token groups of a range
+
+template <int DP, int RT, int TYPE>
+__global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnArgs p) {
+  constexpr int KC = DP / 64;                     // 16-byte chunks of a key a lane holds
+  constexpr int KS = DP / 32;                     // MFMAs of 32 dimensions
+  constexpr int VB = DP / 16;                     // bytes of a value a lane holds
+  constexpr int VW = VB / 4;
+  constexpr int NQ = TYPE == QC_STORAGE_F32 ? 2 : 1;   // f16 terms of q and of the probabilities
+  __shared__ int s_page[kMaxGroups];
+  __shared__ float s_ks[kMaxGroups], s_vs[kMaxGroups];
+  __shared__ float s_red[kWaves], s_m[kWaves][RT * 16], s_l[kWaves][RT * 16];
+  __shared__ f32x4 s_o[kWaves / 2][RT][VB][64];
+
+  const int lane = threadIdx.x & 63, row16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // split fastest, then row block, key head, sequence
+  long long id = blockIdx.x;
+  const int split = static_cast<int>(id % p.splits);
+  id /= p.splits;
+  const int rb = static_cast<int>(id % p.row_blocks);
+  id /= p.row_blocks;
+  const int kvh = static_cast<int>(id % a.kv_heads), seq = static_cast<int>(id / a.kv_heads);
+  Unit u;
+  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return;
+  const int r0 = rb * RT * 16, r1 = min(r0 + RT * 16, u.rows * p.group);
+  if (r0 >= r1) return;
+  int lo, hi;
+  seen_range(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
+  const int base = lo & ~31;
+  const int from = base + split * p.chunk, to = min(hi, from + p.chunk);   // from: multiple of 32
+
+  // page ids and scales of the range's groups of 16 keys, and the largest value scale
+  const int groups = max(0, (to - from + 15) >> 4);
+  float unit = 0.f;
+  for (int i = threadIdx.x; i < groups; i += 64 * kWaves) {
+    const int tok = from + 16 * i;
+    int page = tok + 15 < lo ? -1 : a.table[static_cast<long long>(seq) * a.columns + (tok >> a.page_shift)];
+    float ks = 0.f, vs = 0.f;
+    if (static_cast<unsigned>(page) < static_cast<unsigned>(a.pages)) {
+      const long long at = static_cast<long long>(page) * a.kv_heads + kvh;
+      ks = a.k_scales[at];
+      vs = a.v_scales[at];
+    } else {
+      if (tok + 15 >= lo) *a.status = QC_INVALID_ARGUMENT;
+      page = -1;
+    }
+    s_page[i] = page;
+    s_ks[i] = ks;
+    s_vs[i] = vs;
+    unit = fmaxf(unit, vs);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor(unit, o));
+  if (lane == 0) s_red[wave] = unit;
+
+  // q's fragments: row row16 of tile t, dimensions 64 c + 16 g + 8 h + j
+  f16x8 qf[RT][KS][NQ];
+  float factor[RT];                               // score's scale in log2 units, over q's
+  int row_lo[RT], row_hi[RT];                     // keys the lane's row sees
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = r0 + 16 * t + row16;
+    const bool has = r < r1;
+    const int token = (has ? r : r0) / p.group, head = kvh * p.group + (has ? r : r0) - token * p.group;
+    const long long at = (u.first + token) * p.q_stride + static_cast<long long>(head) * a.head_dim;
+    float v[KS][8], top = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+      load8<TYPE>(p.q, at + d, has && d < a.head_dim, p.vec, v[s]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        top = fmaxf(top, fabsf(v[s][j]));
+        nan = nan || v[s][j] != v[s][j];
+      }
+    }
+    if (nan) top = INFINITY;
+    top = lanes16_max(top);
+    float inverse;
+    const float up = row_scale(top, inverse);
+    factor[t] = p.scale * kLog2e * inverse;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = v[s][j] * up;
+        qf[t][s][0][j] = static_cast<_Float16>(x);
+        if constexpr (NQ == 2) qf[t][s][1][j] = static_cast<_Float16>(x - static_cast<float>(qf[t][s][0][j]));
+      }
+    row_hi[t] = has ? (p.causal ? min(u.kv, u.position(token) + 1) : u.kv) : 0;
+    row_lo[t] = p.window > 0 ? u.position(token) + 1 - p.window : 0;
+  }
+  __syncthreads();
+  unit = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  // probabilities enter the second product as p * (value scale / unit) * 2^15
+  const float per_unit = unit > 0.f ? 32768.0f / unit : 0.f;
+
+  float m[RT], l[RT];
+  f32x4 acc[RT][VB];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int k = 0; k < VB; ++k) acc[t][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  struct Raw {
+    u32x4 k[2][KC];
+    uint32_t v[8][VW];
+  };
+  const long long page_bytes = static_cast<long long>(a.kv_heads) * a.page_tokens * a.head_dim;
+  const long long head_bytes = static_cast<long long>(kvh) * a.page_tokens * a.head_dim;
+  auto load = [&](int tok, Raw& r) {              // 32 keys from tok
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int i = (tok - from) / 16 + t;
+      const int page = i < groups ? __builtin_amdgcn_readfirstlane(s_page[i < groups ? i : 0]) : -1;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) r.k[t][c] = u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) r.v[4 * t + e][w] = 0;
+      if (page < 0) continue;
+      const int slot = (tok + 16 * t) & (a.page_tokens - 1);
+      const long long at = page * page_bytes + head_bytes + static_cast<long long>(slot) * a.head_dim;
+      const int8_t* kp = a.k_codes + at + row16 * a.head_dim + 16 * g;
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+        if (64 * c + 16 * g < a.head_dim) r.k[t][c] = *reinterpret_cast<const u32x4*>(kp + 64 * c);
+      const int8_t* vp = a.v_codes + at + 4 * g * a.head_dim + VB * row16;
+      if (VB * row16 < a.head_dim) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int8_t* q = vp + e * a.head_dim;
+          if constexpr (VW == 1) {
+            r.v[4 * t + e][0] = *reinterpret_cast<const uint32_t*>(q);
+          } else if constexpr (VW == 2) {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(q);
+            r.v[4 * t + e][0] = x[0];
+            r.v[4 * t + e][1] = x[1];
+          } else {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(q);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) r.v[4 * t + e][w] = x[w];
+          }
+        }
+      }
+    }
+  };
+  auto compute = [&](int tok, const Raw& r) {
+    f32x4 s[RT][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t w[4];
+        bytes_to_f16(r.k[t][ks >> 1][2 * (ks & 1)], w[0], w[1]);
+        bytes_to_f16(r.k[t][ks >> 1][2 * (ks & 1) + 1], w[2], w[3]);
+        const f16x8 kf = __builtin_bit_cast(f16x8, u32x4{w[0], w[1], w[2], w[3]});
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+            s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][ks][q], s[rt][t], 0, 0, 0);
+      }
+    }
+    const int i = (tok - from) / 16;
+    const int i1 = min(i + 1, groups - 1);
+    const float ks[2] = {s_ks[i], s_ks[i1]};
+    const float vr[2] = {s_vs[i] * per_unit, s_vs[i1] * per_unit};
+    const bool page_ok[2] = {s_page[i] >= 0, s_page[i1] >= 0};
+    f16x8 pf[RT][NQ];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float z[8], top = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = tok + 16 * t + 4 * g + e;
+          const bool see = j >= row_lo[rt] && j < row_hi[rt] && page_ok[t];
+          z[4 * t + e] = see ? s[rt][t][e] * (ks[t] * factor[rt]) : -INFINITY;
+          top = fmaxf(top, z[4 * t + e]);
+        }
+      top = lanes16_max(top);
+      const float mn = fmaxf(m[rt], top);
+      const float ref = mn == -INFINITY ? 0.f : mn;   // nothing seen yet: all terms are 0
+      if (__any(mn != m[rt])) {
+        const float alpha = exp2f(m[rt] - ref);
+        l[rt] *= alpha;
+#pragma unroll
+        for (int k = 0; k < VB; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[rt][k][e] *= alpha;
+        m[rt] = mn;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float pe = exp2f(z[e] - ref);
+        l[rt] += pe;
+        const float pv = pe * vr[e >> 2];
+        pf[rt][0][e] = static_cast<_Float16>(pv);
+        if constexpr (NQ == 2) pf[rt][1][e] = static_cast<_Float16>(pv - static_cast<float>(pf[rt][0][e]));
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      uint32_t x[2][4], y[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[t][e] = r.v[4 * t + e][w];
+        transpose4(x[t], y[t]);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t f[4];
+        bytes_to_f16(y[0][c], f[0], f[1]);
+        bytes_to_f16(y[1][c], f[2], f[3]);
+        const f16x8 vf = __builtin_bit_cast(f16x8, u32x4{f[0], f[1], f[2], f[3]});
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+            acc[rt][4 * w + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][q], acc[rt][4 * w + c], 0, 0, 0);
+      }
+    }
+  };
+  {
+    const int stride = 32 * kWaves;
+    int tok = from + 32 * wave;
+    if (tok < to) {
+      Raw cur;
+      load(tok, cur);
+      for (; tok + stride < to; tok += stride) {
+        Raw next;
+        load(tok + stride, next);
+        compute(tok, cur);
+        cur = next;
+      }
+      compute(tok, cur);
+    }
+  }
+
+  // join the waves: the common maximum, then the sums pairwise in a fixed order
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    l[t] = lanes16_sum(l[t]);
+    if (g == 0) {
+      s_m[wave][16 * t + row16] = m[t];
+      s_l[wave][16 * t + row16] = l[t];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    float all = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all = fmaxf(all, s_m[w][16 * t + row16]);
+    const float ref = all == -INFINITY ? 0.f : all;
+    const float mine = exp2f(m[t] - ref);
+#pragma unroll
+    for (int k = 0; k < VB; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][k][e] *= mine;
+    l[t] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) l[t] += s_l[w][16 * t + row16] * exp2f(s_m[w][16 * t + row16] - ref);
+    m[t] = all;
+  }
+#pragma unroll
+  for (int half = kWaves / 2; half > 0; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int k = 0; k < VB; ++k) s_o[wave - half][t][k][lane] = acc[t][k];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int k = 0; k < VB; ++k) acc[t][k] += s_o[wave][t][k][lane];
+    }
+    __syncthreads();
+  }
+  if (wave > 0) return;
+  const float back = unit * (1.0f / 32768.0f);
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = r0 + 16 * t + row16;
+    if (r >= r1) continue;
+    const int token = r / p.group, head = kvh * p.group + r - token * p.group;
+    const bool last = p.splits == 1;
+    const float f = last ? (l[t] == 0.f ? 0.f : back / l[t]) : back;
+    const long long row = static_cast<long long>(u.first + token) * p.heads + head;
+    const long long part = (static_cast<long long>(split) * a.tokens * p.heads + row) * a.head_dim;
+    if (!last && g == 0) {
+      float* st = p.stats + 2 * (static_cast<long long>(split) * a.tokens * p.heads + row);
+      st[0] = m[t];
+      st[1] = l[t];
+    }
+    if (!last && l[t] == 0.f) continue;           // saw no key: the join takes nothing of it
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = VB * (4 * g + e);
+      if (d >= a.head_dim) continue;
+      float v[VB];
+#pragma unroll
+      for (int k = 0; k < VB; ++k) v[k] = acc[t][k][e] * f;
+      if (last)
+        store_n<TYPE, VB>(p.out, (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim + d,
+                          p.vec, v);
+      else
+        store_n<QC_STORAGE_F32, VB>(p.part, part + d, true, v);
+    }
+  }
+}
+
+// out = sum over the ranges of 2^(m_s - m) O_s over that of 2^(m_s - m) l_s: a
+// wavefront a row.
+template <int TYPE>
+__global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p) {
   const int lane = threadIdx.x & 63;
-  const int s = blockIdx.y;
-  int first, rows, kv;
-  if (!kv8_sequence(a, s, first, rows, kv)) return;
-  const long long item = static_cast<long long>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
-  const int i = static_cast<int>(item / heads), h = static_cast<int>(item % heads);
-  if (i >= rows) return;
-  const int kvh = h / (heads / a.kv_heads);
-  const int pos = kv - rows + i;
-  const int hi = causal ? min(kv, pos + 1) : kv;
-  const int lo = window > 0 ? max(0, pos + 1 - window) : 0;
-  const raw* q = static_cast<const raw*>(qp) + (first + i) * q_stride + static_cast<long long>(h) * a.head_dim;
-  float qv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int d = lane + 64 * e;
-    qv[e] = d < a.head_dim ? decode<TYPE>(q[d]) : 0.f;
-  }
+  const long long item = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const long long per_seq = static_cast<long long>(a.max_new) * p.heads;
+  const int seq = static_cast<int>(item / per_seq);
+  if (seq >= a.seqs) return;
+  const int rest = static_cast<int>(item - seq * per_seq);
+  const int token = rest / p.heads, head = rest - token * p.heads;
+  Unit u;
+  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv) || token >= u.rows) return;
+  const long long rows = static_cast<long long>(a.tokens) * p.heads;
+  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
   float m = -INFINITY, l = 0.f;
-  for (int j = lo; j < hi; ++j) {
-    const int page = a.table[static_cast<long long>(s) * a.columns + (j >> a.page_shift)];
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) {
-      *a.status = QC_INVALID_ARGUMENT;
-      continue;
-    }
-    const long long unit = static_cast<long long>(page) * a.kv_heads + kvh;
-    const long long at = (unit * a.page_tokens + (j & (a.page_tokens - 1))) * a.head_dim;
-    float dot = 0.f;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.stats[2 * (s * rows + row)]);
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int s = 0; s < p.splits; ++s) {
+    const float ms = p.stats[2 * (s * rows + row)], ls = p.stats[2 * (s * rows + row) + 1];
+    if (ms == -INFINITY && ls == 0.f) continue;   // saw no key (a row that is not finite has a sum of NaN)
+    const float f = exp2f(ms - ref);
+    l += f * ls;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = lane + 64 * e;
-      if (d < a.head_dim) dot = fmaf(qv[e], static_cast<float>(a.k_codes[at + d]), dot);
+      if (d < a.head_dim) v[e] += f * p.part[(s * rows + row) * a.head_dim + d];
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o);
-    const float z = dot * (a.k_scales[unit] * scale);
-    const float mn = fmaxf(m, z);
-    const float alpha = expf(m - mn), p = expf(z - mn);
-    l = l * alpha + p;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = lane + 64 * e;
-      const float v = d < a.head_dim ? static_cast<float>(a.v_codes[at + d]) * a.v_scales[unit] : 0.f;
-      acc[e] = fmaf(p, v, acc[e] * alpha);
-    }
-    m = mn;
   }
-  raw* y = static_cast<raw*>(out) + (first + i) * out_stride + static_cast<long long>(h) * a.head_dim;
+  typedef typename Storage<TYPE>::raw raw;
+  raw* out = static_cast<raw*>(p.out) + (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int d = lane + 64 * e;
-    if (d < a.head_dim) y[d] = encode<TYPE>(l == 0.f ? 0.f : acc[e] / l);
+    if (d < a.head_dim) out[d] = encode<TYPE>(l == 0.f ? 0.f : v[e] / l);
   }
+}
+
+template <int DP, int RT, int TYPE>
+hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
+  const long long rows = static_cast<long long>(a.max_new) * p.group;
+  p.row_blocks = static_cast<int>((rows + RT * 16 - 1) / (RT * 16));
+  // keys a block of rows can see, from a multiple of 32 on
+  long long span = a.max_kv;
+  if (p.window > 0) span = std::min<long long>(span, p.window + (RT * 16 + p.group - 1) / p.group + 32);
+  const long long units = static_cast<long long>(a.seqs) * a.kv_heads * p.row_blocks;
+  const long long want = std::max<long long>(1, 4LL * device_cu_count() / units);
+  long long chunk = (span + want - 1) / want;
+  chunk = std::max<long long>(32 * kWaves, (chunk + 31) / 32 * 32);
+  chunk = std::min<long long>(chunk, 16 * kMaxGroups);
+  p.chunk = static_cast<int>(chunk);
+  p.splits = static_cast<int>((span + chunk - 1) / chunk);
+  const long long grid = units * p.splits;
+  if (grid > INT_MAX) return hipErrorInvalidValue;
+  std::unique_lock<std::mutex> hold;
+  if (p.splits > 1) {
+    StreamWorkspace* ws = nullptr;
+    hipError_t e = stream_workspace(s, &ws);
+    if (e != hipSuccess) return e;
+    hold = std::unique_lock<std::mutex>(ws->call);
+    const size_t outs = static_cast<size_t>(p.splits) * a.tokens * p.heads;
+    void* buf = nullptr;
+    e = stream_buffer(ws, s, outs * (a.head_dim + 2) * sizeof(float), 0, &buf);
+    if (e != hipSuccess) return e;
+    p.part = static_cast<float*>(buf);
+    p.stats = p.part + outs * a.head_dim;
+  }
+  attention_direct<DP, RT, TYPE><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a, p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return e;
+  const long long items = static_cast<long long>(a.seqs) * a.max_new * p.heads;
+  attention_join<TYPE><<<static_cast<unsigned>((items + 3) / 4), 256, 0, s>>>(a, p);
+  return hipGetLastError();
+}
+
+template <int DP, int TYPE>
+hipError_t run_rows(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
+  const long long rows = static_cast<long long>(a.max_new) * p.group;
+  if (rows <= 16 || (DP == 256 && TYPE == QC_STORAGE_F32)) return run_direct<DP, 1, TYPE>(a, p, s);
+  if constexpr (DP < 256 || TYPE != QC_STORAGE_F32) return run_direct<DP, 2, TYPE>(a, p, s);
+  return hipErrorInvalidValue;
+}
+
+template <int TYPE>
+hipError_t run_typed(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
+  if (a.head_dim <= 64) return run_rows<64, TYPE>(a, p, s);
+  if (a.head_dim <= 128) return run_rows<128, TYPE>(a, p, s);
+  return run_rows<256, TYPE>(a, p, s);
 }
 
 }  // namespace
 
 hipError_t launch_kv8_attention(const Kv8Attention& r, int* status, hipStream_t s) {
   const Kv8Args a = kv8_args(*r.cache, *r.batch, status);
-  const long long items = static_cast<long long>(a.max_new) * r.heads;
-  const dim3 grid(static_cast<unsigned>((items + kThreads / 64 - 1) / (kThreads / 64)), a.seqs);
-  const int heads = static_cast<int>(r.heads), window = static_cast<int>(r.window);
+  AttnArgs p = {};
+  p.q = r.q;
+  p.out = r.out;
+  p.q_stride = r.q_stride;
+  p.out_stride = r.out_stride;
+  p.heads = static_cast<int>(r.heads);
+  p.group = p.heads / a.kv_heads;
+  p.scale = r.scale;
+  p.causal = r.causal;
+  p.window = static_cast<int>(r.window);
+  const int size = r.type == QC_STORAGE_F32 ? 4 : 2;
+  p.vec = ((reinterpret_cast<uintptr_t>(r.q) | reinterpret_cast<uintptr_t>(r.out) |
+            static_cast<uintptr_t>(r.q_stride * size) | static_cast<uintptr_t>(r.out_stride * size)) & 15) == 0;
   switch (r.type) {
-    case QC_STORAGE_F32:
-      attention_simple<QC_STORAGE_F32><<<grid, kThreads, 0, s>>>(a, r.q, r.q_stride, r.out, r.out_stride,
-                                                                 heads, r.scale, r.causal, window);
-      break;
-    case QC_STORAGE_F16:
-      attention_simple<QC_STORAGE_F16><<<grid, kThreads, 0, s>>>(a, r.q, r.q_stride, r.out, r.out_stride,
-                                                                 heads, r.scale, r.causal, window);
-      break;
-    default:
-      attention_simple<QC_STORAGE_BF16><<<grid, kThreads, 0, s>>>(a, r.q, r.q_stride, r.out, r.out_stride,
-                                                                  heads, r.scale, r.causal, window);
+    case QC_STORAGE_F32: return run_typed<QC_STORAGE_F32>(a, p, s);
+    case QC_STORAGE_F16: return run_typed<QC_STORAGE_F16>(a, p, s);
+    default: return run_typed<QC_STORAGE_BF16>(a, p, s);
   }
-  return hipGetLastError();
 }
 
 }  // namespace qc
