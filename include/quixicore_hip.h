@@ -425,8 +425,8 @@ typedef struct qc_kv8_batch {
  * nearest 1 / 127, or 0 below 2^-126; codes held
  * become rint(code * (s / s')), new ones clamp(rint(x * (1 / s')), +-127), each
  * step rounded to f32.  A page written by a call must belong to one sequence.
- * A page and head with a non-finite new value, and a sequence of more new tokens than
- * kv_len, are errors and left as they were.  Status: 1 for sizes out of range, 2 for an
+ * A page and head with a non-finite new value or scale held, and a sequence of more
+ * new tokens than kv_len, are errors and left as they were.  Status: 1 for sizes out of range, 2 for an
  * unknown type, 3 for NULL or misaligned pointers. */
 int qc_hip_kv8_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* k,
                       long long k_stride, const void* v, long long v_stride, int type,
@@ -445,7 +445,8 @@ int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void
  * kv_heads, query heads h * heads / kv_heads .. sharing key head h.  Token i of n
  * stands at p = kv_len - n + i and sees the positions j < kv_len; with causal != 0
  * j <= p, and with window > 0 (causal only) j > p - window.  A row that sees nothing
- * (n > kv_len, or kv_len 0) is zeros.  Pages that no row sees are not looked at.
+ * (n > kv_len, or kv_len 0) is zeros.  Pages that no row sees are not looked at; one
+ * that is seen and has a scale that is not finite is an error like a bad page id.
  * 16-bit q: the probabilities enter the product with the values in 11 bits, f32 q: in
  * 22; sums and statistics are f32.  Status: 1 for sizes out of range, 2 for an
  * unknown type, 3 for NULL or misaligned pointers, a scale that is not finite, or a

@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "qc_kv8.h"
+#include "qc_lds_dma.h"
 #include "qc_storage.h"
 
 namespace qc {
@@ -24,6 +25,7 @@ using namespace storage;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -193,18 +195,22 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
     const int tok = from + 16 * i;
     int page = tok + 15 < lo ? -1 : a.table[static_cast<long long>(seq) * a.columns + (tok >> a.page_shift)];
     float ks = 0.f, vs = 0.f;
+    bool ok = false;
     if (static_cast<unsigned>(page) < static_cast<unsigned>(a.pages)) {
       const long long at = static_cast<long long>(page) * a.kv_heads + kvh;
       ks = a.k_scales[at];
       vs = a.v_scales[at];
-    } else {
+      ok = isfinite(ks) && isfinite(vs);
+    }
+    if (!ok) {
       if (tok + 15 >= lo) *a.status = QC_INVALID_ARGUMENT;
       page = -1;
+      ks = vs = 0.f;
     }
     s_page[i] = page;
     s_ks[i] = ks;
     s_vs[i] = vs;
-    unit = fmaxf(unit, vs);
+    unit = fmaxf(unit, fabsf(vs));
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor(unit, o));
@@ -480,6 +486,347 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
   }
 }
 
+// ---- Many rows a key head: both operands through LDS ---------------------------
+//
+// With hundreds of rows a key head each key is used that often, so a first launch
+// lays the codes out as f16 operands, exactly, once: per sequence and key head, for every 32
+// keys the fragments of v_mfma_f32_32x32x16_f16, 1 KB each, in the order they
+// are read.  K fragment s (16 dimensions): lane l key l & 31, dimensions 16 s + 8 (l >> 5)
+// + j.  V fragment (t, k) (32 dimensions, 16 keys): lane l dimension 32 t + (l & 31), keys
+// 16 k + 8 (j >> 2) + 4 (l >> 5) + (j & 3) -- the keys whose scores lane l of S^T = K Q^T
+// holds in registers 8 k + j, so its probabilities are its operand of O^T = V^T P^T.
+// Beside them the magnitudes of the key and value scales of each 16 keys (a negative scale
+// turns its codes' signs); a key scale of -1 marks a group without a page.
+struct Frags {
+  _Float16* k;           // [units][cap / 32][DP / 16][512]
+  _Float16* v;           // [units][cap / 32][DP / 32][2][512]
+  float* ks;             // [units][cap / 16]
+  float* vs;
+  int cap;               // keys laid out per unit: a multiple of 64
+  int unit0;             // the pass's first unit (sequence * kv_heads + key head)
+};
+
+template <int DP>
+__global__ __launch_bounds__(256) void attention_layout(Kv8Args a, Frags f, int tiles, int window) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x % tiles, local = blockIdx.x / tiles;
+  const int unit = f.unit0 + local;
+  const int seq = unit / a.kv_heads, kvh = unit - seq * a.kv_heads;
+  int first, rows, kv;
+  if (!kv8_sequence(a, seq, first, rows, kv) || rows == 0) return;
+  const int lo = window > 0 ? max(0, kv - rows + 1 - window) & ~63 : 0;
+  const int tok = 32 * tile;
+  if (tok < lo || tok >= ((kv + 63) & ~63)) return;
+  const int8_t *kp[2], *vp[2];                    // codes of the tile's two groups of 16 keys
+  bool k_neg[2], v_neg[2], v_zero[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = tok + 16 * i;
+    kp[i] = vp[i] = nullptr;
+    k_neg[i] = v_neg[i] = v_zero[i] = false;
+    float ks = -1.f, vs = 0.f;
+    if (t < kv && (window <= 0 || t + 15 >= kv - rows + 1 - window)) {   // some row sees one of them
+      const int page = a.table[static_cast<long long>(seq) * a.columns + (t >> a.page_shift)];
+      bool ok = false;
+      if (static_cast<unsigned>(page) < static_cast<unsigned>(a.pages)) {
+        const long long at = static_cast<long long>(page) * a.kv_heads + kvh;
+        const float sk = a.k_scales[at], sv = a.v_scales[at];
+        ok = isfinite(sk) && isfinite(sv);
+        if (ok) {
+          const long long off = (at * a.page_tokens + (t & (a.page_tokens - 1))) * a.head_dim;
+          kp[i] = a.k_codes + off;
+          vp[i] = a.v_codes + off;
+          k_neg[i] = sk < 0.f;
+          v_neg[i] = sv < 0.f;
+          v_zero[i] = sv == 0.f;
+          ks = fabsf(sk);
+          vs = fabsf(sv);
+        }
+      }
+      if (!ok && threadIdx.x == 0) *a.status = QC_INVALID_ARGUMENT;
+    }
+    if (threadIdx.x == 0) {
+      const long long at = static_cast<long long>(local) * (f.cap / 16) + t / 16;
+      f.ks[at] = ks;
+      f.vs[at] = vs;
+    }
+  }
+  const long long at32 = static_cast<long long>(local) * (f.cap / 32) + tile;
+  constexpr int NF = DP / 16;                     // fragments of either kind
+  for (int s = wave; s < NF; s += 4) {            // K
+    const int key = lane & 31, d = 16 * s + 8 * (lane >> 5), i = key >> 4;
+    u32x4 o = {0, 0, 0, 0};
+    if (kp[i] != nullptr && d < a.head_dim) {
+      const u32x2 b = *reinterpret_cast<const u32x2*>(kp[i] + (key & 15) * a.head_dim + d);
+      uint32_t w[4];
+      bytes_to_f16(b[0], w[0], w[1]);
+      bytes_to_f16(b[1], w[2], w[3]);
+      const uint32_t sign = k_neg[i] ? 0x80008000u : 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = w[e] ^ sign;
+    }
+    *reinterpret_cast<u32x4*>(f.k + (at32 * NF + s) * 512 + 8 * lane) = o;
+  }
+  for (int s = wave; s < NF; s += 4) {            // V: fragment (t, k) = (s / 2, s % 2)
+    const int i = s & 1, d = 32 * (s >> 1) + (lane & 31);
+    f16x8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = static_cast<_Float16>(0.f);
+    if (vp[i] != nullptr && !v_zero[i] && d < a.head_dim) {
+      const int8_t* p = vp[i] + 4 * (lane >> 5) * a.head_dim + d;
+      const int sign = v_neg[i] ? -1 : 1;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        o[j] = static_cast<_Float16>(sign * p[(8 * (j >> 2) + (j & 3)) * a.head_dim]);
+    }
+    *reinterpret_cast<u32x4*>(f.v + (at32 * NF + s) * 512 + 8 * lane) = __builtin_bit_cast(u32x4, o);
+  }
+}
+
+// Workgroup: NW waves of 32 rows of a key head, a range of keys.  A step is 64 keys,
+// its fragments copied to one of two LDS buffers while the other is used.  A score's
+// exponent is one fused multiply-add: with c the key scale times the row's factor and b =
+// log2(value scale / largest one) + 15 per 16 keys, p' = 2^(s c + b - m) is the
+// probability as it meets the codes of V, and the sum takes p' 2^-b.
+template <int DP, int NW, int TYPE>
+__global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, AttnArgs p, Frags f) {
+  constexpr int NF = DP / 16, DT = DP / 32;
+  constexpr int NQ = TYPE == QC_STORAGE_F32 ? 2 : 1;
+  constexpr int kFragBytes = 2 * NF * 1024;       // 64 keys of K, or of V
+  constexpr int kStage = 2 * kFragBytes;
+  constexpr int LOADS = kStage / 1024 / NW;       // a wave's loads of 1 KB a step
+  static_assert(kStage % (1024 * NW) == 0, "whole loads");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+  __shared__ float s_unit[NW];
+
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // unit fastest: with workgroups dealt to the XCDs in turn, a head's blocks share an L2; the
+  // longest rows (last blocks) first
+  int id = blockIdx.x;
+  const int units = gridDim.x / (p.splits * p.row_blocks);
+  const int local = id % units;
+  id /= units;
+  const int split = id % p.splits;
+  const int rb = p.row_blocks - 1 - id / p.splits;
+  const int unit_id = f.unit0 + local;
+  const int seq = unit_id / a.kv_heads, kvh = unit_id - seq * a.kv_heads;
+  Unit u;
+  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return;
+  const int r0 = rb * NW * 32, r1 = min(r0 + NW * 32, u.rows * p.group);
+  if (r0 >= r1) return;
+  int lo, hi;
+  seen_range(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
+  const int from = (lo & ~63) + split * p.chunk, to = min(hi, from + p.chunk);
+  const int steps = to > from ? (to - from + 63) >> 6 : 0;
+
+  const _Float16* kf = f.k + (static_cast<long long>(local) * (f.cap / 32) + from / 32) * NF * 512;
+  const _Float16* vf = f.v + (static_cast<long long>(local) * (f.cap / 32) + from / 32) * NF * 512;
+  const float* ks = f.ks + static_cast<long long>(local) * (f.cap / 16) + from / 16;
+  const float* vs = f.vs + static_cast<long long>(local) * (f.cap / 16) + from / 16;
+  auto issue = [&](int step, int buf) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int q = wave * LOADS + i;             // uniform
+      const _Float16* src = q < 2 * NF ? kf + (static_cast<long long>(step) * 2 * NF + q) * 512
+                                       : vf + (static_cast<long long>(step) * 2 * NF + q - 2 * NF) * 512;
+      dma16(src, 16 * lane, lds + buf * kStage + q * 1024);
+    }
+  };
+  if (steps > 0) issue(0, 0);
+
+  // the range's largest value scale
+  float unit = 0.f;
+  for (int i = threadIdx.x; i < 4 * steps; i += 64 * NW) unit = fmaxf(unit, vs[i]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor(unit, o));
+  if (lane == 0) s_unit[wave] = unit;
+
+  // q: row lane & 31, dimensions 16 s + 8 half + j
+  f16x8 qf[NF][NQ];
+  const int r = r0 + 32 * wave + (lane & 31);
+  const bool has = r < r1;
+  const int token = (has ? r : r0) / p.group, head = kvh * p.group + (has ? r : r0) - token * p.group;
+  const int row_hi = has ? (p.causal ? min(u.kv, u.position(token) + 1) : u.kv) : 0;
+  const int row_lo = p.window > 0 ? u.position(token) + 1 - p.window : 0;
+  float factor, broken = 0.f;                     // broken: NaN for a row that is not finite
+  {
+    const long long at = (u.first + token) * p.q_stride + static_cast<long long>(head) * a.head_dim;
+    float v[NF][8], top = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int s = 0; s < NF; ++s) {
+      const int d = 16 * s + 8 * half;
+      load8<TYPE>(p.q, at + d, has && d < a.head_dim, p.vec, v[s]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        top = fmaxf(top, fabsf(v[s][j]));
+        nan = nan || v[s][j] != v[s][j];
+      }
+    }
+    if (nan) top = INFINITY;
+    top = fmaxf(top, __shfl_xor(top, 32));
+    float inverse;
+    float up = row_scale(top, inverse);
+    if (inverse != inverse) {
+      broken = inverse;
+      inverse = 1.f;
+      up = 0.f;
+    }
+    factor = fabsf(p.scale) * kLog2e * inverse;
+    if (p.scale < 0.f) up = -up;
+#pragma unroll
+    for (int s = 0; s < NF; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = broken != broken ? 0.f : v[s][j] * up;
+        qf[s][0][j] = static_cast<_Float16>(x);
+        if constexpr (NQ == 2) qf[s][1][j] = static_cast<_Float16>(x - static_cast<float>(qf[s][0][j]));
+      }
+  }
+  // keys every row of the wave sees, and any of them
+  int all_hi = row_hi, any_hi = row_hi, all_lo = row_lo;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all_hi = min(all_hi, __shfl_xor(all_hi, o));
+    any_hi = max(any_hi, __shfl_xor(any_hi, o));
+    all_lo = max(all_lo, __shfl_xor(all_lo, o));
+  }
+  all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+  any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NW; ++w) unit = fmaxf(unit, s_unit[w]);
+  const float log_unit = unit > 0.f ? __log2f(unit) : 0.f;
+
+  constexpr float kLow = -3.0e38f;                // below every score
+  float m = kLow, l = 0.f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
+
+  for (int step = 0; step < steps; ++step) {
+    const int buf = step & 1, tok = from + 64 * step;
+    wait_vmcnt<0>();                              // this wave's loads of the step
+    __syncthreads();                              // everyone's; the other buffer is free
+    if (step + 1 < steps) issue(step + 1, buf ^ 1);
+    if (tok >= any_hi) continue;
+    float c[4], b[4], inv[4];
+    bool whole = tok >= all_lo && tok + 64 <= all_hi;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float k = ks[4 * step + i], v = vs[4 * step + i];
+      whole = whole && k >= 0.f;
+      c[i] = fmaxf(k * factor, 1e-37f);           // above 0: masked scores are -inf
+      const float r = v > 0.f ? fmaxf(__log2f(v) - log_unit, -100.f) : 0.f;
+      b[i] = r + 15.f;
+      inv[i] = __builtin_amdgcn_exp2f(-b[i]);
+    }
+    const uint8_t* kb = lds + buf * kStage + 16 * lane;
+    f32x16 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
+#pragma unroll
+      for (int d = 0; d < NF; ++d) {
+        const f16x8 k = *reinterpret_cast<const f16x8*>(kb + (t * NF + d) * 1024);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[d][q], s[t], 0, 0, 0);
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int j = tok + 32 * t + 8 * (e >> 2) + 4 * half + (e & 3);
+          if (j < row_lo || j >= row_hi || ks[4 * step + 2 * t + (e >> 3)] < 0.f) s[t][e] = -INFINITY;
+        }
+    }
+    float top = kLow;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x16& x = s[i >> 1];
+      const int o = 8 * (i & 1);
+      const float g = fmaxf(fmaxf(fmaxf(x[o], x[o + 1]), fmaxf(x[o + 2], x[o + 3])),
+                            fmaxf(fmaxf(x[o + 4], x[o + 5]), fmaxf(x[o + 6], x[o + 7])));
+      top = fmaxf(top, g * c[i]);
+    }
+    {
+      auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    }
+    const float mn = fmaxf(m, top);
+    if (__any(mn != m)) {
+      const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[t][e] *= alpha;
+      m = mn;
+    }
+    const uint8_t* vb = lds + buf * kStage + kFragBytes + 16 * lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float off = b[i] - m;
+      float sum = 0.f, e8[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e8[j] = __builtin_amdgcn_exp2f(fmaf(s[i >> 1][8 * (i & 1) + j], c[i], off));
+        sum += e8[j];
+      }
+      l = fmaf(sum, inv[i], l);
+      f16x8 pf[NQ];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        pf[0][j] = static_cast<_Float16>(e8[j]);
+        if constexpr (NQ == 2) pf[1][j] = static_cast<_Float16>(e8[j] - static_cast<float>(pf[0][j]));
+      }
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const f16x8 v = *reinterpret_cast<const f16x8*>(vb + ((i >> 1) * NF + 2 * t + (i & 1)) * 1024);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[q], acc[t], 0, 0, 0);
+      }
+    }
+  }
+  l += __shfl_xor(l, 32);
+  if (!has) return;
+  const bool last = p.splits == 1;
+  const float back = unit * (1.0f / 32768.0f) + broken;
+  const float scale = last ? (l == 0.f ? 0.f : back / l) : back;
+  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
+  const long long part = static_cast<long long>(split) * a.tokens * p.heads + row;
+  if (!last) {
+    if (half == 0) {
+      p.stats[2 * part] = l == 0.f ? -INFINITY : m;
+      p.stats[2 * part + 1] = l;
+    }
+    if (l == 0.f) return;
+  }
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int d = 32 * t + 2 * e + 4 * half;
+      if (d >= a.head_dim) continue;
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = l == 0.f ? 0.f : acc[t][e + j] * scale;
+      if (last)
+        store_n<TYPE, 4>(p.out, (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim + d,
+                         p.vec, v);
+      else
+        store_n<QC_STORAGE_F32, 4>(p.part, part * a.head_dim + d, true, v);
+    }
+}
+
 // out = sum over the ranges of 2^(m_s - m) O_s over that of 2^(m_s - m) l_s: a
 // wavefront a row.
 template <int TYPE>
@@ -519,13 +866,34 @@ __global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p) {
   }
 }
 
+// A call's partial sums where its keys are split.
+hipError_t part_buffers(const Kv8Args& a, AttnArgs& p, StreamWorkspace* ws, hipStream_t s) {
+  const size_t outs = static_cast<size_t>(p.splits) * a.tokens * p.heads;
+  void* buf = nullptr;
+  const hipError_t e = stream_buffer(ws, s, outs * (a.head_dim + 2) * sizeof(float), 0, &buf);
+  p.part = static_cast<float*>(buf);
+  p.stats = p.part + outs * a.head_dim;
+  return e;
+}
+
+template <int TYPE>
+hipError_t run_join(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
+  const long long items = static_cast<long long>(a.seqs) * a.max_new * p.heads;
+  attention_join<TYPE><<<static_cast<unsigned>((items + 3) / 4), 256, 0, s>>>(a, p);
+  return hipGetLastError();
+}
+
+// Keys that a block of `rows` rows can see, from a multiple of `align` on.
+long long key_span(const Kv8Args& a, const AttnArgs& p, int rows, int align) {
+  if (p.window <= 0) return a.max_kv;
+  return std::min<long long>(a.max_kv, static_cast<long long>(p.window) + (rows + p.group - 1) / p.group + align);
+}
+
 template <int DP, int RT, int TYPE>
 hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   const long long rows = static_cast<long long>(a.max_new) * p.group;
   p.row_blocks = static_cast<int>((rows + RT * 16 - 1) / (RT * 16));
-  // keys a block of rows can see, from a multiple of 32 on
-  long long span = a.max_kv;
-  if (p.window > 0) span = std::min<long long>(span, p.window + (RT * 16 + p.group - 1) / p.group + 32);
+  const long long span = key_span(a, p, RT * 16, 32);
   const long long units = static_cast<long long>(a.seqs) * a.kv_heads * p.row_blocks;
   const long long want = std::max<long long>(1, 4LL * device_cu_count() / units);
   long long chunk = (span + want - 1) / want;
@@ -541,27 +909,62 @@ hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
     hipError_t e = stream_workspace(s, &ws);
     if (e != hipSuccess) return e;
     hold = std::unique_lock<std::mutex>(ws->call);
-    const size_t outs = static_cast<size_t>(p.splits) * a.tokens * p.heads;
-    void* buf = nullptr;
-    e = stream_buffer(ws, s, outs * (a.head_dim + 2) * sizeof(float), 0, &buf);
-    if (e != hipSuccess) return e;
-    p.part = static_cast<float*>(buf);
-    p.stats = p.part + outs * a.head_dim;
+    if ((e = part_buffers(a, p, ws, s)) != hipSuccess) return e;
   }
   attention_direct<DP, RT, TYPE><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a, p);
-  hipError_t e = hipGetLastError();
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
-  const long long items = static_cast<long long>(a.seqs) * a.max_new * p.heads;
-  attention_join<TYPE><<<static_cast<unsigned>((items + 3) / 4), 256, 0, s>>>(a, p);
-  return hipGetLastError();
+  return run_join<TYPE>(a, p, s);
+}
+
+// Bytes of fragments laid out at a time; a call with more goes in passes of whole units.
+constexpr long long kFragPass = 1LL << 30;
+
+template <int DP, int NW, int TYPE>
+hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
+  const long long rows = static_cast<long long>(a.max_new) * p.group;
+  p.row_blocks = static_cast<int>((rows + 32 * NW - 1) / (32 * NW));
+  const long long span = key_span(a, p, 32 * NW, 64);
+  const long long units = static_cast<long long>(a.seqs) * a.kv_heads;
+  const long long want = std::max<long long>(1, device_cu_count() / (units * p.row_blocks));
+  long long chunk = ((span + want - 1) / want + 63) / 64 * 64;
+  chunk = std::max<long long>(chunk, 512);
+  p.chunk = static_cast<int>(chunk);
+  p.splits = static_cast<int>((span + chunk - 1) / chunk);
+  Frags f = {};
+  f.cap = (a.max_kv + 63) / 64 * 64;
+  const long long unit_bytes = static_cast<long long>(f.cap) * DP * 4 + f.cap / 2;   // two of f16, scales
+  const long long pass = std::min(units, std::max<long long>(1, kFragPass / unit_bytes));
+  if (pass * p.splits * p.row_blocks > INT_MAX || pass * (f.cap / 32) > INT_MAX) return hipErrorInvalidValue;
+  StreamWorkspace* ws = nullptr;
+  hipError_t e = stream_workspace(s, &ws);
+  if (e != hipSuccess) return e;
+  std::unique_lock<std::mutex> hold(ws->call);
+  if (p.splits > 1 && (e = part_buffers(a, p, ws, s)) != hipSuccess) return e;
+  void* buf = nullptr;
+  if ((e = stream_buffer(ws, s, static_cast<size_t>(pass) * unit_bytes, 1, &buf)) != hipSuccess) return e;
+  f.k = static_cast<_Float16*>(buf);
+  f.v = f.k + pass * f.cap * DP;
+  f.ks = reinterpret_cast<float*>(f.v + pass * f.cap * DP);
+  f.vs = f.ks + pass * (f.cap / 16);
+  for (long long u0 = 0; u0 < units; u0 += pass) {
+    const int n = static_cast<int>(std::min(pass, units - u0));
+    f.unit0 = static_cast<int>(u0);
+    const int tiles = f.cap / 32;
+    attention_layout<DP><<<static_cast<unsigned>(n) * tiles, 256, 0, s>>>(a, f, tiles, p.window);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    attention_tiled<DP, NW, TYPE><<<static_cast<unsigned>(n) * p.splits * p.row_blocks, 64 * NW, 0, s>>>(a, p, f);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  return p.splits > 1 ? run_join<TYPE>(a, p, s) : hipSuccess;
 }
 
 template <int DP, int TYPE>
 hipError_t run_rows(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
   const long long rows = static_cast<long long>(a.max_new) * p.group;
-  if (rows <= 16 || (DP == 256 && TYPE == QC_STORAGE_F32)) return run_direct<DP, 1, TYPE>(a, p, s);
-  if constexpr (DP < 256 || TYPE != QC_STORAGE_F32) return run_direct<DP, 2, TYPE>(a, p, s);
-  return hipErrorInvalidValue;
+  if (rows <= 16) return run_direct<DP, 1, TYPE>(a, p, s);
+  if (rows > 64) return run_tiled<DP, DP == 256 ? 4 : 8, TYPE>(a, p, s);
+  return run_direct<DP, DP == 256 && TYPE == QC_STORAGE_F32 ? 1 : 2, TYPE>(a, p, s);
 }
 
 template <int TYPE>

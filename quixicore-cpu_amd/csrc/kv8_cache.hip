@@ -85,6 +85,10 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Kv8Args a, Rows k, Row
     return;
   }
   const float before = lo > p0 ? *scale_at : 0.f;
+  if (!isfinite(before)) {
+    if (threadIdx.x == 0) *a.status = QC_INVALID_ARGUMENT;
+    return;
+  }
   float scale = fmaxf(before, top * (1.0f / 127.0f));
   if (scale < 1.17549435e-38f) scale = 0.f;
   const float inv = scale > 0.f ? 1.0f / scale : 0.f;
@@ -92,7 +96,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Kv8Args a, Rows k, Row
   if (lo > p0 && ratio != 1.0f) {
     const int m = (lo - p0) * a.head_dim;
     for (int i = threadIdx.x; i < m; i += kThreads)
-      codes[i] = static_cast<int8_t>(rintf(static_cast<float>(codes[i]) * ratio));
+      codes[i] = static_cast<int8_t>(fminf(fmaxf(rintf(static_cast<float>(codes[i]) * ratio), -127.f), 127.f));
   }
   int8_t* out = codes + (lo - p0) * a.head_dim;
   for (int i = threadIdx.x; i < n; i += kThreads) {
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(Kv8Args a, void* k, vo
 
 // The figures and table entries that a call goes by.  from_new: it touches the
 // new tokens' pages; else the pages that its queries see (window: see
-// qc_hip_kv8_attention).
+// qc_hip_kv8_attention), and their scales are finite.
 __global__ __launch_bounds__(kThreads) void kv8_check(Kv8Args a, bool from_new, int window) {
   const int q = blockIdx.x;
   int first, rows, kv;
@@ -158,10 +162,18 @@ __global__ __launch_bounds__(kThreads) void kv8_check(Kv8Args a, bool from_new, 
   if (from_new && rows > kv) *a.status = QC_INVALID_ARGUMENT;
   const int from = from_new ? max(kv - rows, 0) : window > 0 ? max(kv - rows + 1 - window, 0) : 0;
   for (int c = (from >> a.page_shift) + threadIdx.x; c < (kv + a.page_tokens - 1) >> a.page_shift;
-       c += kThreads)
-    if (static_cast<unsigned>(a.table[static_cast<long long>(q) * a.columns + c]) >=
-        static_cast<unsigned>(a.pages))
+       c += kThreads) {
+    const int page = a.table[static_cast<long long>(q) * a.columns + c];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) {
       *a.status = QC_INVALID_ARGUMENT;
+      continue;
+    }
+    if (from_new) continue;
+    for (int h = 0; h < a.kv_heads; ++h) {
+      const long long at = static_cast<long long>(page) * a.kv_heads + h;
+      if (!isfinite(a.k_scales[at]) || !isfinite(a.v_scales[at])) *a.status = QC_INVALID_ARGUMENT;
+    }
+  }
 }
 
 // *flag = 3 where a row of the batch's sequences holds NaN or +-inf.

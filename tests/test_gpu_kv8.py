@@ -377,6 +377,11 @@ def test_attention_scales_far_apart(qc, dev, dtype):
         cache.tensors[3].zero_()
         cache.tensors[1].zero_()
         _attend(qc, dev, rng, new, kv, 4, 2, 64, 16, dtype, batch=batch, cache=cache)
+        batch = Ragged(rng, new, kv, 16)
+        cache = _random_cache(qc, dev, rng, batch.pages, 2, 16, 64)
+        for i in (2, 3):                                # negative scales are scales
+            cache.tensors[i][torch.rand(batch.pages, 2, device=dev) < 0.5] *= -1
+        _attend(qc, dev, rng, new, kv, 4, 2, 64, 16, dtype, batch=batch, cache=cache)
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
@@ -453,10 +458,13 @@ def test_attention_errors(qc, dev):
         q = torch.from_numpy(rng.standard_normal((batch.tokens, 4, 64))).to(torch.float16).to(dev)
         want = qc.kv8_attention(cache, batch.device(qc, dev), q)
         a, z = int(batch.start[1]), int(batch.start[2])
-        for bad in ("page", "long", "negative", "start"):
+        for bad in ("page", "scale", "long", "negative", "start"):
             b = batch.device(qc, dev)
             if bad == "page":
                 b.tensors[0][1, 2] = batch.pages
+            elif bad == "scale":
+                held = cache.tensors[3].clone()
+                cache.tensors[3][batch.table[1, 2], 1] = float("inf")
             elif bad == "long":
                 b.tensors[2][1] = batch.max_kv + 1
             elif bad == "negative":
@@ -475,8 +483,14 @@ def test_attention_errors(qc, dev):
                 assert torch.equal(out[a:z], want[a:z]) and bool((out[z:] == 7).all())
             else:
                 assert torch.equal(out[z:], want[z:])
-                if bad != "page":
+                if bad in ("page", "scale"):
+                    # as if the page were not there: the same for both ways to lose it
+                    assert bool(torch.isfinite(out[a:z]).all())
+                else:
                     assert bool((out[a:z] == 7).all())
+            if bad == "scale":
+                assert torch.equal(out[a:z, :2], want[a:z, :2])      # the other key head's rows
+                cache.tensors[3].copy_(held)
 
 
 @pytest.mark.parametrize("new,kv,heads,kvh", [([1] * 5, [900, 1, 64, 500, 333], 8, 2), ([1], [4000], 4, 1),
