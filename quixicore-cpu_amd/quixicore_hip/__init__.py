@@ -355,60 +355,70 @@ class RopeScaling(ctypes.Structure):
                 ("high_turns", ctypes.c_double), ("magnitude", ctypes.c_double)]
 
 
+# The checks run on every call beside kernels of a few us: no tensor is looked at twice,
+# and get_device() stands for comparing device objects.
 _storage_ids = None   # torch dtype -> STORAGE id
 _device = None        # index of the current device
+_types = None         # (int32, uint8, float32)
+
+
+def _start():
+    global _storage_ids, _device, _types
+    import torch
+    torch.cuda.current_stream()   # initialises the device
+    _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    _storage_ids = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    _types = (torch.int32, torch.uint8, torch.float32)
 
 
 def _storage(t):
-    global _storage_ids, _device
+    """STORAGE id of a tensor's type."""
     if _storage_ids is None:
-        import torch
-        torch.cuda.current_stream()   # initialises the device
-        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-        _storage_ids = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        _start()
     st = _storage_ids.get(t.dtype)
     if st is None:
         raise TypeError(f"f32, f16 or bf16 tensors: got {t.dtype}")
-    _here(t)
     return st
 
 
 def _here(*tensors):
-    global _device
+    """The tensors lie on the current device."""
     if _device is None:
-        import torch
-        torch.cuda.current_stream()
-        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        _start()
     now = _device()
     for t in tensors:
-        if t is not None and (t.device.type != "cuda" or t.device.index != now):
+        if t.get_device() != now:
             raise ValueError(f"a tensor on {t.device}: the current device is cuda:{now}")
 
 
 def _flat(what, dtype, *tensors):
     """Contiguous tensors of one type on the current device."""
-    _here(*tensors)
+    now = _device()
     for t in tensors:
-        if t is not None and (t.dtype != dtype or not t.is_contiguous()):
-            raise ValueError(f"{what}: contiguous {dtype} tensors")
+        if t.dtype is not dtype or not t.is_contiguous() or t.get_device() != now:
+            raise ValueError(f"{what}: contiguous {dtype} tensors on cuda:{now}")
 
 
 def _status(dev_status):
-    import torch
-    if dev_status is not None:
-        _flat("dev_status", torch.int32, dev_status)
-    return _ptr(dev_status)
+    if dev_status is None:
+        return None
+    _flat("dev_status", _types[0], dev_status)
+    return dev_status.data_ptr()
 
 
 def _rows(what, t, heads, head_dim):
     """Row stride of token rows [tokens][heads * head_dim] or [tokens][heads][head_dim]."""
-    ok = (t.dim() == 2 and t.shape[1] == heads * head_dim and t.stride(1) == 1) or (
-        t.dim() == 3 and t.shape[1] == heads and t.shape[2] == head_dim and t.stride(2) == 1
-        and (heads == 1 or t.stride(1) == head_dim))
+    shape, stride = t.shape, t.stride()
+    n = len(shape)
+    if n == 3:
+        ok = shape[1] == heads and shape[2] == head_dim and stride[2] == 1 and (
+            heads == 1 or stride[1] == head_dim)
+    else:
+        ok = n == 2 and shape[1] == heads * head_dim and stride[1] == 1
     if not ok:
         raise ValueError(f"{what}: rows of {heads} x {head_dim} elements side by side, got "
-                         f"{tuple(t.shape)} with strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else heads * head_dim
+                         f"{tuple(shape)} with strides {stride}")
+    return stride[0] if shape[0] > 1 else heads * head_dim
 
 
 def rope_table(positions, rotary_dim, base=10000.0, scaling="none", factor=1.0,
@@ -429,24 +439,26 @@ def rope_table(positions, rotary_dim, base=10000.0, scaling="none", factor=1.0,
 def rope(x, cosine, sine, positions, interleaved=False, out=None, dev_status=None):
     """x [tokens][heads][head_dim] (any token and head strides) with the first 2 *
     cosine.shape[1] elements of every head rotated; out may be x."""
-    import torch
     st = _storage(x)
     if x.dim() != 3 or x.stride(2) != 1:
         raise ValueError("rope: x is [tokens][heads][head_dim], elements side by side")
     if out is None:
+        import torch
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.stride(2) != 1 or out.dtype != x.dtype:
+    elif out is not x and (out.shape != x.shape or out.stride(2) != 1 or out.dtype is not x.dtype):
         raise ValueError("rope: out is of x's shape and type")
-    _here(out)
-    _flat("rope tables", torch.float32, cosine, sine)
-    _flat("rope positions", torch.int32, positions)
+    _here(x, out)
+    _flat("rope tables", _types[2], cosine, sine)
+    _flat("rope positions", _types[0], positions)
     tokens, heads, head_dim = x.shape
-    if cosine.dim() != 2 or sine.shape != cosine.shape or positions.numel() != tokens:
+    most, half = cosine.shape
+    if sine.shape != cosine.shape or positions.numel() != tokens:
         raise ValueError("rope: tables [max_position][rotary_dim / 2], a position for each token")
-    _check(lib.qc_hip_rope(_ptr(x), _ptr(out), st, tokens, heads, head_dim, 2 * cosine.shape[1],
-                           x.stride(0), x.stride(1), out.stride(0), out.stride(1), _ptr(cosine),
-                           _ptr(sine), _ptr(positions), cosine.shape[0], int(bool(interleaved)),
-                           _status(dev_status), _stream(None)), "rope")
+    xt, xh, _ = x.stride()
+    yt, yh, _ = out.stride()
+    _check(lib.qc_hip_rope(x.data_ptr(), out.data_ptr(), st, tokens, heads, head_dim, 2 * half, xt,
+                           xh, yt, yh, cosine.data_ptr(), sine.data_ptr(), positions.data_ptr(),
+                           most, 1 if interleaved else 0, _status(dev_status), _stream(None)), "rope")
     return out
 
 
@@ -460,12 +472,14 @@ class Kv8Cache(ctypes.Structure):
 
     def __init__(self, k_codes, v_codes, k_scales, v_scales):
         import torch
+        _here(k_codes)
         _flat("cache codes", torch.int8, k_codes, v_codes)
         _flat("cache scales", torch.float32, k_scales, v_scales)
         if (k_codes.dim() != 4 or v_codes.shape != k_codes.shape
                 or k_scales.shape != k_codes.shape[:2] or v_scales.shape != k_codes.shape[:2]):
             raise ValueError("codes [pages][kv_heads][page_tokens][head_dim], scales [pages][kv_heads]")
         self.tensors = (k_codes, v_codes, k_scales, v_scales)
+        self.device = k_codes.get_device()
         super().__init__(*[t.data_ptr() for t in self.tensors], *k_codes.shape)
 
 
@@ -479,17 +493,26 @@ class Kv8Batch(ctypes.Structure):
 
     def __init__(self, block_table, seq_start, kv_len, tokens, max_new, max_kv):
         import torch
+        _here(block_table)
         _flat("batch", torch.int32, block_table, seq_start, kv_len)
         seqs, columns = block_table.shape
         if seq_start.numel() != seqs + 1 or kv_len.numel() != seqs:
             raise ValueError("block_table [seqs][columns], seq_start [seqs + 1], kv_len [seqs]")
         self.tensors = (block_table, seq_start, kv_len)
+        self.device = block_table.get_device()
         super().__init__(*[t.data_ptr() for t in self.tensors], seqs, columns, tokens, max_new,
                          max_kv)
 
 
-def _kv8_here(cache, batch):
-    _here(cache.tensors[0], batch.tensors[0])
+def _kv8_here(cache, batch, *tensors):
+    """Everything on the current device (types were checked when the handles were made)."""
+    now = _device()
+    if cache.device != now or batch.device != now:
+        raise ValueError(f"a cache on cuda:{cache.device}, a batch on cuda:{batch.device}: the "
+                         f"current device is cuda:{now}")
+    for t in tensors:
+        if t.get_device() != now:
+            raise ValueError(f"a tensor on {t.device}: the current device is cuda:{now}")
 
 
 def kv8_cache(pages, kv_heads, page_tokens, head_dim):
@@ -504,34 +527,34 @@ def kv8_cache(pages, kv_heads, page_tokens, head_dim):
 def kv8_append(cache, batch, k, v, dev_status=None):
     """Writes the batch's new tokens' k and v ([tokens][kv_heads][head_dim] or flat rows)."""
     st = _storage(k)
-    _here(v)
-    _kv8_here(cache, batch)
-    if v.dtype != k.dtype or k.shape[0] != batch.tokens or v.shape[0] != batch.tokens:
+    _kv8_here(cache, batch, k, v)
+    tokens, heads, head_dim = batch.tokens, cache.kv_heads, cache.head_dim
+    if v.dtype is not k.dtype or k.shape[0] != tokens or v.shape[0] != tokens:
         raise ValueError("kv8_append: k and v of one type, a row for each of the batch's tokens")
-    _check(lib.qc_hip_kv8_append(ctypes.addressof(cache), ctypes.addressof(batch), _ptr(k),
-                                 _rows("k", k, cache.kv_heads, cache.head_dim), _ptr(v),
-                                 _rows("v", v, cache.kv_heads, cache.head_dim), st,
-                                 _status(dev_status), _stream(None)), "kv8_append")
+    _check(lib.qc_hip_kv8_append(ctypes.addressof(cache), ctypes.addressof(batch), k.data_ptr(),
+                                 _rows("k", k, heads, head_dim), v.data_ptr(),
+                                 _rows("v", v, heads, head_dim), st, _status(dev_status),
+                                 _stream(None)), "kv8_append")
 
 
 def kv8_gather(cache, batch, dtype=None, k=None, v=None, dev_status=None):
     """(k, v) [tokens][kv_heads][head_dim]: the values the cache holds for the batch's
     tokens.  Rows of no sequence are left as they were (zeros in new tensors)."""
-    import torch
-    shape = (batch.tokens, cache.kv_heads, cache.head_dim)
-    if k is None:
-        k = torch.zeros(shape, dtype=dtype or torch.float32, device=cache.tensors[0].device)
-    if v is None:
-        v = torch.zeros(shape, dtype=k.dtype, device=k.device)
+    tokens, heads, head_dim = batch.tokens, cache.kv_heads, cache.head_dim
+    if k is None or v is None:
+        import torch
+        new = torch.zeros((2, tokens, heads, head_dim), device=cache.tensors[0].device,
+                          dtype=dtype or (torch.float32 if k is None and v is None else
+                                          (v if k is None else k).dtype)).unbind()
+        k, v = new[0] if k is None else k, new[1] if v is None else v
     st = _storage(k)
-    _here(v)
-    _kv8_here(cache, batch)
-    if v.dtype != k.dtype or k.shape[0] != batch.tokens or v.shape[0] != batch.tokens:
+    _kv8_here(cache, batch, k, v)
+    if v.dtype is not k.dtype or k.shape[0] != tokens or v.shape[0] != tokens:
         raise ValueError("kv8_gather: k and v of one type, a row for each of the batch's tokens")
-    _check(lib.qc_hip_kv8_gather(ctypes.addressof(cache), ctypes.addressof(batch), _ptr(k),
-                                 _rows("k", k, cache.kv_heads, cache.head_dim), _ptr(v),
-                                 _rows("v", v, cache.kv_heads, cache.head_dim), st,
-                                 _status(dev_status), _stream(None)), "kv8_gather")
+    _check(lib.qc_hip_kv8_gather(ctypes.addressof(cache), ctypes.addressof(batch), k.data_ptr(),
+                                 _rows("k", k, heads, head_dim), v.data_ptr(),
+                                 _rows("v", v, heads, head_dim), st, _status(dev_status),
+                                 _stream(None)), "kv8_gather")
     return k, v
 
 
@@ -539,23 +562,23 @@ def kv8_attention(cache, batch, q, scale=None, causal=True, window=0, out=None, 
     """softmax(scale q k^T) v of the batch's tokens over the cache: q [tokens][heads][head_dim]
     (rows may be strided), scale 1 / sqrt(head_dim) by default.  Rows of no sequence are left as
     they were (zeros in a new tensor)."""
-    import torch
     st = _storage(q)
-    _kv8_here(cache, batch)
-    if q.dim() != 3 or q.shape[0] != batch.tokens:
+    head_dim, shape = cache.head_dim, q.shape
+    if len(shape) != 3 or shape[0] != batch.tokens:
         raise ValueError("kv8_attention: q is [tokens][heads][head_dim], a row for each of the batch's tokens")
-    heads = q.shape[1]
+    heads = shape[1]
     if out is None:
-        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
+        import torch
+        out = torch.zeros(shape, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.dtype is not q.dtype:
         raise ValueError("kv8_attention: out is of q's shape and type")
-    _here(out)
+    _kv8_here(cache, batch, q, out)
     if scale is None:
-        scale = cache.head_dim ** -0.5
-    _check(lib.qc_hip_kv8_attention(ctypes.addressof(cache), ctypes.addressof(batch), _ptr(q),
-                                    _rows("q", q, heads, cache.head_dim), _ptr(out),
-                                    _rows("out", out, heads, cache.head_dim), st, heads, scale,
-                                    int(bool(causal)), window, _status(dev_status), _stream(None)),
+        scale = head_dim ** -0.5
+    _check(lib.qc_hip_kv8_attention(ctypes.addressof(cache), ctypes.addressof(batch), q.data_ptr(),
+                                    _rows("q", q, heads, head_dim), out.data_ptr(),
+                                    _rows("out", out, heads, head_dim), st, heads, scale,
+                                    1 if causal else 0, window, _status(dev_status), _stream(None)),
            "kv8_attention")
     return out
 
@@ -565,45 +588,55 @@ def quantize_mxfp4(x, dev_status=None):
     strided)."""
     import torch
     st = _storage(x)
+    _here(x)
     if x.dim() != 2 or x.stride(1) != 1:
         raise ValueError("quantize_mxfp4: x is [rows][dim], elements side by side")
     rows, dim = x.shape
     codes = torch.empty((rows, dim // 2), dtype=torch.uint8, device=x.device)
     scales = torch.empty((rows, dim // 32), dtype=torch.uint8, device=x.device)
-    _check(lib.qc_hip_quantize_mxfp4(_ptr(x), st, x.stride(0), _ptr(codes), _ptr(scales), rows,
-                                     dim, _status(dev_status), _stream(None)), "quantize_mxfp4")
+    _check(lib.qc_hip_quantize_mxfp4(x.data_ptr(), st, x.stride(0), codes.data_ptr(),
+                                     scales.data_ptr(), rows, dim, _status(dev_status),
+                                     _stream(None)), "quantize_mxfp4")
     return codes, scales
 
 
 def dequantize_mxfp4(codes, scales, dtype=None, out=None):
     """The values [rows][dim] that MXFP4 codes and scales stand for."""
-    import torch
-    _flat("mxfp4", torch.uint8, codes, scales)
-    rows, dim = codes.shape[0], 2 * codes.shape[1]
+    _here(codes)
+    _flat("mxfp4", _types[1], codes, scales)
+    rows, half = codes.shape
     if out is None:
-        out = torch.empty((rows, dim), dtype=dtype or torch.float32, device=codes.device)
-    if tuple(scales.shape) != (rows, dim // 32) or tuple(out.shape) != (rows, dim) or not out.is_contiguous():
-        raise ValueError("dequantize_mxfp4: codes [rows][dim / 2], scales [rows][dim / 32], out [rows][dim]")
-    _check(lib.qc_hip_dequantize_mxfp4(_ptr(codes), _ptr(scales), _ptr(out), _storage(out), rows,
-                                       dim, _stream(None)), "dequantize_mxfp4")
+        import torch
+        out = torch.empty((rows, 2 * half), dtype=dtype or torch.float32, device=codes.device)
+    elif tuple(out.shape) != (rows, 2 * half) or not out.is_contiguous():
+        raise ValueError("dequantize_mxfp4: out is [rows][dim], contiguous")
+    _here(out)
+    if tuple(scales.shape) != (rows, half // 16):
+        raise ValueError("dequantize_mxfp4: codes [rows][dim / 2], scales [rows][dim / 32]")
+    _check(lib.qc_hip_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), out.data_ptr(),
+                                       _storage(out), rows, 2 * half, _stream(None)),
+           "dequantize_mxfp4")
     return out
 
 
 def mxfp4_gemm(w_codes, w_scales, x_codes, x_scales, dtype=None, y=None):
     """y [m][n] = x . w^T of MXFP4 matrices w [n][k] and x [m][k]."""
-    import torch
-    _flat("mxfp4_gemm", torch.uint8, w_codes, w_scales, x_codes, x_scales)
-    (n, half), m = w_codes.shape, x_codes.shape[0]
-    k = 2 * half
-    if (x_codes.shape[1] != half or tuple(w_scales.shape) != (n, k // 32)
-            or tuple(x_scales.shape) != (m, k // 32)):
+    _here(w_codes)
+    _flat("mxfp4_gemm", _types[1], w_codes, w_scales, x_codes, x_scales)
+    n, half = w_codes.shape
+    m, other = x_codes.shape
+    blocks = half // 16
+    if other != half or tuple(w_scales.shape) != (n, blocks) or tuple(x_scales.shape) != (m, blocks):
         raise ValueError("mxfp4_gemm: codes [rows][k / 2], scales [rows][k / 32]")
     if y is None:
+        import torch
         y = torch.empty((m, n), dtype=dtype or torch.float32, device=x_codes.device)
     elif tuple(y.shape) != (m, n) or not y.is_contiguous():
         raise ValueError("mxfp4_gemm: y is [m][n], contiguous")
-    _check(lib.qc_hip_mxfp4_gemm(_ptr(w_codes), _ptr(w_scales), _ptr(x_codes), _ptr(x_scales),
-                                 _ptr(y), _storage(y), m, n, k, _stream(None)), "mxfp4_gemm")
+    _here(y)
+    _check(lib.qc_hip_mxfp4_gemm(w_codes.data_ptr(), w_scales.data_ptr(), x_codes.data_ptr(),
+                                 x_scales.data_ptr(), y.data_ptr(), _storage(y), m, n, 2 * half,
+                                 _stream(None)), "mxfp4_gemm")
     return y
 
 
