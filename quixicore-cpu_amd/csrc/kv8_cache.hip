@@ -9,6 +9,8 @@
 // 127), ties to even, each step rounded to f32.  So a call's codes are
 // defined bit for bit, and a page that is filled token by token has been rounded
 // at most once for each growth of its scale.
+#include <algorithm>
+
 #include "qc_kv8.h"
 #include "qc_storage.h"
 
@@ -24,68 +26,106 @@ struct Rows {
   long long stride;   // elements between tokens
 };
 
-// Workgroup (page slot, head, K or V) of a sequence: the page's new tokens.
-template <int TYPE>
-__global__ __launch_bounds__(kThreads) void append_kernel(Kv8Args a, Rows k, Rows v, int slots) {
-  typedef typename Storage<TYPE>::raw raw;
-  __shared__ float stop[kThreads / 64];
-  __shared__ int sbad[kThreads / 64];
-  long long id = blockIdx.x;
-  const int which = id & 1;
+// What workgroup `id` of a grid over (sequence, touched page, head, K or V) works on:
+// the page's new tokens, positions [lo, hi) of a page that starts at p0.
+struct Place {
+  int which, head;
+  int lo, hi, p0;
+  int row;                 // token row of position lo
+  long long unit;          // page * kv_heads + head
+};
+
+__device__ __forceinline__ bool place_of(const Kv8Args& a, int slots, Place& w) {
+  int id = blockIdx.x;
+  w.which = id & 1;
   id >>= 1;
-  const int head = id % a.kv_heads;
-  id /= a.kv_heads;
-  const int slot = id % slots;
-  const int q = id / slots;
+  const int rest = id / a.kv_heads;
+  w.head = id - rest * a.kv_heads;
+  const int q = rest / slots, slot = rest - q * slots;
   int first, rows, kv;
-  if (!kv8_sequence(a, q, first, rows, kv)) return;
+  if (!kv8_sequence(a, q, first, rows, kv)) return false;
   const int begin = kv - rows;               // position of the first new token
   if (begin < 0) {
     *a.status = QC_INVALID_ARGUMENT;
-    return;
+    return false;
   }
   const int column = (begin >> a.page_shift) + slot;
-  const int p0 = column << a.page_shift;     // the page's first position
-  const int lo = max(begin, p0), hi = min(kv, p0 + a.page_tokens);
-  if (lo >= hi) return;
+  w.p0 = column << a.page_shift;
+  w.lo = max(begin, w.p0);
+  w.hi = min(kv, w.p0 + a.page_tokens);
+  if (w.lo >= w.hi) return false;
   const int page = a.table[static_cast<long long>(q) * a.columns + column];
   if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) {
     *a.status = QC_INVALID_ARGUMENT;
-    return;
+    return false;
   }
-  const Rows src = which ? v : k;
-  const long long unit = static_cast<long long>(page) * a.kv_heads + head;
-  int8_t* codes = (which ? a.v_codes : a.k_codes) + unit * a.page_tokens * a.head_dim;
-  float* scale_at = (which ? a.v_scales : a.k_scales) + unit;
-  const raw* x = static_cast<const raw*>(src.p) + (first + lo - begin) * src.stride +
-                 static_cast<long long>(head) * a.head_dim;
-  const int n = (hi - lo) * a.head_dim;
-  float top = 0.f;
-  int bad = 0;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int t = i / a.head_dim;
-    const float f = decode<TYPE>(x[t * src.stride + i - t * a.head_dim]);
-    bad |= !isfinite(f);
-    top = fmaxf(top, fabsf(f));
+  w.row = first + w.lo - begin;
+  w.unit = static_cast<long long>(page) * a.kv_heads + w.head;
+  return true;
+}
+
+__device__ __forceinline__ int code_of(float v) {
+  return static_cast<int>(fminf(fmaxf(rintf(v), -127.f), 127.f));
+}
+
+// Chunks of V elements (VEC: 16 bytes of a row, aligned); the first kHeld of a thread
+// stay in registers between the maximum and the codes, the others are read again
+// (from L2).  A page and head is a chain of dependent reads (lengths, page id, rows, scale)
+// with little data behind it, so many small workgroups: 64 threads where a page's
+// head is at most 4096 elements.  10.5 thousand tokens of 8 heads of 128, f16, pages
+// of 16: 39 us with an element a thread, 14 here.
+constexpr int kHeld = 8;
+template <int TYPE, int NT, bool VEC>
+__global__ __launch_bounds__(NT) void append_kernel(Kv8Args a, Rows k, Rows v, int slots) {
+  typedef typename Storage<TYPE>::raw raw;
+  constexpr int V = VEC ? Storage<TYPE>::per16 : 4;
+  __shared__ float stop[NT / 64];
+  Place w;
+  if (!place_of(a, slots, w)) return;
+  const Rows src = w.which ? v : k;
+  int8_t* codes = (w.which ? a.v_codes : a.k_codes) + w.unit * a.page_tokens * a.head_dim;
+  float* scale_at = (w.which ? a.v_scales : a.k_scales) + w.unit;
+  const raw* x = static_cast<const raw*>(src.p) + w.row * src.stride +
+                 static_cast<long long>(w.head) * a.head_dim;
+  const float before = w.lo > w.p0 ? *scale_at : 0.f;
+  const int per_row = a.head_dim / V, n = (w.hi - w.lo) * per_row;
+  auto load = [&](int i, float* f) {
+    const int t = i / per_row;
+    const raw* p = x + t * src.stride + (i - t * per_row) * V;
+    if constexpr (VEC) {
+      decode16<TYPE>(*reinterpret_cast<const u32x4*>(p), f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = decode<TYPE>(p[j]);
+    }
+  };
+  float held[kHeld][V], top = 0.f;
+  auto see = [&](const float* f) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) top = isfinite(f[j]) ? fmaxf(top, fabsf(f[j])) : INFINITY;
+  };
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h) {
+    const int i = threadIdx.x + h * NT;
+    if (i < n) load(i, held[h]);
+  }
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h)
+    if (static_cast<int>(threadIdx.x) + h * NT < n) see(held[h]);
+  for (int i = threadIdx.x + kHeld * NT; i < n; i += NT) {
+    float f[V];
+    load(i, f);
+    see(f);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  bad = __any(bad);
-  if ((threadIdx.x & 63) == 0) {
-    stop[threadIdx.x >> 6] = top;
-    sbad[threadIdx.x >> 6] = bad;
+  if constexpr (NT > 64) {
+    if ((threadIdx.x & 63) == 0) stop[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) top = fmaxf(top, stop[i]);
   }
-  __syncthreads();
-  for (int w = 0; w < kThreads / 64; ++w) {
-    top = fmaxf(top, stop[w]);
-    bad |= sbad[w];
-  }
-  if (bad) {
-    if (threadIdx.x == 0) *a.status = QC_INVALID_ARGUMENT;
-    return;
-  }
-  const float before = lo > p0 ? *scale_at : 0.f;
-  if (!isfinite(before)) {
+  if (top == INFINITY || !isfinite(before)) {
     if (threadIdx.x == 0) *a.status = QC_INVALID_ARGUMENT;
     return;
   }
@@ -93,61 +133,75 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Kv8Args a, Rows k, Row
   if (scale < 1.17549435e-38f) scale = 0.f;
   const float inv = scale > 0.f ? 1.0f / scale : 0.f;
   const float ratio = scale > 0.f ? before / scale : 0.f;
-  if (lo > p0 && ratio != 1.0f) {
-    const int m = (lo - p0) * a.head_dim;
-    for (int i = threadIdx.x; i < m; i += kThreads)
-      codes[i] = static_cast<int8_t>(fminf(fmaxf(rintf(static_cast<float>(codes[i]) * ratio), -127.f), 127.f));
+  if (w.lo > w.p0 && ratio != 1.0f) {
+    uint32_t* old = reinterpret_cast<uint32_t*>(codes);
+    const int m = (w.lo - w.p0) * a.head_dim / 4;
+    for (int i = threadIdx.x; i < m; i += NT) {
+      const uint32_t c = old[i];
+      uint32_t o = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o |= (code_of(static_cast<float>(static_cast<int8_t>(c >> (8 * j))) * ratio) & 0xFF) << (8 * j);
+      old[i] = o;
+    }
   }
-  int8_t* out = codes + (lo - p0) * a.head_dim;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int t = i / a.head_dim;
-    const float f = decode<TYPE>(x[t * src.stride + i - t * a.head_dim]);
-    out[i] = static_cast<int8_t>(fminf(fmaxf(rintf(f * inv), -127.f), 127.f));
+  uint32_t* out = reinterpret_cast<uint32_t*>(codes + (w.lo - w.p0) * a.head_dim);
+  auto put = [&](int i, const float* f) {
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+      uint32_t o = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o |= (code_of(f[4 * j + e] * inv) & 0xFF) << (8 * e);
+      out[i * (V / 4) + j] = o;
+    }
+  };
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h) {
+    const int i = threadIdx.x + h * NT;
+    if (i < n) put(i, held[h]);
   }
-  __syncthreads();                            // every wave has read the scale before
+  for (int i = threadIdx.x + kHeld * NT; i < n; i += NT) {
+    float f[V];
+    load(i, f);
+    put(i, f);
+  }
+  // every wave has read the scale before: at the latest by the barrier above
   if (threadIdx.x == 0) *scale_at = scale;
 }
 
-// The same places read back: code * scale, rounded once.
-template <int TYPE>
+// The same places read back: code * scale, rounded once; four codes a thread and
+// step (8.3 thousand tokens of 8 heads of 128 to f16: 24 us with one, 16 so).
+template <int TYPE, bool VEC>
 __global__ __launch_bounds__(kThreads) void gather_kernel(Kv8Args a, void* k, void* v,
                                                           long long k_stride, long long v_stride,
                                                           int slots) {
   typedef typename Storage<TYPE>::raw raw;
-  long long id = blockIdx.x;
-  const int which = id & 1;
-  id >>= 1;
-  const int head = id % a.kv_heads;
-  id /= a.kv_heads;
-  const int slot = id % slots;
-  const int q = id / slots;
-  int first, rows, kv;
-  if (!kv8_sequence(a, q, first, rows, kv)) return;
-  const int begin = kv - rows;
-  if (begin < 0) {
-    *a.status = QC_INVALID_ARGUMENT;
-    return;
-  }
-  const int column = (begin >> a.page_shift) + slot;
-  const int p0 = column << a.page_shift;
-  const int lo = max(begin, p0), hi = min(kv, p0 + a.page_tokens);
-  if (lo >= hi) return;
-  const int page = a.table[static_cast<long long>(q) * a.columns + column];
-  if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) {
-    *a.status = QC_INVALID_ARGUMENT;
-    return;
-  }
-  const long long unit = static_cast<long long>(page) * a.kv_heads + head;
-  const int8_t* codes = (which ? a.v_codes : a.k_codes) +
-                        (unit * a.page_tokens + lo - p0) * a.head_dim;
-  const float scale = (which ? a.v_scales : a.k_scales)[unit];
-  const long long stride = which ? v_stride : k_stride;
-  raw* out = static_cast<raw*>(which ? v : k) + (first + lo - begin) * stride +
-             static_cast<long long>(head) * a.head_dim;
-  const int n = (hi - lo) * a.head_dim;
+  Place w;
+  if (!place_of(a, slots, w)) return;
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(
+      (w.which ? a.v_codes : a.k_codes) + (w.unit * a.page_tokens + w.lo - w.p0) * a.head_dim);
+  const float scale = (w.which ? a.v_scales : a.k_scales)[w.unit];
+  const long long stride = w.which ? v_stride : k_stride;
+  raw* out = static_cast<raw*>(w.which ? v : k) + w.row * stride +
+             static_cast<long long>(w.head) * a.head_dim;
+  const int per_row = a.head_dim / 4, n = (w.hi - w.lo) * per_row;
+#pragma unroll 4
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int t = i / a.head_dim;
-    out[t * stride + i - t * a.head_dim] = encode<TYPE>(static_cast<float>(codes[i]) * scale);
+    const uint32_t c = codes[i];
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = static_cast<float>(static_cast<int8_t>(c >> (8 * j))) * scale;
+    const int t = i / per_row;
+    raw* o = out + t * stride + (i - t * per_row) * 4;
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = encode<TYPE>(f[j]);
+    } else if constexpr (TYPE == QC_STORAGE_F32) {
+      *reinterpret_cast<u32x4*>(o) = encode16<TYPE>(f);
+    } else {
+      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+      *reinterpret_cast<u32x2*>(o) = u32x2{encode2<TYPE>(f[0], f[1]), encode2<TYPE>(f[2], f[3])};
+    }
   }
 }
 
@@ -240,17 +294,48 @@ hipError_t launch_kv8_nonfinite(const qc_kv8_cache& c, const qc_kv8_batch& b, co
   return hipGetLastError();
 }
 
+namespace {
+
+// Rows of 16-byte chunks (the heads of a row are multiples of 16 elements apart).
+bool wide_rows(const void* p, long long stride, int size) {
+  return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * size)) % 16 == 0;
+}
+
+template <int TYPE>
+void run_append(const Kv8Args& a, const Rows& k, const Rows& v, hipStream_t s) {
+  constexpr int size = TYPE == QC_STORAGE_F32 ? 4 : 2;
+  const int slots = touched_slots(a);
+  const unsigned grid = static_cast<unsigned>(2LL * a.kv_heads * slots * a.seqs);
+  const bool vec = wide_rows(k.p, k.stride, size) && wide_rows(v.p, v.stride, size);
+  const bool small = std::min(a.max_new, a.page_tokens) * a.head_dim <= 4096;
+  if (vec && small) append_kernel<TYPE, 64, true><<<grid, 64, 0, s>>>(a, k, v, slots);
+  else if (vec) append_kernel<TYPE, 256, true><<<grid, 256, 0, s>>>(a, k, v, slots);
+  else append_kernel<TYPE, 256, false><<<grid, 256, 0, s>>>(a, k, v, slots);
+}
+
+template <int TYPE>
+void run_gather(const Kv8Args& a, void* k, void* v, long long k_stride, long long v_stride,
+                hipStream_t s) {
+  constexpr int size = TYPE == QC_STORAGE_F32 ? 4 : 2;
+  const int slots = touched_slots(a);
+  const unsigned grid = static_cast<unsigned>(2LL * a.kv_heads * slots * a.seqs);
+  if (wide_rows(k, k_stride, size) && wide_rows(v, v_stride, size))
+    gather_kernel<TYPE, true><<<grid, kThreads, 0, s>>>(a, k, v, k_stride, v_stride, slots);
+  else
+    gather_kernel<TYPE, false><<<grid, kThreads, 0, s>>>(a, k, v, k_stride, v_stride, slots);
+}
+
+}  // namespace
+
 hipError_t launch_kv8_append(const qc_kv8_cache& c, const qc_kv8_batch& b, const void* k,
                              long long k_stride, const void* v, long long v_stride, int type,
                              int* status, hipStream_t s) {
   const Kv8Args a = kv8_args(c, b, status);
-  const int slots = touched_slots(a);
-  const unsigned grid = static_cast<unsigned>(2LL * a.kv_heads * slots * a.seqs);
   const Rows kr = {k, k_stride}, vr = {v, v_stride};
   switch (type) {
-    case QC_STORAGE_F32: append_kernel<QC_STORAGE_F32><<<grid, kThreads, 0, s>>>(a, kr, vr, slots); break;
-    case QC_STORAGE_F16: append_kernel<QC_STORAGE_F16><<<grid, kThreads, 0, s>>>(a, kr, vr, slots); break;
-    default: append_kernel<QC_STORAGE_BF16><<<grid, kThreads, 0, s>>>(a, kr, vr, slots);
+    case QC_STORAGE_F32: run_append<QC_STORAGE_F32>(a, kr, vr, s); break;
+    case QC_STORAGE_F16: run_append<QC_STORAGE_F16>(a, kr, vr, s); break;
+    default: run_append<QC_STORAGE_BF16>(a, kr, vr, s);
   }
   return hipGetLastError();
 }
@@ -259,17 +344,10 @@ hipError_t launch_kv8_gather(const qc_kv8_cache& c, const qc_kv8_batch& b, void*
                              long long k_stride, void* v, long long v_stride, int type, int* status,
                              hipStream_t s) {
   const Kv8Args a = kv8_args(c, b, status);
-  const int slots = touched_slots(a);
-  const unsigned grid = static_cast<unsigned>(2LL * a.kv_heads * slots * a.seqs);
   switch (type) {
-    case QC_STORAGE_F32:
-      gather_kernel<QC_STORAGE_F32><<<grid, kThreads, 0, s>>>(a, k, v, k_stride, v_stride, slots);
-      break;
-    case QC_STORAGE_F16:
-      gather_kernel<QC_STORAGE_F16><<<grid, kThreads, 0, s>>>(a, k, v, k_stride, v_stride, slots);
-      break;
-    default:
-      gather_kernel<QC_STORAGE_BF16><<<grid, kThreads, 0, s>>>(a, k, v, k_stride, v_stride, slots);
+    case QC_STORAGE_F32: run_gather<QC_STORAGE_F32>(a, k, v, k_stride, v_stride, s); break;
+    case QC_STORAGE_F16: run_gather<QC_STORAGE_F16>(a, k, v, k_stride, v_stride, s); break;
+    default: run_gather<QC_STORAGE_BF16>(a, k, v, k_stride, v_stride, s);
   }
   return hipGetLastError();
 }
