@@ -568,6 +568,17 @@ int qc_hip_set_cint8_dot(int mode);
  * counterpart. */
 int qc_hip_set_qgemm_fold(int mode);
 
+/* Kernels of qc_hip_kv8_attention (process-wide): 0 (default) chooses from the
+ * sizes; 1 / 2 read the cache directly for 16 or 32 rows a workgroup (head_dim above
+ * 128 with f32: always 16); 3 lays it out for MFMA tiles first.  All stay within
+ * the stated precision.  Tuning and test knob with no reference counterpart. */
+int qc_hip_set_kv8_attention_route(int route);
+
+/* Kernels of qc_hip_mxfp4_gemm (process-wide): 0 (default) chooses from the sizes;
+ * 1 = weights streamed to registers; 2 = both operands through LDS (k <= 2^24).
+ * Tuning and test knob with no reference counterpart. */
+int qc_hip_set_mxfp4_gemm_route(int route);
+
 /* on != 0: qc_hip_rms_norm_add_quant_int8 replays the element-order sum of
  * squares for every row instead of only for rows whose float norm the
  * parallel sum cannot settle (process-wide; results are identical either

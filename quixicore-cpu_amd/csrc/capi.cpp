@@ -37,6 +37,8 @@ struct Knobs {
   std::atomic<int> cint8_dot{0};
   std::atomic<int> int8_route{qc::kInt8Auto};
   std::atomic<bool> norm_sequential{false};
+  std::atomic<int> kv8_route{0};
+  std::atomic<int> mxfp4_route{0};
 };
 Knobs g_knobs;
 
@@ -932,6 +934,7 @@ int qc_hip_kv8_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, c
   r.window = std::min<long long>(window, INT_MAX / 2);
   r.scale = scale;
   r.causal = causal != 0;
+  r.route = g_knobs.kv8_route.load(std::memory_order_relaxed);
   const hipStream_t s = as_stream(stream);
   return checked(
       dev_status, s,
@@ -979,6 +982,7 @@ int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uin
       y == nullptr || !aligned16(w_codes) || !aligned16(x_codes))
     return QC_INVALID_ARGUMENT;
   return finish(qc::launch_mxfp4_gemm(w_codes, w_scales, x_codes, x_scales, y, y_type, m, n, k,
+                                      g_knobs.mxfp4_route.load(std::memory_order_relaxed),
                                       as_stream(stream)));
 }
 
@@ -1008,6 +1012,18 @@ int qc_hip_set_qgemm_fold(int mode) {
 
 int qc_hip_set_norm_sequential_sum(int on) {
   g_knobs.norm_sequential.store(on != 0, std::memory_order_relaxed);
+  return QC_OK;
+}
+
+int qc_hip_set_kv8_attention_route(int route) {
+  if (route < 0 || route > 3) return QC_INVALID_ARGUMENT;
+  g_knobs.kv8_route.store(route, std::memory_order_relaxed);
+  return QC_OK;
+}
+
+int qc_hip_set_mxfp4_gemm_route(int route) {
+  if (route < 0 || route > 2) return QC_INVALID_ARGUMENT;
+  g_knobs.mxfp4_route.store(route, std::memory_order_relaxed);
   return QC_OK;
 }
 

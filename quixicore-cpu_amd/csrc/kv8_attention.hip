@@ -49,6 +49,7 @@ struct AttnArgs {
   float* stats;         // [split][tokens * heads][2]: maximum (log2 units), sum
   int splits, chunk;    // key ranges of `chunk` tokens
   int row_blocks;
+  int route;            // host: 0 by size, 1 / 2 one or two row tiles, 3 tiled
 };
 
 // Keys [lo, hi) that rows of tokens t0..t1 (inclusive) see together.
@@ -74,6 +75,13 @@ __device__ __forceinline__ void transpose4(const uint32_t (&r)[4], uint32_t (&t)
   t[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
   t[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
   t[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+// Largest of three (fmaxf would first quiet each value that an MFMA wrote).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
 // Maximum / sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
@@ -156,10 +164,10 @@ __device__ __forceinline__ void store_n(void* out, long long at, bool vec, const
 // lane & 15 at dimension 64 c + 16 g.  V: lane loads DP / 16 bytes of its eight
 // keys at dimension (DP / 16) (lane & 15), transposed in registers.
 constexpr int kWaves = 4;
-constexpr int kMaxGroups = 512;   // 16-token groups of a range
+constexpr int kMaxGroups = 256;   // 16-key groups of a range
 
 template <int DP, int RT, int TYPE>
-__global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnArgs p) {
+__global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STORAGE_F32 ? 4 : 1) void attention_direct(Kv8Args a, AttnArgs p) {
   constexpr int KC = DP / 64;                     // 16-byte chunks of a key a lane holds
   constexpr int KS = DP / 32;                     // MFMAs of 32 dimensions
   constexpr int VB = DP / 16;                     // bytes of a value a lane holds
@@ -173,12 +181,12 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
   const int lane = threadIdx.x & 63, row16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // split fastest, then row block, key head, sequence
-  long long id = blockIdx.x;
-  const int split = static_cast<int>(id % p.splits);
+  int id = blockIdx.x;
+  const int split = id % p.splits;
   id /= p.splits;
-  const int rb = static_cast<int>(id % p.row_blocks);
+  const int rb = id % p.row_blocks;
   id /= p.row_blocks;
-  const int kvh = static_cast<int>(id % a.kv_heads), seq = static_cast<int>(id / a.kv_heads);
+  const int kvh = id % a.kv_heads, seq = id / a.kv_heads;
   Unit u;
   if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return;
   const int r0 = rb * RT * 16, r1 = min(r0 + RT * 16, u.rows * p.group);
@@ -186,26 +194,82 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
   int lo, hi;
   seen_range(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
   const int base = lo & ~31;
-  const int from = base + split * p.chunk, to = min(hi, from + p.chunk);   // from: multiple of 32
+  const int from = __builtin_amdgcn_readfirstlane(base + split * p.chunk);   // a multiple of 32
+  const int to = __builtin_amdgcn_readfirstlane(min(hi, from + p.chunk));
+  const int groups = max(0, (to - from + 15) >> 4);
+  const int* table = a.table + static_cast<long long>(seq) * a.columns;
+  // the page of 16 keys, -1 where no row sees one of them; ids out of range are told apart below
+  auto page_of = [&](int tok) { return tok < to && tok + 15 >= lo ? table[tok >> a.page_shift] : -1; };
+
+  // Codes of 32 keys from tok.  A group without a page reads page 0 and counts for nothing,
+  // lanes past head_dim read dimension 0: q is zero there, and sums there are not stored.
+  u32x4 kr[2][KC];
+  uint32_t vr8[8][VW];
+  const int k_lane = row16 * a.head_dim + (16 * g < a.head_dim ? 16 * g : 0);
+  const int v_lane = 4 * g * a.head_dim + (VB * row16 < a.head_dim ? VB * row16 : 0);
+  int k_off[KC];
+#pragma unroll
+  for (int c = 0; c < KC; ++c) k_off[c] = 64 * c + 16 * g < a.head_dim ? 64 * c : 0;
+  auto code_at = [&](int tok, int id) {
+    id = __builtin_amdgcn_readfirstlane(id);
+    const int page = static_cast<unsigned>(id) < static_cast<unsigned>(a.pages) ? id : 0;
+    return ((static_cast<long long>(page) * a.kv_heads + kvh) * a.page_tokens + (tok & (a.page_tokens - 1))) * a.head_dim;
+  };
+  auto load_k = [&](long long at0, long long at1) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int8_t* kp = a.k_codes + (t ? at1 : at0);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kr[t][c] = *reinterpret_cast<const u32x4*>(kp + k_lane + k_off[c]);
+    }
+  };
+  auto load_v = [&](long long at0, long long at1) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int8_t* vp = a.v_codes + (t ? at1 : at0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int8_t* q = vp + v_lane + e * a.head_dim;
+        if constexpr (VW == 1) {
+          vr8[4 * t + e][0] = *reinterpret_cast<const uint32_t*>(q);
+        } else if constexpr (VW == 2) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(q);
+          vr8[4 * t + e][0] = x[0];
+          vr8[4 * t + e][1] = x[1];
+        } else {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(q);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) vr8[4 * t + e][w] = x[w];
+        }
+      }
+    }
+  };
+  // the wave's first keys are on their way before anything is waited for
+  const int stride = 32 * kWaves, tok0 = from + 32 * wave;
+  if (tok0 < to) {
+    const long long at0 = code_at(tok0, page_of(tok0)), at1 = code_at(tok0 + 16, page_of(tok0 + 16));
+    load_k(at0, at1);
+    load_v(at0, at1);
+  }
 
   // page ids and scales of the range's groups of 16 keys, and the largest value scale
-  const int groups = max(0, (to - from + 15) >> 4);
   float unit = 0.f;
   for (int i = threadIdx.x; i < groups; i += 64 * kWaves) {
-    const int tok = from + 16 * i;
-    int page = tok + 15 < lo ? -1 : a.table[static_cast<long long>(seq) * a.columns + (tok >> a.page_shift)];
+    int page = page_of(from + 16 * i);
     float ks = 0.f, vs = 0.f;
-    bool ok = false;
-    if (static_cast<unsigned>(page) < static_cast<unsigned>(a.pages)) {
-      const long long at = static_cast<long long>(page) * a.kv_heads + kvh;
-      ks = a.k_scales[at];
-      vs = a.v_scales[at];
-      ok = isfinite(ks) && isfinite(vs);
-    }
-    if (!ok) {
-      if (tok + 15 >= lo) *a.status = QC_INVALID_ARGUMENT;
-      page = -1;
-      ks = vs = 0.f;
+    if (from + 16 * i + 15 >= lo) {
+      bool ok = false;
+      if (static_cast<unsigned>(page) < static_cast<unsigned>(a.pages)) {
+        const long long at = static_cast<long long>(page) * a.kv_heads + kvh;
+        ks = a.k_scales[at];
+        vs = a.v_scales[at];
+        ok = isfinite(ks) && isfinite(vs);
+      }
+      if (!ok) {
+        *a.status = QC_INVALID_ARGUMENT;
+        page = -1;
+        ks = vs = 0.f;
+      }
     }
     s_page[i] = page;
     s_ks[i] = ks;
@@ -232,12 +296,14 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
     for (int s = 0; s < KS; ++s) {
       const int d = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
       load8<TYPE>(p.q, at + d, has && d < a.head_dim, p.vec, v[s]);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         top = fmaxf(top, fabsf(v[s][j]));
         nan = nan || v[s][j] != v[s][j];
       }
-    }
     if (nan) top = INFINITY;
     top = lanes16_max(top);
     float inverse;
@@ -254,8 +320,13 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
     row_hi[t] = has ? (p.causal ? min(u.kv, u.position(token) + 1) : u.kv) : 0;
     row_lo[t] = p.window > 0 ? u.position(token) + 1 - p.window : 0;
   }
+  // keys that every row of the block sees (its rows past r1 count for nothing whatever they see)
+  int all_hi = hi, all_lo = lo;
+  if (p.causal) all_hi = min(u.kv, u.position(r0 / p.group) + 1);
+  if (p.window > 0) all_lo = u.position((r1 - 1) / p.group) + 1 - p.window;
   __syncthreads();
-  unit = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) unit = fmaxf(unit, s_red[w]);
   // probabilities enter the second product as p * (value scale / unit) * 2^15
   const float per_unit = unit > 0.f ? 32768.0f / unit : 0.f;
 
@@ -269,51 +340,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
     for (int k = 0; k < VB; ++k) acc[t][k] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  struct Raw {
-    u32x4 k[2][KC];
-    uint32_t v[8][VW];
-  };
-  const long long page_bytes = static_cast<long long>(a.kv_heads) * a.page_tokens * a.head_dim;
-  const long long head_bytes = static_cast<long long>(kvh) * a.page_tokens * a.head_dim;
-  auto load = [&](int tok, Raw& r) {              // 32 keys from tok
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int i = (tok - from) / 16 + t;
-      const int page = i < groups ? __builtin_amdgcn_readfirstlane(s_page[i < groups ? i : 0]) : -1;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) r.k[t][c] = u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int w = 0; w < VW; ++w) r.v[4 * t + e][w] = 0;
-      if (page < 0) continue;
-      const int slot = (tok + 16 * t) & (a.page_tokens - 1);
-      const long long at = page * page_bytes + head_bytes + static_cast<long long>(slot) * a.head_dim;
-      const int8_t* kp = a.k_codes + at + row16 * a.head_dim + 16 * g;
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-        if (64 * c + 16 * g < a.head_dim) r.k[t][c] = *reinterpret_cast<const u32x4*>(kp + 64 * c);
-      const int8_t* vp = a.v_codes + at + 4 * g * a.head_dim + VB * row16;
-      if (VB * row16 < a.head_dim) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int8_t* q = vp + e * a.head_dim;
-          if constexpr (VW == 1) {
-            r.v[4 * t + e][0] = *reinterpret_cast<const uint32_t*>(q);
-          } else if constexpr (VW == 2) {
-            const u32x2 x = *reinterpret_cast<const u32x2*>(q);
-            r.v[4 * t + e][0] = x[0];
-            r.v[4 * t + e][1] = x[1];
-          } else {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(q);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) r.v[4 * t + e][w] = x[w];
-          }
-        }
-      }
-    }
-  };
-  auto compute = [&](int tok, const Raw& r) {
+  for (int tok = tok0; tok < to; tok += stride) {
     f32x4 s[RT][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -322,8 +349,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         uint32_t w[4];
-        bytes_to_f16(r.k[t][ks >> 1][2 * (ks & 1)], w[0], w[1]);
-        bytes_to_f16(r.k[t][ks >> 1][2 * (ks & 1) + 1], w[2], w[3]);
+        bytes_to_f16(kr[t][ks >> 1][2 * (ks & 1)], w[0], w[1]);
+        bytes_to_f16(kr[t][ks >> 1][2 * (ks & 1) + 1], w[2], w[3]);
         const f16x8 kf = __builtin_bit_cast(f16x8, u32x4{w[0], w[1], w[2], w[3]});
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -334,27 +361,43 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
     }
     const int i = (tok - from) / 16;
     const int i1 = min(i + 1, groups - 1);
+    // the next step's keys take the registers of these
+    const bool more = tok + stride < to;
+    long long at0 = 0, at1 = 0;
+    if (more) {
+      const int n = i + stride / 16;
+      at0 = code_at(tok + stride, s_page[n]);
+      at1 = code_at(tok + stride + 16, n + 1 < groups ? s_page[n + 1] : -1);
+      load_k(at0, at1);
+    }
     const float ks[2] = {s_ks[i], s_ks[i1]};
     const float vr[2] = {s_vs[i] * per_unit, s_vs[i1] * per_unit};
-    const bool page_ok[2] = {s_page[i] >= 0, s_page[i1] >= 0};
+    const int page[2] = {s_page[i], s_page[i1]};
+    const bool whole = __builtin_amdgcn_readfirstlane(tok >= all_lo && tok + 32 <= all_hi && tok + 32 <= to &&
+                                                      page[0] >= 0 && page[1] >= 0);
     f16x8 pf[RT][NQ];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float z[8], top = -INFINITY;
+      float z[8];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t) {
+        const float c = ks[t] * factor[rt];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = tok + 16 * t + 4 * g + e;
-          const bool see = j >= row_lo[rt] && j < row_hi[rt] && page_ok[t];
-          z[4 * t + e] = see ? s[rt][t][e] * (ks[t] * factor[rt]) : -INFINITY;
-          top = fmaxf(top, z[4 * t + e]);
+        for (int e = 0; e < 4; ++e) z[4 * t + e] = s[rt][t][e] * c;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = tok + 16 * (e >> 2) + 4 * g + (e & 3);
+          if (j < row_lo[rt] || j >= row_hi[rt] || page[e >> 2] < 0) z[e] = -INFINITY;
         }
+      }
+      float top = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7])));
       top = lanes16_max(top);
       const float mn = fmaxf(m[rt], top);
       const float ref = mn == -INFINITY ? 0.f : mn;   // nothing seen yet: all terms are 0
       if (__any(mn != m[rt])) {
-        const float alpha = exp2f(m[rt] - ref);
+        const float alpha = __builtin_amdgcn_exp2f(m[rt] - ref);
         l[rt] *= alpha;
 #pragma unroll
         for (int k = 0; k < VB; ++k)
@@ -364,7 +407,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float pe = exp2f(z[e] - ref);
+        const float pe = __builtin_amdgcn_exp2f(z[e] - ref);
         l[rt] += pe;
         const float pv = pe * vr[e >> 2];
         pf[rt][0][e] = static_cast<_Float16>(pv);
@@ -377,7 +420,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[t][e] = r.v[4 * t + e][w];
+        for (int e = 0; e < 4; ++e) x[t][e] = vr8[4 * t + e][w];
         transpose4(x[t], y[t]);
       }
 #pragma unroll
@@ -393,21 +436,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
             acc[rt][4 * w + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][q], acc[rt][4 * w + c], 0, 0, 0);
       }
     }
-  };
-  {
-    const int stride = 32 * kWaves;
-    int tok = from + 32 * wave;
-    if (tok < to) {
-      Raw cur;
-      load(tok, cur);
-      for (; tok + stride < to; tok += stride) {
-        Raw next;
-        load(tok + stride, next);
-        compute(tok, cur);
-        cur = next;
-      }
-      compute(tok, cur);
-    }
+    if (more) load_v(at0, at1);
   }
 
   // join the waves: the common maximum, then the sums pairwise in a fixed order
@@ -426,14 +455,15 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) all = fmaxf(all, s_m[w][16 * t + row16]);
     const float ref = all == -INFINITY ? 0.f : all;
-    const float mine = exp2f(m[t] - ref);
+    const float mine = __builtin_amdgcn_exp2f(m[t] - ref);
 #pragma unroll
     for (int k = 0; k < VB; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[t][k][e] *= mine;
     l[t] = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) l[t] += s_l[w][16 * t + row16] * exp2f(s_m[w][16 * t + row16] - ref);
+    for (int w = 0; w < kWaves; ++w)
+      l[t] += s_l[w][16 * t + row16] * __builtin_amdgcn_exp2f(s_m[w][16 * t + row16] - ref);
     m[t] = all;
   }
 #pragma unroll
@@ -451,7 +481,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
 #pragma unroll
         for (int k = 0; k < VB; ++k) acc[t][k] += s_o[wave][t][k][lane];
     }
-    __syncthreads();
+    if (half > 1) __syncthreads();
   }
   if (wave > 0) return;
   const float back = unit * (1.0f / 32768.0f);
@@ -497,6 +527,14 @@ __global__ __launch_bounds__(64 * kWaves) void attention_direct(Kv8Args a, AttnA
 // holds in registers 8 k + j, so its probabilities are its operand of O^T = V^T P^T.
 // Beside them the magnitudes of the key and value scales of each 16 keys (a negative scale
 // turns its codes' signs); a key scale of -1 marks a group without a page.
+// Workgroup barrier after which what the waves have read from LDS may be overwritten.
+__device__ __forceinline__ void ring_sync() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));   // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 struct Frags {
   _Float16* k;           // [units][cap / 32][DP / 16][512]
   _Float16* v;           // [units][cap / 32][DP / 32][2][512]
@@ -584,21 +622,35 @@ __global__ __launch_bounds__(256) void attention_layout(Kv8Args a, Frags f, int 
   }
 }
 
-// Workgroup: NW waves of 32 rows of a key head, a range of keys.  A step is 64 keys,
-// its fragments copied to one of two LDS buffers while the other is used.  A score's
-// exponent is one fused multiply-add: with c the key scale times the row's factor and b =
-// log2(value scale / largest one) + 15 per 16 keys, p' = 2^(s c + b - m) is the
-// probability as it meets the codes of V, and the sum takes p' 2^-b.
+// Workgroup: NW waves of 32 rows of a key head, a range of keys.  A step is 64 keys.
+// A score's exponent is one fused multiply-add: with c the key scale times the row's
+// factor and b = log2(value scale / largest one) + shift per 16 keys, p' = 2^(s c + b - m)
+// is the probability as it meets the codes of V, and the sum takes p' 2^-b.  For 16-bit q
+// the shift is 11, and m follows the running maximum only once that is 4 above it (p' <= 2^15
+// fits f16): of random rows, some maximum among 32 grows in most steps, and each growth
+// rescales all sums.  p' keeps its 11 bits down to 2^-25 of the row's largest that way (with 7
+// and 8, to 2^-21: a row whose largest meets a code of 0 showed it); f32 q, whose second
+// term is 2^-11 smaller, takes 15 and 0.
+//
+// The exponentials of a step and its 32 MFMAs take about the same time, so they have to
+// run beside each other, and waves that meet at a barrier every step do the same thing at
+// the same time: a wave's own stream mixes them.  It computes the scores of step t + 1
+// while step t's exponentials and value products go on, so K is a step ahead of V in the S
+// LDS buffers each has.
+constexpr int kTiledGroups = 1024;   // 16-key groups of a range
+
 template <int DP, int NW, int TYPE>
 __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, AttnArgs p, Frags f) {
   constexpr int NF = DP / 16, DT = DP / 32;
   constexpr int NQ = TYPE == QC_STORAGE_F32 ? 2 : 1;
-  constexpr int kFragBytes = 2 * NF * 1024;       // 64 keys of K, or of V
-  constexpr int kStage = 2 * kFragBytes;
-  constexpr int LOADS = kStage / 1024 / NW;       // a wave's loads of 1 KB a step
-  static_assert(kStage % (1024 * NW) == 0, "whole loads");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+  constexpr int kBytes = 2 * NF * 1024;           // 64 keys of K, or of V
+  constexpr int LOADS = kBytes / 1024 / NW;       // a wave's loads of 1 KB of either a step
+  constexpr int S = 2;                            // buffers (three: 582 -> 605 us)
+  static_assert(kBytes % (1024 * NW) == 0, "whole loads");
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k[S * kBytes], s_v[S * kBytes];
+  __shared__ f32x4 s_c[kTiledGroups / 4], s_b[kTiledGroups / 4], s_inv[kTiledGroups / 4];
   __shared__ float s_unit[NW];
+  __shared__ int s_bad[NW];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -618,30 +670,49 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   if (r0 >= r1) return;
   int lo, hi;
   seen_range(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
-  const int from = (lo & ~63) + split * p.chunk, to = min(hi, from + p.chunk);
+  const int from = __builtin_amdgcn_readfirstlane((lo & ~63) + split * p.chunk);
+  const int to = __builtin_amdgcn_readfirstlane(min(hi, from + p.chunk));
   const int steps = to > from ? (to - from + 63) >> 6 : 0;
 
-  const _Float16* kf = f.k + (static_cast<long long>(local) * (f.cap / 32) + from / 32) * NF * 512;
-  const _Float16* vf = f.v + (static_cast<long long>(local) * (f.cap / 32) + from / 32) * NF * 512;
-  const float* ks = f.ks + static_cast<long long>(local) * (f.cap / 16) + from / 16;
-  const float* vs = f.vs + static_cast<long long>(local) * (f.cap / 16) + from / 16;
-  auto issue = [&](int step, int buf) {
+  const long long tile0 = static_cast<long long>(local) * (f.cap / 32) + from / 32;
+  const _Float16* kf = f.k + tile0 * NF * 512;
+  const _Float16* vf = f.v + tile0 * NF * 512;
+  // Loads of steps past the last repeat it, into buffers that are not read again, so that
+  // the number in flight is the same in every step.
+  auto issue = [&](const _Float16* src, uint8_t* buffer, int step) {
+    const _Float16* from_step = src + static_cast<long long>(min(step, steps - 1)) * 2 * NF * 512;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int q = wave * LOADS + i;             // uniform
-      const _Float16* src = q < 2 * NF ? kf + (static_cast<long long>(step) * 2 * NF + q) * 512
-                                       : vf + (static_cast<long long>(step) * 2 * NF + q - 2 * NF) * 512;
-      dma16(src, 16 * lane, lds + buf * kStage + q * 1024);
+      dma16(from_step + q * 512, 16 * lane, buffer + q * 1024);
     }
   };
-  if (steps > 0) issue(0, 0);
+  if (steps > 0) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      issue(kf, s_k + i * kBytes, i);
+      if (i < S - 1) issue(vf, s_v + i * kBytes, i);
+    }
+  }
 
-  // the range's largest value scale
+  // the range's key scales, and its value scales against the largest
+  constexpr float kLow = -3.0e38f;                // below every score
+  constexpr float kShift = NQ == 2 ? 15.f : 11.f, kSlack = 15.f - kShift;
+  const float* ks = f.ks + static_cast<long long>(local) * (f.cap / 16) + from / 16;
+  const float* vs = f.vs + static_cast<long long>(local) * (f.cap / 16) + from / 16;
   float unit = 0.f;
-  for (int i = threadIdx.x; i < 4 * steps; i += 64 * NW) unit = fmaxf(unit, vs[i]);
+  bool bad = false;
+  for (int i = threadIdx.x; i < 4 * steps; i += 64 * NW) {
+    unit = fmaxf(unit, vs[i]);
+    bad = bad || (ks[i] < 0.f && from + 16 * i < to && from + 16 * i + 15 >= lo);   // a page missing
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor(unit, o));
-  if (lane == 0) s_unit[wave] = unit;
+  bad = __any(bad);
+  if (lane == 0) {
+    s_unit[wave] = unit;
+    s_bad[wave] = bad;
+  }
 
   // q: row lane & 31, dimensions 16 s + 8 half + j
   f16x8 qf[NF][NQ];
@@ -659,12 +730,14 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
     for (int s = 0; s < NF; ++s) {
       const int d = 16 * s + 8 * half;
       load8<TYPE>(p.q, at + d, has && d < a.head_dim, p.vec, v[s]);
+    }
+#pragma unroll
+    for (int s = 0; s < NF; ++s)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         top = fmaxf(top, fabsf(v[s][j]));
         nan = nan || v[s][j] != v[s][j];
       }
-    }
     if (nan) top = INFINITY;
     top = fmaxf(top, __shfl_xor(top, 32));
     float inverse;
@@ -697,72 +770,89 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   any_hi = __builtin_amdgcn_readfirstlane(any_hi);
   all_lo = __builtin_amdgcn_readfirstlane(all_lo);
   __syncthreads();
+  int any_bad = 0;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) unit = fmaxf(unit, s_unit[w]);
-  const float log_unit = unit > 0.f ? __log2f(unit) : 0.f;
+  for (int w = 0; w < NW; ++w) {
+    unit = fmaxf(unit, s_unit[w]);
+    any_bad |= s_bad[w];
+  }
+  any_bad = __builtin_amdgcn_readfirstlane(any_bad);
+  for (int i = threadIdx.x; i < 4 * steps; i += 64 * NW) {
+    // a scale of 0 has codes of 0, so any b will do for it
+    const float b = kShift + (vs[i] > 0.f ? fmaxf(__log2f(vs[i] / unit), -100.f) : 0.f);
+    reinterpret_cast<float*>(s_c)[i] = ks[i];
+    reinterpret_cast<float*>(s_b)[i] = b;
+    reinterpret_cast<float*>(s_inv)[i] = __builtin_amdgcn_exp2f(-b);
+  }
 
-  constexpr float kLow = -3.0e38f;                // below every score
   float m = kLow, l = 0.f;
-  f32x16 acc[DT];
+  f32x16 acc[DT], s[2], sn[2];
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
+  // quarter i of a step's score products: key tile i / 2, one half of the dimensions
+  auto scores = [&](const uint8_t* kb, int i, f32x16 (&o)[2]) {
+    const int t = i >> 1;
+    if ((i & 1) == 0) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
+    }
+#pragma unroll
+    for (int d = (i & 1) * NF / 2; d < ((i & 1) + 1) * NF / 2; ++d) {
+      const f16x8 k = *reinterpret_cast<const f16x8*>(kb + (t * NF + d) * 1024);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[d][q], o[t], 0, 0, 0);
+    }
+  };
+  if (steps > 0) wait_vmcnt<2 * (S - 1) * LOADS>();   // K of step 0
+  __syncthreads();
+  if (steps > 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) scores(s_k + 16 * lane, i, s);
+  }
 
-  for (int step = 0; step < steps; ++step) {
-    const int buf = step & 1, tok = from + 64 * step;
-    wait_vmcnt<0>();                              // this wave's loads of the step
-    __syncthreads();                              // everyone's; the other buffer is free
-    if (step + 1 < steps) issue(step + 1, buf ^ 1);
-    if (tok >= any_hi) continue;
-    float c[4], b[4], inv[4];
-    bool whole = tok >= all_lo && tok + 64 <= all_hi;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float k = ks[4 * step + i], v = vs[4 * step + i];
-      whole = whole && k >= 0.f;
-      c[i] = fmaxf(k * factor, 1e-37f);           // above 0: masked scores are -inf
-      const float r = v > 0.f ? fmaxf(__log2f(v) - log_unit, -100.f) : 0.f;
-      b[i] = r + 15.f;
-      inv[i] = __builtin_amdgcn_exp2f(-b[i]);
-    }
-    const uint8_t* kb = lds + buf * kStage + 16 * lane;
-    f32x16 s[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
-#pragma unroll
-      for (int d = 0; d < NF; ++d) {
-        const f16x8 k = *reinterpret_cast<const f16x8*>(kb + (t * NF + d) * 1024);
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[d][q], s[t], 0, 0, 0);
-      }
-    }
-    if (!whole) {
+  int kbuf = 0, vbuf = 0;                         // buffers of K and V of the step
+  // s: the step's scores; sn: receives the next one's
+  auto run = [&](int step, f32x16 (&s)[2], f32x16 (&sn)[2]) {
+    const int tok = from + 64 * step;
+    wait_vmcnt<2 * (S - 2) * LOADS>();            // this wave's loads of V of the step, K of the next
+    ring_sync();                                  // everyone's; V of the step before, K of this are free
+    const int vfree = vbuf > 0 ? vbuf - 1 : S - 1;
+    issue(vf, s_v + vfree * kBytes, step + S - 1);
+    issue(kf, s_k + kbuf * kBytes, step + S);
+    kbuf = kbuf + 1 < S ? kbuf + 1 : 0;
+    const uint8_t* vb = s_v + vbuf * kBytes + 16 * lane;
+    const uint8_t* kb = s_k + kbuf * kBytes + 16 * lane;   // of the next step
+    vbuf = vbuf + 1 < S ? vbuf + 1 : 0;
+    if (tok >= any_hi) return;                    // none of the wave's rows sees more
+    f32x4 c = s_c[step];
+    const f32x4 b = s_b[step], inv = s_inv[step];
+    if (any_bad || tok < all_lo || tok + 64 > all_hi) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int j = tok + 32 * t + 8 * (e >> 2) + 4 * half + (e & 3);
-          if (j < row_lo || j >= row_hi || ks[4 * step + 2 * t + (e >> 3)] < 0.f) s[t][e] = -INFINITY;
+          if (j < row_lo || j >= row_hi || c[2 * t + (e >> 3)] < 0.f) s[t][e] = -INFINITY;
         }
     }
     float top = kLow;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      c[i] = fmaxf(c[i] * factor, 1e-37f);        // above 0: masked scores stay -inf
       const f32x16& x = s[i >> 1];
       const int o = 8 * (i & 1);
-      const float g = fmaxf(fmaxf(fmaxf(x[o], x[o + 1]), fmaxf(x[o + 2], x[o + 3])),
-                            fmaxf(fmaxf(x[o + 4], x[o + 5]), fmaxf(x[o + 6], x[o + 7])));
+      const float g = max3(max3(x[o], x[o + 1], x[o + 2]), max3(x[o + 3], x[o + 4], x[o + 5]),
+                           max3(x[o + 6], x[o + 7], x[o + 7]));
       top = fmaxf(top, g * c[i]);
     }
     {
       auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       top = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
     }
-    const float mn = fmaxf(m, top);
-    if (__any(mn != m)) {
+    if (__any(top > m + kSlack)) {
+      const float mn = fmaxf(m, top);
       const float alpha = __builtin_amdgcn_exp2f(m - mn);
       l *= alpha;
 #pragma unroll
@@ -771,23 +861,22 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
         for (int e = 0; e < 16; ++e) acc[t][e] *= alpha;
       m = mn;
     }
-    const uint8_t* vb = lds + buf * kStage + kFragBytes + 16 * lane;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      scores(kb, i, sn);                          // past the last step: of no use, and not used
       const float off = b[i] - m;
-      float sum = 0.f, e8[8];
+      float e8[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        e8[j] = __builtin_amdgcn_exp2f(fmaf(s[i >> 1][8 * (i & 1) + j], c[i], off));
-        sum += e8[j];
-      }
-      l = fmaf(sum, inv[i], l);
+      for (int j = 0; j < 8; ++j) e8[j] = __builtin_amdgcn_exp2f(fmaf(s[i >> 1][8 * (i & 1) + j], c[i], off));
       f16x8 pf[NQ];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         pf[0][j] = static_cast<_Float16>(e8[j]);
         if constexpr (NQ == 2) pf[1][j] = static_cast<_Float16>(e8[j] - static_cast<float>(pf[0][j]));
       }
+      // (an f16 dot for the sum would lose the probabilities that are subnormal there)
+      const float sum = ((e8[0] + e8[1]) + (e8[2] + e8[3])) + ((e8[4] + e8[5]) + (e8[6] + e8[7]));
+      l = fmaf(sum, inv[i], l);
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
         const f16x8 v = *reinterpret_cast<const f16x8*>(vb + ((i >> 1) * NF + 2 * t + (i & 1)) * 1024);
@@ -795,11 +884,16 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
         for (int q = 0; q < NQ; ++q) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[q], acc[t], 0, 0, 0);
       }
     }
+  };
+  for (int step = 0; step < steps; step += 2) {
+    run(step, s, sn);
+    if (step + 1 < steps) run(step + 1, sn, s);
   }
+  wait_vmcnt<0>();   // no load may land in LDS that is no longer this workgroup's
   l += __shfl_xor(l, 32);
   if (!has) return;
   const bool last = p.splits == 1;
-  const float back = unit * (1.0f / 32768.0f) + broken;
+  const float back = unit * (NQ == 2 ? 1.0f / 32768.0f : 1.0f / 2048.0f) + broken;   // 2^-kShift
   const float scale = last ? (l == 0.f ? 0.f : back / l) : back;
   const long long row = static_cast<long long>(u.first + token) * p.heads + head;
   const long long part = static_cast<long long>(split) * a.tokens * p.heads + row;
@@ -828,42 +922,117 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
 }
 
 // out = sum over the ranges of 2^(m_s - m) O_s over that of 2^(m_s - m) l_s: a
-// wavefront a row.
+// workgroup a row.  256 / L groups of L threads (L >= head_dim / 4, a power of two) take the
+// ranges in turn, four loads ahead, and meet in LDS in a fixed order.  (A wavefront a
+// row, its ranges one after the other: 128 ranges of 32 rows 30 us, 5 so.)
 template <int TYPE>
-__global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p) {
-  const int lane = threadIdx.x & 63;
-  const long long item = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const long long per_seq = static_cast<long long>(a.max_new) * p.heads;
-  const int seq = static_cast<int>(item / per_seq);
-  if (seq >= a.seqs) return;
-  const int rest = static_cast<int>(item - seq * per_seq);
+__global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p, int shift) {
+  __shared__ float s_w[256], s_red[8];
+  __shared__ f32x4 s_o[256];
+  const int tid = threadIdx.x;
+  const unsigned item = blockIdx.x, per_seq = static_cast<unsigned>(a.max_new) * p.heads;
+  const int seq = item / per_seq;
+  const int rest = item - seq * per_seq;
   const int token = rest / p.heads, head = rest - token * p.heads;
   Unit u;
   if (!kv8_sequence(a, seq, u.first, u.rows, u.kv) || token >= u.rows) return;
   const long long rows = static_cast<long long>(a.tokens) * p.heads;
   const long long row = static_cast<long long>(u.first + token) * p.heads + head;
-  float m = -INFINITY, l = 0.f;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.stats[2 * (s * rows + row)]);
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const float* stats = p.stats + 2 * row;
+  float m = -INFINITY;
+  for (int s = tid; s < p.splits; s += 256) m = fmaxf(m, stats[2 * s * rows]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if ((tid & 63) == 0) s_red[tid >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
   const float ref = m == -INFINITY ? 0.f : m;
-  for (int s = 0; s < p.splits; ++s) {
-    const float ms = p.stats[2 * (s * rows + row)], ls = p.stats[2 * (s * rows + row) + 1];
-    if (ms == -INFINITY && ls == 0.f) continue;   // saw no key (a row that is not finite has a sum of NaN)
-    const float f = exp2f(ms - ref);
-    l += f * ls;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = lane + 64 * e;
-      if (d < a.head_dim) v[e] += f * p.part[(s * rows + row) * a.head_dim + d];
+  const int group = tid >> shift, groups = 256 >> shift, d = 4 * (tid & ((1 << shift) - 1));
+  float l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < p.splits; s0 += 256) {
+    float w = 0.f;
+    const int n = min(256, p.splits - s0);
+    if (tid < n) {
+      const float ls = stats[2 * (s0 + tid) * rows + 1];
+      // a range with no key the row sees has no sums (one of a row that is not finite has a
+      // sum of NaN): -1 marks it
+      w = ls == 0.f ? -1.f : __builtin_amdgcn_exp2f(stats[2 * (s0 + tid) * rows] - ref);
+      if (ls != 0.f) l = fmaf(w, ls, l);
     }
-  }
-  typedef typename Storage<TYPE>::raw raw;
-  raw* out = static_cast<raw*>(p.out) + (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim;
+    s_w[tid] = w;
+    __syncthreads();
+    if (d < a.head_dim) {
+      const float* o = p.part + (s0 * rows + row) * a.head_dim + d;
+#pragma unroll 4
+      for (int s = group; s < n; s += groups) {
+        const float f = s_w[s];
+        if (f == -1.f) continue;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(o + s * rows * a.head_dim);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int d = lane + 64 * e;
-    if (d < a.head_dim) out[d] = encode<TYPE>(l == 0.f ? 0.f : v[e] / l);
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, x[e], acc[e]);
+      }
+    }
+    __syncthreads();
   }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  if ((tid & 63) == 0) s_red[4 + (tid >> 6)] = l;
+  s_o[tid] = acc;
+  __syncthreads();
+  if (group > 0 || d >= a.head_dim) return;
+  for (int g = 1; g < groups; ++g) acc += s_o[(g << shift) + tid];
+  l = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = l == 0.f ? 0.f : acc[e] / l;
+  store_n<TYPE, 4>(p.out, (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim + d, p.vec, v);
+}
+
+// The same for a few ranges: L threads a row, each through all of them.  Prompts split in
+// two or four have thousands of rows, and a workgroup for each is mostly its own start.
+constexpr int kFewSplits = 8;
+template <int TYPE>
+__global__ __launch_bounds__(256) void attention_join_few(Kv8Args a, AttnArgs p, int shift) {
+  const unsigned item = (blockIdx.x * 256 + threadIdx.x) >> shift, per_seq = static_cast<unsigned>(a.max_new) * p.heads;
+  const int seq = item / per_seq;
+  if (seq >= a.seqs) return;
+  const int rest = item - seq * per_seq;
+  const int token = rest / p.heads, head = rest - token * p.heads;
+  const int d = 4 * (threadIdx.x & ((1 << shift) - 1));
+  Unit u;
+  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv) || token >= u.rows || d >= a.head_dim) return;
+  const long long rows = static_cast<long long>(a.tokens) * p.heads;
+  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
+  float ms[kFewSplits], ls[kFewSplits], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    ms[s] = -INFINITY;
+    ls[s] = 0.f;
+    if (s < p.splits) {
+      ms[s] = p.stats[2 * (s * rows + row)];
+      ls[s] = p.stats[2 * (s * rows + row) + 1];
+    }
+    m = fmaxf(m, ms[s]);
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  f32x4 x[kFewSplits], acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (ls[s] != 0.f) x[s] = *reinterpret_cast<const f32x4*>(p.part + (s * rows + row) * a.head_dim + d);
+  }
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    const float w = __builtin_amdgcn_exp2f(ms[s] - ref);
+    l = fmaf(w, ls[s], l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, x[s][e], acc[e]);
+  }
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = l == 0.f ? 0.f : acc[e] / l;
+  store_n<TYPE, 4>(p.out, (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim + d, p.vec, v);
 }
 
 // A call's partial sums where its keys are split.
@@ -879,7 +1048,15 @@ hipError_t part_buffers(const Kv8Args& a, AttnArgs& p, StreamWorkspace* ws, hipS
 template <int TYPE>
 hipError_t run_join(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
   const long long items = static_cast<long long>(a.seqs) * a.max_new * p.heads;
-  attention_join<TYPE><<<static_cast<unsigned>((items + 3) / 4), 256, 0, s>>>(a, p);
+  int shift = 2;
+  while ((4 << shift) < a.head_dim) ++shift;
+  if (items > (INT_MAX >> shift)) return hipErrorInvalidValue;
+  if (p.splits <= kFewSplits) {
+    const unsigned grid = static_cast<unsigned>(((items << shift) + 255) / 256);
+    attention_join_few<TYPE><<<grid, 256, 0, s>>>(a, p, shift);
+    return hipGetLastError();
+  }
+  attention_join<TYPE><<<static_cast<unsigned>(items), 256, 0, s>>>(a, p, shift);
   return hipGetLastError();
 }
 
@@ -895,7 +1072,7 @@ hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   p.row_blocks = static_cast<int>((rows + RT * 16 - 1) / (RT * 16));
   const long long span = key_span(a, p, RT * 16, 32);
   const long long units = static_cast<long long>(a.seqs) * a.kv_heads * p.row_blocks;
-  const long long want = std::max<long long>(1, 4LL * device_cu_count() / units);
+  const long long want = std::max<long long>(1, 2LL * device_cu_count() / units);
   long long chunk = (span + want - 1) / want;
   chunk = std::max<long long>(32 * kWaves, (chunk + 31) / 32 * 32);
   chunk = std::min<long long>(chunk, 16 * kMaxGroups);
@@ -928,7 +1105,8 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   const long long units = static_cast<long long>(a.seqs) * a.kv_heads;
   const long long want = std::max<long long>(1, device_cu_count() / (units * p.row_blocks));
   long long chunk = ((span + want - 1) / want + 63) / 64 * 64;
-  chunk = std::max<long long>(chunk, 512);
+  chunk = std::max<long long>(chunk, 1024);
+  chunk = std::min<long long>(chunk, 16 * kTiledGroups);
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((span + chunk - 1) / chunk);
   Frags f = {};
@@ -959,12 +1137,30 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   return p.splits > 1 ? run_join<TYPE>(a, p, s) : hipSuccess;
 }
 
+// The tiled form lays the cache out first (and reads 64 keys for 256 rows at a time), so it
+// takes prompts: 2048 rows a key head or more, and 2^24 pairs of a row and a key it
+// sees, counted in heads of 128.  us, direct / tiled, 8 key heads of 128, bf16, new tokens of
+// all: 512 of 512 19 / 28, 1024 of 1024 (2^24) 49 / 44, 256 of 4096 (1024 rows) 48 / 48, 1024 of
+// 4096 138 / 84, 2048 of 2048 twice 149 / 88, 8192 of 8192 2068 / 530.
+//
+// Below it, one tile of 16 rows a workgroup or two: two read the keys half as often,
+// one makes twice the workgroups.  us, one / two, 4 query heads a key head: 8 new of 8192
+// 18 / 24, 64 of 4096 28 / 29, 16 of 4096 four times (2^19 = row tiles x keys) 27 / 26, eight
+// times 43 / 37, 100 of 16384 106 / 79.
 template <int DP, int TYPE>
 hipError_t run_rows(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
-  const long long rows = static_cast<long long>(a.max_new) * p.group;
-  if (rows <= 16) return run_direct<DP, 1, TYPE>(a, p, s);
-  if (rows > 64) return run_tiled<DP, DP == 256 ? 4 : 8, TYPE>(a, p, s);
-  return run_direct<DP, DP == 256 && TYPE == QC_STORAGE_F32 ? 1 : 2, TYPE>(a, p, s);
+  const double units = static_cast<double>(a.seqs) * a.kv_heads;
+  const double rows = static_cast<double>(a.max_new) * p.group;
+  double keys = a.max_kv;
+  if (p.causal) keys -= 0.5 * std::min(a.max_new, a.max_kv);
+  if (p.window > 0) keys = std::min<double>(keys, p.window);
+  const bool many = rows >= 2048 && units * rows * keys * a.head_dim >= 0x1p31;
+  if (p.route == 0 ? many : p.route == 3)
+    return run_tiled<DP, DP == 256 ? 4 : 8, TYPE>(a, p, s);
+  const bool two = p.route == 0 ? rows > 16 && units * (rows / 16) * keys >= 0x1p19 : p.route == 2;
+  if constexpr (DP < 256 || TYPE != QC_STORAGE_F32)   // (two of f32 256 do not fit the registers)
+    if (two) return run_direct<DP, 2, TYPE>(a, p, s);
+  return run_direct<DP, 1, TYPE>(a, p, s);
 }
 
 template <int TYPE>
@@ -988,6 +1184,7 @@ hipError_t launch_kv8_attention(const Kv8Attention& r, int* status, hipStream_t 
   p.scale = r.scale;
   p.causal = r.causal;
   p.window = static_cast<int>(r.window);
+  p.route = r.route;
   const int size = r.type == QC_STORAGE_F32 ? 4 : 2;
   p.vec = ((reinterpret_cast<uintptr_t>(r.q) | reinterpret_cast<uintptr_t>(r.out) |
             static_cast<uintptr_t>(r.q_stride * size) | static_cast<uintptr_t>(r.out_stride * size)) & 15) == 0;

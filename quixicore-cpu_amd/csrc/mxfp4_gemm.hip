@@ -411,12 +411,15 @@ hipError_t run_ring(const Operands& o, int scale_stride, hipStream_t s) {
 }
 
 template <int TYPE>
-hipError_t run_gemm(Operands o, hipStream_t s) {
-  if (o.m <= 16) return run_direct<1, TYPE>(o, s);
-  if (o.m <= 32) return run_direct<2, TYPE>(o, s);
-  if (o.m <= 64) return run_direct<4, TYPE>(o, s);
+hipError_t run_gemm(Operands o, int route, hipStream_t s) {
   // the ring addresses a tile's codes with 32 bits
-  if (o.m <= 128 || o.blocks > (1 << 19)) return run_direct<8, TYPE>(o, s);
+  const bool ring = o.blocks <= (1 << 19) && (route == 0 ? o.m > 128 : route == 2);
+  if (!ring) {
+    if (o.m <= 16) return run_direct<1, TYPE>(o, s);
+    if (o.m <= 32) return run_direct<2, TYPE>(o, s);
+    if (o.m <= 64) return run_direct<4, TYPE>(o, s);
+    return run_direct<8, TYPE>(o, s);
+  }
   StreamWorkspace* ws = nullptr;
   std::unique_lock<std::mutex> hold;
   int stride = o.blocks;
@@ -443,12 +446,12 @@ hipError_t run_gemm(Operands o, hipStream_t s) {
 
 hipError_t launch_mxfp4_gemm(const uint8_t* w, const uint8_t* ws, const uint8_t* x,
                              const uint8_t* xs, void* y, int type, long long m, long long n,
-                             long long k, hipStream_t s) {
+                             long long k, int route, hipStream_t s) {
   const Operands o = {w, ws, x, xs, y, static_cast<int>(m), static_cast<int>(n), static_cast<int>(k / 32)};
   switch (type) {
-    case QC_STORAGE_F32: return run_gemm<QC_STORAGE_F32>(o, s);
-    case QC_STORAGE_F16: return run_gemm<QC_STORAGE_F16>(o, s);
-    default: return run_gemm<QC_STORAGE_BF16>(o, s);
+    case QC_STORAGE_F32: return run_gemm<QC_STORAGE_F32>(o, route, s);
+    case QC_STORAGE_F16: return run_gemm<QC_STORAGE_F16>(o, route, s);
+    default: return run_gemm<QC_STORAGE_BF16>(o, route, s);
   }
 }
 

@@ -303,6 +303,7 @@ struct Kv8Attention {
   long long heads = 0, window = 0;
   float scale = 1.f;
   int causal = 1;
+  int route = 0;        // 0 by size, 1 / 2 straight from the cache, one or two row tiles, 3 tiled
 };
 hipError_t launch_kv8_attention(const Kv8Attention& r, int* status, hipStream_t s);
 
@@ -318,6 +319,6 @@ hipError_t launch_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, 
                                    long long rows, long long dim, hipStream_t s);
 hipError_t launch_mxfp4_gemm(const uint8_t* w, const uint8_t* ws, const uint8_t* x,
                              const uint8_t* xs, void* y, int type, long long m, long long n,
-                             long long k, hipStream_t s);
+                             long long k, int route, hipStream_t s);   // route: 0 by size, 1 direct, 2 ring
 
 }  // namespace qc

@@ -80,6 +80,8 @@ _SIGS = {
                              _I),
     "qc_hip_quantize_mxfp4": ([_P, _I, _LL, _P, _P, _LL, _LL, _P, _P], _I),
     "qc_hip_dequantize_mxfp4": ([_P, _P, _P, _I, _LL, _LL, _P], _I),
+    "qc_hip_set_kv8_attention_route": ([_I], _I),
+    "qc_hip_set_mxfp4_gemm_route": ([_I], _I),
     "qc_hip_mxfp4_gemm": ([_P, _P, _P, _P, _P, _I, _LL, _LL, _LL, _P], _I),
 }
 for _name, (_args, _res) in _SIGS.items():
@@ -638,6 +640,17 @@ def mxfp4_gemm(w_codes, w_scales, x_codes, x_scales, dtype=None, y=None):
                                  x_scales.data_ptr(), y.data_ptr(), _storage(y), m, n, 2 * half,
                                  _stream(None)), "mxfp4_gemm")
     return y
+
+
+def set_kv8_attention_route(route=0):
+    """0 = from the sizes, 1 / 2 = the cache read directly for 16 / 32 rows a workgroup,
+    3 = laid out for MFMA tiles first."""
+    _check(lib.qc_hip_set_kv8_attention_route(route), "set_kv8_attention_route")
+
+
+def set_mxfp4_gemm_route(route=0):
+    """0 = from the sizes, 1 = weights streamed to registers, 2 = both operands through LDS."""
+    _check(lib.qc_hip_set_mxfp4_gemm_route(route), "set_mxfp4_gemm_route")
 
 
 def set_gemv_rows_per_wave(rows):

@@ -231,6 +231,14 @@ def test_append_errors(qc, dev):
 
 # ---- attention --------------------------------------------------------------------
 
+@pytest.fixture(params=[0, 1, 2, 3], ids=["auto", "direct16", "direct32", "tiled"])
+def route(request, qc):
+    """Every kernel of the attention at every size."""
+    qc.set_kv8_attention_route(request.param)
+    yield request.param
+    qc.set_kv8_attention_route(0)
+
+
 def _attention_reference(host, batch, q, heads, scale, causal, window, half):
     """(out, tolerance) in f64: out is softmax(scale q k^T + mask) v; the tolerance counts
     f32 dots, q and the probabilities in 11 (16-bit q) or 22 bits, f32 sums, one
@@ -273,10 +281,15 @@ def _attention_reference(host, batch, q, heads, scale, causal, window, half):
             small = abs(scale) * np.abs(Q).max(1) * np.abs(K).sum(1).max(initial=0) * 2.0 ** -38
             ds = size * ((hd + 8) * 2.0 ** -24 + qbits) + small + (np.abs(top) + size) * 2.0 ** -22
             spread = p @ np.abs(V)
+            # a probability times its page's share of the largest value scale is held in f16
+            # times 2^11 (f32 q: 2^15 and a second term): below 2^-14 the half step there is
+            # 2^-25, so each key adds at most 2^-36 (2^-40) of that scale times its code
+            C = np.where(used[:, None], np.abs(vc[pid, h // g, slot].astype(np.float64)), 0)
+            floor = (2.0 ** -36 if half > 2.0 ** -24 else 2.0 ** -40) * np.abs(np.where(used, vs[pid, h // g], 0)).max(initial=0) * (seen @ C)
             out[batch.start[s]:batch.start[s + 1], h] = o
             tol[batch.start[s]:batch.start[s + 1], h] = (
                 spread * (bits + 2 * ds[:, None] + (length / 16 + 16) * 2.0 ** -23)
-                + half * (1 + 2.0 ** -10) * np.abs(o) + 2.0 ** -25)
+                + floor + half * (1 + 2.0 ** -10) * np.abs(o) + 2.0 ** -25)
     return out, tol
 
 
@@ -310,7 +323,7 @@ def _attend(qc, dev, rng, new, kv, heads, kvh, hd, page, dtype="bfloat16", causa
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("kv", [[1], [2, 15, 16], [17, 31, 32, 33], [63, 64, 65], [127, 128, 129, 200], [600],
                                 [1000, 1, 513]])
-def test_attention_single_tokens(qc, dev, dtype, kv):
+def test_attention_single_tokens(qc, dev, route, dtype, kv):
     print(f"kv8 attention {dtype} one token each, kv {kv}", flush=True)
     rng = np.random.default_rng(sum(kv))
     _attend(qc, dev, rng, [1] * len(kv), kv, 8, 2, 128, 64, dtype)
@@ -321,7 +334,7 @@ def test_attention_single_tokens(qc, dev, dtype, kv):
     (1, 1, 16, 16), (2, 1, 32, 16), (7, 1, 64, 32), (14, 2, 64, 128), (8, 8, 80, 64), (6, 2, 96, 16), (16, 1, 128, 64),
     (32, 2, 128, 256), (48, 2, 128, 32), (4, 2, 176, 64), (8, 1, 256, 16), (16, 1, 240, 128), (40, 1, 128, 16)])
 @pytest.mark.parametrize("new,kv", [([1, 1], [150, 37]), ([5, 3, 9], [70, 3, 140])])
-def test_attention_heads(qc, dev, heads, kvh, hd, page, new, kv):
+def test_attention_heads(qc, dev, route, heads, kvh, hd, page, new, kv):
     print(f"kv8 attention heads {heads}/{kvh} hd {hd} page {page} new {new}", flush=True)
     rng = np.random.default_rng(heads * hd + page)
     for dtype in ("bfloat16", "float32"):
@@ -337,7 +350,7 @@ def test_attention_heads(qc, dev, heads, kvh, hd, page, new, kv):
     ([33], [400], 8, 1, 128, 16, True, 64), ([70, 70], [70, 200], 2, 1, 256, 64, True, 0),
     ([260], [520], 16, 2, 128, 64, True, 129), ([513], [513], 2, 1, 128, 16, True, 0),
     ([40, 600], [1000, 600], 12, 4, 128, 64, True, 0)])
-def test_attention_prompts(qc, dev, dtype, new, kv, heads, kvh, hd, page, causal, window):
+def test_attention_prompts(qc, dev, route, dtype, new, kv, heads, kvh, hd, page, causal, window):
     print(f"kv8 attention {dtype} new {new} kv {kv} heads {heads}/{kvh} hd {hd} page {page} {causal} {window}", flush=True)
     rng = np.random.default_rng(sum(new) + hd)
     _attend(qc, dev, rng, new, kv, heads, kvh, hd, page, dtype, causal, window, spare=2)
@@ -346,7 +359,7 @@ def test_attention_prompts(qc, dev, dtype, new, kv, heads, kvh, hd, page, causal
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("new,kv", [([5, 1, 3], [2, 0, 3]), ([200, 7], [100, 0]), ([300], [40]), ([40, 33], [0, 31])])
 @pytest.mark.parametrize("causal", [True, False])
-def test_attention_rows_that_see_nothing(qc, dev, dtype, new, kv, causal):
+def test_attention_rows_that_see_nothing(qc, dev, route, dtype, new, kv, causal):
     """More new tokens than the cache holds, and empty caches: rows before position 0, or
     with no key at all, are zeros."""
     print(f"kv8 attention empty rows {dtype} new {new} kv {kv} causal {causal}", flush=True)
@@ -357,7 +370,7 @@ def test_attention_rows_that_see_nothing(qc, dev, dtype, new, kv, causal):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-def test_attention_scales_far_apart(qc, dev, dtype):
+def test_attention_scales_far_apart(qc, dev, route, dtype):
     """Pages' scales spread over e^+-4, sharp scores, large and small q, and scales of zero."""
     import torch
     rng = np.random.default_rng(12)
@@ -370,7 +383,7 @@ def test_attention_scales_far_apart(qc, dev, dtype):
         batch = Ragged(rng, new, kv, 16)
         cache = _random_cache(qc, dev, rng, batch.pages, 2, 16, 64)
         for i in (0, 1):                                # some pages hold zeros under a scale of zero
-            zero = torch.rand(batch.pages, 2, device=dev) < 0.4
+            zero = torch.from_numpy(rng.random((batch.pages, 2)) < 0.4).to(dev)
             cache.tensors[i][zero] = 0
             cache.tensors[2 + i][zero] = 0
         _attend(qc, dev, rng, new, kv, 4, 2, 64, 16, dtype, batch=batch, cache=cache)
@@ -380,12 +393,12 @@ def test_attention_scales_far_apart(qc, dev, dtype):
         batch = Ragged(rng, new, kv, 16)
         cache = _random_cache(qc, dev, rng, batch.pages, 2, 16, 64)
         for i in (2, 3):                                # negative scales are scales
-            cache.tensors[i][torch.rand(batch.pages, 2, device=dev) < 0.5] *= -1
+            cache.tensors[i][torch.from_numpy(rng.random((batch.pages, 2)) < 0.5).to(dev)] *= -1
         _attend(qc, dev, rng, new, kv, 4, 2, 64, 16, dtype, batch=batch, cache=cache)
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-def test_attention_peaked_q(qc, dev, dtype):
+def test_attention_peaked_q(qc, dev, route, dtype):
     """One channel of q far above the rest where the keys hold zero: the others keep
     their bits."""
     import torch
@@ -399,7 +412,7 @@ def test_attention_peaked_q(qc, dev, dtype):
         _attend(qc, dev, rng, new, kv, 4, 2, 64, 32, dtype, batch=batch, cache=cache, q=q)
 
 
-def test_attention_nonfinite_q_stays_in_its_row(qc, dev):
+def test_attention_nonfinite_q_stays_in_its_row(qc, dev, route):
     import torch
     rng = np.random.default_rng(6)
     for dtype in (torch.float32, torch.float16, torch.bfloat16):
@@ -418,7 +431,7 @@ def test_attention_nonfinite_q_stays_in_its_row(qc, dev):
             assert not bool(torch.isfinite(got[0, 0]).any()) and not bool(torch.isfinite(got[2, 7]).any())
 
 
-def test_attention_ignores_what_it_does_not_see(qc, dev):
+def test_attention_ignores_what_it_does_not_see(qc, dev, route):
     """Slots past the length, pages before a window and unused table entries may hold
     anything, NaN scales too."""
     import torch
@@ -447,7 +460,7 @@ def test_attention_ignores_what_it_does_not_see(qc, dev):
         assert st.item() == 0
 
 
-def test_attention_errors(qc, dev):
+def test_attention_errors(qc, dev, route):
     """A bad page or length sets the status; a sequence whose figures are wrong stays
     unwritten and the others are done."""
     import torch
@@ -495,7 +508,7 @@ def test_attention_errors(qc, dev):
 
 @pytest.mark.parametrize("new,kv,heads,kvh", [([1] * 5, [900, 1, 64, 500, 333], 8, 2), ([1], [4000], 4, 1),
                                               ([150, 40], [400, 64], 8, 2), ([20, 3], [2000, 64], 8, 2)])
-def test_attention_repeats_and_graph(qc, dev, new, kv, heads, kvh):
+def test_attention_repeats_and_graph(qc, dev, route, new, kv, heads, kvh):
     """Bit-identical reruns; captured and replayed with eager calls of other sizes on
     the same stream between."""
     import torch
@@ -539,7 +552,7 @@ def test_attention_repeats_and_graph(qc, dev, new, kv, heads, kvh):
     del graph
 
 
-def test_attention_strided_rows(qc, dev):
+def test_attention_strided_rows(qc, dev, route):
     """q inside fused projection rows, out inside wider rows; odd element offsets."""
     import torch
     rng = np.random.default_rng(50)
@@ -559,7 +572,7 @@ def test_attention_strided_rows(qc, dev):
                 assert torch.equal(wide[:, :288].reshape(t, 6, 48), want) and bool((wide[:, 288:] == 7).all())
 
 
-def test_attention_far_into_a_large_cache(qc, dev):
+def test_attention_far_into_a_large_cache(qc, dev, route):
     """Pages whose byte offsets pass 32 bits."""
     import torch
     pages, kvh, page, hd = 18000, 8, 256, 128            # 4.7 GB each of K and V
@@ -593,7 +606,7 @@ def test_attention_far_into_a_large_cache(qc, dev):
     assert np.all(np.abs(out.double().cpu().numpy() - want) <= tol)
 
 
-def test_a_low_bit_layer(qc, dev):
+def test_a_low_bit_layer(qc, dev, route):
     """Projections in MXFP4, rotation, append and attention of a ragged batch, step by step
     over a prompt and two decoding steps: the same as each operator alone on the values
     that the one before gave, and near full precision."""
@@ -647,3 +660,74 @@ def test_a_low_bit_layer(qc, dev):
                 got = out[a:e, h].double()
                 assert ((got - want).norm() / want.norm()).item() < 0.03
     assert st.item() == 0
+
+
+def test_attention_passes_of_the_layout(qc, dev):
+    """More keys than are laid out at a time (1 GB): several passes, the same values as read
+    directly, within both forms' rounding."""
+    import torch
+    rng = np.random.default_rng(70)
+    seqs, kvh, hd, kv = 70, 8, 128, 4096
+    batch = Ragged(rng, [1] * seqs, [kv - 37 * (s % 5) for s in range(seqs)], 64)
+    g = torch.Generator(device=dev).manual_seed(3)
+    shape = (batch.pages, kvh, 64, hd)
+    codes = [torch.randint(-127, 128, shape, generator=g, device=dev, dtype=torch.int8) for _ in range(2)]
+    scales = [torch.rand(batch.pages, kvh, generator=g, device=dev) / 60 for _ in range(2)]
+    cache = qc.Kv8Cache(*codes, *scales)
+    q = torch.randn(batch.tokens, 16, hd, generator=g, device=dev)
+    b = batch.device(qc, dev)
+    try:
+        qc.set_kv8_attention_route(1)
+        direct = qc.kv8_attention(cache, b, q)
+        qc.set_kv8_attention_route(3)
+        tiled = qc.kv8_attention(cache, b, q)
+    finally:
+        qc.set_kv8_attention_route(0)
+    # f32 q: 22 bits of each operand, 64 tiles' f32 sums: 2^-18 of the values' size
+    assert ((direct - tiled).abs().max() / direct.abs().max()).item() < 2.0 ** -14
+
+
+@pytest.mark.parametrize("dtype,new,kv,heads,kvh,hd,window", [
+    ("bfloat16", [1024, 700], [2100, 700], 16, 4, 128, 0), ("float32", [2100], [2100], 16, 4, 64, 0),
+    ("float16", [513, 1000], [900, 3000], 8, 2, 256, 700), ("bfloat16", [2700], [2700], 8, 8, 80, 0)])
+def test_attention_long_prompts(qc, dev, dtype, new, kv, heads, kvh, hd, window):
+    """Sizes at which the tiled kernels are chosen, and splits of their keys; against 64 bits
+    on the GPU, and against the other kernels."""
+    import torch
+    rng = np.random.default_rng(sum(kv))
+    batch = Ragged(rng, new, kv, 32, 3)
+    cache = _random_cache(qc, dev, rng, batch.pages, kvh, 32, hd, 0.3)
+    q = torch.from_numpy(rng.standard_normal((batch.tokens, heads, hd))).to(getattr(torch, dtype)).to(dev)
+    b = batch.device(qc, dev)
+    want = torch.zeros(q.shape, dtype=torch.float64, device=dev)
+    size, score = torch.zeros_like(want), 0.0
+    for s in range(len(kv)):
+        pid, slot = (torch.from_numpy(x).to(dev) for x in batch.places(s, 0, kv[s]))
+        K, V = (cache.tensors[i][pid.long(), :, slot].double() * cache.tensors[2 + i][pid.long()].double()[..., None]
+                for i in range(2))
+        at = torch.arange(kv[s] - new[s], kv[s], device=dev)[:, None]
+        j = torch.arange(kv[s], device=dev)[None]
+        hide = j > at
+        if window:
+            hide = hide | (j <= at - window)
+        a, e = batch.start[s], batch.start[s + 1]
+        for h in range(heads):
+            z = (q[a:e, h].double() @ K[:, h // (heads // kvh)].T.contiguous()) * float(np.float32(hd ** -0.5))
+            score = max(score, z.abs().max().item())
+            p = torch.softmax(z.masked_fill(hide, -math.inf), -1)
+            want[a:e, h] = p @ V[:, h // (heads // kvh)]
+            size[a:e, h] = p @ V[:, h // (heads // kvh)].abs()
+    # probabilities in 11 (22) bits; scores of f32 dots whose terms' magnitudes sum to a few
+    # times the largest score; sums over up to 3000 keys in steps of 16; the output's rounding
+    bits = 2.0 ** -11 if dtype != "float32" else 2.0 ** -21
+    tol = size * (bits + 2 * 4 * score * (hd + 8) * 2.0 ** -24 + 200 * 2.0 ** -23) + HALF[dtype] * (1 + 2.0 ** -10) * want.abs() + 2.0 ** -24
+    outs = []
+    try:
+        for r in (0, 1, 3):
+            qc.set_kv8_attention_route(r)
+            out = qc.kv8_attention(cache, b, q, window=window)
+            assert bool(((out.double() - want).abs() <= tol)[:batch.start[-1]].all()), r
+            outs.append(out)
+    finally:
+        qc.set_kv8_attention_route(0)
+    assert torch.equal(outs[0], outs[2])       # the sizes choose the tiled kernels

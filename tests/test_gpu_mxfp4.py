@@ -117,6 +117,14 @@ def test_quantize_nonfinite(qc, dev, dtype):
             assert scales[r, b].item() == (9 if bad else wscale[r, b])
 
 
+@pytest.fixture(params=[0, 1, 2], ids=["auto", "direct", "ring"])
+def route(request, qc):
+    """Every kernel of the product at every size."""
+    qc.set_mxfp4_gemm_route(request.param)
+    yield request.param
+    qc.set_mxfp4_gemm_route(0)
+
+
 def _matrix(g, rows, k, sigma=1.0, spread=2):
     """Random codes (all 16) and scale bytes."""
     codes = g.integers(0, 256, (rows, k // 2), dtype=np.uint8)
@@ -147,26 +155,26 @@ def _product(qc, dev, g, m, n, k, dtype="float32", spread=2, offset=0):
     (33, 65, 2048), (48, 130, 160), (64, 64, 256), (65, 255, 800), (77, 341, 2752), (100, 31, 4096),
     (128, 128, 512), (129, 257, 608), (200, 1000, 768), (257, 300, 32), (300, 513, 1056),
     (511, 129, 2048), (700, 1025, 320)])
-def test_product_shapes(qc, dev, m, n, k):
+def test_product_shapes(qc, dev, route, m, n, k):
     print(f"mxfp4 product {m}x{n}x{k}", flush=True)
     _product(qc, dev, np.random.default_rng(m * n + k), m, n, k)
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("m,n,k", [(1, 512, 1024), (12, 200, 1056), (40, 77, 512), (300, 260, 608)])
-def test_product_types(qc, dev, dtype, m, n, k):
+def test_product_types(qc, dev, route, dtype, m, n, k):
     # scales that keep the sums within f16
     _product(qc, dev, np.random.default_rng(k + m), m, n, k, dtype, spread=1)
 
 
 @pytest.mark.parametrize("m", [1, 9, 40, 150])
-def test_product_wide_scales(qc, dev, m):
+def test_product_wide_scales(qc, dev, route, m):
     """Scales over 2^+-40: a block's product is exact whatever the others are."""
     _product(qc, dev, np.random.default_rng(m), m, 70, 640, spread=20)
 
 
 @pytest.mark.parametrize("m", [1, 5, 33, 140])
-def test_product_special_scales(qc, dev, m):
+def test_product_special_scales(qc, dev, route, m):
     """A NaN scale of a row reaches that row's (column's) outputs only; the smallest and
     largest scales."""
     import torch
@@ -208,7 +216,7 @@ def test_quantized_product_of_floats(qc, dev):
     assert ((y - full).norm() / full.norm()).item() < 0.25
 
 
-def test_product_repeats_bit_for_bit(qc, dev):
+def test_product_repeats_bit_for_bit(qc, dev, route):
     import torch
     g = np.random.default_rng(8)
     for m in (1, 24, 130):
@@ -219,7 +227,7 @@ def test_product_repeats_bit_for_bit(qc, dev):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 1000, 4096), (20, 300, 2048), (260, 512, 1024)])
-def test_graph_replay(qc, dev, m, n, k):
+def test_graph_replay(qc, dev, route, m, n, k):
     """quantise + product captured, replayed with other work between on the same stream."""
     import torch
     g = torch.Generator(device=dev).manual_seed(2)

@@ -125,6 +125,12 @@ def test_kv8_refusals(q, entry):
             assert call(ref(cache), ref(batch), **bad) == 3, bad
 
 
+def test_knobs(q):
+    for f, most in ((q.lib.qc_hip_set_kv8_attention_route, 3), (q.lib.qc_hip_set_mxfp4_gemm_route, 2)):
+        assert f(-1) == 3 and f(most + 1) == 3
+        assert f(most) == 0 and f(0) == 0
+
+
 def test_mxfp4_refusals(q):
     lib = q.lib
     quant = lambda x=P, type=0, stride=64, c=P, s=P, rows=4, dim=64: lib.qc_hip_quantize_mxfp4(
