@@ -477,7 +477,7 @@ int qc_hip_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, void* o
 
 /* y[m][n] = x . w^T of two MXFP4 matrices, w [n][k] and x [m][k]: products exact,
  * sums f32, y of y_type.  A scale byte of 255 makes the outputs of its row NaN.
- * Status: 1 for sizes that are not positive or k not a multiple of 32, 2 for an
+ * Status: 1 for sizes that are not positive, k above 2^27 or not a multiple of 32, 2 for an
  * unknown type, 3 for NULL pointers or codes that are not 16-byte aligned. */
 int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* x_codes,
                       const uint8_t* x_scales, void* y, int y_type, long long m, long long n,
@@ -574,9 +574,10 @@ int qc_hip_set_qgemm_fold(int mode);
  * the stated precision.  Tuning and test knob with no reference counterpart. */
 int qc_hip_set_kv8_attention_route(int route);
 
-/* Kernels of qc_hip_mxfp4_gemm (process-wide): 0 (default) chooses from the sizes;
- * 1 = weights streamed to registers; 2 = both operands through LDS (k <= 2^24).
- * Tuning and test knob with no reference counterpart. */
+/* Tile of qc_hip_mxfp4_gemm (process-wide): 0 (default) chooses from the sizes; 1..7 =
+ * 32 x 32, 64 x 32, 64 x 64, 128 x 64, 128 x 128, 256 x 128, 256 x 256 rows of w and x
+ * (k above 2^24: always the first).  Tuning and test knob with no reference
+ * counterpart. */
 int qc_hip_set_mxfp4_gemm_route(int route);
 
 /* on != 0: qc_hip_rms_norm_add_quant_int8 replays the element-order sum of

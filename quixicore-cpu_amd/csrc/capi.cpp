@@ -976,7 +976,7 @@ int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uin
                       long long k, void* stream) {
   if (!valid_product({m, n, 4}) || !valid_product({m, k}) || !valid_product({n, k}) || k % 32 != 0)
     return QC_INVALID_SHAPE;
-  if (m > INT_MAX / 2 || n > INT_MAX / 2 || k > INT_MAX / 2) return QC_INVALID_SHAPE;
+  if (m > INT_MAX / 2 || n > INT_MAX / 2 || k > (1LL << 27)) return QC_INVALID_SHAPE;
   if (!known_storage(y_type)) return QC_UNSUPPORTED_FORMAT;
   if (w_codes == nullptr || w_scales == nullptr || x_codes == nullptr || x_scales == nullptr ||
       y == nullptr || !aligned16(w_codes) || !aligned16(x_codes))
@@ -1022,7 +1022,7 @@ int qc_hip_set_kv8_attention_route(int route) {
 }
 
 int qc_hip_set_mxfp4_gemm_route(int route) {
-  if (route < 0 || route > 2) return QC_INVALID_ARGUMENT;
+  if (route < 0 || route > 7) return QC_INVALID_ARGUMENT;
   g_knobs.mxfp4_route.store(route, std::memory_order_relaxed);
   return QC_OK;
 }

@@ -7,6 +7,7 @@
 // meet in one instruction is free as long as both operands agree.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 #include "qc_internal.h"
@@ -58,111 +59,24 @@ __device__ __forceinline__ void store4(void* y, long long at, int left, const fl
   }
 }
 
-// ---- Few rows of x: weights straight from memory ------------------------------
+// A workgroup owns TN rows of w and TM rows of x, cut into WGN x WGM wave tiles of 32 x
+// 32 instructions; KG waves share a wave tile, each with 4 / KG of every step's quarters,
+// and add their sums at the end.  A K step is one 128-byte line of codes (8 blocks) of every
+// row and its 8 scale bytes, copied to a stage of an S-deep LDS ring by global_load_lds: codes
+// 8 rows an instruction, 16-byte chunk c of row r at position c ^ ((r >> 1) & 7); scales
+// 32 rows an instruction, lane l the bytes 4 (l >> 5) .. + 3 of row l & 31.  Quarter q of a
+// step multiplies, with v_mfma_scale_f32_32x32x64, chunks q and 4 + q of the rows: lane l
+// holds chunk 4 (l >> 5) + q of row l & 31, whose scale is byte q of the dword that it
+// holds for the whole step.
 //
-// A workgroup owns 16 rows of w and MT tiles of 16 rows of x; its four waves take the
-// windows of 16 blocks (256 bytes of a row) in turn and add their sums in LDS.
-// In a window, instruction t multiplies blocks 4 t .. 4 t + 3: lane l holds block
-// 4 t + (l >> 4) of row l & 15, so a load covers 64 bytes of each row.
-constexpr int kDirectWaves = 4;
-
-// The scale bytes of blocks 4 t + g of a window, t = 0..3, in byte 0 of s[t].
-__device__ __forceinline__ void window_scales(const uint8_t* row, int g, int left, uint32_t (&s)[4]) {
-  if (left >= 16) {
-    uint32_t d[4];
-    __builtin_memcpy(d, row, 16);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) s[t] = d[t] >> (8 * g);
-  } else {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) s[t] = 4 * t + g < left ? row[4 * t + g] : 0;
-  }
-}
-
-template <int MT, int TYPE>
-__global__ __launch_bounds__(64 * kDirectWaves) void mxfp4_direct(
-    const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws, const uint8_t* __restrict__ x,
-    const uint8_t* __restrict__ xs, void* __restrict__ y, int m, int n, int blocks) {
-  __shared__ f32x4 sums[kDirectWaves - 1][MT][64];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = lane & 15, g = lane >> 4;
-  const int n0 = 16 * blockIdx.x, m0 = 16 * MT * blockIdx.y;
-  const long long wr = min(n0 + row, n - 1);
-  const uint8_t* wp = w + wr * blocks * 16 + 16 * g;
-  const uint8_t* wsp = ws + wr * blocks;
-  const uint8_t* xp[MT];
-  const uint8_t* xsp[MT];
-  bool has[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int r = m0 + 16 * i + row;
-    has[i] = r < m;                              // lanes of rows past m load nothing
-    xp[i] = x + static_cast<long long>(has[i] ? r : 0) * blocks * 16 + 16 * g;
-    xsp[i] = xs + static_cast<long long>(has[i] ? r : 0) * blocks;
-  }
-  f32x4 acc[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int b0 = 16 * wave; b0 < blocks; b0 += 16 * kDirectWaves) {
-    const int left = blocks - b0;
-    uint32_t sw[4];
-    window_scales(wsp + b0, g, left, sw);
-    i32x4 a[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      a[t] = i32x4{0, 0, 0, 0};
-      if (4 * t + g < left)
-        a[t] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wp + 16LL * (b0 + 4 * t)));
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      uint32_t sx[4] = {0, 0, 0, 0};
-      i32x4 b[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) b[t] = i32x4{0, 0, 0, 0};
-      if (has[i]) {
-        window_scales(xsp[i] + b0, g, left, sx);
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          if (4 * t + g < left) b[t] = *reinterpret_cast<const i32x4*>(xp[i] + 16LL * (b0 + 4 * t));
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-            fp4_operand(a[t]), fp4_operand(b[t]), acc[i], 4, 4, 0, static_cast<int>(sw[t]), 0,
-            static_cast<int>(sx[t]));
-    }
-  }
-  if (wave > 0) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sums[wave - 1][i][lane] = acc[i];
-  }
-  __syncthreads();
-  if (wave > 0) return;
-  // lane l: row l & 15 of x, rows 4 (l >> 4) .. + 3 of w
-  const int nc = n0 + 4 * g;
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-#pragma unroll
-    for (int k = 0; k < kDirectWaves - 1; ++k) acc[i] += sums[k][i][lane];
-    if (!has[i] || nc >= n) continue;
-    const float v[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
-    store4<TYPE>(y, static_cast<long long>(m0 + 16 * i + row) * n + nc, n - nc, v,
-                 n % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0);
-  }
-}
-
-// ---- Many rows: both operands through an LDS ring ---------------------------
-//
-// A workgroup of WGN x WGM waves owns TN rows of w and TM rows of x.  A K step is
-// one 128-byte line of codes (8 blocks) of every row and its 8 scale bytes, copied to a
-// stage of an S-deep ring by global_load_lds: codes 8 rows an instruction, 16-byte chunk
-// c of row r at position c ^ ((r >> 1) & 7); scales 32 rows an instruction, lane l
-// the bytes 4 (l >> 5) .. + 3 of row l & 31.  Quarter q of a step multiplies, with
-// v_mfma_scale_f32_32x32x64, chunks q and 4 + q of the rows: lane l holds chunk
-// 4 (l >> 5) + q of row l & 31, whose scale is byte q of the dword that it holds for
-// the whole step.
+// What bounds it: with few rows of x the stream of w (M = 1, 14336 x 4096: 31 MB, 7.8 us, of
+// which a launch and the first bytes are about 3; a form without LDS, 16 rows a workgroup and
+// the codes straight to registers, took 9.2, M = 32 17 against 8.3); with many, a step's chain
+// of barrier, LDS reads and MFMAs, the LDS traffic (a 256 x 256 tile reads its 64 KB stage
+// three times and writes it once, as many cycles as its MFMAs) and MFMA power: M = 4096,
+// 14336 x 4096, 162 us = 2.97 PFLOP/s, of it about 25 for the outputs' burst.  More waves
+// for the same tile are faster than larger wave tiles everywhere (256 x 256: 16 waves of 64 x 64
+// 162, 8 of 64 x 128 164, 4 of 128 x 128 174; 128 x 128, M = 512: 8 waves 16, 4 waves 24).
 __device__ __forceinline__ void ring_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -183,18 +97,20 @@ __device__ __forceinline__ void tile_at(int b, int total, int tiles_n, int tiles
   tm = band * kBand + rem % gm;
 }
 
-template <int TN, int TM, int S, int WGN, int WGM, int TYPE>
-__global__ __launch_bounds__(64 * WGN * WGM, 1) void mxfp4_ring(
+template <int TN, int TM, int S, int WGN, int WGM, int KG, int TYPE>
+__global__ __launch_bounds__(64 * WGN * WGM * KG, 1) void mxfp4_ring(
     const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws, const uint8_t* __restrict__ x,
     const uint8_t* __restrict__ xs, void* __restrict__ y, int m, int n, int blocks,
     int scale_stride, int tiles_n, int tiles_m) {
-  constexpr int NW = WGN * WGM;
+  constexpr int NW = WGN * WGM * KG;
+  constexpr int QN = 4 / KG;                        // quarters of a step that a wave multiplies
   constexpr int FN = TN / WGN / 32, FM = TM / WGM / 32;
   constexpr int R = TN + TM;                        // rows of a stage, w's first
-  constexpr int GC = R / 8 / NW, GS = (R / 32 + NW - 1) / NW;   // loads a wave and step
+  // loads a wave and step (beyond the stage's share the last one again: the same bytes)
+  constexpr int GC = (R / 8 + NW - 1) / NW, GS = (R / 32 + NW - 1) / NW;
   constexpr int G = GC + GS;
   constexpr int kStage = R * 136;                   // codes, then scales
-  static_assert(R % (8 * NW) == 0 && FN >= 1 && FM >= 1 && S >= 2 && G * (S - 1) < 64, "tile");
+  static_assert(FN >= 1 && FM >= 1 && S >= 2 && G * (S - 1) < 64, "tile");
   static_assert(S * kStage <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[S * kStage];
 
@@ -213,7 +129,7 @@ __global__ __launch_bounds__(64 * WGN * WGM, 1) void mxfp4_ring(
   int ccol[GC];
 #pragma unroll
   for (int j = 0; j < GC; ++j) {
-    const int r8 = 8 * (wave * GC + j);             // uniform
+    const int r8 = 8 * min(wave * GC + j, R / 8 - 1);   // uniform
     const bool is_w = r8 < TN;
     const int first = is_w ? n0 : m0, limit = is_w ? n : m, base = is_w ? r8 : r8 - TN;
     cbase[j] = (is_w ? w : x) + static_cast<long long>(first) * bytes;
@@ -238,7 +154,7 @@ __global__ __launch_bounds__(64 * WGN * WGM, 1) void mxfp4_ring(
       if (j < from || j >= to) continue;
       if (j < GC) {
         const int col = min(128 * step + ccol[j < GC ? j : 0], bytes - 16);
-        dma16(cbase[j < GC ? j : 0], cvo[j < GC ? j : 0] + col, base + (wave * GC + j) * 1024);
+        dma16(cbase[j < GC ? j : 0], cvo[j < GC ? j : 0] + col, base + min(wave * GC + j, R / 8 - 1) * 1024);
       } else {
         const int i = j - GC;
         const int col = min(8 * step + 4 * (lane >> 5), scale_stride - 4);
@@ -248,12 +164,14 @@ __global__ __launch_bounds__(64 * WGN * WGM, 1) void mxfp4_ring(
     }
   };
 
-  const int wn = (wave / WGM) * FN * 32, wm = (wave % WGM) * FM * 32;
+  const int kg = wave / (WGN * WGM), tile = wave % (WGN * WGM);
+  const int wn = (tile / WGM) * FN * 32, wm = (tile % WGM) * FM * 32;
+  const int q0 = kg * QN;
   const int key = (lane >> 1) & 7;
   i32x4 fa[2][FN], fb[2][FM];
   int sa[2][FN], sb[2][FM];                         // scales of this step and the next
-  auto read_frags = [&](int stage, int q, int slot) {
-    const uint8_t* base = lds + stage * kStage + (lane & 31) * 128 + (((4 * (lane >> 5) + q) ^ key) * 16);
+  auto read_frags = [&](int stage, int j, int slot) {     // quarter q0 + j
+    const uint8_t* base = lds + stage * kStage + (lane & 31) * 128 + (((4 * (lane >> 5) + q0 + j) ^ key) * 16);
 #pragma unroll
     for (int i = 0; i < FN; ++i) fa[slot][i] = *reinterpret_cast<const i32x4*>(base + (wn + 32 * i) * 128);
 #pragma unroll
@@ -262,9 +180,11 @@ __global__ __launch_bounds__(64 * WGN * WGM, 1) void mxfp4_ring(
   auto read_scales = [&](int stage, int slot) {
     const uint8_t* base = lds + stage * kStage + R * 128 + 4 * lane;
 #pragma unroll
-    for (int i = 0; i < FN; ++i) sa[slot][i] = *reinterpret_cast<const int*>(base + (wn / 32 + i) * 256);
+    for (int i = 0; i < FN; ++i)
+      sa[slot][i] = *reinterpret_cast<const int*>(base + (wn / 32 + i) * 256) >> (8 * q0);
 #pragma unroll
-    for (int j = 0; j < FM; ++j) sb[slot][j] = *reinterpret_cast<const int*>(base + ((TN + wm) / 32 + j) * 256);
+    for (int j = 0; j < FM; ++j)
+      sb[slot][j] = *reinterpret_cast<const int*>(base + ((TN + wm) / 32 + j) * 256) >> (8 * q0);
   };
   f32x16 acc[FN][FM];
 #pragma unroll
@@ -291,14 +211,21 @@ __global__ __launch_bounds__(64 * WGN * WGM, 1) void mxfp4_ring(
   read_scales(0, 0);
   read_frags(0, 0, 0);
   int stage = 0;
+  // slots: quarter j of a step in j & 1, the next step's first in the one not in use
   auto step = [&](int k, auto par) {
     constexpr int P = decltype(par)::value;
-    read_frags(stage, 1, 1);
-    mfmas(std::integral_constant<int, 0>(), 0, P);
-    read_frags(stage, 2, 0);
-    mfmas(std::integral_constant<int, 1>(), 1, P);
-    read_frags(stage, 3, 1);
-    mfmas(std::integral_constant<int, 2>(), 0, P);
+    constexpr int FIRST = QN == 1 ? P : 0, LAST = QN == 1 ? P : 1;
+    if constexpr (QN == 4) {
+      read_frags(stage, 1, 1);
+      mfmas(std::integral_constant<int, 0>(), 0, P);
+      read_frags(stage, 2, 0);
+      mfmas(std::integral_constant<int, 1>(), 1, P);
+      read_frags(stage, 3, 1);
+      mfmas(std::integral_constant<int, 2>(), 0, P);
+    } else if constexpr (QN == 2) {
+      read_frags(stage, 1, 1);
+      mfmas(std::integral_constant<int, 0>(), 0, P);
+    }
     // step k + 1 is in; every wave has read all of stage
     wait_vmcnt<(S - 2) * G>();
     __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));   // lgkmcnt(0)
@@ -306,8 +233,8 @@ __global__ __launch_bounds__(64 * WGN * WGM, 1) void mxfp4_ring(
     issue(min(k + S, nk - 1), stage, 0, G);
     stage = stage + 1 < S ? stage + 1 : 0;
     read_scales(stage, P ^ 1);
-    read_frags(stage, 0, 0);
-    mfmas(std::integral_constant<int, 3>(), 1, P);
+    read_frags(stage, 0, FIRST ^ (QN == 1 ? 1 : 0));
+    mfmas(std::integral_constant<int, QN - 1>(), LAST, P);
   };
   int k = 0;
   for (; k + 2 < nk; k += 2) {
@@ -330,7 +257,7 @@ __global__ __launch_bounds__(64 * WGN * WGM, 1) void mxfp4_ring(
     auto last = [&](auto quarter) {
       constexpr int Q = decltype(quarter)::value;
       read_frags(stage, Q, 0);
-      const bool in = 4 * (lane >> 5) + Q < left;
+      const bool in = 4 * (lane >> 5) + q0 + Q < left;
       const i32x4 zero = {0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < FN; ++i) {
@@ -344,12 +271,37 @@ __global__ __launch_bounds__(64 * WGN * WGM, 1) void mxfp4_ring(
       }
       mfmas(quarter, 0, 0);
     };
-    last(std::integral_constant<int, 0>());
-    if (left > 1) last(std::integral_constant<int, 1>());
-    if (left > 2) last(std::integral_constant<int, 2>());
-    if (left > 3) last(std::integral_constant<int, 3>());
+    if (left > q0) last(std::integral_constant<int, 0>());
+    if constexpr (QN > 1)
+      if (left > q0 + 1) last(std::integral_constant<int, 1>());
+    if constexpr (QN > 2) {
+      if (left > 2) last(std::integral_constant<int, 2>());
+      if (left > 3) last(std::integral_constant<int, 3>());
+    }
   }
   wait_vmcnt<0>();   // no load may land in LDS that is no longer this workgroup's
+  if constexpr (KG > 1) {
+    // the quarters' sums meet in the ring's LDS, added in their order
+    static_assert((KG - 1) * WGN * WGM * FN * FM * 4096 <= S * kStage, "sums fit the ring");
+    f32x16* sums = reinterpret_cast<f32x16*>(lds);
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));
+    __syncthreads();
+    if (kg > 0) {
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+          sums[((((kg - 1) * WGN * WGM + tile) * FN + i) * FM + j) * 64 + lane] = acc[i][j];
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] += sums[(((g * WGN * WGM + tile) * FN + i) * FM + j) * 64 + lane];
+  }
 
   // lane l: row wm + 32 j + (l & 31) of x; register e: row 8 (e >> 2) + 4 (l >> 5) + (e & 3) of w
   const bool vec = n % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
@@ -395,31 +347,54 @@ struct Operands {
   int m, n, blocks;
 };
 
-template <int MT, int TYPE>
-hipError_t run_direct(const Operands& o, hipStream_t s) {
-  const dim3 grid((o.n + 15) / 16, (o.m + 16 * MT - 1) / (16 * MT));
-  mxfp4_direct<MT, TYPE><<<grid, 64 * kDirectWaves, 0, s>>>(o.w, o.ws, o.x, o.xs, o.y, o.m, o.n, o.blocks);
-  return hipGetLastError();
+// The tiles, and what they cost: us of one round of workgroups on the CUs and of each
+// further one, K = 4096 (measured over M = 1 to 4096, N = 1000 to 14336; longer rows scale
+// all alike).  us at K = 4096 by tile, M x N:
+//            32x32  64x32  64x64  128x64  128x128  256x128  256x256
+// 1 x 14336    8.0    7.8    8.4    10.0     12.5     20.7     29.8
+// 64 x 4096    5.7    7.0    7.9    10.1     12.0     19.5     26.1
+// 128 x 14336 23.0   20.7   15.6    13.2     16.6     25.2     33.5
+// 512 x 4096  24.1   23.4   15.4    13.2     16.2     24.4     37.2
+// 512 x 14336 72.4   65.0   43.3    38.5     31.6     29.0     42.2
+// 2048 x 14336 273    241    159     138      108      103       87
+struct Tile {
+  int tn, tm;
+  bool whole_rounds;     // one workgroup a CU: a started round costs a round
+  double first, more;
+};
+constexpr int kTiles = 7;
+constexpr Tile kTile[kTiles] = {{32, 32, false, 5.6, 3.2},  {64, 32, false, 7.4, 5.4},   {64, 64, false, 9.4, 6.5},
+                                {128, 64, false, 13.0, 9.0}, {128, 128, true, 18.0, 15.0}, {256, 128, true, 29.0, 25.0},
+                                {256, 256, true, 42.0, 42.0}};
+
+int choose_tile(long long m, long long n, int cus) {
+  int best = 0;
+  double least = 0.0;
+  for (int i = 0; i < kTiles; ++i) {
+    const Tile& t = kTile[i];
+    const double tiles = static_cast<double>((n + t.tn - 1) / t.tn) * static_cast<double>((m + t.tm - 1) / t.tm);
+    double rounds = tiles / cus;
+    if (t.whole_rounds) rounds = std::ceil(rounds);
+    const double cost = t.first + t.more * std::max(0.0, rounds - 1.0);
+    if (i == 0 || cost < least) {
+      least = cost;
+      best = i;
+    }
+  }
+  return best;
 }
 
-template <int TN, int TM, int S, int WGN, int WGM, int TYPE>
+template <int TN, int TM, int S, int WGN, int WGM, int KG, int TYPE>
 hipError_t run_ring(const Operands& o, int scale_stride, hipStream_t s) {
   const int tiles_n = (o.n + TN - 1) / TN, tiles_m = (o.m + TM - 1) / TM;
-  mxfp4_ring<TN, TM, S, WGN, WGM, TYPE><<<static_cast<unsigned>(tiles_n) * tiles_m, 64 * WGN * WGM, 0, s>>>(
+  if (static_cast<long long>(tiles_n) * tiles_m > INT_MAX) return hipErrorInvalidValue;
+  mxfp4_ring<TN, TM, S, WGN, WGM, KG, TYPE><<<static_cast<unsigned>(tiles_n) * tiles_m, 64 * WGN * WGM * KG, 0, s>>>(
       o.w, o.ws, o.x, o.xs, o.y, o.m, o.n, o.blocks, scale_stride, tiles_n, tiles_m);
   return hipGetLastError();
 }
 
 template <int TYPE>
 hipError_t run_gemm(Operands o, int route, hipStream_t s) {
-  // the ring addresses a tile's codes with 32 bits
-  const bool ring = o.blocks <= (1 << 19) && (route == 0 ? o.m > 128 : route == 2);
-  if (!ring) {
-    if (o.m <= 16) return run_direct<1, TYPE>(o, s);
-    if (o.m <= 32) return run_direct<2, TYPE>(o, s);
-    if (o.m <= 64) return run_direct<4, TYPE>(o, s);
-    return run_direct<8, TYPE>(o, s);
-  }
   StreamWorkspace* ws = nullptr;
   std::unique_lock<std::mutex> hold;
   int stride = o.blocks;
@@ -439,7 +414,17 @@ hipError_t run_gemm(Operands o, int route, hipStream_t s) {
     o.ws = static_cast<const uint8_t*>(buf);
     o.xs = o.ws + static_cast<long long>(o.n) * stride;
   }
-  return run_ring<256, 256, 2, 4, 2, TYPE>(o, stride, s);
+  // a tile's codes are addressed with 32 bits: 32 rows of long ones
+  const int tile = o.blocks > (1 << 19) ? 0 : route > 0 ? route - 1 : choose_tile(o.m, o.n, device_cu_count());
+  switch (tile) {
+    case 0: return run_ring<32, 32, 4, 1, 1, 2, TYPE>(o, stride, s);
+    case 1: return run_ring<64, 32, 4, 2, 1, 1, TYPE>(o, stride, s);
+    case 2: return run_ring<64, 64, 4, 2, 2, 1, TYPE>(o, stride, s);
+    case 3: return run_ring<128, 64, 3, 4, 2, 1, TYPE>(o, stride, s);
+    case 4: return run_ring<128, 128, 4, 4, 2, 1, TYPE>(o, stride, s);
+    case 5: return run_ring<256, 128, 3, 4, 2, 1, TYPE>(o, stride, s);
+    default: return run_ring<256, 256, 2, 4, 4, 1, TYPE>(o, stride, s);
+  }
 }
 
 }  // namespace

@@ -319,6 +319,6 @@ hipError_t launch_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, 
                                    long long rows, long long dim, hipStream_t s);
 hipError_t launch_mxfp4_gemm(const uint8_t* w, const uint8_t* ws, const uint8_t* x,
                              const uint8_t* xs, void* y, int type, long long m, long long n,
-                             long long k, int route, hipStream_t s);   // route: 0 by size, 1 direct, 2 ring
+                             long long k, int route, hipStream_t s);   // route: 0 by size, 1..7 a tile
 
 }  // namespace qc

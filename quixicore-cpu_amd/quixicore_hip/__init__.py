@@ -649,7 +649,7 @@ def set_kv8_attention_route(route=0):
 
 
 def set_mxfp4_gemm_route(route=0):
-    """0 = from the sizes, 1 = weights streamed to registers, 2 = both operands through LDS."""
+    """0 = from the sizes, 1..7 = tiles of 32 x 32 to 256 x 256 rows of w and x."""
     _check(lib.qc_hip_set_mxfp4_gemm_route(route), "set_mxfp4_gemm_route")
 
 

@@ -117,9 +117,9 @@ def test_quantize_nonfinite(qc, dev, dtype):
             assert scales[r, b].item() == (9 if bad else wscale[r, b])
 
 
-@pytest.fixture(params=[0, 1, 2], ids=["auto", "direct", "ring"])
+@pytest.fixture(params=range(8), ids=["auto", "32x32", "64x32", "64x64", "128x64", "128x128", "256x128", "256x256"])
 def route(request, qc):
-    """Every kernel of the product at every size."""
+    """Every tile of the product at every size."""
     qc.set_mxfp4_gemm_route(request.param)
     yield request.param
     qc.set_mxfp4_gemm_route(0)

@@ -126,7 +126,7 @@ def test_kv8_refusals(q, entry):
 
 
 def test_knobs(q):
-    for f, most in ((q.lib.qc_hip_set_kv8_attention_route, 3), (q.lib.qc_hip_set_mxfp4_gemm_route, 2)):
+    for f, most in ((q.lib.qc_hip_set_kv8_attention_route, 3), (q.lib.qc_hip_set_mxfp4_gemm_route, 7)):
         assert f(-1) == 3 and f(most + 1) == 3
         assert f(most) == 0 and f(0) == 0
 
@@ -151,7 +151,7 @@ def test_mxfp4_refusals(q):
     gemm = lambda w=P, ws=P, x=P, xs=P, y=P, type=0, m=2, n=3, k=64: lib.qc_hip_mxfp4_gemm(
         w, ws, x, xs, y, type, m, n, k, None)
     for bad in (dict(m=0), dict(n=0), dict(k=0), dict(k=31), dict(m=1 << 62), dict(n=1 << 40),
-                dict(k=1 << 40), dict(m=1 << 31)):
+                dict(k=1 << 40), dict(m=1 << 31), dict(k=(1 << 27) + 32)):
         assert gemm(**bad) == 1, bad
     assert gemm(type=9) == 2
     for bad in (dict(w=None), dict(ws=None), dict(x=None), dict(xs=None), dict(y=None),
