@@ -74,9 +74,9 @@ __device__ __forceinline__ void store4(void* y, long long at, int left, const fl
 // the codes straight to registers, took 9.2, M = 32 17 against 8.3); with many, a step's chain
 // of barrier, LDS reads and MFMAs, the LDS traffic (a 256 x 256 tile reads its 64 KB stage
 // three times and writes it once, as many cycles as its MFMAs) and MFMA power: M = 4096,
-// 14336 x 4096, 162 us = 2.97 PFLOP/s, of it about 25 for the outputs' burst.  More waves
-// for the same tile are faster than larger wave tiles everywhere (256 x 256: 16 waves of 64 x 64
-// 162, 8 of 64 x 128 164, 4 of 128 x 128 174; 128 x 128, M = 512: 8 waves 16, 4 waves 24).
+// 14336 x 4096, quantised normal values, 182 us = 2.64 PFLOP/s, of it about 25 for the
+// outputs' burst.  Eight waves of 64 x 128 there: four of 128 x 128 are 6% slower, sixteen of
+// 64 x 64 3%; 128 x 128 tiles (M = 512) take 16 us with eight waves, 24 with four.
 __device__ __forceinline__ void ring_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -356,7 +356,7 @@ struct Operands {
 // 128 x 14336 23.0   20.7   15.6    13.2     16.6     25.2     33.5
 // 512 x 4096  24.1   23.4   15.4    13.2     16.2     24.4     37.2
 // 512 x 14336 72.4   65.0   43.3    38.5     31.6     29.0     42.2
-// 2048 x 14336 273    241    159     138      108      103       87
+// 2048 x 14336 273    241    159     138      108      103       90
 struct Tile {
   int tn, tm;
   bool whole_rounds;     // one workgroup a CU: a started round costs a round
@@ -423,7 +423,7 @@ hipError_t run_gemm(Operands o, int route, hipStream_t s) {
     case 3: return run_ring<128, 64, 3, 4, 2, 1, TYPE>(o, stride, s);
     case 4: return run_ring<128, 128, 4, 4, 2, 1, TYPE>(o, stride, s);
     case 5: return run_ring<256, 128, 3, 4, 2, 1, TYPE>(o, stride, s);
-    default: return run_ring<256, 256, 2, 4, 4, 1, TYPE>(o, stride, s);
+    default: return run_ring<256, 256, 2, 4, 2, 1, TYPE>(o, stride, s);
   }
 }
 
