@@ -172,7 +172,10 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
   constexpr int KS = DP / 32;                     // MFMAs of 32 dimensions
   constexpr int VB = DP / 16;                     // bytes of a value a lane holds
   constexpr int VW = VB / 4;
-  constexpr int NQ = TYPE == QC_STORAGE_F32 ? 2 : 1;   // f16 terms of q and of the probabilities
+  constexpr int NQ = TYPE == QC_STORAGE_F32 ? 2 : 1;   // f16 terms of q
+  // and of the probabilities: one rounded to 11 bits weighs as much as an f16 output's own
+  // rounding where few keys do, and the second term costs nothing beside the loads
+  constexpr int NP = TYPE == QC_STORAGE_BF16 ? 1 : 2;
   __shared__ int s_page[kMaxGroups];
   __shared__ float s_ks[kMaxGroups], s_vs[kMaxGroups];
   __shared__ float s_red[kWaves], s_m[kWaves][RT * 16], s_l[kWaves][RT * 16];
@@ -313,7 +316,7 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = v[s][j] * up;
+        const float x = in_f32(v[s][j] * up);
         qf[t][s][0][j] = static_cast<_Float16>(x);
         if constexpr (NQ == 2) qf[t][s][1][j] = static_cast<_Float16>(x - static_cast<float>(qf[t][s][0][j]));
       }
@@ -375,7 +378,7 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
     const int page[2] = {s_page[i], s_page[i1]};
     const bool whole = __builtin_amdgcn_readfirstlane(tok >= all_lo && tok + 32 <= all_hi && tok + 32 <= to &&
                                                       page[0] >= 0 && page[1] >= 0);
-    f16x8 pf[RT][NQ];
+    f16x8 pf[RT][NP];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float z[8];
@@ -409,9 +412,9 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
       for (int e = 0; e < 8; ++e) {
         const float pe = __builtin_amdgcn_exp2f(z[e] - ref);
         l[rt] += pe;
-        const float pv = pe * vr[e >> 2];
+        const float pv = in_f32(pe * vr[e >> 2]);
         pf[rt][0][e] = static_cast<_Float16>(pv);
-        if constexpr (NQ == 2) pf[rt][1][e] = static_cast<_Float16>(pv - static_cast<float>(pf[rt][0][e]));
+        if constexpr (NP == 2) pf[rt][1][e] = static_cast<_Float16>(pv - static_cast<float>(pf[rt][0][e]));
       }
     }
 #pragma unroll
@@ -432,7 +435,7 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int q = 0; q < NQ; ++q)
+          for (int q = 0; q < NP; ++q)
             acc[rt][4 * w + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][q], acc[rt][4 * w + c], 0, 0, 0);
       }
     }
@@ -753,7 +756,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
     for (int s = 0; s < NF; ++s)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = broken != broken ? 0.f : v[s][j] * up;
+        const float x = in_f32(broken != broken ? 0.f : v[s][j] * up);
         qf[s][0][j] = static_cast<_Float16>(x);
         if constexpr (NQ == 2) qf[s][1][j] = static_cast<_Float16>(x - static_cast<float>(qf[s][0][j]));
       }

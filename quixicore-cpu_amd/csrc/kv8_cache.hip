@@ -185,7 +185,6 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(Kv8Args a, void* k, vo
   raw* out = static_cast<raw*>(w.which ? v : k) + w.row * stride +
              static_cast<long long>(w.head) * a.head_dim;
   const int per_row = a.head_dim / 4, n = (w.hi - w.lo) * per_row;
-#pragma unroll 4
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint32_t c = codes[i];
     float f[4];

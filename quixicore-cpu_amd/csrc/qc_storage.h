@@ -33,11 +33,19 @@ __device__ __forceinline__ float decode(typename Storage<TYPE>::raw b) {
   else return __uint_as_float(static_cast<uint32_t>(b) << 16);
 }
 
+// The value as it stands in f32.  A conversion to f16 that the compiler sees beside the
+// product it takes becomes one instruction without the f32 rounding between, in some of the
+// places that use it and not in others.
+__device__ __forceinline__ float in_f32(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+
 template <int TYPE>
 __device__ __forceinline__ typename Storage<TYPE>::raw encode(float v) {
   if constexpr (TYPE == QC_STORAGE_F32) return __float_as_uint(v);
   else if constexpr (TYPE == QC_STORAGE_F16)
-    return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+    return __builtin_bit_cast(uint16_t, static_cast<_Float16>(in_f32(v)));
   else return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
 }
 
@@ -45,7 +53,7 @@ __device__ __forceinline__ typename Storage<TYPE>::raw encode(float v) {
 template <int TYPE>
 __device__ __forceinline__ uint32_t encode2(float a, float b) {
   static_assert(TYPE != QC_STORAGE_F32, "16-bit types");
-  const f32x2 v = {a, b};
+  const f32x2 v = {in_f32(a), in_f32(b)};
   if constexpr (TYPE == QC_STORAGE_F16)
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
   else

@@ -412,6 +412,15 @@ def test_attention_peaked_q(qc, dev, route, dtype):
         _attend(qc, dev, rng, new, kv, 4, 2, 64, 32, dtype, batch=batch, cache=cache, q=q)
 
 
+def test_attention_f32_keeps_its_second_terms(qc, dev, route):
+    """Many probabilities of some size over pages of several scales, beside small scores, so that
+    the bound is near 2^-18 of the values' sum: a probability whose two f16 terms do not belong together (one product rounded
+    in two ways, once in some 2^13) is 2^-11 of itself off."""
+    rng = np.random.default_rng(8)
+    _attend(qc, dev, rng, [1] * 256, [20 + s % 31 for s in range(256)], 16, 4, 16, 16, "float32", qmag=0.3, spread=0.3)
+    _attend(qc, dev, rng, [60] * 12, [60] * 12, 16, 4, 16, 16, "float32", qmag=0.3, spread=0.3)
+
+
 def test_attention_nonfinite_q_stays_in_its_row(qc, dev, route):
     import torch
     rng = np.random.default_rng(6)
