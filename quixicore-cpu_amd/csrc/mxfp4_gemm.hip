@@ -321,8 +321,8 @@ __global__ __launch_bounds__(64 * WGN * WGM * KG, 1) void mxfp4_ring(
   }
 }
 
-// Scale rows at a stride that is a multiple of 4 bytes: the ring's loads are
-// dwords.  Bytes past a row's blocks are zero.
+// Scale rows that begin at a multiple of 4 bytes, which the caller's need not: the
+// ring's loads are dwords.  Bytes past a row's blocks are zero.
 __global__ __launch_bounds__(256) void pad_scales(const uint8_t* __restrict__ ws, long long n,
                                                   const uint8_t* __restrict__ xs, long long m,
                                                   int blocks, int stride, uint32_t* __restrict__ out) {
@@ -398,7 +398,7 @@ hipError_t run_gemm(Operands o, int route, hipStream_t s) {
   StreamWorkspace* ws = nullptr;
   std::unique_lock<std::mutex> hold;
   int stride = o.blocks;
-  if (o.blocks % 4 != 0) {
+  if (o.blocks % 4 != 0 || ((reinterpret_cast<uintptr_t>(o.ws) | reinterpret_cast<uintptr_t>(o.xs)) & 3) != 0) {
     hipError_t e = stream_workspace(s, &ws);
     if (e != hipSuccess) return e;
     hold = std::unique_lock<std::mutex>(ws->call);

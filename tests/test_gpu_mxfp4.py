@@ -173,6 +173,27 @@ def test_product_wide_scales(qc, dev, route, m):
     _product(qc, dev, np.random.default_rng(m), m, 70, 640, spread=20)
 
 
+@pytest.mark.parametrize("at", [(1, 0), (0, 3), (2, 1)])
+def test_product_scales_at_any_byte(qc, dev, route, at):
+    """Scales cut out of a larger array begin at any byte; so may y's elements."""
+    import torch
+    g = np.random.default_rng(6)
+    m, n, k = 37, 70, 384
+    w, ws = _matrix(g, n, k)
+    x, xs = _matrix(g, m, k)
+    up = lambda a: torch.from_numpy(a).to(dev)
+
+    def cut(a, off):
+        room = torch.zeros(a.size + 8, dtype=torch.uint8, device=dev)
+        view = room[off:off + a.size].view(a.shape)
+        view.copy_(up(a))
+        return view
+    want = qc.mxfp4_gemm(up(w), up(ws), up(x), up(xs))
+    y = torch.zeros(m * n + 1, device=dev)[1:].view(m, n)
+    qc.mxfp4_gemm(up(w), cut(ws, at[0]), up(x), cut(xs, at[1]), y=y)
+    assert torch.equal(y, want)
+
+
 @pytest.mark.parametrize("m", [1, 5, 33, 140])
 def test_product_special_scales(qc, dev, route, m):
     """A NaN scale of a row reaches that row's (column's) outputs only; the smallest and
