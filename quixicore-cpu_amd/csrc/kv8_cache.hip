@@ -229,16 +229,17 @@ __global__ __launch_bounds__(kThreads) void kv8_check(Kv8Args a, bool from_new, 
   }
 }
 
-// *flag = 3 where a row of the batch's sequences holds NaN or +-inf.
+// *flag = 3 where a row of the batch's sequences holds NaN or +-inf; `parts` workgroups a
+// sequence for K and V each.
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void kv8_nonfinite(Kv8Args a, Rows k, Rows v) {
+__global__ __launch_bounds__(kThreads) void kv8_nonfinite(Kv8Args a, Rows k, Rows v, int parts) {
   typedef typename Storage<TYPE>::raw raw;
-  const int q = blockIdx.x >> 1;
+  const int part = (blockIdx.x >> 1) % parts, q = (blockIdx.x >> 1) / parts;
   int first, rows, kv;
   if (!kv8_sequence(a, q, first, rows, kv)) return;
   const Rows src = blockIdx.x & 1 ? v : k;
   const int row = a.kv_heads * a.head_dim;
-  for (int t = 0; t < rows; ++t)
+  for (int t = part; t < rows; t += parts)
     for (int i = threadIdx.x; i < row; i += kThreads)
       if (!isfinite(decode<TYPE>(static_cast<const raw*>(src.p)[(first + t) * src.stride + i])))
         *a.status = QC_INVALID_ARGUMENT;
@@ -284,11 +285,12 @@ hipError_t launch_kv8_nonfinite(const qc_kv8_cache& c, const qc_kv8_batch& b, co
                                 int* flag, hipStream_t s) {
   const Kv8Args a = kv8_args(c, b, flag);
   const Rows kr = {k, k_stride}, vr = {v, v_stride};
-  const unsigned grid = 2u * static_cast<unsigned>(a.seqs);
+  const int parts = touched_slots(a);
+  const unsigned grid = static_cast<unsigned>(2LL * parts * a.seqs);
   switch (type) {
-    case QC_STORAGE_F32: kv8_nonfinite<QC_STORAGE_F32><<<grid, kThreads, 0, s>>>(a, kr, vr); break;
-    case QC_STORAGE_F16: kv8_nonfinite<QC_STORAGE_F16><<<grid, kThreads, 0, s>>>(a, kr, vr); break;
-    default: kv8_nonfinite<QC_STORAGE_BF16><<<grid, kThreads, 0, s>>>(a, kr, vr);
+    case QC_STORAGE_F32: kv8_nonfinite<QC_STORAGE_F32><<<grid, kThreads, 0, s>>>(a, kr, vr, parts); break;
+    case QC_STORAGE_F16: kv8_nonfinite<QC_STORAGE_F16><<<grid, kThreads, 0, s>>>(a, kr, vr, parts); break;
+    default: kv8_nonfinite<QC_STORAGE_BF16><<<grid, kThreads, 0, s>>>(a, kr, vr, parts);
   }
   return hipGetLastError();
 }
