@@ -25,7 +25,8 @@
  *   - Results are deterministic: rerunning a call gives bit-identical output.
  *   - Scratch: entry points whose kernels need device scratch (qc_hip_qgemm
  *     from M = 2, the canonical int8 projections from M = 2, the affine
- *     canonical W8A8 route) take it from a per-(device, stream) cache that
+ *     canonical W8A8 route, qc_hip_kv8_attention of long caches and of long prompts,
+ *     qc_hip_mxfp4_gemm of scale rows that do not begin at multiples of 4 bytes) take it from a per-(device, stream) cache that
  *     only grows; the first call on a stream, or one needing more, allocates
  *     (hipMalloc), later calls do not.  Calls on one stream share its buffers
  *     in stream order; graphs captured on a stream keep that stream's buffers
@@ -405,7 +406,8 @@ typedef struct qc_kv8_cache {
  * rows from seq_start[seqs] on belong to no one and are neither read nor written.
  * A sequence whose figures break these bounds, or a page id that a call needs and
  * that is not in [0, pages), is an error: the sequence is left out (append,
- * gather: that page of it; attention: its rows see the other pages). */
+ * gather: that page of it; attention: its rows see the other pages).  Where
+ * sequences' rows overlap (starts that run backwards), attention may leave out others too. */
 typedef struct qc_kv8_batch {
   const int* block_table;   /* [seqs][columns] */
   const int* seq_start;     /* [seqs + 1] */
@@ -445,7 +447,7 @@ int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void
  * kv_heads, query heads h * heads / kv_heads .. sharing key head h.  Token i of n
  * stands at p = kv_len - n + i and sees the positions j < kv_len; with causal != 0
  * j <= p, and with window > 0 (causal only) j > p - window.  A row that sees nothing
- * (n > kv_len, or kv_len 0) is zeros.  Pages that no row sees are not looked at; one
+ * (n > kv_len, or kv_len 0) is zeros.  q and out do not overlap.  Pages that no row sees are not looked at; one
  * that is seen and has a scale that is not finite is an error like a bad page id.
  * The probabilities enter the product with the values in 11 bits (bf16 q, and f16 q
  * of prompts of some thousand tokens) or 22; dots, sums and statistics are f32.  Status: 1 for sizes out of range, 2 for an

@@ -48,9 +48,76 @@ struct AttnArgs {
   float* part;          // [split][tokens * heads][head_dim], then statistics
   float* stats;         // [split][tokens * heads][2]: maximum (log2 units), sum
   int splits, chunk;    // key ranges of `chunk` tokens
-  int row_blocks;
+  int per, row_blocks;  // rows of a row block, row blocks of a sequence's key head at most
+  int rows_from, rows_to;   // sequences of [rows_from, rows_to) rows a key head are worked on
+  int listed;           // what blocks are counted by: kPadded, kBlocks, kSequences
   int route;            // host: 0 by size, 1 / 2 one or two row tiles, 3 tiled
 };
+
+// Row blocks of a ragged batch.  kPadded: every sequence has row_blocks of them, most of
+// them empty where one sequence is much longer than the others (and empty workgroups
+// between those with work leave them on few of the shader engines that the grid is dealt to in
+// turn).  kBlocks: only those there are, found by a scan over the sequences; the grid
+// is what the batch's tokens allow at most, its empty workgroups last.  kSequences: those with
+// rows in range, counted alike.  us, 32 / 8 heads of 128, bf16: 256 new tokens beside 127
+// sequences of one, 1000 to 2000 keys, 1907 padded, 121 listed.
+enum { kPadded, kBlocks, kSequences };
+
+// The sequence that has the b-th of what is listed, b's place in it and the number of
+// listed sequences before it.  (The first workgroup looks at every sequence, so that a bad
+// one is told of.)
+struct Listed {
+  int seq, at, before;
+};
+__device__ __forceinline__ bool find_listed(const Kv8Args& a, const AttnArgs& p, int b, Listed& out) {
+  b = __builtin_amdgcn_readfirstlane(b);
+  const int lane = threadIdx.x & 63;
+  bool found = false;
+  int before = 0;
+  for (int base = 0; base < a.seqs; base += 64) {
+    int n = 0, first, rows, kv;
+    if (base + lane < a.seqs && kv8_sequence(a, base + lane, first, rows, kv)) {
+      const int all = rows * p.group;
+      if (all > 0 && all >= p.rows_from && all < p.rows_to) n = p.listed == kBlocks ? (all + p.per - 1) / p.per : 1;
+    }
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int below = __shfl_up(sum, o);
+      if (lane >= o) sum += below;
+    }
+    const uint64_t past = __ballot(sum > b), some = __ballot(n > 0);
+    if (past != 0 && !found) {
+      const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      out.seq = base + l;
+      out.at = b - __builtin_amdgcn_readlane(sum - n, l);
+      out.before = before + __popcll(some & ((1ull << l) - 1));
+      found = out.at >= 0;
+      if (blockIdx.x != 0) return found;
+    }
+    b -= __builtin_amdgcn_readlane(sum, 63);
+    before += __popcll(some);
+  }
+  return found;
+}
+
+// What block `id` of a grid over row blocks is: the same for a whole wavefront where
+// the grid is listed.
+__device__ __forceinline__ bool block_of(const Kv8Args& a, const AttnArgs& p, int id, int& seq, int& kvh, int& rb) {
+  if (p.listed == kPadded) {
+    rb = id % p.row_blocks;
+    id /= p.row_blocks;
+    kvh = id % a.kv_heads;
+    seq = id / a.kv_heads;
+    return true;
+  }
+  kvh = id % a.kv_heads;
+  Listed l;
+  const bool found = find_listed(a, p, id / a.kv_heads, l);
+  seq = l.seq;
+  rb = l.at;
+  return found;
+}
 
 // Keys [lo, hi) that rows of tokens t0..t1 (inclusive) see together.
 __device__ __forceinline__ void seen_range(const AttnArgs& p, const Unit& u, int t0, int t1, int& lo,
@@ -164,7 +231,7 @@ __device__ __forceinline__ void store_n(void* out, long long at, bool vec, const
 // lane & 15 at dimension 64 c + 16 g.  V: lane loads DP / 16 bytes of its eight
 // keys at dimension (DP / 16) (lane & 15), transposed in registers.
 constexpr int kWaves = 4;
-constexpr int kMaxGroups = 256;   // 16-key groups of a range
+constexpr int kMaxGroups = 1024;   // 16-key groups of a range
 
 template <int DP, int RT, int TYPE>
 __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STORAGE_F32 ? 4 : 1) void attention_direct(Kv8Args a, AttnArgs p) {
@@ -184,14 +251,11 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
   const int lane = threadIdx.x & 63, row16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // split fastest, then row block, key head, sequence
-  int id = blockIdx.x;
-  const int split = id % p.splits;
-  id /= p.splits;
-  const int rb = id % p.row_blocks;
-  id /= p.row_blocks;
-  const int kvh = id % a.kv_heads, seq = id / a.kv_heads;
+  const int split = blockIdx.x % p.splits;
+  int seq, kvh, rb;
+  if (!block_of(a, p, blockIdx.x / p.splits, seq, kvh, rb)) return;
   Unit u;
-  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return;
+  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv) || u.rows * p.group >= p.rows_to) return;
   const int r0 = rb * RT * 16, r1 = min(r0 + RT * 16, u.rows * p.group);
   if (r0 >= r1) return;
   int lo, hi;
@@ -544,17 +608,22 @@ struct Frags {
   float* ks;             // [units][cap / 16]
   float* vs;
   int cap;               // keys laid out per unit: a multiple of 64
-  int unit0;             // the pass's first unit (sequence * kv_heads + key head)
+  int unit0, units;      // the pass's units (sequence, of the listed ones, * kv_heads + key head)
 };
 
 template <int DP>
-__global__ __launch_bounds__(256) void attention_layout(Kv8Args a, Frags f, int tiles, int window) {
+__global__ __launch_bounds__(256) void attention_layout(Kv8Args a, AttnArgs p, Frags f, int tiles) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = blockIdx.x % tiles, local = blockIdx.x / tiles;
-  const int unit = f.unit0 + local;
-  const int seq = unit / a.kv_heads, kvh = unit - seq * a.kv_heads;
-  int first, rows, kv;
+  const int window = p.window;
+  const int unit = f.unit0 + local, kvh = unit % a.kv_heads;
+  int seq = unit / a.kv_heads, first, rows, kv;
+  if (p.listed != kPadded) {
+    Listed l;
+    if (!find_listed(a, p, seq, l)) return;
+    seq = l.seq;
+  }
   if (!kv8_sequence(a, seq, first, rows, kv) || rows == 0) return;
   const int lo = window > 0 ? max(0, kv - rows + 1 - window) & ~63 : 0;
   const int tok = 32 * tile;
@@ -615,11 +684,11 @@ __global__ __launch_bounds__(256) void attention_layout(Kv8Args a, Frags f, int 
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[j] = static_cast<_Float16>(0.f);
     if (vp[i] != nullptr && !v_zero[i] && d < a.head_dim) {
-      const int8_t* p = vp[i] + 4 * (lane >> 5) * a.head_dim + d;
+      const int8_t* from = vp[i] + 4 * (lane >> 5) * a.head_dim + d;
       const int sign = v_neg[i] ? -1 : 1;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        o[j] = static_cast<_Float16>(sign * p[(8 * (j >> 2) + (j & 3)) * a.head_dim]);
+        o[j] = static_cast<_Float16>(sign * from[(8 * (j >> 2) + (j & 3)) * a.head_dim]);
     }
     *reinterpret_cast<u32x4*>(f.v + (at32 * NF + s) * 512 + 8 * lane) = __builtin_bit_cast(u32x4, o);
   }
@@ -657,18 +726,31 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // unit fastest: with workgroups dealt to the XCDs in turn, a head's blocks share an L2; the
-  // longest rows (last blocks) first
-  int id = blockIdx.x;
-  const int units = gridDim.x / (p.splits * p.row_blocks);
-  const int local = id % units;
-  id /= units;
-  const int split = id % p.splits;
-  const int rb = p.row_blocks - 1 - id / p.splits;
-  const int unit_id = f.unit0 + local;
-  const int seq = unit_id / a.kv_heads, kvh = unit_id - seq * a.kv_heads;
+  // unit (listed: key head) fastest: with workgroups dealt to the XCDs in turn, a head's
+  // blocks share an L2; the longest rows (last blocks) first
+  int id = blockIdx.x, local, split, rb, seq;
   Unit u;
-  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return;
+  if (p.listed == kPadded) {
+    const int units = gridDim.x / (p.splits * p.row_blocks);
+    local = id % units;
+    id /= units;
+    split = id % p.splits;
+    rb = p.row_blocks - 1 - id / p.splits;
+    seq = (f.unit0 + local) / a.kv_heads;
+    if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return;
+  } else {
+    local = id % a.kv_heads;
+    id /= a.kv_heads;
+    split = id % p.splits;
+    Listed l;
+    if (!find_listed(a, p, id / p.splits, l)) return;
+    seq = l.seq;
+    local += l.before * a.kv_heads - f.unit0;
+    if (local < 0 || local >= f.units || !kv8_sequence(a, seq, u.first, u.rows, u.kv)) return;
+    rb = (u.rows * p.group + p.per - 1) / p.per - 1 - l.at;
+    if (rb < 0) return;
+  }
+  const int kvh = (f.unit0 + local) % a.kv_heads;
   const int r0 = rb * NW * 32, r1 = min(r0 + NW * 32, u.rows * p.group);
   if (r0 >= r1) return;
   int lo, hi;
@@ -924,21 +1006,32 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
     }
 }
 
+// Row `item` of a join's grid: `per` rows of each row block.
+__device__ __forceinline__ bool join_row(const Kv8Args& a, const AttnArgs& p, int item, int per, Unit& u, int& token,
+                                         int& head) {
+  int seq, kvh, rb;
+  if (!block_of(a, p, item / per, seq, kvh, rb) || seq >= a.seqs) return false;
+  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return false;
+  const int r = rb * p.per + item % per, all = u.rows * p.group;
+  if (r >= all || all < p.rows_from || all >= p.rows_to) return false;
+  token = r / p.group;
+  head = kvh * p.group + r - token * p.group;
+  return true;
+}
+
 // out = sum over the ranges of 2^(m_s - m) O_s over that of 2^(m_s - m) l_s: a
 // workgroup a row.  256 / L groups of L threads (L >= head_dim / 4, a power of two) take the
 // ranges in turn, four loads ahead, and meet in LDS in a fixed order.  (A wavefront a
-// row, its ranges one after the other: 128 ranges of 32 rows 30 us, 5 so.)
+// row, its ranges one after the other: 128 ranges of 32 rows 30 us, 5 so.)  `per`: rows of
+// a block that are launched.
 template <int TYPE>
-__global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p, int shift) {
+__global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p, int per, int shift) {
   __shared__ float s_w[256], s_red[8];
   __shared__ f32x4 s_o[256];
   const int tid = threadIdx.x;
-  const unsigned item = blockIdx.x, per_seq = static_cast<unsigned>(a.max_new) * p.heads;
-  const int seq = item / per_seq;
-  const int rest = item - seq * per_seq;
-  const int token = rest / p.heads, head = rest - token * p.heads;
   Unit u;
-  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv) || token >= u.rows) return;
+  int token, head;
+  if (!join_row(a, p, blockIdx.x, per, u, token, head)) return;
   const long long rows = static_cast<long long>(a.tokens) * p.heads;
   const long long row = static_cast<long long>(u.first + token) * p.heads + head;
   const float* stats = p.stats + 2 * row;
@@ -996,15 +1089,12 @@ __global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p, int
 // two or four have thousands of rows, and a workgroup for each is mostly its own start.
 constexpr int kFewSplits = 8;
 template <int TYPE>
-__global__ __launch_bounds__(256) void attention_join_few(Kv8Args a, AttnArgs p, int shift) {
-  const unsigned item = (blockIdx.x * 256 + threadIdx.x) >> shift, per_seq = static_cast<unsigned>(a.max_new) * p.heads;
-  const int seq = item / per_seq;
-  if (seq >= a.seqs) return;
-  const int rest = item - seq * per_seq;
-  const int token = rest / p.heads, head = rest - token * p.heads;
+__global__ __launch_bounds__(256) void attention_join_few(Kv8Args a, AttnArgs p, int per, int shift) {
   const int d = 4 * (threadIdx.x & ((1 << shift) - 1));
   Unit u;
-  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv) || token >= u.rows || d >= a.head_dim) return;
+  int token, head;
+  // (a wavefront's rows, 16 at most, are one block's where blocks are listed)
+  if (!join_row(a, p, blockIdx.x * (256 >> shift) + (threadIdx.x >> shift), per, u, token, head) || d >= a.head_dim) return;
   const long long rows = static_cast<long long>(a.tokens) * p.heads;
   const long long row = static_cast<long long>(u.first + token) * p.heads + head;
   float ms[kFewSplits], ls[kFewSplits], m = -INFINITY, l = 0.f;
@@ -1048,18 +1138,21 @@ hipError_t part_buffers(const Kv8Args& a, AttnArgs& p, StreamWorkspace* ws, hipS
   return e;
 }
 
+// blocks: row blocks of all key heads (what block_of takes).
 template <int TYPE>
-hipError_t run_join(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
-  const long long items = static_cast<long long>(a.seqs) * a.max_new * p.heads;
+hipError_t run_join(const Kv8Args& a, const AttnArgs& p, long long blocks, hipStream_t s) {
   int shift = 2;
   while ((4 << shift) < a.head_dim) ++shift;
-  if (items > (INT_MAX >> shift)) return hipErrorInvalidValue;
+  const bool one = p.listed != kBlocks && p.row_blocks == 1;
+  const int per = one ? std::min<long long>(p.per, static_cast<long long>(a.max_new) * p.group) : p.per;
+  const long long items = blocks * per;
+  if (items > INT_MAX - 256) return hipErrorInvalidValue;
   if (p.splits <= kFewSplits) {
-    const unsigned grid = static_cast<unsigned>(((items << shift) + 255) / 256);
-    attention_join_few<TYPE><<<grid, 256, 0, s>>>(a, p, shift);
+    const int rows = 256 >> shift;
+    attention_join_few<TYPE><<<static_cast<unsigned>((items + rows - 1) / rows), 256, 0, s>>>(a, p, per, shift);
     return hipGetLastError();
   }
-  attention_join<TYPE><<<static_cast<unsigned>(items), 256, 0, s>>>(a, p, shift);
+  attention_join<TYPE><<<static_cast<unsigned>(items), 256, 0, s>>>(a, p, per, shift);
   return hipGetLastError();
 }
 
@@ -1071,14 +1164,20 @@ long long key_span(const Kv8Args& a, const AttnArgs& p, int rows, int align) {
 
 template <int DP, int RT, int TYPE>
 hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
-  const long long rows = static_cast<long long>(a.max_new) * p.group;
-  p.row_blocks = static_cast<int>((rows + RT * 16 - 1) / (RT * 16));
+  const long long rows = std::min<long long>(static_cast<long long>(a.max_new) * p.group, p.rows_to - 1);
+  p.per = RT * 16;
+  p.row_blocks = static_cast<int>((rows + p.per - 1) / p.per);
   const long long span = key_span(a, p, RT * 16, 32);
-  const long long units = static_cast<long long>(a.seqs) * a.kv_heads * p.row_blocks;
+  const long long padded = static_cast<long long>(a.seqs) * p.row_blocks;
+  const long long there = static_cast<long long>(a.tokens) * p.group / p.per + a.seqs;   // at most
+  p.listed = 2 * padded > 3 * there ? kBlocks : kPadded;
+  const long long units = std::min(padded, p.listed == kBlocks ? there : padded) * a.kv_heads;
   const long long want = std::max<long long>(1, 2LL * device_cu_count() / units);
   long long chunk = (span + want - 1) / want;
   chunk = std::max<long long>(32 * kWaves, (chunk + 31) / 32 * 32);
-  chunk = std::min<long long>(chunk, 16 * kMaxGroups);
+  // ranges of 4096 keys at most, or of 16384 where their sums would take more than 1 GB
+  const long long range_bytes = static_cast<long long>(a.tokens) * p.heads * (a.head_dim + 2) * 4;
+  chunk = std::min<long long>(chunk, (span + 4095) / 4096 * range_bytes > (1LL << 30) ? 16 * kMaxGroups : 4096);
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((span + chunk - 1) / chunk);
   const long long grid = units * p.splits;
@@ -1094,7 +1193,7 @@ hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   attention_direct<DP, RT, TYPE><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
-  return run_join<TYPE>(a, p, s);
+  return run_join<TYPE>(a, p, units, s);
 }
 
 // Bytes of fragments laid out at a time; a call with more goes in passes of whole units.
@@ -1103,10 +1202,16 @@ constexpr long long kFragPass = 1LL << 30;
 template <int DP, int NW, int TYPE>
 hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   const long long rows = static_cast<long long>(a.max_new) * p.group;
-  p.row_blocks = static_cast<int>((rows + 32 * NW - 1) / (32 * NW));
+  p.per = 32 * NW;
+  p.row_blocks = static_cast<int>((rows + p.per - 1) / p.per);
   const long long span = key_span(a, p, 32 * NW, 64);
-  const long long units = static_cast<long long>(a.seqs) * a.kv_heads;
-  const long long want = std::max<long long>(1, device_cu_count() / (units * p.row_blocks));
+  const long long all = static_cast<long long>(a.tokens) * p.group;
+  const long long seqs = p.rows_from > 0 ? std::min<long long>(a.seqs, all / p.rows_from) : a.seqs;
+  const long long units = seqs * a.kv_heads;
+  const long long padded = seqs * p.row_blocks, there = all / p.per + seqs;   // at most
+  p.listed = p.rows_from > 0 || padded > there ? kBlocks : kPadded;
+  const long long blocks = p.listed == kBlocks ? std::min(padded, there) : padded;
+  const long long want = std::max<long long>(1, device_cu_count() / (blocks * a.kv_heads));
   long long chunk = ((span + want - 1) / want + 63) / 64 * 64;
   chunk = std::max<long long>(chunk, 1024);
   chunk = std::min<long long>(chunk, 16 * kTiledGroups);
@@ -1116,7 +1221,7 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   f.cap = (a.max_kv + 63) / 64 * 64;
   const long long unit_bytes = static_cast<long long>(f.cap) * DP * 4 + f.cap / 2;   // two of f16, scales
   const long long pass = std::min(units, std::max<long long>(1, kFragPass / unit_bytes));
-  if (pass * p.splits * p.row_blocks > INT_MAX || pass * (f.cap / 32) > INT_MAX) return hipErrorInvalidValue;
+  if (blocks * a.kv_heads * p.splits > INT_MAX || pass * (f.cap / 32) > INT_MAX) return hipErrorInvalidValue;
   StreamWorkspace* ws = nullptr;
   hipError_t e = stream_workspace(s, &ws);
   if (e != hipSuccess) return e;
@@ -1131,13 +1236,17 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   for (long long u0 = 0; u0 < units; u0 += pass) {
     const int n = static_cast<int>(std::min(pass, units - u0));
     f.unit0 = static_cast<int>(u0);
+    f.units = n;
     const int tiles = f.cap / 32;
-    attention_layout<DP><<<static_cast<unsigned>(n) * tiles, 256, 0, s>>>(a, f, tiles, p.window);
+    AttnArgs lay = p;
+    if (p.listed != kPadded) lay.listed = kSequences;
+    attention_layout<DP><<<static_cast<unsigned>(n) * tiles, 256, 0, s>>>(a, lay, f, tiles);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    attention_tiled<DP, NW, TYPE><<<static_cast<unsigned>(n) * p.splits * p.row_blocks, 64 * NW, 0, s>>>(a, p, f);
+    const long long grid = (p.listed == kPadded ? n * p.row_blocks : blocks * a.kv_heads) * p.splits;
+    attention_tiled<DP, NW, TYPE><<<static_cast<unsigned>(grid), 64 * NW, 0, s>>>(a, p, f);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  return p.splits > 1 ? run_join<TYPE>(a, p, s) : hipSuccess;
+  return p.splits > 1 ? run_join<TYPE>(a, p, blocks * a.kv_heads, s) : hipSuccess;
 }
 
 // The tiled form lays the cache out first (and reads 64 keys for 256 rows at a time), so it
@@ -1150,20 +1259,37 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
 // one makes twice the workgroups.  us, one / two, 4 query heads a key head: 8 new of 8192
 // 18 / 24, 64 of 4096 28 / 29, 16 of 4096 four times (2^19 = row tiles x keys) 27 / 26, eight
 // times 43 / 37, 100 of 16384 106 / 79.
+//
+// A ragged batch may hold both kinds: the rows counted are those that its tokens allow, and where
+// not every sequence can have 2048 a key head, those that have are laid out and the others
+// read directly: 4096 new tokens beside 63 sequences of one, 4000 to 8000 keys, 2317 us
+// with all laid out, 695 so (the prompt alone 480, the others 170).
 template <int DP, int TYPE>
-hipError_t run_rows(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
-  const double units = static_cast<double>(a.seqs) * a.kv_heads;
-  const double rows = static_cast<double>(a.max_new) * p.group;
+hipError_t run_rows(const Kv8Args& a, AttnArgs p, hipStream_t s) {
+  constexpr int kLong = 2048;
+  const double rows = static_cast<double>(a.max_new) * p.group, tokens_rows = static_cast<double>(a.tokens) * p.group;
+  const double all = std::min(a.seqs * rows, tokens_rows) * a.kv_heads;
   double keys = a.max_kv;
   if (p.causal) keys -= 0.5 * std::min(a.max_new, a.max_kv);
   if (p.window > 0) keys = std::min<double>(keys, p.window);
-  const bool many = rows >= 2048 && units * rows * keys * a.head_dim >= 0x1p31;
-  if (p.route == 0 ? many : p.route == 3)
-    return run_tiled<DP, DP == 256 ? 4 : 8, TYPE>(a, p, s);
-  const bool two = p.route == 0 ? rows > 16 && units * (rows / 16) * keys >= 0x1p19 : p.route == 2;
-  if constexpr (DP < 256 || TYPE != QC_STORAGE_F32)   // (two of f32 256 do not fit the registers)
-    if (two) return run_direct<DP, 2, TYPE>(a, p, s);
-  return run_direct<DP, 1, TYPE>(a, p, s);
+  const bool many = rows >= kLong && all * keys * a.head_dim >= 0x1p31;
+  constexpr int NW = DP == 256 ? 4 : 8;
+  p.rows_to = INT_MAX;
+  if (p.route == 3 || (p.route == 0 && many && tokens_rows >= static_cast<double>(a.seqs) * kLong))
+    return run_tiled<DP, NW, TYPE>(a, p, s);
+  const bool both = p.route == 0 && many;
+  if (both) p.rows_to = kLong;
+  const bool two = p.route == 0 ? rows > 16 && (all / 16) * keys >= 0x1p19 : p.route == 2;
+  hipError_t e = hipSuccess;
+  if constexpr (DP < 256 || TYPE != QC_STORAGE_F32) {   // (two of f32 256 do not fit the registers)
+    e = two ? run_direct<DP, 2, TYPE>(a, p, s) : run_direct<DP, 1, TYPE>(a, p, s);
+  } else {
+    e = run_direct<DP, 1, TYPE>(a, p, s);
+  }
+  if (!both || e != hipSuccess) return e;
+  p.rows_from = kLong;
+  p.rows_to = INT_MAX;
+  return run_tiled<DP, NW, TYPE>(a, p, s);
 }
 
 template <int TYPE>

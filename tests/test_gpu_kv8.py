@@ -356,6 +356,21 @@ def test_attention_prompts(qc, dev, route, dtype, new, kv, heads, kvh, hd, page,
     _attend(qc, dev, rng, new, kv, heads, kvh, hd, page, dtype, causal, window, spare=2)
 
 
+@pytest.mark.parametrize("dtype,new,kv,heads,kvh,hd,page,window", [
+    ("bfloat16", [1] * 30 + [90] + [0, 1, 1], [200] * 30 + [120] + [0, 64, 33], 8, 2, 64, 16, 0),
+    ("float32", [70] + [2] * 70, [70] + [2 + 7 * i for i in range(70)], 4, 2, 32, 16, 0),
+    ("float16", [1] * 129 + [200, 0, 3], [1 + i for i in range(129)] + [210, 40, 3], 6, 1, 80, 32, 40),
+    ("bfloat16", [1, 600, 0, 2, 1, 200, 90, 129, 128, 127], [700, 4200, 9, 2, 0, 200, 800, 129, 4000, 300], 32, 2, 64, 64, 0),
+    ("bfloat16", [400] + [1] * 9, [9000] + [8990 - 997 * i for i in range(9)], 16, 1, 128, 128, 0),
+    ("float32", [1] * 5 + [500] + [3, 130], [50] * 5 + [4500] + [4400, 2000], 16, 1, 64, 16, 0)])
+def test_attention_ragged(qc, dev, route, dtype, new, kv, heads, kvh, hd, page, window):
+    """Batches whose longest sequence is far longer than most: the row blocks there are
+    get listed, and with 2048 rows a key head and enough work long and short go ways of their own."""
+    print(f"kv8 attention ragged {dtype} {len(new)} sequences, heads {heads}/{kvh} hd {hd} {window}", flush=True)
+    rng = np.random.default_rng(len(new))
+    _attend(qc, dev, rng, new, kv, heads, kvh, hd, page, dtype, window=window, spare=3)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("new,kv", [([5, 1, 3], [2, 0, 3]), ([200, 7], [100, 0]), ([300], [40]), ([40, 33], [0, 31])])
 @pytest.mark.parametrize("causal", [True, False])
@@ -561,6 +576,37 @@ def test_attention_repeats_and_graph(qc, dev, route, new, kv, heads, kvh):
     del graph
 
 
+def test_attention_from_threads(qc, dev):
+    """Calls of several host threads, on one stream and on streams of their own, each with
+    keys that are split and joined: every result is the lone call's."""
+    import threading
+    import torch
+    rng = np.random.default_rng(17)
+    batch = Ragged(rng, [1, 40, 1], [1500, 900, 30], 32)
+    cache = _random_cache(qc, dev, rng, batch.pages, 2, 32, 64)
+    b = batch.device(qc, dev)
+    qs = [torch.from_numpy(rng.standard_normal((batch.tokens, 8, 64))).to(dev, torch.bfloat16) for _ in range(4)]
+    want = [qc.kv8_attention(cache, b, q) for q in qs]
+    torch.cuda.synchronize()
+    shared, wrong = torch.cuda.Stream(), []
+
+    def work(i):
+        st = torch.zeros(1, dtype=torch.int32, device=dev)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(shared if i < 2 else torch.cuda.Stream()):
+            for _ in range(25):
+                out = qc.kv8_attention(cache, b, qs[i], dev_status=st)
+                if not torch.equal(out, want[i]):
+                    wrong.append(i)
+                    return
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_attention_strided_rows(qc, dev, route):
     """q inside fused projection rows, out inside wider rows; odd element offsets."""
     import torch
@@ -671,13 +717,15 @@ def test_a_low_bit_layer(qc, dev, route):
     assert st.item() == 0
 
 
-def test_attention_passes_of_the_layout(qc, dev):
+@pytest.mark.parametrize("new,kv,route", [
+    ([1] * 70, 4096, 3), ([1] * 40 + [260] + [1] * 29, 4096, 3), ([1] * 9 + [1024] * 17 + [1] * 50, 16384, 0)])
+def test_attention_passes_of_the_layout(qc, dev, new, kv, route):
     """More keys than are laid out at a time (1 GB): several passes, the same values as read
     directly, within both forms' rounding."""
     import torch
     rng = np.random.default_rng(70)
-    seqs, kvh, hd, kv = 70, 8, 128, 4096
-    batch = Ragged(rng, [1] * seqs, [kv - 37 * (s % 5) for s in range(seqs)], 64)
+    seqs, kvh, hd = len(new), 8, 128
+    batch = Ragged(rng, new, [kv - 37 * (s % 5) for s in range(seqs)], 64)
     g = torch.Generator(device=dev).manual_seed(3)
     shape = (batch.pages, kvh, 64, hd)
     codes = [torch.randint(-127, 128, shape, generator=g, device=dev, dtype=torch.int8) for _ in range(2)]
@@ -688,7 +736,7 @@ def test_attention_passes_of_the_layout(qc, dev):
     try:
         qc.set_kv8_attention_route(1)
         direct = qc.kv8_attention(cache, b, q)
-        qc.set_kv8_attention_route(3)
+        qc.set_kv8_attention_route(route)
         tiled = qc.kv8_attention(cache, b, q)
     finally:
         qc.set_kv8_attention_route(0)
