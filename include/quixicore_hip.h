@@ -407,7 +407,7 @@ typedef struct qc_kv8_cache {
  * A sequence whose figures break these bounds, or a page id that a call needs and
  * that is not in [0, pages), is an error: the sequence is left out (append,
  * gather: that page of it; attention: its rows see the other pages).  Where
- * sequences' rows overlap (starts that run backwards), attention may leave out others too. */
+ * sequences' rows overlap (starts that run backwards), others may be left out too. */
 typedef struct qc_kv8_batch {
   const int* block_table;   /* [seqs][columns] */
   const int* seq_start;     /* [seqs + 1] */

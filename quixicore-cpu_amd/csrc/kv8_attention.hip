@@ -54,51 +54,18 @@ struct AttnArgs {
   int route;            // host: 0 by size, 1 / 2 one or two row tiles, 3 tiled
 };
 
-// Row blocks of a ragged batch.  kPadded: every sequence has row_blocks of them, most of
-// them empty where one sequence is much longer than the others (and empty workgroups
-// between those with work leave them on few of the shader engines that the grid is dealt to in
-// turn).  kBlocks: only those there are, found by a scan over the sequences; the grid
-// is what the batch's tokens allow at most, its empty workgroups last.  kSequences: those with
-// rows in range, counted alike.  us, 32 / 8 heads of 128, bf16: 256 new tokens beside 127
-// sequences of one, 1000 to 2000 keys, 1907 padded, 121 listed.
+// How blocks are counted.  kPadded: every sequence has row_blocks of them.  kBlocks:
+// only those there are.  kSequences: one for each sequence with rows in range.  us, 32 / 8
+// heads of 128, bf16: 256 new tokens beside 127 sequences of one, 1000 to 2000 keys, 1907
+// padded, 118 listed.
 enum { kPadded, kBlocks, kSequences };
 
-// The sequence that has the b-th of what is listed, b's place in it and the number of
-// listed sequences before it.  (The first workgroup looks at every sequence, so that a bad
-// one is told of.)
-struct Listed {
-  int seq, at, before;
-};
-__device__ __forceinline__ bool find_listed(const Kv8Args& a, const AttnArgs& p, int b, Listed& out) {
-  b = __builtin_amdgcn_readfirstlane(b);
-  const int lane = threadIdx.x & 63;
-  bool found = false;
-  int before = 0;
-  for (int base = 0; base < a.seqs; base += 64) {
-    int n = 0, first, rows, kv;
-    if (base + lane < a.seqs && kv8_sequence(a, base + lane, first, rows, kv)) {
-      const int all = rows * p.group;
-      if (all > 0 && all >= p.rows_from && all < p.rows_to) n = p.listed == kBlocks ? (all + p.per - 1) / p.per : 1;
-    }
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int below = __shfl_up(sum, o);
-      if (lane >= o) sum += below;
-    }
-    const uint64_t past = __ballot(sum > b), some = __ballot(n > 0);
-    if (past != 0 && !found) {
-      const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      out.seq = base + l;
-      out.at = b - __builtin_amdgcn_readlane(sum - n, l);
-      out.before = before + __popcll(some & ((1ull << l) - 1));
-      found = out.at >= 0;
-      if (blockIdx.x != 0) return found;
-    }
-    b -= __builtin_amdgcn_readlane(sum, 63);
-    before += __popcll(some);
-  }
-  return found;
+__device__ __forceinline__ bool find_listed(const Kv8Args& a, const AttnArgs& p, int b, Kv8Listed& out) {
+  return kv8_find(a, b, out, [&](int rows, int) {
+    const int all = rows * p.group;
+    if (all < p.rows_from || all >= p.rows_to) return 0;
+    return p.listed == kBlocks ? (all + p.per - 1) / p.per : 1;
+  });
 }
 
 // What block `id` of a grid over row blocks is: the same for a whole wavefront where
@@ -112,7 +79,7 @@ __device__ __forceinline__ bool block_of(const Kv8Args& a, const AttnArgs& p, in
     return true;
   }
   kvh = id % a.kv_heads;
-  Listed l;
+  Kv8Listed l;
   const bool found = find_listed(a, p, id / a.kv_heads, l);
   seq = l.seq;
   rb = l.at;
@@ -620,7 +587,7 @@ __global__ __launch_bounds__(256) void attention_layout(Kv8Args a, AttnArgs p, F
   const int unit = f.unit0 + local, kvh = unit % a.kv_heads;
   int seq = unit / a.kv_heads, first, rows, kv;
   if (p.listed != kPadded) {
-    Listed l;
+    Kv8Listed l;
     if (!find_listed(a, p, seq, l)) return;
     seq = l.seq;
   }
@@ -742,7 +709,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
     local = id % a.kv_heads;
     id /= a.kv_heads;
     split = id % p.splits;
-    Listed l;
+    Kv8Listed l;
     if (!find_listed(a, p, id / p.splits, l)) return;
     seq = l.seq;
     local += l.before * a.kv_heads - f.unit0;
@@ -1170,7 +1137,7 @@ hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   const long long span = key_span(a, p, RT * 16, 32);
   const long long padded = static_cast<long long>(a.seqs) * p.row_blocks;
   const long long there = static_cast<long long>(a.tokens) * p.group / p.per + a.seqs;   // at most
-  p.listed = 2 * padded > 3 * there ? kBlocks : kPadded;
+  p.listed = kv8_listed(padded, there) ? kBlocks : kPadded;
   const long long units = std::min(padded, p.listed == kBlocks ? there : padded) * a.kv_heads;
   const long long want = std::max<long long>(1, 2LL * device_cu_count() / units);
   long long chunk = (span + want - 1) / want;

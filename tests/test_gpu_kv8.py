@@ -96,7 +96,10 @@ def _same_cache(cache, host):
     (3, 80, 32, [0, 5, 33, 70], [9, 5, 64, 131], 4),
     (5, 96, 128, [200, 0, 1], [300, 0, 129], 0),
     (2, 256, 256, [257, 3], [600, 3], 1),
-    (4, 48, 16, [100, 31, 16, 15], [100, 47, 32, 30], 7)])
+    (4, 48, 16, [100, 31, 16, 15], [100, 47, 32, 30], 7),
+    # one sequence far longer than the others
+    (2, 32, 16, [1] * 70 + [150, 0, 20], [1 + 3 * i for i in range(70)] + [155, 0, 20], 3),
+    (1, 64, 32, [400] + [0] * 9 + [3, 1], [400] + [5] * 9 + [40, 1], 1)])
 def test_append_gather(qc, dev, dtype, heads, hd, page, new, kv, spare):
     import torch
     print(f"kv8 append {dtype} heads {heads} hd {hd} page {page} new {new} kv {kv}", flush=True)
@@ -227,6 +230,52 @@ def test_append_errors(qc, dev):
         st = torch.zeros(1, dtype=torch.int32, device=dev)
         qc.kv8_append(cache, b, up(np.abs(k)), up(np.abs(v)), dev_status=st)
         assert st.item() == 3
+
+
+def test_errors_in_ragged_batches(qc, dev, route):
+    """Bad sequences anywhere in a batch whose blocks are listed, the last one among them, are
+    told of and left out; the others are done."""
+    import torch
+    rng = np.random.default_rng(21)
+    new, kv = [150] + [1] * 130, [150] + [1 + i for i in range(130)]
+    heads, hd = 2, 64
+    for bad in (1, 63, 64, 130):
+        batch = Ragged(rng, new, kv, 16)
+        cache = _random_cache(qc, dev, rng, batch.pages, heads, 16, hd)
+        k, v, q = (torch.from_numpy(rng.standard_normal((batch.tokens, n, hd)).astype(np.float32)).to(dev)
+                   for n in (heads, heads, 8))
+        row = int(batch.start[bad])
+        rest = torch.arange(batch.tokens, device=dev) != row
+        for figure in (-1, 0, batch.max_kv + 1):
+            host = _host(cache)
+            good = batch.device(qc, dev)
+            want = qc.kv8_attention(cache, good, q)
+            b = batch.device(qc, dev)
+            b.tensors[2][bad] = figure
+            st = torch.zeros(1, dtype=torch.int32, device=dev)
+            out = torch.full_like(q, 7.0)
+            qc.kv8_attention(cache, b, q, out=out, dev_status=st)
+            assert torch.equal(out[rest], want[rest])
+            if figure == 0:                       # no error here: a row that sees nothing
+                assert st.item() == 0 and bool((out[row] == 0).all())
+            else:
+                assert st.item() == 3 and bool((out[row] == 7).all())
+            st.zero_()
+            gk = torch.full_like(k, 7.0)
+            gv = torch.full_like(v, 7.0)
+            qc.kv8_gather(cache, b, k=gk, v=gv, dev_status=st)
+            assert st.item() == 3
+            full = qc.kv8_gather(cache, good)
+            assert torch.equal(gk[rest], full[0][rest]) and torch.equal(gv[rest], full[1][rest])
+            assert bool((gk[row] == 7).all()) and bool((gv[row] == 7).all())
+            st.zero_()
+            qc.kv8_append(cache, b, k, v, dev_status=st)
+            assert st.item() == 3
+            sub = Ragged(rng, batch.new, batch.kv, 16)
+            sub.table, sub.pages = batch.table, batch.pages
+            sub.new = [n if s != bad else 0 for s, n in enumerate(batch.new)]
+            _append_reference(host, sub, k.cpu().numpy(), v.cpu().numpy())
+            _same_cache(cache, host)
 
 
 # ---- attention --------------------------------------------------------------------
