@@ -402,7 +402,8 @@ typedef struct qc_kv8_cache {
  * the batch's `tokens` token rows are sequence s's new tokens (none is allowed);
  * kv_len[s] counts its tokens in the cache, the new ones last.  Position p of it
  * lies in page block_table[s * columns + p / page_tokens], slot p % page_tokens.
- * Host bounds: no sequence has more than max_new new tokens or max_kv tokens;
+ * Host bounds: no sequence has more than max_new new tokens (which may exceed tokens)
+ * or max_kv tokens (at most columns * page_tokens);
  * rows from seq_start[seqs] on belong to no one and are neither read nor written.
  * A sequence whose figures break these bounds, or a page id that a call needs and
  * that is not in [0, pages), is an error: the sequence is left out (append,

@@ -202,9 +202,9 @@ bool kv8_shapes(const qc_kv8_cache& c, const qc_kv8_batch& b) {
   if (c.pages > INT_MAX || c.kv_heads > INT_MAX / 256 || b.seqs > INT_MAX - 1 || b.tokens > INT_MAX ||
       b.columns * c.page_tokens > INT_MAX - 512)
     return false;
-  if (b.max_new > b.tokens || b.max_kv > b.columns * c.page_tokens) return false;
+  if (b.max_kv > b.columns * c.page_tokens) return false;
   // a workgroup per sequence, touched page and head
-  const long long slots = (b.max_new + c.page_tokens - 2) / c.page_tokens + 1;
+  const long long slots = (std::min(b.max_new, b.tokens) + c.page_tokens - 2) / c.page_tokens + 1;
   return valid_product({2, c.kv_heads, slots, b.seqs}) && 2 * c.kv_heads * slots * b.seqs <= INT_MAX;
 }
 
@@ -915,7 +915,7 @@ int qc_hip_kv8_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, c
   if (heads <= 0 || heads % cache->kv_heads != 0 || heads > INT_MAX / 256 || window < 0)
     return QC_INVALID_SHAPE;
   // rows of a sequence and key head are counted in an int
-  if (batch->max_new * (heads / cache->kv_heads) > INT_MAX / 2) return QC_INVALID_SHAPE;
+  if (std::min(batch->max_new, batch->tokens) * (heads / cache->kv_heads) > INT_MAX / 2) return QC_INVALID_SHAPE;
   const long long row = heads * cache->head_dim, most = LLONG_MAX / 8 / batch->tokens;
   if (q_stride < row || out_stride < row || q_stride > most || out_stride > most)
     return QC_INVALID_SHAPE;

@@ -292,7 +292,7 @@ Kv8Args kv8_args(const qc_kv8_cache& c, const qc_kv8_batch& b, int* status) {
   a.seqs = static_cast<int>(b.seqs);
   a.columns = static_cast<int>(b.columns);
   a.tokens = static_cast<int>(b.tokens);
-  a.max_new = static_cast<int>(b.max_new);
+  a.max_new = static_cast<int>(std::min(b.max_new, b.tokens));
   a.max_kv = static_cast<int>(b.max_kv);
   a.status = status;
   return a;

@@ -11,7 +11,7 @@ namespace qc {
 
 // A call's cache and batch with the limits the host checked: pages, heads,
 // page_tokens (a power of two, 16..256), head_dim (a multiple of 16, 16..256), seqs,
-// columns, tokens, max_new and max_kv positive and within int.
+// columns, tokens, max_new (at most tokens) and max_kv positive and within int.
 struct Kv8Args {
   int8_t* k_codes;
   int8_t* v_codes;

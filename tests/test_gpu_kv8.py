@@ -232,6 +232,28 @@ def test_append_errors(qc, dev):
         assert st.item() == 3
 
 
+@pytest.mark.parametrize("bound", [9, 1000, 1 << 40])
+def test_loose_bound_of_new_tokens(qc, dev, bound):
+    """max_new is a bound only: one above the batch's tokens changes nothing."""
+    import torch
+    rng = np.random.default_rng(2)
+    batch = Ragged(rng, [1, 3], [17, 20], 16)
+    cache = _random_cache(qc, dev, rng, batch.pages, 2, 16, 32)
+    exact = batch.device(qc, dev)
+    loose = qc.Kv8Batch(*exact.tensors, batch.tokens, bound, batch.max_kv)
+    host = _host(cache)
+    k, v = (torch.from_numpy(rng.standard_normal((batch.tokens, 2, 32)).astype(np.float32)).to(dev) for _ in range(2))
+    q = torch.randn(batch.tokens, 4, 32, device=dev)
+    st = torch.zeros(1, dtype=torch.int32, device=dev)
+    qc.kv8_append(cache, loose, k, v, dev_status=st)
+    _append_reference(host, batch, k.cpu().numpy(), v.cpu().numpy())
+    _same_cache(cache, host)
+    for a, b in zip(qc.kv8_gather(cache, loose, dev_status=st), qc.kv8_gather(cache, exact)):
+        assert torch.equal(a, b)
+    assert torch.equal(qc.kv8_attention(cache, loose, q), qc.kv8_attention(cache, exact, q))
+    assert st.item() == 0
+
+
 def test_errors_in_ragged_batches(qc, dev, route):
     """Bad sequences anywhere in a batch whose blocks are listed, the last one among them, are
     told of and left out; the others are done."""
