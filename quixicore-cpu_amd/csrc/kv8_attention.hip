@@ -844,24 +844,36 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
   // quarter i of a step's score products: key tile i / 2, one half of the dimensions
-  auto scores = [&](const uint8_t* kb, int i, f32x16 (&o)[2]) {
+  auto scores = [&](const f16x8 (&k)[NF / 2], int i, f32x16 (&o)[2]) {
     const int t = i >> 1;
     if ((i & 1) == 0) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
     }
 #pragma unroll
-    for (int d = (i & 1) * NF / 2; d < ((i & 1) + 1) * NF / 2; ++d) {
-      const f16x8 k = *reinterpret_cast<const f16x8*>(kb + (t * NF + d) * 1024);
+    for (int d = 0; d < NF / 2; ++d)
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[d][q], o[t], 0, 0, 0);
-    }
+      for (int q = 0; q < NQ; ++q)
+        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[d], qf[(i & 1) * (NF / 2) + d][q], o[t], 0, 0, 0);
+  };
+  // The compiler reads a fragment from LDS just before the MFMA that takes it; reads kept where
+  // they are written have a quarter's arithmetic to arrive in (us, heads of 64 / 128 / 256: 99.6
+  // -> 95.1 / 533 -> 528 / 193 -> 174).  With two terms the registers do not hold V's beside K's, and
+  // the compiler keeps the order (f32, 128: 116 -> 113; pinned 191).
+  auto pin = [] {
+    if constexpr (NQ == 1) __builtin_amdgcn_sched_barrier(0);
   };
   if (steps > 0) wait_vmcnt<2 * (S - 1) * LOADS>();   // K of step 0
   __syncthreads();
   if (steps > 0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) scores(s_k + 16 * lane, i, s);
+    for (int i = 0; i < 4; ++i) {
+      f16x8 kq[NF / 2];
+#pragma unroll
+      for (int d = 0; d < NF / 2; ++d)
+        kq[d] = *reinterpret_cast<const f16x8*>(s_k + 16 * lane + ((i >> 1) * NF + (i & 1) * (NF / 2) + d) * 1024);
+      scores(kq, i, s);
+    }
   }
 
   int kbuf = 0, vbuf = 0;                         // buffers of K and V of the step
@@ -878,6 +890,18 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
     const uint8_t* kb = s_k + kbuf * kBytes + 16 * lane;   // of the next step
     vbuf = vbuf + 1 < S ? vbuf + 1 : 0;
     if (tok >= any_hi) return;                    // none of the wave's rows sees more
+    f16x8 kq[NF / 2], vq[DT];                     // a quarter's fragments of K and of V
+    auto load_k = [&](int i) {
+#pragma unroll
+      for (int d = 0; d < NF / 2; ++d)
+        kq[d] = *reinterpret_cast<const f16x8*>(kb + ((i >> 1) * NF + (i & 1) * (NF / 2) + d) * 1024);
+    };
+    auto load_v = [&](int i) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t) vq[t] = *reinterpret_cast<const f16x8*>(vb + ((i >> 1) * NF + 2 * t + (i & 1)) * 1024);
+    };
+    load_k(0);
+    pin();
     f32x4 c = s_c[step];
     const f32x4 b = s_b[step], inv = s_inv[step];
     if (any_bad || tok < all_lo || tok + 64 > all_hi) {
@@ -915,7 +939,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      scores(kb, i, sn);                          // past the last step: of no use, and not used
+      if constexpr (NQ == 1) load_v(i);
+      pin();
+      scores(kq, i, sn);                          // past the last step: of no use, and not used
+      if constexpr (NQ == 2) load_v(i);
       const float off = b[i] - m;
       float e8[8];
 #pragma unroll
@@ -929,12 +956,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
       // (an f16 dot for the sum would lose the probabilities that are subnormal there)
       const float sum = ((e8[0] + e8[1]) + (e8[2] + e8[3])) + ((e8[4] + e8[5]) + (e8[6] + e8[7]));
       l = fmaf(sum, inv[i], l);
+      if (i < 3) load_k(i + 1);
+      pin();
 #pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        const f16x8 v = *reinterpret_cast<const f16x8*>(vb + ((i >> 1) * NF + 2 * t + (i & 1)) * 1024);
+      for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[q], acc[t], 0, 0, 0);
-      }
+        for (int q = 0; q < NQ; ++q) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vq[t], pf[q], acc[t], 0, 0, 0);
     }
   };
   for (int step = 0; step < steps; step += 2) {
