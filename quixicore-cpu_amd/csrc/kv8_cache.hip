@@ -88,7 +88,7 @@ __device__ __forceinline__ int code_of(float v) {
 // (from L2).  A page and head is a chain of dependent reads (lengths, page id, rows, scale)
 // with little data behind it, so many small workgroups: 64 threads where a page's
 // head is at most 4096 elements.  10.5 thousand tokens of 8 heads of 128, f16, pages
-// of 16: 39 us with an element a thread, 14 here.
+// of 16 (64 MB): 39 us with an element a thread, 14 here (4.5 TB/s).
 constexpr int kHeld = 8;
 template <int TYPE, int NT, bool VEC>
 __global__ __launch_bounds__(NT) void append_kernel(Kv8Args a, Rows k, Rows v, int slots) {
@@ -184,37 +184,45 @@ __global__ __launch_bounds__(NT) void append_kernel(Kv8Args a, Rows k, Rows v, i
   if (threadIdx.x == 0) *scale_at = scale;
 }
 
-// The same places read back: code * scale, rounded once; four codes a thread and
-// step (8.3 thousand tokens of 8 heads of 128 to f16: 24 us with one, 16 so).
-template <int TYPE, bool VEC>
-__global__ __launch_bounds__(kThreads) void gather_kernel(Kv8Args a, void* k, void* v,
-                                                          long long k_stride, long long v_stride,
-                                                          int slots) {
+// The same places read back: code * scale, rounded once; eight codes a thread and step, kHeld
+// loads ahead of the stores.  Bound by memory: 10.5 thousand tokens of 8 heads of 128 to f16,
+// pages of 16 (64 MB): 17 us with four codes and a load a step and 256 threads, 11 here (5.8 TB/s).
+template <int TYPE, int NT, bool VEC>
+__global__ __launch_bounds__(NT) void gather_kernel(Kv8Args a, void* k, void* v, long long k_stride,
+                                                    long long v_stride, int slots) {
   typedef typename Storage<TYPE>::raw raw;
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   Place w;
   if (!place_of(a, slots, w)) return;
-  const uint32_t* codes = reinterpret_cast<const uint32_t*>(
+  const u32x2* codes = reinterpret_cast<const u32x2*>(
       (w.which ? a.v_codes : a.k_codes) + (w.unit * a.page_tokens + w.lo - w.p0) * a.head_dim);
   const float scale = (w.which ? a.v_scales : a.k_scales)[w.unit];
   const long long stride = w.which ? v_stride : k_stride;
   raw* out = static_cast<raw*>(w.which ? v : k) + w.row * stride +
              static_cast<long long>(w.head) * a.head_dim;
-  const int per_row = a.head_dim / 4, n = (w.hi - w.lo) * per_row;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint32_t c = codes[i];
-    float f[4];
+  const int per_row = a.head_dim / 8, n = (w.hi - w.lo) * per_row;
+  for (int i0 = threadIdx.x; i0 < n; i0 += kHeld * NT) {
+    u32x2 held[kHeld];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = static_cast<float>(static_cast<int8_t>(c >> (8 * j))) * scale;
-    const int t = i / per_row;
-    raw* o = out + t * stride + (i - t * per_row) * 4;
-    if constexpr (!VEC) {
+    for (int h = 0; h < kHeld; ++h)
+      if (i0 + h * NT < n) held[h] = codes[i0 + h * NT];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] = encode<TYPE>(f[j]);
-    } else if constexpr (TYPE == QC_STORAGE_F32) {
-      *reinterpret_cast<u32x4*>(o) = encode16<TYPE>(f);
-    } else {
-      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-      *reinterpret_cast<u32x2*>(o) = u32x2{encode2<TYPE>(f[0], f[1]), encode2<TYPE>(f[2], f[3])};
+    for (int h = 0; h < kHeld; ++h) {
+      const int i = i0 + h * NT;
+      if (i >= n) break;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        f[j] = static_cast<float>(static_cast<int8_t>(held[h][j >> 2] >> (8 * (j & 3)))) * scale;
+      const int t = i / per_row;
+      raw* o = out + t * stride + (i - t * per_row) * 8;
+      if constexpr (VEC) {
+#pragma unroll
+        for (int j = 0; j < 8; j += Storage<TYPE>::per16) *reinterpret_cast<u32x4*>(o + j) = encode16<TYPE>(f + j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = encode<TYPE>(f[j]);
+      }
     }
   }
 }
@@ -345,10 +353,11 @@ void run_gather(const Kv8Args& a, void* k, void* v, long long k_stride, long lon
   constexpr int size = TYPE == QC_STORAGE_F32 ? 4 : 2;
   int slots;
   const unsigned grid = touched_grid(a, slots);
-  if (wide_rows(k, k_stride, size) && wide_rows(v, v_stride, size))
-    gather_kernel<TYPE, true><<<grid, kThreads, 0, s>>>(a, k, v, k_stride, v_stride, slots);
-  else
-    gather_kernel<TYPE, false><<<grid, kThreads, 0, s>>>(a, k, v, k_stride, v_stride, slots);
+  const bool vec = wide_rows(k, k_stride, size) && wide_rows(v, v_stride, size);
+  const bool small = std::min(a.max_new, a.page_tokens) * a.head_dim <= 4096;
+  if (vec && small) gather_kernel<TYPE, 64, true><<<grid, 64, 0, s>>>(a, k, v, k_stride, v_stride, slots);
+  else if (vec) gather_kernel<TYPE, 256, true><<<grid, 256, 0, s>>>(a, k, v, k_stride, v_stride, slots);
+  else gather_kernel<TYPE, 256, false><<<grid, 256, 0, s>>>(a, k, v, k_stride, v_stride, slots);
 }
 
 }  // namespace
