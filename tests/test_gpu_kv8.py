@@ -788,6 +788,61 @@ def test_a_low_bit_layer(qc, dev, route):
     assert st.item() == 0
 
 
+def test_a_captured_decoding_step(qc, dev):
+    """The layer's operators captured once for a batch whose lengths, positions and rows change
+    between the replays; another captured batch and eager calls share the stream's workspaces.
+    Every replay is the eager step's, bit for bit, cache and all."""
+    import torch
+    torch.manual_seed(1)
+    heads, kvh, hd, hidden, page = 8, 2, 64, 224, 16
+    wc, ws = qc.quantize_mxfp4(0.06 * torch.randn((heads + 2 * kvh) * hd, hidden, device=dev))
+    cosine, sine = qc.rope_table(2048, hd)
+    rng = np.random.default_rng(5)
+    st = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def step(cache, b, x, pos):
+        xc, xs = qc.quantize_mxfp4(x, dev_status=st)
+        y = qc.mxfp4_gemm(wc, ws, xc, xs, dtype=torch.bfloat16)
+        qk = y[:, :(heads + kvh) * hd].unflatten(1, (heads + kvh, hd))
+        qc.rope(qk, cosine, sine, pos, out=qk, dev_status=st)
+        qc.kv8_append(cache, b, y[:, heads * hd:(heads + kvh) * hd], y[:, (heads + kvh) * hd:], dev_status=st)
+        return qc.kv8_attention(cache, b, y[:, :heads * hd].unflatten(1, (heads, hd)), dev_status=st)
+
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    runs = []
+    with torch.cuda.stream(stream):
+        for held in ([700, 15, 1300, 0], [40, 1, 64]):
+            batch = Ragged(rng, [1] * len(held), [h + 40 for h in held], page)
+            b = batch.device(qc, dev)
+            b.tensors[2].copy_(torch.tensor([h + 1 for h in held], dtype=torch.int32))
+            cache = _random_cache(qc, dev, rng, batch.pages, kvh, page, hd)
+            x = torch.randn(len(held), hidden, device=dev, dtype=torch.bfloat16)
+            pos = (b.tensors[2] - 1).clone()
+            keep = [c.clone() for c in cache.tensors]
+            step(cache, b, x, pos)                # sizes the workspaces
+            for c, k in zip(cache.tensors, keep):
+                c.copy_(k)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                out = step(cache, b, x, pos)
+            runs.append((cache, b, x, pos, graph, out))
+        for rep in range(6):
+            for cache, b, x, pos, graph, out in runs:
+                x.copy_(torch.randn_like(x))
+                other = qc.Kv8Cache(*[c.clone() for c in cache.tensors])
+                graph.replay()
+                got = out.clone()
+                assert torch.equal(got, step(other, b, x, pos))
+                for c, o in zip(cache.tensors, other.tensors):
+                    assert torch.equal(c, o)
+                b.tensors[2].add_(1 + rep % 2 * 3)      # (slots between hold what they held)
+                pos.copy_(b.tensors[2] - 1)
+                torch.cuda.synchronize()
+    assert st.item() == 0
+
+
 @pytest.mark.parametrize("new,kv,route", [
     ([1] * 70, 4096, 3), ([1] * 40 + [260] + [1] * 29, 4096, 3), ([1] * 9 + [1024] * 17 + [1] * 50, 16384, 0)])
 def test_attention_passes_of_the_layout(qc, dev, new, kv, route):
