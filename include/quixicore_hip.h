@@ -403,7 +403,7 @@ typedef struct qc_kv8_cache {
  * kv_len[s] counts its tokens in the cache, the new ones last.  Position p of it
  * lies in page block_table[s * columns + p / page_tokens], slot p % page_tokens.
  * Host bounds: no sequence has more than max_new new tokens (which may exceed tokens)
- * or max_kv tokens (at most columns * page_tokens);
+ * or max_kv tokens (at most columns * page_tokens, which is at most 2^30);
  * rows from seq_start[seqs] on belong to no one and are neither read nor written.
  * A sequence whose figures break these bounds, or a page id that a call needs and
  * that is not in [0, pages), is an error: the sequence is left out (append,

@@ -200,7 +200,7 @@ bool kv8_shapes(const qc_kv8_cache& c, const qc_kv8_batch& b) {
       b.max_kv <= 0)
     return false;
   if (c.pages > INT_MAX || c.kv_heads > INT_MAX / 256 || b.seqs > INT_MAX - 1 || b.tokens > INT_MAX ||
-      b.columns * c.page_tokens > INT_MAX - 512)
+      b.columns * c.page_tokens > (1LL << 30))
     return false;
   if (b.max_kv > b.columns * c.page_tokens) return false;
   // a workgroup per sequence, touched page and head

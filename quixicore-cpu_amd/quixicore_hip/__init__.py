@@ -440,13 +440,14 @@ def rope_table(positions, rotary_dim, base=10000.0, scaling="none", factor=1.0,
 
 def rope(x, cosine, sine, positions, interleaved=False, out=None, dev_status=None):
     """x [tokens][heads][head_dim] (any token and head strides) with the first 2 *
-    cosine.shape[1] elements of every head rotated; out may be x."""
+    cosine.shape[1] elements of every head rotated; out may be x.  Tokens at position -1 are
+    left as they were (zeros in a new tensor)."""
     st = _storage(x)
     if x.dim() != 3 or x.stride(2) != 1:
         raise ValueError("rope: x is [tokens][heads][head_dim], elements side by side")
     if out is None:
         import torch
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
     elif out is not x and (out.shape != x.shape or out.stride(2) != 1 or out.dtype is not x.dtype):
         raise ValueError("rope: out is of x's shape and type")
     _here(x, out)
@@ -587,7 +588,7 @@ def kv8_attention(cache, batch, q, scale=None, causal=True, window=0, out=None, 
 
 def quantize_mxfp4(x, dev_status=None):
     """(codes [rows][dim / 2], scales [rows][dim / 32]) uint8 of x [rows][dim] (rows may be
-    strided)."""
+    strided).  Where dev_status becomes 3, the blocks in error hold anything."""
     import torch
     st = _storage(x)
     _here(x)

@@ -647,6 +647,18 @@ def test_attention_repeats_and_graph(qc, dev, route, new, kv, heads, kvh):
     del graph
 
 
+def test_attention_shared_pages(qc, dev, route):
+    """Sequences that share their first pages, and a page that one sequence holds twice."""
+    import torch
+    rng = np.random.default_rng(33)
+    batch = Ragged(rng, [1, 40, 2], [100, 90, 70], 16)
+    batch.table[1, :4] = batch.table[0, :4]
+    batch.table[2, :3] = batch.table[0, :3]
+    batch.table[2, 3] = batch.table[2, 1]
+    for dtype in ("float32", "bfloat16"):
+        _attend(qc, dev, rng, batch.new, batch.kv, 8, 2, 64, 16, dtype, batch=batch)
+
+
 def test_attention_from_threads(qc, dev):
     """Calls of several host threads, on one stream and on streams of their own, each with
     keys that are split and joined: every result is the lone call's."""

@@ -137,6 +137,7 @@ def test_padding_and_bad_positions(qc, dev):
     pos = torch.tensor([3, -1, 9, -1, -1, 0], dtype=torch.int32, device=dev)
     qc.rope(x, c, s, pos, out=out)
     assert torch.equal(out[0], want[0]) and torch.all(out[1] == 5.0)
+    assert torch.all(qc.rope(x, c, s, pos)[1] == 0.0)
 
 
 def test_tables_serve_the_single_token_seam(qc, oracle, dev):

@@ -82,7 +82,7 @@ CACHE_SHAPES = (dict(pages=0), dict(kv_heads=0), dict(page_tokens=8), dict(page_
                 dict(head_dim=0), dict(pages=1 << 31), dict(pages=1 << 62), dict(kv_heads=1 << 30))
 BATCH_SHAPES = (dict(seqs=0), dict(columns=0), dict(tokens=0), dict(max_new=0), dict(max_kv=0),
                 dict(max_kv=65), dict(seqs=1 << 31), dict(tokens=1 << 31),
-                dict(columns=1 << 30), dict(seqs=1 << 62))
+                dict(columns=1 << 30), dict(columns=(1 << 26) + 1), dict(seqs=1 << 62))
 
 
 @pytest.mark.parametrize("entry", ["append", "gather", "attention"])
