@@ -26,7 +26,8 @@
  *   - Scratch: entry points whose kernels need device scratch (qc_hip_qgemm
  *     from M = 2, the canonical int8 projections from M = 2, the affine
  *     canonical W8A8 route, qc_hip_kv8_attention of long caches and of long prompts,
- *     qc_hip_mxfp4_gemm of scale rows that do not begin at multiples of 4 bytes) take it from a per-(device, stream) cache that
+ *     qc_hip_mxfp4_gemm of scale arrays that do not begin at a multiple of 4 bytes, or of
+ *     many rows of x whose scale rows do not) take it from a per-(device, stream) cache that
  *     only grows; the first call on a stream, or one needing more, allocates
  *     (hipMalloc), later calls do not.  Calls on one stream share its buffers
  *     in stream order; graphs captured on a stream keep that stream's buffers

@@ -97,7 +97,12 @@ __device__ __forceinline__ void tile_at(int b, int total, int tiles_n, int tiles
   tm = band * kBand + rem % gm;
 }
 
-template <int TN, int TM, int S, int WGN, int WGM, int KG, int TYPE>
+// PACKED: scale rows of any number of bytes, so that a row begins at any byte of a dword. A step
+// then loads the three dwords that its 8 bytes lie in, the third by 64 rows an instruction, and the
+// two that hold a lane's four bytes are shifted together.  (The array itself begins at a
+// dword; the one that holds its last bytes is read whole.)  Against rows laid out by a launch before:
+// M = 1, 14336 x 4064 11.4 -> 8.5 us, M = 77, 5461 x 2752 9.9 -> 8.4.
+template <int TN, int TM, int S, int WGN, int WGM, int KG, int TYPE, bool PACKED>
 __global__ __launch_bounds__(64 * WGN * WGM * KG, 1) void mxfp4_ring(
     const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws, const uint8_t* __restrict__ x,
     const uint8_t* __restrict__ xs, void* __restrict__ y, int m, int n, int blocks,
@@ -108,8 +113,10 @@ __global__ __launch_bounds__(64 * WGN * WGM * KG, 1) void mxfp4_ring(
   constexpr int R = TN + TM;                        // rows of a stage, w's first
   // loads a wave and step (beyond the stage's share the last one again: the same bytes)
   constexpr int GC = (R / 8 + NW - 1) / NW, GS = (R / 32 + NW - 1) / NW;
-  constexpr int G = GC + GS;
-  constexpr int kStage = R * 136;                   // codes, then scales
+  constexpr int X = PACKED ? (R + 63) / 64 : 0;     // loads of third dwords
+  constexpr int GX = (X + NW - 1) / NW;
+  constexpr int G = GC + GS + GX;
+  constexpr int kStage = R * 136 + X * 256;         // codes, scales, third dwords
   static_assert(FN >= 1 && FM >= 1 && S >= 2 && G * (S - 1) < 64, "tile");
   static_assert(S * kStage <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[S * kStage];
@@ -138,14 +145,34 @@ __global__ __launch_bounds__(64 * WGN * WGM * KG, 1) void mxfp4_ring(
     cvo[j] = static_cast<uint32_t>(r) * bytes;
   }
   const uint8_t* sbase[GS];
-  uint32_t svo[GS];
+  uint32_t svo[GS], slast[GS];                      // slast: the array's last dword
 #pragma unroll
   for (int j = 0; j < GS; ++j) {
     const int r32 = 32 * min(wave * GS + j, R / 32 - 1);
     const bool is_w = r32 < TN;
     const int first = is_w ? n0 : m0, limit = is_w ? n : m, base = is_w ? r32 : r32 - TN;
-    sbase[j] = (is_w ? ws : xs) + static_cast<long long>(first) * scale_stride;
-    svo[j] = static_cast<uint32_t>(min(first + base + (lane & 31), limit - 1) - first) * scale_stride;
+    const long long at = static_cast<long long>(first) * scale_stride;
+    const int r = min(first + base + (lane & 31), limit - 1) - first;
+    sbase[j] = (is_w ? ws : xs) + (PACKED ? at & ~3ll : at);
+    svo[j] = static_cast<uint32_t>(r) * scale_stride;
+    slast[j] = 0;
+    if constexpr (PACKED) {
+      svo[j] = (static_cast<uint32_t>(at & 3) + svo[j]) & ~3u;
+      const long long last = ((static_cast<long long>(limit) * scale_stride - 1) & ~3ll) - (at & ~3ll);
+      slast[j] = static_cast<uint32_t>(last < 0x7FFFFFFF ? last : 0x7FFFFFFF);
+    }
+  }
+  const uint8_t* xat[GX ? GX : 1];                  // third dword of the lane's row at step 0
+  const uint8_t* xlast[GX ? GX : 1];
+#pragma unroll
+  for (int j = 0; j < GX; ++j) {
+    const int rr = min(64 * min(wave * GX + j, X - 1) + lane, R - 1);
+    const bool is_w = rr < TN;
+    const int limit = is_w ? n : m;
+    const long long row = min((is_w ? n0 + rr : m0 + rr - TN), limit - 1);
+    const uint8_t* array = is_w ? ws : xs;
+    xat[j] = array + ((row * scale_stride) & ~3ll) + 8;
+    xlast[j] = array + ((static_cast<long long>(limit) * scale_stride - 1) & ~3ll);
   }
   auto issue = [&](int step, int stage, int from, int to) {
     uint8_t* base = lds + stage * kStage;
@@ -155,11 +182,15 @@ __global__ __launch_bounds__(64 * WGN * WGM * KG, 1) void mxfp4_ring(
       if (j < GC) {
         const int col = min(128 * step + ccol[j < GC ? j : 0], bytes - 16);
         dma16(cbase[j < GC ? j : 0], cvo[j < GC ? j : 0] + col, base + min(wave * GC + j, R / 8 - 1) * 1024);
-      } else {
-        const int i = j - GC;
-        const int col = min(8 * step + 4 * (lane >> 5), scale_stride - 4);
-        dma4(sbase[i < GS ? i : 0], svo[i < GS ? i : 0] + col,
+      } else if (j < GC + GS) {
+        const int i = j - GC < GS ? j - GC : 0;
+        const int col = 8 * step + 4 * (lane >> 5);
+        dma4(sbase[i], PACKED ? min(svo[i] + col, slast[i]) : svo[i] + min(col, scale_stride - 4),
              base + R * 128 + min(wave * GS + i, R / 32 - 1) * 256);
+      } else {
+        const int i = j - GC - GS;
+        const uint8_t* at = xat[i] + 8 * step;
+        dma4_addr(at < xlast[i] ? at : xlast[i], base + R * 136 + min(wave * GX + i, X - 1) * 256);
       }
     }
   };
@@ -177,14 +208,27 @@ __global__ __launch_bounds__(64 * WGN * WGM * KG, 1) void mxfp4_ring(
 #pragma unroll
     for (int j = 0; j < FM; ++j) fb[slot][j] = *reinterpret_cast<const i32x4*>(base + (TN + wm + 32 * j) * 128);
   };
+  uint32_t ba[FN], bb[FM];                          // PACKED: the byte of a dword that a row begins at
+  if constexpr (PACKED) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) ba[i] = (static_cast<uint32_t>(min(n0 + wn + 32 * i + (lane & 31), n - 1)) * scale_stride) & 3;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) bb[j] = (static_cast<uint32_t>(min(m0 + wm + 32 * j + (lane & 31), m - 1)) * scale_stride) & 3;
+  }
+  // the dword after a lane's: its row's second or third
+  const int after = (lane < 32 ? R * 128 + 128 : R * 136) + 4 * (lane & 31), after_by = lane < 32 ? 256 : 128;
   auto read_scales = [&](int stage, int slot) {
-    const uint8_t* base = lds + stage * kStage + R * 128 + 4 * lane;
+    const uint8_t* base = lds + stage * kStage;
+    auto read = [&](int rows32, uint32_t byte) {
+      const uint32_t v = *reinterpret_cast<const uint32_t*>(base + R * 128 + 4 * lane + rows32 * 256);
+      if constexpr (!PACKED) return static_cast<int>(v) >> (8 * q0);
+      const uint32_t next = *reinterpret_cast<const uint32_t*>(base + after + rows32 * after_by);
+      return static_cast<int>(__builtin_amdgcn_alignbyte(next, v, byte)) >> (8 * q0);
+    };
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
-      sa[slot][i] = *reinterpret_cast<const int*>(base + (wn / 32 + i) * 256) >> (8 * q0);
+    for (int i = 0; i < FN; ++i) sa[slot][i] = read(wn / 32 + i, PACKED ? ba[i] : 0);
 #pragma unroll
-    for (int j = 0; j < FM; ++j)
-      sb[slot][j] = *reinterpret_cast<const int*>(base + ((TN + wm) / 32 + j) * 256) >> (8 * q0);
+    for (int j = 0; j < FM; ++j) sb[slot][j] = read((TN + wm) / 32 + j, PACKED ? bb[j] : 0);
   };
   f32x16 acc[FN][FM];
 #pragma unroll
@@ -321,8 +365,8 @@ __global__ __launch_bounds__(64 * WGN * WGM * KG, 1) void mxfp4_ring(
   }
 }
 
-// Scale rows that begin at a multiple of 4 bytes, which the caller's need not: the
-// ring's loads are dwords.  Bytes past a row's blocks are zero.
+// Scale rows laid out for the ring, whose loads are dwords (arrays that begin at any byte, and rows of any
+// length for the largest tile).  Bytes past a row's blocks are zero.
 __global__ __launch_bounds__(256) void pad_scales(const uint8_t* __restrict__ ws, long long n,
                                                   const uint8_t* __restrict__ xs, long long m,
                                                   int blocks, int stride, uint32_t* __restrict__ out) {
@@ -388,7 +432,10 @@ template <int TN, int TM, int S, int WGN, int WGM, int KG, int TYPE>
 hipError_t run_ring(const Operands& o, int scale_stride, hipStream_t s) {
   const int tiles_n = (o.n + TN - 1) / TN, tiles_m = (o.m + TM - 1) / TM;
   if (static_cast<long long>(tiles_n) * tiles_m > INT_MAX) return hipErrorInvalidValue;
-  mxfp4_ring<TN, TM, S, WGN, WGM, KG, TYPE><<<static_cast<unsigned>(tiles_n) * tiles_m, 64 * WGN * WGM * KG, 0, s>>>(
+  auto kernel = mxfp4_ring<TN, TM, S, WGN, WGM, KG, TYPE, false>;
+  if constexpr (TN * TM < 256 * 256)
+    if (scale_stride % 4 != 0) kernel = mxfp4_ring<TN, TM, S, WGN, WGM, KG, TYPE, true>;
+  kernel<<<static_cast<unsigned>(tiles_n) * tiles_m, 64 * WGN * WGM * KG, 0, s>>>(
       o.w, o.ws, o.x, o.xs, o.y, o.m, o.n, o.blocks, scale_stride, tiles_n, tiles_m);
   return hipGetLastError();
 }
@@ -397,8 +444,13 @@ template <int TYPE>
 hipError_t run_gemm(Operands o, int route, hipStream_t s) {
   StreamWorkspace* ws = nullptr;
   std::unique_lock<std::mutex> hold;
+  // a tile's codes are addressed with 32 bits: 32 rows of long ones
+  const int tile = o.blocks > (1 << 19) ? 0 : route > 0 ? route - 1 : choose_tile(o.m, o.n, device_cu_count());
   int stride = o.blocks;
-  if (o.blocks % 4 != 0 || ((reinterpret_cast<uintptr_t>(o.ws) | reinterpret_cast<uintptr_t>(o.xs)) & 3) != 0) {
+  // Rows of scales that do not begin at dwords: laid out first for the largest tile, whose LDS
+  // has no time for the third dwords (us, laid out / in the ring, K = 4064, N = 14336: M = 1 11.4 /
+  // 8.5, 512 35.2 / 34.6, 2048 97.4 / 100.9, 4096 209.7 / 214.6).
+  if ((o.blocks % 4 != 0 && tile == kTiles - 1) || ((reinterpret_cast<uintptr_t>(o.ws) | reinterpret_cast<uintptr_t>(o.xs)) & 3) != 0) {
     hipError_t e = stream_workspace(s, &ws);
     if (e != hipSuccess) return e;
     hold = std::unique_lock<std::mutex>(ws->call);
@@ -414,8 +466,6 @@ hipError_t run_gemm(Operands o, int route, hipStream_t s) {
     o.ws = static_cast<const uint8_t*>(buf);
     o.xs = o.ws + static_cast<long long>(o.n) * stride;
   }
-  // a tile's codes are addressed with 32 bits: 32 rows of long ones
-  const int tile = o.blocks > (1 << 19) ? 0 : route > 0 ? route - 1 : choose_tile(o.m, o.n, device_cu_count());
   switch (tile) {
     case 0: return run_ring<32, 32, 4, 1, 1, 2, TYPE>(o, stride, s);
     case 1: return run_ring<64, 32, 4, 2, 1, 1, TYPE>(o, stride, s);
