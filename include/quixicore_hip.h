@@ -438,10 +438,12 @@ int qc_hip_kv8_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch, cons
 
 /* The same places read back: k and v rows of the batch's tokens receive the
  * values held at positions kv_len - n .. kv_len - 1 (a seq_start that spans whole
- * sequences reads all of them).  Status and errors as for qc_hip_kv8_append. */
+ * sequences reads all of them).  zero_rest != 0: rows of k and v that receive nothing (of no
+ * sequence, or left out by an error) become zeros; else they stay as they were.  Status and
+ * errors as for qc_hip_kv8_append. */
 int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void* k,
-                      long long k_stride, void* v, long long v_stride, int type, int* dev_status,
-                      void* stream);
+                      long long k_stride, void* v, long long v_stride, int type, int zero_rest,
+                      int* dev_status, void* stream);
 
 /* out = softmax(scale * q k^T + mask) v over the cache, for the new tokens of
  * every sequence (which the cache holds already).  q and out: [tokens][heads *

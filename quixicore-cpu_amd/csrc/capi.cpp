@@ -889,8 +889,8 @@ int qc_hip_kv8_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch, cons
 }
 
 int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void* k,
-                      long long k_stride, void* v, long long v_stride, int type, int* dev_status,
-                      void* stream) {
+                      long long k_stride, void* v, long long v_stride, int type, int zero_rest,
+                      int* dev_status, void* stream) {
   if (cache == nullptr || batch == nullptr) return QC_INVALID_ARGUMENT;
   if (!kv8_shapes(*cache, *batch)) return QC_INVALID_SHAPE;
   const long long row = cache->kv_heads * cache->head_dim, most = LLONG_MAX / 8 / batch->tokens;
@@ -902,7 +902,7 @@ int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void
       dev_status, s,
       [&](int* flag) { return qc::launch_kv8_check(*cache, *batch, true, 0, flag, s); },
       [&](int* flag) {
-        return qc::launch_kv8_gather(*cache, *batch, k, k_stride, v, v_stride, type, flag, s);
+        return qc::launch_kv8_gather(*cache, *batch, k, k_stride, v, v_stride, type, zero_rest != 0, flag, s);
       });
 }
 

@@ -35,7 +35,7 @@ struct Place {
   int which, head;
   int lo, hi, p0;
   int row;                 // token row of position lo
-  long long unit;          // page * kv_heads + head
+  long long unit;          // page * kv_heads + head; -1 where the page id is out of range
 };
 
 __device__ __forceinline__ bool place_of(const Kv8Args& a, int slots, Place& w) {
@@ -70,12 +70,10 @@ __device__ __forceinline__ bool place_of(const Kv8Args& a, int slots, Place& w) 
   w.hi = min(kv, w.p0 + a.page_tokens);
   if (w.lo >= w.hi) return false;
   const int page = a.table[static_cast<long long>(q) * a.columns + column];
-  if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pages)) {
-    *a.status = QC_INVALID_ARGUMENT;
-    return false;
-  }
+  const bool in = static_cast<unsigned>(page) < static_cast<unsigned>(a.pages);
+  if (!in) *a.status = QC_INVALID_ARGUMENT;
   w.row = first + w.lo - begin;
-  w.unit = static_cast<long long>(page) * a.kv_heads + w.head;
+  w.unit = in ? static_cast<long long>(page) * a.kv_heads + w.head : -1;
   return true;
 }
 
@@ -96,7 +94,7 @@ __global__ __launch_bounds__(NT) void append_kernel(Kv8Args a, Rows k, Rows v, i
   constexpr int V = VEC ? Storage<TYPE>::per16 : 4;
   __shared__ float stop[NT / 64];
   Place w;
-  if (!place_of(a, slots, w)) return;
+  if (!place_of(a, slots, w) || w.unit < 0) return;
   const Rows src = w.which ? v : k;
   int8_t* codes = (w.which ? a.v_codes : a.k_codes) + w.unit * a.page_tokens * a.head_dim;
   float* scale_at = (w.which ? a.v_scales : a.k_scales) + w.unit;
@@ -184,16 +182,62 @@ __global__ __launch_bounds__(NT) void append_kernel(Kv8Args a, Rows k, Rows v, i
   if (threadIdx.x == 0) *scale_at = scale;
 }
 
+// Which of the 64 token rows from t0 on belong to no sequence that has its tokens in the cache.
+__device__ __forceinline__ uint64_t rows_of_none(const Kv8Args& a, int t0) {
+  const int n = min(64, a.tokens - t0);
+  uint64_t taken = n < 64 ? ~0ull << n : 0;
+  for (int i = threadIdx.x & 63; i < a.seqs; i += 64) {
+    int first, rows, kv;
+    if (!kv8_sequence(a, i, first, rows, kv) || rows > kv) continue;
+    const int lo = max(first - t0, 0), hi = min(first + rows - t0, 64);
+    if (lo < hi) taken |= (~0ull >> (64 - (hi - lo))) << lo;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1)
+    taken |= static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(taken), o));
+  return ~taken;
+}
+
+template <int TYPE, int NT, bool VEC>
+__device__ __forceinline__ void zero_row(typename Storage<TYPE>::raw* p, int n) {
+  constexpr int V = VEC ? Storage<TYPE>::per16 : 1;
+  for (int i = threadIdx.x * V; i < n; i += NT * V) {
+    if constexpr (VEC) *reinterpret_cast<u32x4*>(p + i) = u32x4{0, 0, 0, 0};
+    else p[i] = 0;
+  }
+}
+
 // The same places read back: code * scale, rounded once; eight codes a thread and step, kHeld
 // loads ahead of the stores.  Bound by memory: 10.5 thousand tokens of 8 heads of 128 to f16,
 // pages of 16 (64 MB): 17 us with four codes and a load a step and 256 threads, 11 here (5.8 TB/s).
+// rest: workgroups from it on, two for each 64 token rows (K and V), set those to zero that no
+// sequence has; 0 where such rows stay as they are.  (A fill of all rows before the call: 6 us more, and
+// as many of the host's.)
 template <int TYPE, int NT, bool VEC>
 __global__ __launch_bounds__(NT) void gather_kernel(Kv8Args a, void* k, void* v, long long k_stride,
-                                                    long long v_stride, int slots) {
+                                                    long long v_stride, int slots, unsigned rest) {
   typedef typename Storage<TYPE>::raw raw;
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  if (rest > 0 && blockIdx.x >= rest) {
+    const int which = (blockIdx.x - rest) & 1, t0 = (blockIdx.x - rest) / 2 * 64;
+    uint64_t empty = rows_of_none(a, t0);
+    raw* rows = static_cast<raw*>(which ? v : k);
+    for (; empty != 0; empty &= empty - 1) {
+      const int t = t0 + __ffsll(static_cast<unsigned long long>(empty)) - 1;
+      zero_row<TYPE, NT, VEC>(rows + t * (which ? v_stride : k_stride), a.kv_heads * a.head_dim);
+    }
+    return;
+  }
   Place w;
   if (!place_of(a, slots, w)) return;
+  if (w.unit < 0) {                               // a page that is not there
+    if (rest == 0) return;
+    for (int t = 0; t < w.hi - w.lo; ++t)
+      zero_row<TYPE, NT, VEC>(static_cast<raw*>(w.which ? v : k) + (w.row + t) * (w.which ? v_stride : k_stride) +
+                                  static_cast<long long>(w.head) * a.head_dim,
+                              a.head_dim);
+    return;
+  }
   const u32x2* codes = reinterpret_cast<const u32x2*>(
       (w.which ? a.v_codes : a.k_codes) + (w.unit * a.page_tokens + w.lo - w.p0) * a.head_dim);
   const float scale = (w.which ? a.v_scales : a.k_scales)[w.unit];
@@ -348,16 +392,18 @@ void run_append(const Kv8Args& a, const Rows& k, const Rows& v, hipStream_t s) {
 }
 
 template <int TYPE>
-void run_gather(const Kv8Args& a, void* k, void* v, long long k_stride, long long v_stride,
+void run_gather(const Kv8Args& a, void* k, void* v, long long k_stride, long long v_stride, bool zero_rest,
                 hipStream_t s) {
   constexpr int size = TYPE == QC_STORAGE_F32 ? 4 : 2;
   int slots;
-  const unsigned grid = touched_grid(a, slots);
+  unsigned grid = touched_grid(a, slots);
+  const unsigned rest = zero_rest ? grid : 0;
+  if (zero_rest) grid += 2u * static_cast<unsigned>((a.tokens + 63LL) / 64);
   const bool vec = wide_rows(k, k_stride, size) && wide_rows(v, v_stride, size);
   const bool small = std::min(a.max_new, a.page_tokens) * a.head_dim <= 4096;
-  if (vec && small) gather_kernel<TYPE, 64, true><<<grid, 64, 0, s>>>(a, k, v, k_stride, v_stride, slots);
-  else if (vec) gather_kernel<TYPE, 256, true><<<grid, 256, 0, s>>>(a, k, v, k_stride, v_stride, slots);
-  else gather_kernel<TYPE, 256, false><<<grid, 256, 0, s>>>(a, k, v, k_stride, v_stride, slots);
+  if (vec && small) gather_kernel<TYPE, 64, true><<<grid, 64, 0, s>>>(a, k, v, k_stride, v_stride, slots, rest);
+  else if (vec) gather_kernel<TYPE, 256, true><<<grid, 256, 0, s>>>(a, k, v, k_stride, v_stride, slots, rest);
+  else gather_kernel<TYPE, 256, false><<<grid, 256, 0, s>>>(a, k, v, k_stride, v_stride, slots, rest);
 }
 
 }  // namespace
@@ -376,13 +422,13 @@ hipError_t launch_kv8_append(const qc_kv8_cache& c, const qc_kv8_batch& b, const
 }
 
 hipError_t launch_kv8_gather(const qc_kv8_cache& c, const qc_kv8_batch& b, void* k,
-                             long long k_stride, void* v, long long v_stride, int type, int* status,
-                             hipStream_t s) {
+                             long long k_stride, void* v, long long v_stride, int type, bool zero_rest,
+                             int* status, hipStream_t s) {
   const Kv8Args a = kv8_args(c, b, status);
   switch (type) {
-    case QC_STORAGE_F32: run_gather<QC_STORAGE_F32>(a, k, v, k_stride, v_stride, s); break;
-    case QC_STORAGE_F16: run_gather<QC_STORAGE_F16>(a, k, v, k_stride, v_stride, s); break;
-    default: run_gather<QC_STORAGE_BF16>(a, k, v, k_stride, v_stride, s);
+    case QC_STORAGE_F32: run_gather<QC_STORAGE_F32>(a, k, v, k_stride, v_stride, zero_rest, s); break;
+    case QC_STORAGE_F16: run_gather<QC_STORAGE_F16>(a, k, v, k_stride, v_stride, zero_rest, s); break;
+    default: run_gather<QC_STORAGE_BF16>(a, k, v, k_stride, v_stride, zero_rest, s);
   }
   return hipGetLastError();
 }

@@ -291,8 +291,8 @@ hipError_t launch_kv8_append(const qc_kv8_cache& c, const qc_kv8_batch& b, const
                              long long k_stride, const void* v, long long v_stride, int type,
                              int* status, hipStream_t s);
 hipError_t launch_kv8_gather(const qc_kv8_cache& c, const qc_kv8_batch& b, void* k,
-                             long long k_stride, void* v, long long v_stride, int type, int* status,
-                             hipStream_t s);
+                             long long k_stride, void* v, long long v_stride, int type, bool zero_rest,
+                             int* status, hipStream_t s);
 struct Kv8Attention {
   const qc_kv8_cache* cache = nullptr;
   const qc_kv8_batch* batch = nullptr;

@@ -75,7 +75,7 @@ _SIGS = {
     "qc_hip_rope": ([_P, _P, _I, _LL, _LL, _LL, _LL, _LL, _LL, _LL, _LL, _P, _P, _P, _LL, _I, _P,
                      _P], _I),
     "qc_hip_kv8_append": ([_P, _P, _P, _LL, _P, _LL, _I, _P, _P], _I),
-    "qc_hip_kv8_gather": ([_P, _P, _P, _LL, _P, _LL, _I, _P, _P], _I),
+    "qc_hip_kv8_gather": ([_P, _P, _P, _LL, _P, _LL, _I, _I, _P, _P], _I),
     "qc_hip_kv8_attention": ([_P, _P, _P, _LL, _P, _LL, _I, _LL, ctypes.c_float, _I, _LL, _P, _P],
                              _I),
     "qc_hip_quantize_mxfp4": ([_P, _I, _LL, _P, _P, _LL, _LL, _P, _P], _I),
@@ -544,19 +544,24 @@ def kv8_gather(cache, batch, dtype=None, k=None, v=None, dev_status=None):
     """(k, v) [tokens][kv_heads][head_dim]: the values the cache holds for the batch's
     tokens.  Rows of no sequence are left as they were (zeros in new tensors)."""
     tokens, heads, head_dim = batch.tokens, cache.kv_heads, cache.head_dim
-    if k is None or v is None:
+    rest = 0
+    if k is None and v is None:
         import torch
-        new = torch.zeros((2, tokens, heads, head_dim), device=cache.tensors[0].device,
-                          dtype=dtype or (torch.float32 if k is None and v is None else
-                                          (v if k is None else k).dtype)).unbind()
-        k, v = new[0] if k is None else k, new[1] if v is None else v
+        k, v = torch.empty((2, tokens, heads, head_dim), dtype=dtype or torch.float32,
+                           device=cache.tensors[0].device).unbind()
+        rest = 1
+    elif k is None or v is None:
+        import torch
+        given = v if k is None else k
+        new = torch.zeros((tokens, heads, head_dim), dtype=given.dtype, device=given.device)
+        k, v = (new, v) if k is None else (k, new)
     st = _storage(k)
     _kv8_here(cache, batch, k, v)
     if v.dtype is not k.dtype or k.shape[0] != tokens or v.shape[0] != tokens:
         raise ValueError("kv8_gather: k and v of one type, a row for each of the batch's tokens")
     _check(lib.qc_hip_kv8_gather(ctypes.addressof(cache), ctypes.addressof(batch), k.data_ptr(),
                                  _rows("k", k, heads, head_dim), v.data_ptr(),
-                                 _rows("v", v, heads, head_dim), st, _status(dev_status),
+                                 _rows("v", v, heads, head_dim), st, rest, _status(dev_status),
                                  _stream(None)), "kv8_gather")
     return k, v
 

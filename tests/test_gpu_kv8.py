@@ -232,6 +232,50 @@ def test_append_errors(qc, dev):
         assert st.item() == 3
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("new,spare", [([3, 0, 20, 1, 70], 5), ([1] * 90 + [200], 130), ([64], 64), ([1], 0)])
+def test_gather_into_new_tensors(qc, dev, dtype, new, spare):
+    """Rows that receive nothing are zeros in tensors that the call makes: those of no sequence,
+    of bad lengths (too long, fewer than the new ones), of bad starts and of bad pages."""
+    import torch
+    dt = getattr(torch, dtype)
+    rng = np.random.default_rng(spare)
+    heads, hd, page = 3, 48, 16
+    batch = Ragged(rng, new, [n + 5 for n in new], page, spare)
+    cache = _random_cache(qc, dev, rng, batch.pages, heads, page, hd)
+    st = torch.zeros(1, dtype=torch.int32, device=dev)
+    last = len(new) - 1
+    a, e = int(batch.start[last]), int(batch.start[last + 1])
+    bad_page = (new[last] + 4) // page                # of the last token
+    for bad in ("nothing", "long", "short", "page", "start"):
+        b = batch.device(qc, dev)
+        left = torch.zeros(batch.tokens, dtype=torch.bool, device=dev)
+        left[e:] = True
+        if bad == "long":
+            b.tensors[2][last] = batch.max_kv + 1
+            left[a:e] = True
+        elif bad == "short":
+            b.tensors[2][last] = new[last] - 1
+            left[a:e] = True
+        elif bad == "page":
+            b.tensors[0][last, bad_page] = batch.pages
+            left[e - ((new[last] + 4) % page + 1 if bad_page * page > 5 else new[last]):e] = True
+        elif bad == "start":
+            b.tensors[1][last + 1] = batch.tokens + 1
+            left[a:] = True
+        given = [torch.full((batch.tokens, heads, hd), 7.0, dtype=dt, device=dev) for _ in range(2)]
+        qc.kv8_gather(cache, b, k=given[0], v=given[1], dev_status=st)
+        junk = torch.full((2, batch.tokens, heads, hd), float("nan"), dtype=dt, device=dev)
+        del junk                                        # what the new tensors are likely to lie on
+        st.zero_()
+        for got, want in zip(qc.kv8_gather(cache, b, dtype=dt, dev_status=st), given):
+            assert bool((want[left] == 7).all()) and bool((got[left] == 0).all()), bad
+            assert torch.equal(got[~left], want[~left])
+        assert st.item() == (0 if bad == "nothing" else 3)
+    one = qc.kv8_gather(cache, batch.device(qc, dev), k=given[0], dev_status=st)
+    assert one[0] is given[0] and bool((one[1][e:] == 0).all())
+
+
 @pytest.mark.parametrize("bound", [9, 1000, 1 << 40])
 def test_loose_bound_of_new_tokens(qc, dev, bound):
     """max_new is a bound only: one above the batch's tokens changes nothing."""

@@ -96,8 +96,9 @@ def test_kv8_refusals(q, entry):
         if entry == "attention":
             return lib.qc_hip_kv8_attention(cache, batch, a, sa, b, sb, type, heads, scale, causal,
                                             window, P, None)
-        f = lib.qc_hip_kv8_append if entry == "append" else lib.qc_hip_kv8_gather
-        return f(cache, batch, a, sa, b, sb, type, P, None)
+        if entry == "append":
+            return lib.qc_hip_kv8_append(cache, batch, a, sa, b, sb, type, P, None)
+        return lib.qc_hip_kv8_gather(cache, batch, a, sa, b, sb, type, 1, P, None)
 
     cache, batch = _cache(q), _batch(q)
     ref = ctypes.byref
