@@ -404,7 +404,8 @@ def _flat(what, dtype, *tensors):
 def _status(dev_status):
     if dev_status is None:
         return None
-    _flat("dev_status", _types[0], dev_status)
+    if dev_status.dtype is not _types[0] or dev_status.get_device() != _device():
+        _flat("dev_status", _types[0], dev_status)
     return dev_status.data_ptr()
 
 
@@ -448,17 +449,17 @@ def rope(x, cosine, sine, positions, interleaved=False, out=None, dev_status=Non
     if out is None:
         import torch
         out = torch.zeros(x.shape, dtype=x.dtype, device=x.device)
-    elif out is not x and (out.shape != x.shape or out.stride(2) != 1 or out.dtype is not x.dtype):
+    tokens, heads, head_dim = shape = x.shape
+    xt, xh, _ = x.stride()
+    yt, yh, side = out.stride()
+    if out is not x and (side != 1 or out.shape != shape or out.dtype is not x.dtype):
         raise ValueError("rope: out is of x's shape and type")
     _here(x, out)
     _flat("rope tables", _types[2], cosine, sine)
     _flat("rope positions", _types[0], positions)
-    tokens, heads, head_dim = x.shape
-    most, half = cosine.shape
-    if sine.shape != cosine.shape or positions.numel() != tokens:
+    most, half = table = cosine.shape
+    if sine.shape != table or positions.numel() != tokens:
         raise ValueError("rope: tables [max_position][rotary_dim / 2], a position for each token")
-    xt, xh, _ = x.stride()
-    yt, yh, _ = out.stride()
     _check(lib.qc_hip_rope(x.data_ptr(), out.data_ptr(), st, tokens, heads, head_dim, 2 * half, xt,
                            xh, yt, yh, cosine.data_ptr(), sine.data_ptr(), positions.data_ptr(),
                            most, 1 if interleaved else 0, _status(dev_status), _stream(None)), "rope")
@@ -597,12 +598,13 @@ def quantize_mxfp4(x, dev_status=None):
     import torch
     st = _storage(x)
     _here(x)
-    if x.dim() != 2 or x.stride(1) != 1:
+    stride = x.stride()
+    if len(stride) != 2 or stride[1] != 1:
         raise ValueError("quantize_mxfp4: x is [rows][dim], elements side by side")
     rows, dim = x.shape
     codes = torch.empty((rows, dim // 2), dtype=torch.uint8, device=x.device)
     scales = torch.empty((rows, dim // 32), dtype=torch.uint8, device=x.device)
-    _check(lib.qc_hip_quantize_mxfp4(x.data_ptr(), st, x.stride(0), codes.data_ptr(),
+    _check(lib.qc_hip_quantize_mxfp4(x.data_ptr(), st, stride[0], codes.data_ptr(),
                                      scales.data_ptr(), rows, dim, _status(dev_status),
                                      _stream(None)), "quantize_mxfp4")
     return codes, scales
@@ -610,16 +612,18 @@ def quantize_mxfp4(x, dev_status=None):
 
 def dequantize_mxfp4(codes, scales, dtype=None, out=None):
     """The values [rows][dim] that MXFP4 codes and scales stand for."""
-    _here(codes)
+    if _device is None:
+        _start()
     _flat("mxfp4", _types[1], codes, scales)
     rows, half = codes.shape
     if out is None:
         import torch
         out = torch.empty((rows, 2 * half), dtype=dtype or torch.float32, device=codes.device)
-    elif tuple(out.shape) != (rows, 2 * half) or not out.is_contiguous():
+    elif out.shape != (rows, 2 * half) or not out.is_contiguous():
         raise ValueError("dequantize_mxfp4: out is [rows][dim], contiguous")
-    _here(out)
-    if tuple(scales.shape) != (rows, half // 16):
+    else:
+        _here(out)
+    if scales.shape != (rows, half // 16):
         raise ValueError("dequantize_mxfp4: codes [rows][dim / 2], scales [rows][dim / 32]")
     _check(lib.qc_hip_dequantize_mxfp4(codes.data_ptr(), scales.data_ptr(), out.data_ptr(),
                                        _storage(out), rows, 2 * half, _stream(None)),
@@ -629,19 +633,21 @@ def dequantize_mxfp4(codes, scales, dtype=None, out=None):
 
 def mxfp4_gemm(w_codes, w_scales, x_codes, x_scales, dtype=None, y=None):
     """y [m][n] = x . w^T of MXFP4 matrices w [n][k] and x [m][k]."""
-    _here(w_codes)
+    if _device is None:
+        _start()
     _flat("mxfp4_gemm", _types[1], w_codes, w_scales, x_codes, x_scales)
     n, half = w_codes.shape
     m, other = x_codes.shape
     blocks = half // 16
-    if other != half or tuple(w_scales.shape) != (n, blocks) or tuple(x_scales.shape) != (m, blocks):
+    if other != half or w_scales.shape != (n, blocks) or x_scales.shape != (m, blocks):
         raise ValueError("mxfp4_gemm: codes [rows][k / 2], scales [rows][k / 32]")
     if y is None:
         import torch
         y = torch.empty((m, n), dtype=dtype or torch.float32, device=x_codes.device)
-    elif tuple(y.shape) != (m, n) or not y.is_contiguous():
+    elif y.shape != (m, n) or not y.is_contiguous():
         raise ValueError("mxfp4_gemm: y is [m][n], contiguous")
-    _here(y)
+    else:
+        _here(y)
     _check(lib.qc_hip_mxfp4_gemm(w_codes.data_ptr(), w_scales.data_ptr(), x_codes.data_ptr(),
                                  x_scales.data_ptr(), y.data_ptr(), _storage(y), m, n, 2 * half,
                                  _stream(None)), "mxfp4_gemm")
