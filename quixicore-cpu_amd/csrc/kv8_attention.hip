@@ -1204,24 +1204,34 @@ hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
 // Bytes of fragments laid out at a time; a call with more goes in passes of whole units.
 constexpr long long kFragPass = 1LL << 30;
 
-template <int DP, int NW, int TYPE>
-hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
+// The tiled form's grid for sequences of p.rows_from rows or more: units laid out at most, row
+// blocks of a key head, ranges of keys.
+struct TiledPlan {
+  long long units, blocks;
+};
+TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per) {
   const long long rows = static_cast<long long>(a.max_new) * p.group;
-  p.per = 32 * NW;
-  p.row_blocks = static_cast<int>((rows + p.per - 1) / p.per);
-  const long long span = key_span(a, p, 32 * NW, 64);
+  p.per = per;
+  p.row_blocks = static_cast<int>((rows + per - 1) / per);
+  const long long span = key_span(a, p, per, 64);
   const long long all = static_cast<long long>(a.tokens) * p.group;
   const long long seqs = p.rows_from > 0 ? std::min<long long>(a.seqs, all / p.rows_from) : a.seqs;
-  const long long units = seqs * a.kv_heads;
-  const long long padded = seqs * p.row_blocks, there = all / p.per + seqs;   // at most
+  const long long padded = seqs * p.row_blocks, there = all / per + seqs;   // at most
   p.listed = p.rows_from > 0 || padded > there ? kBlocks : kPadded;
-  const long long blocks = p.listed == kBlocks ? std::min(padded, there) : padded;
+  const long long blocks = std::min(padded, p.listed == kBlocks ? there : padded);
   const long long want = std::max<long long>(1, device_cu_count() / (blocks * a.kv_heads));
   long long chunk = ((span + want - 1) / want + 63) / 64 * 64;
   chunk = std::max<long long>(chunk, 1024);
   chunk = std::min<long long>(chunk, 16 * kTiledGroups);
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((span + chunk - 1) / chunk);
+  return {seqs * a.kv_heads, blocks};
+}
+
+template <int DP, int NW, int TYPE>
+hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
+  const TiledPlan plan = plan_tiled(a, p, 32 * NW);
+  const long long units = plan.units, blocks = plan.blocks;
   Frags f = {};
   f.cap = (a.max_kv + 63) / 64 * 64;
   const long long unit_bytes = static_cast<long long>(f.cap) * DP * 4 + f.cap / 2;   // two of f16, scales
@@ -1254,47 +1264,58 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   return p.splits > 1 ? run_join<TYPE>(a, p, blocks * a.kv_heads, s) : hipSuccess;
 }
 
-// The tiled form lays the cache out first (and reads 64 keys for 256 rows at a time), so it
-// takes prompts: 2048 rows a key head or more, and 2^24 pairs of a row and a key it
-// sees, counted in heads of 128.  us, direct / tiled, 8 key heads of 128, bf16, new tokens of
-// all: 512 of 512 19 / 28, 1024 of 1024 (2^24) 49 / 44, 256 of 4096 (1024 rows) 48 / 48, 1024 of
-// 4096 138 / 84, 2048 of 2048 twice 149 / 88, 8192 of 8192 2068 / 530.
-//
-// Below it, one tile of 16 rows a workgroup or two: two read the keys half as often,
-// one makes twice the workgroups.  us, one / two, 4 query heads a key head: 8 new of 8192
-// 18 / 24, 64 of 4096 28 / 29, 16 of 4096 four times (2^19 = row tiles x keys) 27 / 26, eight
-// times 43 / 37, 100 of 16384 106 / 79.
+// The tiled form lays the cache out first and reads 64 keys for 256 rows (128 of heads above 128) at
+// a time, so it takes prompts: sequences of 512 rows a key head or more, and three workgroups
+// to four CUs; up to 1024 keys, where the direct form is mostly its workgroups' starts, 256
+// rows and one to two CUs.  Below that, one tile of 16 rows a workgroup or two: two read the keys
+// half as often, one makes twice the workgroups (heads above 128: of less than half the
+// registers).  us, one / two / tiled, causal, key heads x rows x keys:
+//                        8 x 512 x 8000     16 x 1024 x 500    16 x 2048 x 2000     64 x 512 x 2000
+//   bf16, heads of 64     45 / 36 / 44        14 / 14 / 21       62 / 50 / 45         65 / 50 / 49
+//   bf16, 128             64 / 51 / 55        22 / 20 / 29      102 / 81 / 62        104 / 82 / 73
+//   bf16, 256             99 / 103 / 82       42 / 47 / 42      183 / 191 / 103      198 / 192 / 126
+//   f32, 128              76 / 62 / 78        27 / 25 / 41      125 / 100 / 86       127 / 102 / 100
+// and, bf16, 128, 192 x 256 x 500 57 / 57 / 44, 16 x 2048 x 500 (128 workgroups) 33 / 36 / 30.  Over
+// 2000 cases of 2 to 192 key heads, 48 to 2048 rows and 500 to 8000 keys the rule is 0.6%
+// off the best of the three.
 //
 // A ragged batch may hold both kinds: the rows counted are those that its tokens allow, and where
-// not every sequence can have 2048 a key head, those that have are laid out and the others
+// not every sequence can have as many, those that have are laid out and the others
 // read directly: 4096 new tokens beside 63 sequences of one, 4000 to 8000 keys, 2317 us
-// with all laid out, 695 so (the prompt alone 480, the others 170).
+// with all laid out, 700 so (the prompt alone 460, the others 170).
 template <int DP, int TYPE>
 hipError_t run_rows(const Kv8Args& a, AttnArgs p, hipStream_t s) {
-  constexpr int kLong = 2048;
-  const double rows = static_cast<double>(a.max_new) * p.group, tokens_rows = static_cast<double>(a.tokens) * p.group;
-  const double all = std::min(a.seqs * rows, tokens_rows) * a.kv_heads;
+  constexpr int NW = DP == 256 ? 4 : 8;
+  const bool brief = a.max_kv <= 1024;
+  const int many = brief ? 256 : 512;
+  const long long rows = static_cast<long long>(a.max_new) * p.group;
+  const long long all = std::min(a.seqs * rows, static_cast<long long>(a.tokens) * p.group);   // of a key head
+  p.rows_to = INT_MAX;
+  bool tiled = p.route == 3;
+  if (p.route == 0 && rows >= many) {
+    AttnArgs q = p;
+    if (all < static_cast<long long>(a.seqs) * many) q.rows_from = many;
+    const long long groups = plan_tiled(a, q, 32 * NW).blocks * a.kv_heads * q.splits;
+    tiled = 4 * groups >= (brief ? 2 : 3) * device_cu_count();
+    if (tiled) p.rows_from = q.rows_from;
+  }
+  if (tiled && p.rows_from == 0) return run_tiled<DP, NW, TYPE>(a, p, s);
   double keys = a.max_kv;
   if (p.causal) keys -= 0.5 * std::min(a.max_new, a.max_kv);
   if (p.window > 0) keys = std::min<double>(keys, p.window);
-  const bool many = rows >= kLong && all * keys * a.head_dim >= 0x1p31;
-  constexpr int NW = DP == 256 ? 4 : 8;
-  p.rows_to = INT_MAX;
-  if (p.route == 3 || (p.route == 0 && many && tokens_rows >= static_cast<double>(a.seqs) * kLong))
-    return run_tiled<DP, NW, TYPE>(a, p, s);
-  const bool both = p.route == 0 && many;
-  if (both) p.rows_to = kLong;
-  const bool two = p.route == 0 ? rows > 16 && (all / 16) * keys >= 0x1p19 : p.route == 2;
+  const double pairs = static_cast<double>(all) * a.kv_heads / 16 * keys;
+  const bool two = p.route == 0 ? rows > 16 && (DP <= 128 ? pairs >= 0x1p19 : keys >= 600 && pairs >= 0x1p20)
+                                : p.route == 2;
+  AttnArgs few = p;
+  few.rows_from = 0;
+  if (tiled) few.rows_to = many;
   hipError_t e = hipSuccess;
   if constexpr (DP < 256 || TYPE != QC_STORAGE_F32) {   // (two of f32 256 do not fit the registers)
-    e = two ? run_direct<DP, 2, TYPE>(a, p, s) : run_direct<DP, 1, TYPE>(a, p, s);
+    e = two ? run_direct<DP, 2, TYPE>(a, few, s) : run_direct<DP, 1, TYPE>(a, few, s);
   } else {
-    e = run_direct<DP, 1, TYPE>(a, p, s);
+    e = run_direct<DP, 1, TYPE>(a, few, s);
   }
-  if (!both || e != hipSuccess) return e;
-  p.rows_from = kLong;
-  p.rows_to = INT_MAX;
-  return run_tiled<DP, NW, TYPE>(a, p, s);
+  return tiled && e == hipSuccess ? run_tiled<DP, NW, TYPE>(a, p, s) : e;
 }
 
 template <int TYPE>

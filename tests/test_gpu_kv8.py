@@ -962,11 +962,11 @@ def test_attention_long_prompts(qc, dev, dtype, new, kv, heads, kvh, hd, window)
     tol = size * (bits + 2 * 4 * score * (hd + 8) * 2.0 ** -24 + 200 * 2.0 ** -23) + HALF[dtype] * (1 + 2.0 ** -10) * want.abs() + 2.0 ** -24
     outs = []
     try:
-        for r in (0, 1, 3):
+        for r in (0, 1, 2, 3):
             qc.set_kv8_attention_route(r)
             out = qc.kv8_attention(cache, b, q, window=window)
             assert bool(((out.double() - want).abs() <= tol)[:batch.start[-1]].all()), r
             outs.append(out)
     finally:
         qc.set_kv8_attention_route(0)
-    assert torch.equal(outs[0], outs[2])       # the sizes choose the tiled kernels
+    assert any(torch.equal(outs[0], o) for o in outs[1:])     # the sizes choose one of them
