@@ -401,35 +401,35 @@ struct Operands {
   int m, n, blocks;
 };
 
-// The tiles, and what they cost: us of one round of workgroups on the CUs and of each
-// further one, K = 4096 (measured over M = 1 to 4096, N = 1000 to 14336; longer rows scale
-// all alike).  us at K = 4096 by tile, M x N:
+// The tiles, and what a product of K costs with each: fixed + K / 4096 (first + more (rounds - 1)) us,
+// rounds being the tiles over the CUs, of which `whole` counts started rounds whole. Fitted
+// to 730 sizes of M 1 to 4096, N 256 to 16384, K 256 to 14336, over which the tile chosen is 0.2%
+// slower than the best (a fit to half of them, on the other half: 0.3%).  us at K = 4096:
 //            32x32  64x32  64x64  128x64  128x128  256x128  256x256
-// 1 x 14336    8.0    7.8    8.4    10.0     12.5     20.7     29.8
-// 64 x 4096    5.7    7.0    7.9    10.1     12.0     19.5     26.1
-// 128 x 14336 23.0   20.7   15.6    13.2     16.6     25.2     33.5
-// 512 x 4096  24.1   23.4   15.4    13.2     16.2     24.4     37.2
-// 512 x 14336 72.4   65.0   43.3    38.5     31.6     29.0     42.2
-// 2048 x 14336 273    241    159     138      108      103       90
+// 1 x 14336    7.7    7.5    8.4     9.8     12.3     20.4     30.4
+// 64 x 4096    5.4    6.7    7.8    10.4     11.7     19.7     27.8
+// 128 x 14336 23.1   20.4   14.5    12.4     14.9     22.2     32.3
+// 512 x 4096  23.3   22.6   14.0    12.0     14.4     21.5     32.2
+// 512 x 14336 72.0   62.4   40.9    37.3     28.7     25.3     36.0
+// 2048 x 14336 261    230    154     133      103       97       80
 struct Tile {
   int tn, tm;
-  bool whole_rounds;     // one workgroup a CU: a started round costs a round
-  double first, more;
+  double fixed, first, more, whole;
 };
 constexpr int kTiles = 7;
-constexpr Tile kTile[kTiles] = {{32, 32, false, 5.6, 3.2},  {64, 32, false, 7.4, 5.4},   {64, 64, false, 9.4, 6.5},
-                                {128, 64, false, 13.0, 9.0}, {128, 128, true, 18.0, 15.0}, {256, 128, true, 29.0, 25.0},
-                                {256, 256, true, 42.0, 42.0}};
+constexpr Tile kTile[kTiles] = {{32, 32, 3.3, 3.0, 3.9, 0.7},     {64, 32, 3.3, 4.8, 6.3, 1.0},
+                                {64, 64, 3.6, 5.2, 8.7, 1.0},     {128, 64, 3.2, 11.1, 11.3, 1.0},
+                                {128, 128, 4.8, 12.4, 22.1, 1.0}, {256, 128, 5.7, 25.5, 40.3, 0.7},
+                                {256, 256, 20.5, 27.9, 48.1, 1.0}};
 
-int choose_tile(long long m, long long n, int cus) {
+int choose_tile(long long m, long long n, long long k, int cus) {
   int best = 0;
   double least = 0.0;
   for (int i = 0; i < kTiles; ++i) {
     const Tile& t = kTile[i];
     const double tiles = static_cast<double>((n + t.tn - 1) / t.tn) * static_cast<double>((m + t.tm - 1) / t.tm);
-    double rounds = tiles / cus;
-    if (t.whole_rounds) rounds = std::ceil(rounds);
-    const double cost = t.first + t.more * std::max(0.0, rounds - 1.0);
+    const double rounds = t.whole * std::ceil(tiles / cus) + (1.0 - t.whole) * tiles / cus;
+    const double cost = t.fixed + static_cast<double>(k) / 4096.0 * (t.first + t.more * std::max(0.0, rounds - 1.0));
     if (i == 0 || cost < least) {
       least = cost;
       best = i;
@@ -455,7 +455,7 @@ hipError_t run_gemm(Operands o, int route, hipStream_t s) {
   StreamWorkspace* ws = nullptr;
   std::unique_lock<std::mutex> hold;
   // a tile's codes are addressed with 32 bits: 32 rows of long ones
-  const int tile = o.blocks > (1 << 19) ? 0 : route > 0 ? route - 1 : choose_tile(o.m, o.n, device_cu_count());
+  const int tile = o.blocks > (1 << 19) ? 0 : route > 0 ? route - 1 : choose_tile(o.m, o.n, 32LL * o.blocks, device_cu_count());
   int stride = o.blocks;
   // Rows of scales that do not begin at dwords: laid out first for the largest tile, whose LDS
   // has no time for the third dwords (us, laid out / in the ring, K = 4064, N = 14336: M = 1 11.4 /
