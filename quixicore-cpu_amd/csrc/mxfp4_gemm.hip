@@ -44,14 +44,14 @@ __device__ __forceinline__ i32x8 fp4_operand(const i32x4& v) {
 // holds chunk 4 (l >> 5) + q of row l & 31, whose scale is byte q of the dword that it
 // holds for the whole step.
 //
-// What bounds it: with few rows of x the stream of w (M = 1, 14336 x 4096: 31 MB, 7.8 us, of
+// What bounds it: with few rows of x the stream of w (M = 1, 14336 x 4096: 31 MB, 7.1 us, of
 // which a launch and the first bytes are about 3; a form without LDS, 16 rows a workgroup and
-// the codes straight to registers, took 9.2, M = 32 17 against 8.3); with many, a step's chain
+// the codes straight to registers, took 9.2, M = 32 17 against 8); with many, a step's chain
 // of barrier, LDS reads and MFMAs, the LDS traffic (a 256 x 256 tile reads its 64 KB stage
 // three times and writes it once, as many cycles as its MFMAs) and MFMA power: M = 4096,
-// 14336 x 4096, quantised normal values, 182 us = 2.64 PFLOP/s, of it about 25 for the
-// outputs' burst.  Eight waves of 64 x 128 there: four of 128 x 128 are 6% slower, sixteen of
-// 64 x 64 3%; 128 x 128 tiles (M = 512) take 16 us with eight waves, 24 with four.
+// 14336 x 4096, quantised normal values, 155 us = 3.1 PFLOP/s, the matrix cores busy half of
+// it. Eight waves of 64 x 128 there: four of 128 x 128 are 6% slower, sixteen of
+// 64 x 64 3%; 128 x 128 tiles (M = 512) take 14 us with eight waves, 24 with four.
 __device__ __forceinline__ void ring_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
