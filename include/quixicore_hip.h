@@ -454,7 +454,9 @@ int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void
  * (n > kv_len, or kv_len 0) is zeros.  q and out do not overlap.  Pages that no row sees are not looked at; one
  * that is seen and has a scale that is not finite is an error like a bad page id.
  * The probabilities enter the product with the values in 11 bits (bf16 q, and f16 q
- * of prompts of some thousand tokens) or 22; dots, sums and statistics are f32.  Status: 1 for sizes out of range, 2 for an
+ * of prompts of some hundred tokens) or 22; dots, sums and statistics are f32.  They are held
+ * relative to their row's largest and their page's value scale to the largest of the keys
+ * read together: a product of both below 2^-25 loses bits.  Status: 1 for sizes out of range, 2 for an
  * unknown type, 3 for NULL or misaligned pointers, a scale that is not finite, or a
  * window without causal. */
 int qc_hip_kv8_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* q,

@@ -687,7 +687,10 @@ __global__ __launch_bounds__(256) void attention_layout(Kv8Args a, AttnArgs p, F
 // PFLOP/s of both (a plain f16 product of 8192^3 reaches 1.11).  MFMAs and VALU are each busy
 // half of the SIMDs' cycles and the clock is at 1.9 GHz: what bounds it is issue and power.
 // Priorities by wave or phase change nothing or cost 4%.
-constexpr int kTiledGroups = 1024;   // 16-key groups of a range
+// 16-key groups of a range: what LDS holds beside the buffers. (Each range of a prompt's keys
+// takes its rows' sums in memory: 17 GB for 131072 tokens of 32 heads in ranges of 16384.)
+template <int DP>
+constexpr int kTiledGroups = DP == 256 ? 1024 : 4096;
 
 template <int DP, int NW, int TYPE>
 __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, AttnArgs p, Frags f) {
@@ -698,7 +701,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   constexpr int S = 2;                            // buffers (three: 582 -> 605 us)
   static_assert(kBytes % (1024 * NW) == 0, "whole loads");
   __shared__ __attribute__((aligned(1024))) uint8_t s_k[S * kBytes], s_v[S * kBytes];
-  __shared__ f32x4 s_c[kTiledGroups / 4], s_b[kTiledGroups / 4], s_inv[kTiledGroups / 4];
+  __shared__ f32x4 s_c[kTiledGroups<DP> / 4], s_b[kTiledGroups<DP> / 4], s_inv[kTiledGroups<DP> / 4];
   __shared__ float s_unit[NW];
   __shared__ int s_bad[NW];
 
@@ -1209,7 +1212,7 @@ constexpr long long kFragPass = 1LL << 30;
 struct TiledPlan {
   long long units, blocks;
 };
-TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per) {
+TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per, int max_groups) {
   const long long rows = static_cast<long long>(a.max_new) * p.group;
   p.per = per;
   p.row_blocks = static_cast<int>((rows + per - 1) / per);
@@ -1222,7 +1225,7 @@ TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per) {
   const long long want = std::max<long long>(1, device_cu_count() / (blocks * a.kv_heads));
   long long chunk = ((span + want - 1) / want + 63) / 64 * 64;
   chunk = std::max<long long>(chunk, 1024);
-  chunk = std::min<long long>(chunk, 16 * kTiledGroups);
+  chunk = std::min<long long>(chunk, 16 * max_groups);
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((span + chunk - 1) / chunk);
   return {seqs * a.kv_heads, blocks};
@@ -1230,7 +1233,7 @@ TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per) {
 
 template <int DP, int NW, int TYPE>
 hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
-  const TiledPlan plan = plan_tiled(a, p, 32 * NW);
+  const TiledPlan plan = plan_tiled(a, p, 32 * NW, kTiledGroups<DP>);
   const long long units = plan.units, blocks = plan.blocks;
   Frags f = {};
   f.cap = (a.max_kv + 63) / 64 * 64;
@@ -1295,7 +1298,7 @@ hipError_t run_rows(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   if (p.route == 0 && rows >= many) {
     AttnArgs q = p;
     if (all < static_cast<long long>(a.seqs) * many) q.rows_from = many;
-    const long long groups = plan_tiled(a, q, 32 * NW).blocks * a.kv_heads * q.splits;
+    const long long groups = plan_tiled(a, q, 32 * NW, kTiledGroups<DP>).blocks * a.kv_heads * q.splits;
     tiled = 4 * groups >= (brief ? 2 : 3) * device_cu_count();
     if (tiled) p.rows_from = q.rows_from;
   }

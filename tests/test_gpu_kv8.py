@@ -900,9 +900,10 @@ def test_a_captured_decoding_step(qc, dev):
 
 
 @pytest.mark.parametrize("new,kv,route", [
-    ([1] * 70, 4096, 3), ([1] * 40 + [260] + [1] * 29, 4096, 3), ([1] * 9 + [1024] * 17 + [1] * 50, 16384, 0)])
+    ([1] * 70, 4096, 3), ([1] * 40 + [260] + [1] * 29, 4096, 3), ([1] * 9 + [1024] * 17 + [1] * 50, 16384, 0),
+    ([1, 300, 2], 40000, 3), ([700], 70000, 3)])
 def test_attention_passes_of_the_layout(qc, dev, new, kv, route):
-    """More keys than are laid out at a time (1 GB): several passes, the same values as read
+    """More keys than are laid out at a time (1 GB) or than one range holds: the same values as read
     directly, within both forms' rounding."""
     import torch
     rng = np.random.default_rng(70)
