@@ -14,6 +14,7 @@
 #include <initializer_list>
 #include <limits>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -177,17 +178,31 @@ bool known_storage(int type) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// No exception leaves a C entry.
+template <class F>
+int guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return QC_OUT_OF_MEMORY;
+  } catch (...) {
+    return QC_DEVICE_ERROR;
+  }
+}
+
 // dev_status set: launch(dev_status), asynchronous.  NULL: check(flag) first,
 // 3 and nothing written if it set the flag, then launch and wait.
 template <class Check, class Launch>
 int checked(int* dev_status, hipStream_t s, Check&& check, Launch&& launch) {
-  if (dev_status != nullptr) return finish(launch(dev_status));
-  int bad = 0;
-  int st = with_flag(s, &bad, check);
-  if (st != QC_OK) return st;
-  if (bad) return QC_INVALID_ARGUMENT;
-  st = with_flag(s, &bad, launch);
-  return st == QC_OK && bad ? QC_INVALID_ARGUMENT : st;
+  return guarded([&] {
+    if (dev_status != nullptr) return finish(launch(dev_status));
+    int bad = 0;
+    int st = with_flag(s, &bad, check);
+    if (st != QC_OK) return st;
+    if (bad) return static_cast<int>(QC_INVALID_ARGUMENT);
+    st = with_flag(s, &bad, launch);
+    return st == QC_OK && bad ? static_cast<int>(QC_INVALID_ARGUMENT) : st;
+  });
 }
 
 // Sizes of a cache and a batch; 64-bit element offsets, int counts.
@@ -815,8 +830,9 @@ int qc_hip_rope_table(float* cosine, float* sine, long long first_position, long
     keep = std::min(std::max(keep, 0.0), 1.0);
     f.w[i] = keep * w + (1.0 - keep) * w / factor;
   }
-  return finish(qc::launch_rope_table(cosine, sine, first_position, positions, half, f,
-                                      as_stream(stream)));
+  return guarded([&] {
+    return finish(qc::launch_rope_table(cosine, sine, first_position, positions, half, f, as_stream(stream)));
+  });
 }
 
 int qc_hip_rope(const void* x, void* y, int type, long long tokens, long long heads,
@@ -968,7 +984,8 @@ int qc_hip_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, void* o
   if (!known_storage(type)) return QC_UNSUPPORTED_FORMAT;
   if (codes == nullptr || scales == nullptr || out == nullptr || !aligned16(codes))
     return QC_INVALID_ARGUMENT;
-  return finish(qc::launch_dequantize_mxfp4(codes, scales, out, type, rows, dim, as_stream(stream)));
+  return guarded(
+      [&] { return finish(qc::launch_dequantize_mxfp4(codes, scales, out, type, rows, dim, as_stream(stream))); });
 }
 
 int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* x_codes,
@@ -981,9 +998,11 @@ int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uin
   if (w_codes == nullptr || w_scales == nullptr || x_codes == nullptr || x_scales == nullptr ||
       y == nullptr || !aligned16(w_codes) || !aligned16(x_codes))
     return QC_INVALID_ARGUMENT;
-  return finish(qc::launch_mxfp4_gemm(w_codes, w_scales, x_codes, x_scales, y, y_type, m, n, k,
-                                      g_knobs.mxfp4_route.load(std::memory_order_relaxed),
-                                      as_stream(stream)));
+  return guarded([&] {
+    return finish(qc::launch_mxfp4_gemm(w_codes, w_scales, x_codes, x_scales, y, y_type, m, n, k,
+                                        g_knobs.mxfp4_route.load(std::memory_order_relaxed),
+                                        as_stream(stream)));
+  });
 }
 
 int qc_hip_set_qgemm_panel(int mode) {

@@ -57,7 +57,10 @@ hipError_t stream_buffer(StreamWorkspace* w, hipStream_t s, size_t bytes, int ta
     w->bytes[tag] = 0;
   }
   void* p = nullptr;
-  if ((e = hipMalloc(&p, bytes ? bytes : 256)) != hipSuccess) return e;
+  if ((e = hipMalloc(&p, bytes ? bytes : 256)) != hipSuccess) {
+    (void)hipGetLastError();   // reported here, not by the next launch
+    return e;
+  }
   w->ptr[tag] = p;
   w->bytes[tag] = bytes ? bytes : 256;
   w->captured[tag] = capturing;

@@ -734,6 +734,27 @@ def test_attention_from_threads(qc, dev):
     assert not wrong
 
 
+def test_attention_without_room_for_its_sums(qc, dev):
+    """A bound of keys whose ranges would take more memory than the device has is an error, with
+    nothing written; the next call is none the worse."""
+    import torch
+    rng = np.random.default_rng(1)
+    batch = Ragged(rng, [8192], [8192], 256, columns=1 << 22)
+    cache = _random_cache(qc, dev, rng, batch.pages, 1, 256, 16)
+    q = torch.randn(8192, 32, 16, device=dev)
+    out = torch.full_like(q, 7.0)
+    st = torch.zeros(1, dtype=torch.int32, device=dev)
+    try:
+        qc.set_kv8_attention_route(1)
+        with pytest.raises(qc.QcError) as e:
+            qc.kv8_attention(cache, batch.device(qc, dev, max_kv=1 << 30), q, out=out, dev_status=st)
+        assert e.value.status in (4, 5)
+    finally:
+        qc.set_kv8_attention_route(0)
+    assert bool((out == 7).all()) and st.item() == 0
+    _attend(qc, dev, rng, [1, 40], [100, 700], 8, 2, 64, 16)
+
+
 def test_attention_strided_rows(qc, dev, route):
     """q inside fused projection rows, out inside wider rows; odd element offsets."""
     import torch
