@@ -149,6 +149,18 @@ __device__ __forceinline__ float row_scale(float top, float& inverse) {
   return ldexpf(1.0f, 15 - e);
 }
 
+// A value that all lanes hold, in a scalar register.
+__device__ __forceinline__ float uniform(float v) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
+}
+
+// unit = m 2^e of a workgroup's largest value scale, m 0 or in [1/2, 1).
+__device__ __forceinline__ float split_unit(float unit, int& e) {
+  const float m = frexpf(unit, &e);
+  e = __builtin_amdgcn_readfirstlane(e);
+  return uniform(m);
+}
+
 // Elements d, .., d + 7 of a q row (zeros at and past head_dim, a multiple of 16).
 template <int TYPE>
 __device__ __forceinline__ void load8(const void* q, long long at, bool in, bool vec, float* v) {
@@ -367,8 +379,11 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) unit = fmaxf(unit, s_red[w]);
-  // probabilities enter the second product as p * (value scale / unit) * 2^15
-  const float per_unit = unit > 0.f ? 32768.0f / unit : 0.f;
+  // Probabilities enter the second product as p * (value scale / unit) * 2^15, the power of two
+  // in either scale taken out first: 2^15 / unit alone is infinite from 9.6e-35 down.
+  int unit_e;
+  const float unit_m = split_unit(unit, unit_e);
+  const float per_unit = uniform(unit > 0.f ? 32768.0f / unit_m : 0.f);
 
   float m[RT], l[RT];
   f32x4 acc[RT][VB];
@@ -411,7 +426,7 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
       load_k(at0, at1);
     }
     const float ks[2] = {s_ks[i], s_ks[i1]};
-    const float vr[2] = {s_vs[i] * per_unit, s_vs[i1] * per_unit};
+    const float vr[2] = {ldexpf(s_vs[i], -unit_e) * per_unit, ldexpf(s_vs[i1], -unit_e) * per_unit};
     const int page[2] = {s_page[i], s_page[i1]};
     const bool whole = __builtin_amdgcn_readfirstlane(tok >= all_lo && tok + 32 <= all_hi && tok + 32 <= to &&
                                                       page[0] >= 0 && page[1] >= 0);
@@ -524,7 +539,7 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
     if (half > 1) __syncthreads();
   }
   if (wave > 0) return;
-  const float back = unit * (1.0f / 32768.0f);
+  const float back = unit_m * (1.0f / 32768.0f);  // (times 2^unit_e, last: no factor underflows)
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = r0 + 16 * t + row16;
@@ -546,7 +561,7 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
       if (d >= a.head_dim) continue;
       float v[VB];
 #pragma unroll
-      for (int k = 0; k < VB; ++k) v[k] = acc[t][k][e] * f;
+      for (int k = 0; k < VB; ++k) v[k] = ldexpf(acc[t][k][e] * f, unit_e);
       if (last)
         store_n<TYPE, VB>(p.out, (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim + d,
                           p.vec, v);
@@ -986,7 +1001,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   l += __shfl_xor(l, 32);
   if (!has) return;
   const bool last = p.splits == 1;
-  const float back = unit * (NQ == 2 ? 1.0f / 32768.0f : 1.0f / 2048.0f) + broken;   // 2^-kShift
+  int unit_e;                                     // its power of two comes last: no factor underflows
+  const float unit_m = split_unit(unit, unit_e);
+  const float back = unit_m * (NQ == 2 ? 1.0f / 32768.0f : 1.0f / 2048.0f) + broken;   // 2^-kShift
   const float scale = last ? (l == 0.f ? 0.f : back / l) : back;
   const long long row = static_cast<long long>(u.first + token) * p.heads + head;
   const long long part = static_cast<long long>(split) * a.tokens * p.heads + row;
@@ -1005,7 +1022,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
       if (d >= a.head_dim) continue;
       float v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = l == 0.f ? 0.f : acc[t][e + j] * scale;
+      for (int j = 0; j < 4; ++j) v[j] = l == 0.f ? 0.f : ldexpf(acc[t][e + j] * scale, unit_e);
       if (last)
         store_n<TYPE, 4>(p.out, (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim + d,
                          p.vec, v);

@@ -528,6 +528,50 @@ def test_attention_scales_far_apart(qc, dev, route, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("new,kv", [([1, 1], [300, 90]), ([70], [300]), ([1], [4000]), ([40, 3], [1500, 31])])
+@pytest.mark.parametrize("down", [107, 113, 121])
+def test_attention_tiny_value_scales(qc, dev, route, dtype, new, kv, down):
+    """Value scales near 1e-34, 1e-36 and 2^-126 (some below it), some of them 0: outputs are those of
+    scales 2^down times as large, over 2^down, to within the tolerance there and the spacing of
+    the type's subnormals."""
+    import torch
+    print(f"kv8 attention tiny value scales {dtype} new {new} kv {kv} 2^-{down}", flush=True)
+    rng = np.random.default_rng(down + len(new))
+    batch = Ragged(rng, new, kv, 16)
+    cache = _random_cache(qc, dev, rng, batch.pages, 2, 16, 64)
+    # few bits, so that 2^-down of them is exact where it is subnormal too
+    vs = rng.integers(0, 256, (batch.pages, 2)).astype(np.float32) * np.float32(2.0 ** -13)
+    cache.tensors[3].copy_(torch.from_numpy(vs * np.float32(2.0 ** -down)))
+    q = torch.from_numpy(rng.standard_normal((batch.tokens, 4, 64))).to(getattr(torch, dtype))
+    st = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = qc.kv8_attention(cache, batch.device(qc, dev), q.to(dev), dev_status=st)
+    assert st.item() == 0
+    if dtype == "float16":
+        assert bool((out == 0).all())                 # below half of 2^-24
+        return
+    host = _host(cache)
+    host[3] = vs
+    want, tol = _attention_reference(host, batch, q.float().numpy(), 4, 0.125, True, 0, HALF[dtype])
+    # half a step of subnormal outputs; the sums of at most 40 ranges are stored in f32
+    tol += 2.0 ** (down - (150 if dtype == "float32" else 134)) + 40 * 2.0 ** (down - 150)
+    err = np.abs(out.double().cpu().numpy() * 2.0 ** down - want)
+    assert np.all(err <= tol), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("new", [1, 30])
+@pytest.mark.parametrize("scale", [1e-34, 1e-36, 2.0 ** -126])
+def test_attention_tiny_value_scales_in_some_ranges(qc, dev, route, dtype, new, scale):
+    """Whole key ranges of tiny values between normal ones change nothing beyond their own share."""
+    rng = np.random.default_rng(new)
+    batch = Ragged(rng, [new], [4000], 16)
+    cache = _random_cache(qc, dev, rng, batch.pages, 2, 16, 64)
+    pid, _ = batch.places(0, 512, 3072)
+    cache.tensors[3][np.unique(pid)] = scale
+    _attend(qc, dev, rng, [new], [4000], 4, 2, 64, 16, dtype, batch=batch, cache=cache)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 def test_attention_peaked_q(qc, dev, route, dtype):
     """One channel of q far above the rest where the keys hold zero: the others keep
     their bits."""
