@@ -429,8 +429,8 @@ typedef struct qc_kv8_batch {
  * nearest 1 / 127, or 0 below 2^-126; codes held
  * become rint(code * (s / s')), new ones clamp(rint(x * (1 / s')), +-127), each
  * step rounded to f32.  A page written by a call must belong to one sequence.
- * A page and head with a non-finite new value or scale held, and a sequence of more
- * new tokens than kv_len, are errors and left as they were.  Status: 1 for sizes out of range, 2 for an
+ * A page and head with a non-finite new value, or a non-finite scale held where the page has tokens
+ * before the new ones, and a sequence of more new tokens than kv_len, are errors and left as they were.  Status: 1 for sizes out of range, 2 for an
  * unknown type, 3 for NULL or misaligned pointers. */
 int qc_hip_kv8_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* k,
                       long long k_stride, const void* v, long long v_stride, int type,
@@ -439,8 +439,9 @@ int qc_hip_kv8_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch, cons
 /* The same places read back: k and v rows of the batch's tokens receive the
  * values held at positions kv_len - n .. kv_len - 1 (a seq_start that spans whole
  * sequences reads all of them).  zero_rest != 0: rows of k and v that receive nothing (of no
- * sequence, or left out by an error) become zeros; else they stay as they were.  Status and
- * errors as for qc_hip_kv8_append. */
+ * sequence, or left out by an error) become zeros; else they stay as they were.  Errors: a sequence of
+ * more new tokens than kv_len, and a page and head with a scale that is not finite, are left out.  Status as
+ * for qc_hip_kv8_append. */
 int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void* k,
                       long long k_stride, void* v, long long v_stride, int type, int zero_rest,
                       int* dev_status, void* stream);

@@ -895,7 +895,7 @@ int qc_hip_kv8_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch, cons
   return checked(
       dev_status, s,
       [&](int* flag) {
-        hipError_t e = qc::launch_kv8_check(*cache, *batch, true, 0, flag, s);
+        hipError_t e = qc::launch_kv8_check(*cache, *batch, qc::Kv8Call::kAppend, 0, flag, s);
         if (e == hipSuccess) e = qc::launch_kv8_nonfinite(*cache, *batch, k, k_stride, v, v_stride, type, flag, s);
         return e;
       },
@@ -916,7 +916,7 @@ int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void
   const hipStream_t s = as_stream(stream);
   return checked(
       dev_status, s,
-      [&](int* flag) { return qc::launch_kv8_check(*cache, *batch, true, 0, flag, s); },
+      [&](int* flag) { return qc::launch_kv8_check(*cache, *batch, qc::Kv8Call::kGather, 0, flag, s); },
       [&](int* flag) {
         return qc::launch_kv8_gather(*cache, *batch, k, k_stride, v, v_stride, type, zero_rest != 0, flag, s);
       });
@@ -955,7 +955,7 @@ int qc_hip_kv8_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, c
   return checked(
       dev_status, s,
       [&](int* flag) {
-        return qc::launch_kv8_check(*cache, *batch, false, static_cast<int>(r.window), flag, s);
+        return qc::launch_kv8_check(*cache, *batch, qc::Kv8Call::kAttention, static_cast<int>(r.window), flag, s);
       },
       [&](int* flag) { return qc::launch_kv8_attention(r, flag, s); });
 }

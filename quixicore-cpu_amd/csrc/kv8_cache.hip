@@ -230,57 +230,61 @@ __global__ __launch_bounds__(NT) void gather_kernel(Kv8Args a, void* k, void* v,
   }
   Place w;
   if (!place_of(a, slots, w)) return;
-  if (w.unit < 0) {                               // a page that is not there
-    if (rest == 0) return;
-    for (int t = 0; t < w.hi - w.lo; ++t)
-      zero_row<TYPE, NT, VEC>(static_cast<raw*>(w.which ? v : k) + (w.row + t) * (w.which ? v_stride : k_stride) +
-                                  static_cast<long long>(w.head) * a.head_dim,
-                              a.head_dim);
-    return;
-  }
-  const u32x2* codes = reinterpret_cast<const u32x2*>(
-      (w.which ? a.v_codes : a.k_codes) + (w.unit * a.page_tokens + w.lo - w.p0) * a.head_dim);
-  const float scale = (w.which ? a.v_scales : a.k_scales)[w.unit];
   const long long stride = w.which ? v_stride : k_stride;
   raw* out = static_cast<raw*>(w.which ? v : k) + w.row * stride +
              static_cast<long long>(w.head) * a.head_dim;
-  const int per_row = a.head_dim / 8, n = (w.hi - w.lo) * per_row;
-  for (int i0 = threadIdx.x; i0 < n; i0 += kHeld * NT) {
-    u32x2 held[kHeld];
+  if (w.unit >= 0) {
+    const u32x2* codes = reinterpret_cast<const u32x2*>(
+        (w.which ? a.v_codes : a.k_codes) + (w.unit * a.page_tokens + w.lo - w.p0) * a.head_dim);
+    const float scale = (w.which ? a.v_scales : a.k_scales)[w.unit];
+    // looked at in the loop, where the codes are on their way (ahead of them: 0.2 us a call)
+    float s = scale;
+    const int per_row = a.head_dim / 8, n = (w.hi - w.lo) * per_row;
+    for (int i0 = threadIdx.x; i0 < n; i0 += kHeld * NT) {
+      u32x2 held[kHeld];
 #pragma unroll
-    for (int h = 0; h < kHeld; ++h)
-      if (i0 + h * NT < n) held[h] = codes[i0 + h * NT];
+      for (int h = 0; h < kHeld; ++h)
+        if (i0 + h * NT < n) held[h] = codes[i0 + h * NT];
+      asm volatile("" : "+s"(s));
+      if (!isfinite(s)) break;
 #pragma unroll
-    for (int h = 0; h < kHeld; ++h) {
-      const int i = i0 + h * NT;
-      if (i >= n) break;
-      float f[8];
+      for (int h = 0; h < kHeld; ++h) {
+        const int i = i0 + h * NT;
+        if (i >= n) break;
+        float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        f[j] = static_cast<float>(static_cast<int8_t>(held[h][j >> 2] >> (8 * (j & 3)))) * scale;
-      const int t = i / per_row;
-      raw* o = out + t * stride + (i - t * per_row) * 8;
-      if constexpr (VEC) {
+        for (int j = 0; j < 8; ++j)
+          f[j] = static_cast<float>(static_cast<int8_t>(held[h][j >> 2] >> (8 * (j & 3)))) * s;
+        const int t = i / per_row;
+        raw* o = out + t * stride + (i - t * per_row) * 8;
+        if constexpr (VEC) {
 #pragma unroll
-        for (int j = 0; j < 8; j += Storage<TYPE>::per16) *reinterpret_cast<u32x4*>(o + j) = encode16<TYPE>(f + j);
-      } else {
+          for (int j = 0; j < 8; j += Storage<TYPE>::per16) *reinterpret_cast<u32x4*>(o + j) = encode16<TYPE>(f + j);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = encode<TYPE>(f[j]);
+          for (int j = 0; j < 8; ++j) o[j] = encode<TYPE>(f[j]);
+        }
       }
     }
+    if (isfinite(scale)) return;
+    if (threadIdx.x == 0) *a.status = QC_INVALID_ARGUMENT;
   }
+  // a page that is not there, or without a scale
+  if (rest == 0) return;
+  for (int t = 0; t < w.hi - w.lo; ++t) zero_row<TYPE, NT, VEC>(out + t * stride, a.head_dim);
 }
 
-// The figures and table entries that a call goes by.  from_new: it touches the
-// new tokens' pages; else the pages that its queries see (window: see
-// qc_hip_kv8_attention), and their scales are finite.
-__global__ __launch_bounds__(kThreads) void kv8_check(Kv8Args a, bool from_new, int window) {
+// The figures, table entries and scales that a call goes by: append and gather touch the new
+// tokens' pages, attention those that its queries see (window: see qc_hip_kv8_attention).
+// An append goes by the scales of pages that hold tokens before the new ones, the others by all.
+__global__ __launch_bounds__(kThreads) void kv8_check(Kv8Args a, Kv8Call call, int window) {
   const int q = blockIdx.x;
   int first, rows, kv;
   if (!kv8_sequence(a, q, first, rows, kv)) return;
   if (rows == 0) return;
-  if (from_new && rows > kv) *a.status = QC_INVALID_ARGUMENT;
-  const int from = from_new ? max(kv - rows, 0) : window > 0 ? max(kv - rows + 1 - window, 0) : 0;
+  const bool attention = call == Kv8Call::kAttention;
+  if (!attention && rows > kv) *a.status = QC_INVALID_ARGUMENT;
+  const int from = !attention ? max(kv - rows, 0) : window > 0 ? max(kv - rows + 1 - window, 0) : 0;
   for (int c = (from >> a.page_shift) + threadIdx.x; c < (kv + a.page_tokens - 1) >> a.page_shift;
        c += kThreads) {
     const int page = a.table[static_cast<long long>(q) * a.columns + c];
@@ -288,7 +292,7 @@ __global__ __launch_bounds__(kThreads) void kv8_check(Kv8Args a, bool from_new, 
       *a.status = QC_INVALID_ARGUMENT;
       continue;
     }
-    if (from_new) continue;
+    if (call == Kv8Call::kAppend && c << a.page_shift >= kv - rows) continue;
     for (int h = 0; h < a.kv_heads; ++h) {
       const long long at = static_cast<long long>(page) * a.kv_heads + h;
       if (!isfinite(a.k_scales[at]) || !isfinite(a.v_scales[at])) *a.status = QC_INVALID_ARGUMENT;
@@ -350,10 +354,10 @@ Kv8Args kv8_args(const qc_kv8_cache& c, const qc_kv8_batch& b, int* status) {
   return a;
 }
 
-hipError_t launch_kv8_check(const qc_kv8_cache& c, const qc_kv8_batch& b, bool from_new, int window,
+hipError_t launch_kv8_check(const qc_kv8_cache& c, const qc_kv8_batch& b, Kv8Call call, int window,
                             int* flag, hipStream_t s) {
   const Kv8Args a = kv8_args(c, b, flag);
-  kv8_check<<<a.seqs, kThreads, 0, s>>>(a, from_new, window);
+  kv8_check<<<a.seqs, kThreads, 0, s>>>(a, call, window);
   return hipGetLastError();
 }
 

@@ -282,7 +282,8 @@ hipError_t launch_rope_table(float* cosine, float* sine, long long first, long l
 
 // The 8-bit key/value cache (qc_hip_kv8_*); shapes and pointers checked by the
 // caller, the device's lengths and page ids by the kernels (*status = 3).
-hipError_t launch_kv8_check(const qc_kv8_cache& c, const qc_kv8_batch& b, bool from_new, int window,
+enum class Kv8Call { kAppend, kGather, kAttention };
+hipError_t launch_kv8_check(const qc_kv8_cache& c, const qc_kv8_batch& b, Kv8Call call, int window,
                             int* flag, hipStream_t s);
 hipError_t launch_kv8_nonfinite(const qc_kv8_cache& c, const qc_kv8_batch& b, const void* k,
                                 long long k_stride, const void* v, long long v_stride, int type,

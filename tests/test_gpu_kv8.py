@@ -232,6 +232,94 @@ def test_append_errors(qc, dev):
         assert st.item() == 3
 
 
+@pytest.mark.parametrize("which", [2, 3], ids=["k", "v"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_append_errors_of_held_scales(qc, dev, which, value):
+    """A scale held that is not finite: an error where the page has tokens before the new ones, and
+    of no meaning where it has none.  The blocking form writes nothing; the other leaves that page and
+    head and does the rest."""
+    import torch
+    rng = np.random.default_rng(14)
+    heads, hd, page = 2, 32, 16
+    batch = Ragged(rng, [3, 20, 2, 70], [10, 36, 18, 75], page)
+    cache = _random_cache(qc, dev, rng, batch.pages, heads, page, hd)
+    k, v = (rng.standard_normal((batch.tokens, heads, hd)).astype(np.float32) for _ in range(2))
+    K, V = torch.from_numpy(k).to(dev), torch.from_numpy(v).to(dev)
+    b = batch.device(qc, dev)
+    touched = [(s, c) for s in range(4) for c in range((batch.kv[s] - batch.new[s]) // page, -(-batch.kv[s] // page))]
+    held = [(s, c) for s, c in touched if c * page < batch.kv[s] - batch.new[s]]   # tokens before the new ones
+    assert held == [(0, 0), (3, 0)]
+    for s, c in held:
+        keep = [t.clone() for t in cache.tensors]
+        cache.tensors[which][batch.table[s, c], 1] = value
+        host = _host(cache)
+        with pytest.raises(qc.QcError) as e:
+            qc.kv8_append(cache, b, K, V)
+        assert e.value.status == 3
+        _same_cache(cache, host)
+        st = torch.zeros(1, dtype=torch.int32, device=dev)
+        qc.kv8_append(cache, b, K, V, dev_status=st)
+        assert st.item() == 3
+        want = [h.copy() for h in host]
+        with np.errstate(invalid="ignore"):           # (that page and head, put back below)
+            _append_reference(want, batch, k, v)
+        pid = batch.table[s, c]
+        for w in (which - 2, which):
+            want[w][pid, 1] = host[w][pid, 1]
+        _same_cache(cache, want)
+        for t, o in zip(cache.tensors, keep):
+            t.copy_(o)
+    # pages that hold nothing yet, and pages of no sequence
+    unused = np.setdiff1d(np.arange(batch.pages), batch.table[batch.table >= 0])
+    for pid in [batch.table[at] for at in touched if at not in held] + list(unused):
+        cache.tensors[which][int(pid)] = value
+    host = _host(cache)
+    qc.kv8_append(cache, b, K, V)
+    _append_reference(host, batch, k, v)
+    _same_cache(cache, host)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("which", [2, 3], ids=["k", "v"])
+@pytest.mark.parametrize("new,kv,page,hd", [([1, 1, 1], [10, 33, 16], 16, 32), ([3, 150, 0], [40, 150, 9], 16, 64),
+                                            ([300, 7], [310, 500], 256, 128)])
+def test_gather_errors_of_scales(qc, dev, dtype, which, new, kv, page, hd):
+    """A page and head whose scale is not finite is left out (zeros in new tensors) and told
+    of, the rest is read; the blocking form writes nothing.  Pages that the call does not read may hold anything."""
+    import torch
+    dt = getattr(torch, dtype)
+    rng = np.random.default_rng(15)
+    heads = 2
+    batch = Ragged(rng, new, kv, page, 2)
+    cache = _random_cache(qc, dev, rng, batch.pages, heads, page, hd)
+    b = batch.device(qc, dev)
+    read = np.concatenate([batch.places(s, kv[s] - new[s], kv[s])[0] for s in range(len(kv))])
+    cache.tensors[which][torch.from_numpy(np.setdiff1d(np.arange(batch.pages), read)).to(dev)] = float("nan")
+    full = qc.kv8_gather(cache, b, dtype=dt)
+    for value in (float("nan"), float("inf")):
+        pid = int(read[-1])
+        keep = cache.tensors[which].clone()
+        cache.tensors[which][pid, 1] = value
+        out = [torch.full((batch.tokens, heads, hd), 7.0, dtype=dt, device=dev) for _ in range(2)]
+        with pytest.raises(qc.QcError) as e:
+            qc.kv8_gather(cache, b, k=out[0], v=out[1])
+        assert e.value.status == 3 and all(bool((o == 7).all()) for o in out)
+        for given, rest in ((out, 7.0), (None, 0.0)):
+            st = torch.zeros(1, dtype=torch.int32, device=dev)
+            if given is None:
+                got = qc.kv8_gather(cache, b, dtype=dt, dev_status=st)
+            else:
+                got = qc.kv8_gather(cache, b, k=out[0], v=out[1], dev_status=st)
+            assert st.item() == 3
+            for i in range(2):
+                want = full[i].clone()
+                want[len(read):] = rest
+                if i == which - 2:
+                    want[torch.from_numpy(np.flatnonzero(read == pid)).to(dev), 1] = rest
+                assert torch.equal(got[i], want)
+        cache.tensors[which].copy_(keep)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("new,spare", [([3, 0, 20, 1, 70], 5), ([1] * 90 + [200], 130), ([64], 64), ([1], 0)])
 def test_gather_into_new_tensors(qc, dev, dtype, new, spare):
