@@ -371,12 +371,12 @@ int qc_hip_rope_table(float* cosine, float* sine, long long first_position, long
  * f32), c and s from row positions[token] of the tables [max_position][rotary_dim / 2].
  * Element (t, h, d) of x is x[t * x_token_stride + h * x_head_stride + d], of y
  * likewise, so Q and K heads that lie side by side in one projection's rows are one
- * call.  y may be x (same strides): the elements past rotary_dim are then not
+ * call; a token's heads lie before the next token's, or (head-major) a head's tokens before the next head's.  y may be x (same strides): the elements past rotary_dim are then not
  * touched, else they are copied.  Other overlaps of x and y are not allowed.  A token
  * at position -1 is padding and left as it was; a position below -1 or from
  * max_position on is an error and its token left as it was.  Status: 1 for sizes
  * that are not positive, rotary_dim odd or above head_dim, strides shorter than what
- * they step over (a stride of one element's count 1 is not read), 2 for an unknown
+ * they step over in both orders (a stride of one element's count 1 is not read), 2 for an unknown
  * type, 3 for NULL pointers or a bad layout. */
 int qc_hip_rope(const void* x, void* y, int type, long long tokens, long long heads,
                 long long head_dim, long long rotary_dim, long long x_token_stride,

@@ -845,13 +845,14 @@ int qc_hip_rope(const void* x, void* y, int type, long long tokens, long long he
     return QC_INVALID_SHAPE;
   if (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > head_dim) return QC_INVALID_SHAPE;
   if (max_position <= 0 || max_position > INT_MAX) return QC_INVALID_SHAPE;
-  // heads do not overlap within a token, nor tokens each other
+  // no element is two tokens' or heads': a token's heads lie before the next token, or a head's
+  // tokens before the next head
   const long long strides[2][2] = {{x_token_stride, x_head_stride}, {y_token_stride, y_head_stride}};
   for (const auto& st : strides) {
-    const long long token = st[0], head = heads > 1 ? st[1] : head_dim;
+    const long long token = tokens > 1 ? st[0] : LLONG_MAX / 8, head = heads > 1 ? st[1] : head_dim;
     if (head < head_dim || head > LLONG_MAX / heads / 8) return QC_INVALID_SHAPE;
-    if (tokens > 1 && token < (heads - 1) * head + head_dim) return QC_INVALID_SHAPE;
-    if (tokens > 1 && token > LLONG_MAX / tokens / 8) return QC_INVALID_SHAPE;
+    if (token < head_dim || token > LLONG_MAX / tokens / 8) return QC_INVALID_SHAPE;
+    if (token < (heads - 1) * head + head_dim && head < (tokens - 1) * token + head_dim) return QC_INVALID_SHAPE;
   }
   if (!known_storage(type)) return QC_UNSUPPORTED_FORMAT;
   if (layout != QC_ROPE_HALF && layout != QC_ROPE_INTERLEAVED) return QC_INVALID_ARGUMENT;

@@ -440,7 +440,7 @@ def rope_table(positions, rotary_dim, base=10000.0, scaling="none", factor=1.0,
 
 
 def rope(x, cosine, sine, positions, interleaved=False, out=None, dev_status=None):
-    """x [tokens][heads][head_dim] (any token and head strides) with the first 2 *
+    """x [tokens][heads][head_dim] (token-major, head-major or strided) with the first 2 *
     cosine.shape[1] elements of every head rotated; out may be x.  Tokens at position -1 are
     left as they were (zeros in a new tensor)."""
     st = _storage(x)

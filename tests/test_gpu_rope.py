@@ -116,6 +116,34 @@ def test_strided_rows_of_a_projection(qc, dev):
             assert torch.equal(rows[:, (hq + hk) * hd:], before[:, (hq + hk) * hd:])
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("tokens,heads,hd,rd,interleaved,gap", [
+    (1, 5, 64, 64, False, 0), (9, 1, 64, 32, True, 0), (7, 6, 64, 64, False, 0), (33, 4, 128, 64, True, 1),
+    (300, 40, 128, 128, False, 0), (5, 3, 48, 24, False, 3)])
+def test_head_major_rows(qc, dev, dtype, tokens, heads, hd, rd, interleaved, gap):
+    """A view [tokens][heads] of tensors that lie [heads][tokens] (rows `gap` tokens longer than
+    what is rotated): out of place, into and from token-major rows, and in place."""
+    import torch
+    dt = getattr(torch, dtype)
+    g = torch.Generator(device=dev).manual_seed(hd)
+    held = torch.randn(heads, tokens + gap, hd, generator=g, device=dev).to(dt)
+    x = held[:, :tokens].transpose(0, 1)
+    pos = torch.arange(tokens, dtype=torch.int32, device=dev) * 3 % 128
+    c, s = qc.rope_table(128, rd)
+    flat = x.clone(memory_format=torch.contiguous_format)
+    want = qc.rope(flat, c, s, pos, interleaved=interleaved)
+    assert torch.equal(qc.rope(x, c, s, pos, interleaved=interleaved), want)
+    other = torch.full_like(held, 7.0)
+    out = other[:, :tokens].transpose(0, 1)
+    for source in (x, flat):
+        out.fill_(3.0)
+        qc.rope(source, c, s, pos, interleaved=interleaved, out=out)
+        assert torch.equal(out, want) and bool((other[:, tokens:] == 7).all())
+    before = held.clone()
+    qc.rope(x, c, s, pos, interleaved=interleaved, out=x)
+    assert torch.equal(x, want) and torch.equal(held[:, tokens:], before[:, tokens:])
+
+
 def test_padding_and_bad_positions(qc, dev):
     import torch
     x = torch.randn(6, 2, 32, device=dev)

@@ -57,6 +57,15 @@ def test_rope_refusals(q):
         assert rope(**bad) == 3, bad
 
 
+def test_rope_strides_that_overlap(q):
+    """Tokens and heads in neither order apart: refused, for x and for y; the pointers are not read."""
+    call = q.lib.qc_hip_rope
+    for tokens, heads, token, head in ((4, 2, 64, 192), (4, 2, 127, 255), (2, 3, 128, 100), (3, 3, 64, 64),
+                                       (4, 2, 63, 1024), (4, 2, 1 << 62, 64), (4, 2, 64, 1 << 62), (4, 2, 64, -256)):
+        for x, y in (((token, head), (1024, 64)), ((1024, 64), (token, head))):
+            assert call(P, P, 0, tokens, heads, 64, 64, *x, *y, P, P, P, 16, 0, P, None) == 1, (tokens, heads, token, head)
+
+
 def _cache(q, **kw):
     f = dict(k_codes=P, v_codes=P, k_scales=P, v_scales=P, pages=8, kv_heads=2, page_tokens=16,
              head_dim=64)
