@@ -1172,8 +1172,9 @@ hipError_t run_join(const Kv8Args& a, const AttnArgs& p, long long blocks, hipSt
   const int per = one ? std::min<long long>(p.per, static_cast<long long>(a.max_new) * p.group) : p.per;
   const long long items = blocks * per;
   if (items > INT_MAX - 256) return hipErrorInvalidValue;
+  const int rows = p.splits <= kFewSplits ? 256 >> shift : 1;   // of a workgroup
+  if (!kv8_grid_fits((items + rows - 1) / rows, 256)) return hipErrorInvalidValue;
   if (p.splits <= kFewSplits) {
-    const int rows = 256 >> shift;
     attention_join_few<TYPE><<<static_cast<unsigned>((items + rows - 1) / rows), 256, 0, s>>>(a, p, per, shift);
     return hipGetLastError();
   }
@@ -1206,7 +1207,7 @@ hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((span + chunk - 1) / chunk);
   const long long grid = units * p.splits;
-  if (grid > INT_MAX) return hipErrorInvalidValue;
+  if (!kv8_grid_fits(grid, 64 * kWaves)) return hipErrorInvalidValue;
   std::unique_lock<std::mutex> hold;
   if (p.splits > 1) {
     StreamWorkspace* ws = nullptr;
@@ -1256,7 +1257,9 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   f.cap = (a.max_kv + 63) / 64 * 64;
   const long long unit_bytes = static_cast<long long>(f.cap) * DP * 4 + f.cap / 2;   // two of f16, scales
   const long long pass = std::min(units, std::max<long long>(1, kFragPass / unit_bytes));
-  if (blocks * a.kv_heads * p.splits > INT_MAX || pass * (f.cap / 32) > INT_MAX) return hipErrorInvalidValue;
+  if (!kv8_grid_fits((p.listed == kPadded ? pass * p.row_blocks : blocks * a.kv_heads) * p.splits, 64 * NW) ||
+      !kv8_grid_fits(pass * (f.cap / 32), 256))
+    return hipErrorInvalidValue;
   StreamWorkspace* ws = nullptr;
   hipError_t e = stream_workspace(s, &ws);
   if (e != hipSuccess) return e;

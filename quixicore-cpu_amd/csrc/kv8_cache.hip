@@ -357,6 +357,7 @@ Kv8Args kv8_args(const qc_kv8_cache& c, const qc_kv8_batch& b, int* status) {
 hipError_t launch_kv8_check(const qc_kv8_cache& c, const qc_kv8_batch& b, Kv8Call call, int window,
                             int* flag, hipStream_t s) {
   const Kv8Args a = kv8_args(c, b, flag);
+  if (!kv8_grid_fits(a.seqs, kThreads)) return hipErrorInvalidValue;
   kv8_check<<<a.seqs, kThreads, 0, s>>>(a, call, window);
   return hipGetLastError();
 }
@@ -366,7 +367,9 @@ hipError_t launch_kv8_nonfinite(const qc_kv8_cache& c, const qc_kv8_batch& b, co
                                 int* flag, hipStream_t s) {
   const Kv8Args a = kv8_args(c, b, flag);
   const Rows kr = {k, k_stride}, vr = {v, v_stride};
-  const int parts = touched_slots(a);
+  // (of many sequences under a loose bound each takes its rows in more turns)
+  const int parts = std::min(touched_slots(a), std::max(1, (1 << 18) / a.seqs));
+  if (!kv8_grid_fits(2LL * parts * a.seqs, kThreads)) return hipErrorInvalidValue;
   const unsigned grid = static_cast<unsigned>(2LL * parts * a.seqs);
   switch (type) {
     case QC_STORAGE_F32: kv8_nonfinite<QC_STORAGE_F32><<<grid, kThreads, 0, s>>>(a, kr, vr, parts); break;
@@ -384,20 +387,22 @@ bool wide_rows(const void* p, long long stride, int size) {
 }
 
 template <int TYPE>
-void run_append(const Kv8Args& a, const Rows& k, const Rows& v, hipStream_t s) {
+hipError_t run_append(const Kv8Args& a, const Rows& k, const Rows& v, hipStream_t s) {
   constexpr int size = TYPE == QC_STORAGE_F32 ? 4 : 2;
   int slots;
   const unsigned grid = touched_grid(a, slots);
   const bool vec = wide_rows(k.p, k.stride, size) && wide_rows(v.p, v.stride, size);
   const bool small = std::min(a.max_new, a.page_tokens) * a.head_dim <= 4096;
+  if (!kv8_grid_fits(grid, vec && small ? 64 : 256)) return hipErrorInvalidValue;
   if (vec && small) append_kernel<TYPE, 64, true><<<grid, 64, 0, s>>>(a, k, v, slots);
   else if (vec) append_kernel<TYPE, 256, true><<<grid, 256, 0, s>>>(a, k, v, slots);
   else append_kernel<TYPE, 256, false><<<grid, 256, 0, s>>>(a, k, v, slots);
+  return hipGetLastError();
 }
 
 template <int TYPE>
-void run_gather(const Kv8Args& a, void* k, void* v, long long k_stride, long long v_stride, bool zero_rest,
-                hipStream_t s) {
+hipError_t run_gather(const Kv8Args& a, void* k, void* v, long long k_stride, long long v_stride, bool zero_rest,
+                      hipStream_t s) {
   constexpr int size = TYPE == QC_STORAGE_F32 ? 4 : 2;
   int slots;
   unsigned grid = touched_grid(a, slots);
@@ -405,9 +410,11 @@ void run_gather(const Kv8Args& a, void* k, void* v, long long k_stride, long lon
   if (zero_rest) grid += 2u * static_cast<unsigned>((a.tokens + 63LL) / 64);
   const bool vec = wide_rows(k, k_stride, size) && wide_rows(v, v_stride, size);
   const bool small = std::min(a.max_new, a.page_tokens) * a.head_dim <= 4096;
+  if (!kv8_grid_fits(grid, vec && small ? 64 : 256)) return hipErrorInvalidValue;
   if (vec && small) gather_kernel<TYPE, 64, true><<<grid, 64, 0, s>>>(a, k, v, k_stride, v_stride, slots, rest);
   else if (vec) gather_kernel<TYPE, 256, true><<<grid, 256, 0, s>>>(a, k, v, k_stride, v_stride, slots, rest);
   else gather_kernel<TYPE, 256, false><<<grid, 256, 0, s>>>(a, k, v, k_stride, v_stride, slots, rest);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -418,11 +425,10 @@ hipError_t launch_kv8_append(const qc_kv8_cache& c, const qc_kv8_batch& b, const
   const Kv8Args a = kv8_args(c, b, status);
   const Rows kr = {k, k_stride}, vr = {v, v_stride};
   switch (type) {
-    case QC_STORAGE_F32: run_append<QC_STORAGE_F32>(a, kr, vr, s); break;
-    case QC_STORAGE_F16: run_append<QC_STORAGE_F16>(a, kr, vr, s); break;
-    default: run_append<QC_STORAGE_BF16>(a, kr, vr, s);
+    case QC_STORAGE_F32: return run_append<QC_STORAGE_F32>(a, kr, vr, s);
+    case QC_STORAGE_F16: return run_append<QC_STORAGE_F16>(a, kr, vr, s);
+    default: return run_append<QC_STORAGE_BF16>(a, kr, vr, s);
   }
-  return hipGetLastError();
 }
 
 hipError_t launch_kv8_gather(const qc_kv8_cache& c, const qc_kv8_batch& b, void* k,
@@ -430,11 +436,10 @@ hipError_t launch_kv8_gather(const qc_kv8_cache& c, const qc_kv8_batch& b, void*
                              int* status, hipStream_t s) {
   const Kv8Args a = kv8_args(c, b, status);
   switch (type) {
-    case QC_STORAGE_F32: run_gather<QC_STORAGE_F32>(a, k, v, k_stride, v_stride, zero_rest, s); break;
-    case QC_STORAGE_F16: run_gather<QC_STORAGE_F16>(a, k, v, k_stride, v_stride, zero_rest, s); break;
-    default: run_gather<QC_STORAGE_BF16>(a, k, v, k_stride, v_stride, zero_rest, s);
+    case QC_STORAGE_F32: return run_gather<QC_STORAGE_F32>(a, k, v, k_stride, v_stride, zero_rest, s);
+    case QC_STORAGE_F16: return run_gather<QC_STORAGE_F16>(a, k, v, k_stride, v_stride, zero_rest, s);
+    default: return run_gather<QC_STORAGE_BF16>(a, k, v, k_stride, v_stride, zero_rest, s);
   }
-  return hipGetLastError();
 }
 
 }  // namespace qc

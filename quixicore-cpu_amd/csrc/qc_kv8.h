@@ -25,6 +25,11 @@ struct Kv8Args {
   int* status;
 };
 
+// A launch's work-items are counted in 32 bits.
+inline bool kv8_grid_fits(long long groups, int threads) {
+  return groups >= 0 && groups <= static_cast<long long>(UINT32_MAX) / threads;
+}
+
 Kv8Args kv8_args(const qc_kv8_cache& c, const qc_kv8_batch& b, int* status);
 
 #ifdef __HIPCC__

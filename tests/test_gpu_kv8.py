@@ -232,6 +232,31 @@ def test_append_errors(qc, dev):
         assert st.item() == 3
 
 
+def test_append_of_many_sequences_and_a_long_one(qc, dev):
+    """A padded grid of this batch (1024 sequences, 8193 pages each at most) would have more work-items than
+    a launch may: the blocking form looks at all rows all the same, the last ones of the long sequence too."""
+    import torch
+    rng = np.random.default_rng(11)
+    page, hd = 16, 16
+    new = [1] * 500 + [131072 - 1023] + [1] * 523
+    batch = Ragged(rng, new, new, page)
+    cache = _random_cache(qc, dev, rng, batch.pages, 1, page, hd)
+    host = _host(cache)
+    k, v = (rng.standard_normal((batch.tokens, 1, hd)).astype(np.float32) for _ in range(2))
+    K, V = torch.from_numpy(k).to(dev), torch.from_numpy(v).to(dev)
+    b = qc.Kv8Batch(*batch.device(qc, dev).tensors, batch.tokens, batch.tokens, batch.max_kv)
+    for at in (int(batch.start[500]), int(batch.start[501]) - 1, batch.tokens - 1):
+        V[at, 0, 3] = float("nan")
+        with pytest.raises(qc.QcError) as e:
+            qc.kv8_append(cache, b, K, V)
+        assert e.value.status == 3
+        _same_cache(cache, host)
+        V[at, 0, 3] = float(v[at, 0, 3])
+    qc.kv8_append(cache, b, K, V)
+    _append_reference(host, batch, k, v)
+    _same_cache(cache, host)
+
+
 @pytest.mark.parametrize("which", [2, 3], ids=["k", "v"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
 def test_append_errors_of_held_scales(qc, dev, which, value):
