@@ -47,7 +47,8 @@ struct AttnArgs {
   int vec;              // q and out rows allow 16-byte accesses
   float* part;          // [split][tokens * heads][head_dim], then statistics
   float* stats;         // [split][tokens * heads][2]: maximum (log2 units), sum
-  int splits, chunk;    // key ranges of `chunk` tokens
+  int splits, chunk;    // key ranges, and tokens of one, at most
+  int want, span;       // ranges to cut the keys into, at most; keys that a row block sees at most
   int per, row_blocks;  // rows of a row block, row blocks of a sequence's key head at most
   int rows_from, rows_to;   // sequences of [rows_from, rows_to) rows a key head are worked on
   int listed;           // what blocks are counted by: kPadded, kBlocks, kSequences
@@ -91,6 +92,39 @@ __device__ __forceinline__ void seen_range(const AttnArgs& p, const Unit& u, int
                                            int& hi) {
   hi = p.causal ? min(u.kv, u.position(t1) + 1) : u.kv;
   lo = p.window > 0 ? max(0, u.position(t0) + 1 - p.window) : 0;
+}
+
+// The most keys of a sequence with rows; for all lanes.
+__device__ __forceinline__ int longest(const Kv8Args& a) {
+  int n = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x & 63; i < a.seqs; i += 64) {
+    const int kv = a.kv_len[i];
+    if (a.seq_start[i + 1] > a.seq_start[i] && kv <= a.max_kv) n = max(n, kv);
+  }
+  // lanes 1, 2, then 4 and 8 (mirrors) away, then the rows of 16
+  n = max(n, __builtin_amdgcn_update_dpp(0, n, 0xB1, 0xF, 0xF, true));
+  n = max(n, __builtin_amdgcn_update_dpp(0, n, 0x4E, 0xF, 0xF, true));
+  n = max(n, __builtin_amdgcn_update_dpp(0, n, 0x141, 0xF, 0xF, true));
+  n = max(n, __builtin_amdgcn_update_dpp(0, n, 0x140, 0xF, 0xF, true));
+  const auto r = __builtin_amdgcn_permlane16_swap(n, n, false, false);
+  n = max(static_cast<int>(r[0]), static_cast<int>(r[1]));
+  const auto h = __builtin_amdgcn_permlane32_swap(n, n, false, false);
+  return __builtin_amdgcn_readfirstlane(max(static_cast<int>(h[0]), static_cast<int>(h[1])));
+}
+
+// Keys of a range, from the batch's longest sequence and not from the host's bound, which a captured step
+// has far above its lengths (8 sequences of 16384 keys, 32 / 8 heads of 128, bound 131072: 192 us with
+// ranges cut from the bound, 51 so, 49 with the bound at the length).  used: ranges that hold keys.  All
+// keys are covered: n <= splits * chunk, want <= splits; `least` and chunk are multiples of `step`.
+__device__ __forceinline__ int range_keys(const Kv8Args& a, const AttnArgs& p, int least, int step, int& used) {
+  used = p.splits;
+  if (p.chunk <= least || p.splits == 1) return p.chunk;
+  const int n = min(longest(a), p.span);
+  if (n == p.span) return p.chunk;
+  const int keys = min(max(least, ((n + p.want - 1) / p.want + step - 1) / step * step), p.chunk);
+  used = max(1, (n + keys - 1) / keys);
+  return keys;
 }
 
 // Four signed bytes as f16: 0x6400 | u is 1024 + u for a byte u, and u = code + 128.
@@ -235,10 +269,20 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
 
   const int lane = threadIdx.x & 63, row16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // split fastest, then row block, key head, sequence
-  const int split = blockIdx.x % p.splits;
+  // split fastest, then row block, key head, sequence; the ranges past every length after all of these
+  int used;
+  const int chunk = range_keys(a, p, 32 * kWaves, 32, used);
+  int id = blockIdx.x / used, split = blockIdx.x - id * used;
+  if (used < p.splits) {
+    const int blocks = gridDim.x / p.splits;
+    if (id >= blocks) {
+      const int past = blockIdx.x - blocks * used;
+      split = used + past / blocks;
+      id = past % blocks;
+    }
+  }
   int seq, kvh, rb;
-  if (!block_of(a, p, blockIdx.x / p.splits, seq, kvh, rb)) return;
+  if (!block_of(a, p, id, seq, kvh, rb)) return;
   Unit u;
   if (!kv8_sequence(a, seq, u.first, u.rows, u.kv) || u.rows * p.group >= p.rows_to) return;
   const int r0 = rb * RT * 16, r1 = min(r0 + RT * 16, u.rows * p.group);
@@ -246,8 +290,17 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
   int lo, hi;
   seen_range(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
   const int base = lo & ~31;
-  const int from = __builtin_amdgcn_readfirstlane(base + split * p.chunk);   // a multiple of 32
-  const int to = __builtin_amdgcn_readfirstlane(min(hi, from + p.chunk));
+  const int from = __builtin_amdgcn_readfirstlane(base + split * chunk);   // a multiple of 32
+  const int to = __builtin_amdgcn_readfirstlane(min(hi, from + chunk));
+  if (from >= to && p.splits > 1) {               // a range without keys
+    for (int r = r0 + threadIdx.x; r < r1; r += 64 * kWaves) {
+      const int token = r / p.group, head = kvh * p.group + r - token * p.group;
+      float* st = p.stats + 2 * ((static_cast<long long>(split) * a.tokens + u.first + token) * p.heads + head);
+      st[0] = -INFINITY;
+      st[1] = 0.f;
+    }
+    return;
+  }
   const int groups = max(0, (to - from + 15) >> 4);
   const int* table = a.table + static_cast<long long>(seq) * a.columns;
   // the page of 16 keys, -1 where no row sees one of them; ids out of range are told apart below
@@ -706,6 +759,7 @@ __global__ __launch_bounds__(256) void attention_layout(Kv8Args a, AttnArgs p, F
 // takes its rows' sums in memory: 17 GB for 131072 tokens of 32 heads in ranges of 16384.)
 template <int DP>
 constexpr int kTiledGroups = DP == 256 ? 1024 : 4096;
+constexpr int kTiledLeast = 1024;   // keys of a range, where there are as many
 
 template <int DP, int NW, int TYPE>
 __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, AttnArgs p, Frags f) {
@@ -751,8 +805,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   if (r0 >= r1) return;
   int lo, hi;
   seen_range(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
-  const int from = __builtin_amdgcn_readfirstlane((lo & ~63) + split * p.chunk);
-  const int to = __builtin_amdgcn_readfirstlane(min(hi, from + p.chunk));
+  int used;
+  const int chunk = range_keys(a, p, kTiledLeast, 64, used);
+  const int from = __builtin_amdgcn_readfirstlane((lo & ~63) + split * chunk);
+  const int to = __builtin_amdgcn_readfirstlane(min(hi, from + chunk));
   const int steps = to > from ? (to - from + 63) >> 6 : 0;
 
   const long long tile0 = static_cast<long long>(local) * (f.cap / 32) + from / 32;
@@ -1206,6 +1262,8 @@ hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   chunk = std::min<long long>(chunk, (span + 4095) / 4096 * range_bytes > (1LL << 30) ? 16 * kMaxGroups : 4096);
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((span + chunk - 1) / chunk);
+  p.want = static_cast<int>(std::min<long long>(want, p.splits));
+  p.span = static_cast<int>(span);
   const long long grid = units * p.splits;
   if (!kv8_grid_fits(grid, 64 * kWaves)) return hipErrorInvalidValue;
   std::unique_lock<std::mutex> hold;
@@ -1242,10 +1300,12 @@ TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per, int max_groups) {
   const long long blocks = std::min(padded, p.listed == kBlocks ? there : padded);
   const long long want = std::max<long long>(1, device_cu_count() / (blocks * a.kv_heads));
   long long chunk = ((span + want - 1) / want + 63) / 64 * 64;
-  chunk = std::max<long long>(chunk, 1024);
+  chunk = std::max<long long>(chunk, kTiledLeast);
   chunk = std::min<long long>(chunk, 16 * max_groups);
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((span + chunk - 1) / chunk);
+  p.want = static_cast<int>(std::min<long long>(want, p.splits));
+  p.span = static_cast<int>(span);
   return {seqs * a.kv_heads, blocks};
 }
 

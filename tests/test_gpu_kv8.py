@@ -848,6 +848,90 @@ def test_attention_repeats_and_graph(qc, dev, route, new, kv, heads, kvh):
     del graph
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("new,kv,heads,kvh,window", [
+    ([1], [4000], 8, 2, 0), ([1, 0, 1], [2500, 9000, 3000], 8, 2, 0), ([12, 3], [1500, 4000], 4, 2, 0),
+    ([1], [9000], 4, 1, 2000), ([1] * 8, [3000 + 500 * i for i in range(8)], 8, 2, 0)])
+def test_attention_under_a_loose_bound(qc, dev, dtype, new, kv, heads, kvh, window):
+    """Key ranges are cut from the lengths, not from max_kv: a bound far above them gives the bits of the
+    tight one where both join more than 8 ranges, as here (256 CUs).  Sequences without new tokens, and
+    those of bad figures, do not count."""
+    import torch
+    print(f"kv8 attention loose bound {dtype} new {new} kv {kv} {window}", flush=True)
+    rng = np.random.default_rng(len(new))
+    columns = 131072 // 16
+    batch = Ragged(rng, new, kv, 16, columns=columns)
+    cache = _random_cache(qc, dev, rng, batch.pages, kvh, 16, 64)
+    q = torch.from_numpy(rng.standard_normal((batch.tokens, heads, 64))).to(getattr(torch, dtype)).to(dev)
+    most = max(k for n, k in zip(new, kv) if n)
+    bounds = [131072] if window else [16384, 65536, 131072]
+    try:
+        for r in (0, 1, 2):
+            qc.set_kv8_attention_route(r)
+            st = torch.zeros(1, dtype=torch.int32, device=dev)
+            tight = None
+            if 0 not in new:
+                tight = qc.kv8_attention(cache, batch.device(qc, dev, max_kv=most), q, window=window, dev_status=st)
+            for bound in bounds:
+                got = qc.kv8_attention(cache, batch.device(qc, dev, max_kv=bound), q, window=window, dev_status=st)
+                if tight is None:                    # (the sequence without new tokens breaks the tight bound)
+                    tight = got
+                assert torch.equal(got, tight), (r, bound)
+            assert st.item() == 0
+            if 0 in new:
+                b = batch.device(qc, dev, max_kv=131072)
+                b.tensors[2][new.index(0)] = 1
+                assert torch.equal(qc.kv8_attention(cache, b, q, window=window, dev_status=st), tight)
+            if len(new) == 8:                        # the longest goes bad: the others' ranges are their own longest's
+                b = batch.device(qc, dev, max_kv=131072)
+                b.tensors[2][7] = 131073
+                c = Ragged(rng, new[:7], kv[:7], 16, columns=columns)
+                c.table = batch.table[:7]
+                got = qc.kv8_attention(cache, b, q, window=window, dev_status=st)
+                alone = qc.kv8_attention(cache, c.device(qc, dev, max_kv=131072), q[:7], window=window)
+                assert st.item() == 3 and torch.equal(got[:7], alone)
+    finally:
+        qc.set_kv8_attention_route(0)
+
+
+@pytest.mark.parametrize("new,heads,kvh", [(1, 8, 2), (5, 8, 1), (90, 4, 2)])
+def test_attention_replayed_as_lengths_grow(qc, dev, route, new, heads, kvh):
+    """Captured once under a bound of 65536 keys, replayed at lengths from one to 20000: each time the
+    eager call's bits, and right against 64 bits."""
+    import torch
+    rng = np.random.default_rng(new)
+    full = Ragged(rng, [new, new], [20000, 9000], 16, columns=65536 // 16)
+    cache = _random_cache(qc, dev, rng, full.pages, kvh, 16, 64)
+    q = torch.from_numpy(rng.standard_normal((full.tokens, heads, 64))).to(torch.bfloat16)
+    Q, st = q.to(dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    b = full.device(qc, dev, max_kv=65536)
+    out = torch.zeros_like(Q)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        qc.kv8_attention(cache, b, Q, out=out, dev_status=st)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        qc.kv8_attention(cache, b, Q, out=out, dev_status=st)
+    host = _host(cache)
+    for kv in ([new, 0], [new + 30, new], [600, 90], [5000, 300], [20000, 9000]):
+        b.tensors[2].copy_(torch.tensor(kv, dtype=torch.int32))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            out.fill_(float("nan"))
+            graph.replay()
+            eager = qc.kv8_attention(cache, b, Q, dev_status=st)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        at = Ragged(rng, [new, new], kv, 16, columns=full.columns)
+        at.table = full.table
+        want, tol = _attention_reference(host, at, q.float().numpy(), heads, 0.125, True, 0, HALF["bfloat16"])
+        assert np.all(np.abs(out.double().cpu().numpy() - want) <= tol), kv
+    assert st.item() == 0
+    del graph
+
+
 def test_attention_shared_pages(qc, dev, route):
     """Sequences that share their first pages, and a page that one sequence holds twice."""
     import torch
