@@ -1233,3 +1233,76 @@ def test_attention_long_prompts(qc, dev, dtype, new, kv, heads, kvh, hd, window)
     finally:
         qc.set_kv8_attention_route(0)
     assert any(torch.equal(outs[0], o) for o in outs[1:])     # the sizes choose one of them
+
+
+@pytest.mark.parametrize("dtype,long,short,kv_long,kv_short,heads,kvh,hd,window", [
+    # 512 rows a key head and more are laid out, the others read directly
+    ("bfloat16", [900, 128, 900], [127] + [1] * 27 + [0, 9], [1500, 2000, 900], 3000, 32, 8, 128, 0),
+    ("float16", [600, 512, 700], [511] + [1] * 16 + [100, 0, 2], [2500, 512, 1800], 2400, 16, 16, 80, 700),
+    ("float32", [1500, 256], [255] + [1] * 9 + [7], [3000, 1100], 2900, 6, 3, 256, 0),
+    # up to 1024 keys: 256 rows and more
+    ("bfloat16", [300, 64, 250], [63] + [1] * 36 + [20, 0], [300, 1000, 700], 1024, 32, 8, 64, 0),
+    ("float32", [300, 260], [40] + [3] * 30, [900, 260], 1000, 32, 8, 32, 100)])
+def test_attention_mixed_batches(qc, dev, dtype, long, short, kv_long, kv_short, heads, kvh, hd, window):
+    """Batches of a few long prompts and many short ones at which each kind goes to a kernel of its own (checked
+    against the other kernels' bits); sequences at the border, without rows and without keys; against 64 bits."""
+    import torch
+    print(f"kv8 attention mixed {dtype} {len(long)}+{len(short)} heads {heads}/{kvh} hd {hd} {window}", flush=True)
+    rng = np.random.default_rng(len(short) + hd)
+    kv_few = [max(n, kv_short - 61 * i) for i, n in enumerate(short)]
+    kv_few[3] = 0                                     # one row that sees nothing
+    order = rng.permutation(len(long) + len(short))
+    new, kv = [(long + short)[i] for i in order], [(kv_long + kv_few)[i] for i in order]
+    is_long = [bool(i < len(long)) for i in order]
+    batch = Ragged(rng, new, kv, 32, 3)
+    cache = _random_cache(qc, dev, rng, batch.pages, kvh, 32, hd, 0.3)
+    q = torch.from_numpy(rng.standard_normal((batch.tokens, heads, hd))).to(getattr(torch, dtype)).to(dev)
+    q[-3:] = float("nan")
+    b = batch.device(qc, dev)
+    group = heads // kvh
+    want = torch.zeros(q.shape, dtype=torch.float64, device=dev)
+    size, score = torch.zeros_like(want), 0.0
+    rows_long = torch.zeros(batch.tokens, dtype=torch.bool, device=dev)
+    for s in range(len(kv)):
+        a, e = int(batch.start[s]), int(batch.start[s + 1])
+        rows_long[a:e] = is_long[s]
+        if e == a or kv[s] == 0:
+            continue
+        pid, slot = (torch.from_numpy(x).to(dev) for x in batch.places(s, 0, kv[s]))
+        K, V = (cache.tensors[i][pid.long(), :, slot].double() * cache.tensors[2 + i][pid.long()].double()[..., None]
+                for i in range(2))
+        at = torch.arange(kv[s] - new[s], kv[s], device=dev)[:, None]
+        j = torch.arange(kv[s], device=dev)[None]
+        hide = (j > at) | (j <= at - window) if window else j > at
+        for h in range(heads):
+            z = (q[a:e, h].double() @ K[:, h // group].T.contiguous()) * float(np.float32(hd ** -0.5))
+            score = max(score, z.abs().max().item())
+            p = torch.softmax(z.masked_fill(hide, -math.inf), -1)
+            want[a:e, h] = p @ V[:, h // group]
+            size[a:e, h] = p @ V[:, h // group].abs()
+    # as in test_attention_long_prompts: probabilities in 11 (22) bits; scores of f32 dots whose terms' magnitudes sum
+    # to a few times the largest score; sums over up to 3000 keys in steps of 16; the output's rounding
+    bits = 2.0 ** -11 if dtype != "float32" else 2.0 ** -21
+    tol = size * (bits + 2 * 4 * score * (hd + 8) * 2.0 ** -24 + 200 * 2.0 ** -23) + HALF[dtype] * (1 + 2.0 ** -10) * want.abs() + 2.0 ** -24
+    used = int(batch.start[-1])
+    outs = []
+    try:
+        for r in (0, 1, 2, 3):
+            qc.set_kv8_attention_route(r)
+            st = torch.zeros(1, dtype=torch.int32, device=dev)
+            out = torch.full_like(q, 7.0)
+            qc.kv8_attention(cache, b, q, window=window, out=out, dev_status=st)
+            assert st.item() == 0 and bool((out[used:] == 7).all())
+            assert bool(((out.double() - want).abs() <= tol)[:used].all()), r
+            if r == 0:
+                for _ in range(2):
+                    again = torch.full_like(q, 7.0)
+                    qc.kv8_attention(cache, b, q, window=window, out=again, dev_status=st)
+                    assert torch.equal(again, out)
+            outs.append(out)
+    finally:
+        qc.set_kv8_attention_route(0)
+    short_rows = ~rows_long
+    short_rows[used:] = False
+    assert not torch.equal(outs[0][rows_long], outs[1][rows_long]) and not torch.equal(outs[0][rows_long], outs[2][rows_long])
+    assert not torch.equal(outs[0][short_rows], outs[3][short_rows])
