@@ -116,10 +116,11 @@ __device__ __forceinline__ int longest(const Kv8Args& a) {
 // Keys of a range, from the batch's longest sequence and not from the host's bound, which a captured step
 // has far above its lengths (8 sequences of 16384 keys, 32 / 8 heads of 128, bound 131072: 192 us with
 // ranges cut from the bound, 51 so, 49 with the bound at the length).  used: ranges that hold keys.  All
-// keys are covered: n <= splits * chunk, want <= splits; `least` and chunk are multiples of `step`.
+// keys are covered: n <= splits * chunk, want <= splits; `least` and chunk are multiples of `step`.  (Where the
+// blocks alone fill the chip, want is 1 and ranges are cut for LDS only: nothing to look up.)
 __device__ __forceinline__ int range_keys(const Kv8Args& a, const AttnArgs& p, int least, int step, int& used) {
   used = p.splits;
-  if (p.chunk <= least || p.splits == 1) return p.chunk;
+  if (p.chunk <= least || p.splits == 1 || p.want == 1) return p.chunk;
   const int n = min(longest(a), p.span);
   if (n == p.span) return p.chunk;
   const int keys = min(max(least, ((n + p.want - 1) / p.want + step - 1) / step * step), p.chunk);
@@ -269,16 +270,20 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
 
   const int lane = threadIdx.x & 63, row16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // split fastest, then row block, key head, sequence; the ranges past every length after all of these
+  // Range fastest, then row block, key head, sequence; ranges past every length after all of these.
+  // With blocks enough to fill the chip the range is slowest: workgroups are dealt to the XCDs in turn, and short
+  // sequences' empty ranges would leave some idle (128 sequences of up to 6000 keys, heads of 64, 141 -> 110 us; with
+  // fewer blocks 32 x 16384 keys 154 -> 162, and row blocks that share keys on several XCDs).
   int used;
   const int chunk = range_keys(a, p, 32 * kWaves, 32, used);
+  const bool slowest = p.want == 1 && p.splits > 1;
   int id = blockIdx.x / used, split = blockIdx.x - id * used;
-  if (used < p.splits) {
-    const int blocks = gridDim.x / p.splits;
-    if (id >= blocks) {
-      const int past = blockIdx.x - blocks * used;
-      split = used + past / blocks;
-      id = past % blocks;
+  if (slowest || used < p.splits) {
+    const int blocks = gridDim.x / p.splits, first = slowest ? 0 : blocks * used;   // of the workgroups in that order
+    if (static_cast<int>(blockIdx.x) >= first) {
+      const int more = (blockIdx.x - first) / blocks;
+      split = (slowest ? 0 : used) + more;
+      id = blockIdx.x - first - more * blocks;
     }
   }
   int seq, kvh, rb;

@@ -894,6 +894,23 @@ def test_attention_under_a_loose_bound(qc, dev, dtype, new, kv, heads, kvh, wind
         qc.set_kv8_attention_route(0)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("new,kv,heads,kvh", [
+    ([1] * 70, [5000 - 70 * i for i in range(70)], 8, 8), ([1] * 40 + [30] + [2] * 29, [4200 - 59 * i for i in range(70)], 16, 8)])
+def test_attention_of_many_sequences_under_a_loose_bound(qc, dev, dtype, new, kv, heads, kvh):
+    """Blocks enough to fill the chip, and ranges besides: against 64 bits, and the tight bound's bits."""
+    import torch
+    rng = np.random.default_rng(heads)
+    batch = Ragged(rng, new, kv, 16, spare=1, columns=32768 // 16)
+    cache = _random_cache(qc, dev, rng, batch.pages, kvh, 16, 16)
+    _attend(qc, dev, rng, new, kv, heads, kvh, 16, 16, dtype, spare=1, cache=cache, batch=batch)
+    rng = np.random.default_rng(5)
+    q = torch.from_numpy(rng.standard_normal((batch.tokens, heads, 16))).to(getattr(torch, dtype)).to(dev)
+    tight = qc.kv8_attention(cache, batch.device(qc, dev), q)
+    for bound in (8192, 16384, 32768):
+        assert torch.equal(qc.kv8_attention(cache, batch.device(qc, dev, max_kv=bound), q), tight), bound
+
+
 @pytest.mark.parametrize("new,heads,kvh", [(1, 8, 2), (5, 8, 1), (90, 4, 2)])
 def test_attention_replayed_as_lengths_grow(qc, dev, route, new, heads, kvh):
     """Captured once under a bound of 65536 keys, replayed at lengths from one to 20000: each time the
