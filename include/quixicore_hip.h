@@ -455,9 +455,10 @@ int qc_hip_kv8_gather(const qc_kv8_cache* cache, const qc_kv8_batch* batch, void
  * (n > kv_len, or kv_len 0) is zeros.  q and out do not overlap.  Pages that no row sees are not looked at; one
  * that is seen and has a scale that is not finite is an error like a bad page id.
  * The probabilities enter the product with the values in 11 bits (bf16 q, and f16 q
- * of prompts of some hundred tokens) or 22; dots, sums and statistics are f32.  They are held
- * relative to their row's largest and their page's value scale to the largest of the keys
- * read together: a product of both below 2^-25 loses bits.  Status: 1 for sizes out of range, 2 for an
+ * of prompts of some hundred tokens, for which qc_hip_set_kv8_attention_route(2) keeps 22) or 22;
+ * dots, sums and statistics are f32.  Probabilities are held relative to their row's largest and
+ * their page's value scale to the largest of the keys read together (of a range of up to 65536, some of them not
+ * seen by the row): a product of both below 2^-25 loses bits, below about 2^-36 it counts as 0.  Status: 1 for sizes out of range, 2 for an
  * unknown type, 3 for NULL or misaligned pointers, a scale that is not finite, or a
  * window without causal. */
 int qc_hip_kv8_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* q,
@@ -485,7 +486,8 @@ int qc_hip_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, void* o
                             long long rows, long long dim, void* stream);
 
 /* y[m][n] = x . w^T of two MXFP4 matrices, w [n][k] and x [m][k]: products exact,
- * sums f32, y of y_type.  A scale byte of 255 makes the outputs of its row NaN.
+ * sums f32, y of y_type.  A scale byte of 255 makes the outputs of its row NaN.  Scales are
+ * read by aligned 4 bytes, those that hold an array's last one whole: up to 3 bytes past it are read, and not used.
  * Status: 1 for sizes that are not positive, k above 2^27 or not a multiple of 32, 2 for an
  * unknown type, 3 for NULL pointers or codes that are not 16-byte aligned. */
 int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* x_codes,

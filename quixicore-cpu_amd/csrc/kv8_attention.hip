@@ -245,8 +245,8 @@ __device__ __forceinline__ void store_n(void* out, long long at, bool vec, const
 // lane & 15 at dimension 64 c + 16 g.  V: lane loads DP / 16 bytes of its eight
 // keys at dimension (DP / 16) (lane & 15), transposed in registers.
 //
-// Bound by memory where the cache is long: 32 sequences of 16384 keys, 32 / 8 heads of 128,
-// bf16 (711 MB), 143 us, 4.9 TB/s, and 3 to 5 for the join; one of 600 keys, f32, 7.9 and
+// Bound by memory where the cache is long: 32 sequences of 4096 to 16384 keys, 32 / 8 heads of 128,
+// bf16 (711 MB), 143 to 151 us by session, 4.7 to 5.0 TB/s, and 3 to 5 for the join; one of 600 keys, f32, 7.9 and
 // 2.8: a launch, then figures, page id, codes and the waves' join, each waiting for the one
 // before.  A single workgroup of 8 or 16 waves in place of ranges and their join is slower
 // (500 keys, bf16: 13.7 us against 10.0).
@@ -260,8 +260,10 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
   constexpr int VB = DP / 16;                     // bytes of a value a lane holds
   constexpr int VW = VB / 4;
   constexpr int NQ = TYPE == QC_STORAGE_F32 ? 2 : 1;   // f16 terms of q
-  // and of the probabilities: one rounded to 11 bits weighs as much as an f16 output's own
-  // rounding where few keys do, and the second term costs nothing beside the loads
+  // And of the probabilities: one rounded to 11 bits weighs as much as an f16 output's own
+  // rounding, and the second term costs little beside the loads.  A bf16 output's is 8 times as
+  // coarse: a second term would change its error against 64 bits by less than 1% (single outputs take the
+  // next bf16 step) and cost 2% of decoding (32 x 16384 keys, 154 -> 157 us), 8 to 15% of prompts of 16 to 100 tokens.
   constexpr int NP = TYPE == QC_STORAGE_BF16 ? 1 : 2;
   __shared__ int s_page[kMaxGroups];
   __shared__ float s_ks[kMaxGroups], s_vs[kMaxGroups];
@@ -743,8 +745,11 @@ __global__ __launch_bounds__(256) void attention_layout(Kv8Args a, AttnArgs p, F
 // Workgroup: NW waves of 32 rows of a key head, a range of keys.  A step is 64 keys.
 // A score's exponent is one fused multiply-add: with c the key scale times the row's
 // factor and b = log2(value scale / largest one) + shift per 16 keys, p' = 2^(s c + b - m)
-// is the probability as it meets the codes of V, and the sum takes p' 2^-b.  For 16-bit q
-// the shift is 11, and m follows the running maximum only once that is 4 above it (p' <= 2^15
+// is the probability as it meets the codes of V, and the sum takes p' 2^-b.  For 16-bit q p' is one
+// f16, 11 bits.  That is as coarse as an f16 output, whose error against 64 bits it takes from 2.1e-4 to 2.8e-4 of the
+// outputs' size (bf16: 1.66e-3 to 1.67e-3); a second term for f16 q, as the direct form has, costs 19 to 40% (8192
+// tokens, heads of 128, 536 -> 747 us): half again the MFMAs of a loop that they bound.
+// The shift is 11 there, and m follows the running maximum only once that is 4 above it (p' <= 2^15
 // fits f16): of random rows, some maximum among 32 grows in most steps, and each growth
 // rescales all sums.  p' keeps its 11 bits down to 2^-25 of the row's largest that way (with 7
 // and 8, to 2^-21: a row whose largest meets a code of 0 showed it); f32 q, whose second
@@ -756,8 +761,8 @@ __global__ __launch_bounds__(256) void attention_layout(Kv8Args a, AttnArgs p, F
 // while step t's exponentials and value products go on, so K is a step ahead of V in the S
 // LDS buffers each has.
 //
-// 8192 tokens, 32 / 8 heads of 128, bf16, causal (550 GFLOP): 510 us and 13 for the layout, 1.05
-// PFLOP/s of both (a plain f16 product of 8192^3 reaches 1.11).  MFMAs and VALU are each busy
+// 8192 tokens, 32 / 8 heads of 128, bf16, causal (550 GFLOP): 510 to 550 us by session and 13 for the layout, 0.98 to
+// 1.05 PFLOP/s of both (a plain f16 product of 8192^3 reaches 1.1 to 1.3).  MFMAs and VALU are each busy
 // half of the SIMDs' cycles and the clock is at 1.9 GHz: what bounds it is issue and power.
 // Priorities by wave or phase change nothing or cost 4%.
 // 16-key groups of a range: what LDS holds beside the buffers. (Each range of a prompt's keys

@@ -85,8 +85,9 @@ __device__ __forceinline__ int code_of(float v) {
 // stay in registers between the maximum and the codes, the others are read again
 // (from L2).  A page and head is a chain of dependent reads (lengths, page id, rows, scale)
 // with little data behind it, so many small workgroups: 64 threads where a page's
-// head is at most 4096 elements.  10.5 thousand tokens of 8 heads of 128, f16, pages
-// of 16 (64 MB): 39 us with an element a thread, 14 here (4.5 TB/s).
+// head is at most 4096 elements.  7152 tokens of 8 heads of 128, f16, pages of 16 (29 MB of rows
+// read, 15 of codes written): 39 us with an element a thread, 14.8 here: 3.0 TB/s, 1.7 times what the bytes
+// take at a copy's rate, for that chain and the VALU (busy two thirds of the time).
 constexpr int kHeld = 8;
 template <int TYPE, int NT, bool VEC>
 __global__ __launch_bounds__(NT) void append_kernel(Kv8Args a, Rows k, Rows v, int slots) {
@@ -208,8 +209,8 @@ __device__ __forceinline__ void zero_row(typename Storage<TYPE>::raw* p, int n) 
 }
 
 // The same places read back: code * scale, rounded once; eight codes a thread and step, kHeld
-// loads ahead of the stores.  Bound by memory: 10.5 thousand tokens of 8 heads of 128 to f16,
-// pages of 16 (64 MB): 17 us with four codes and a load a step and 256 threads, 11 here (5.8 TB/s).
+// loads ahead of the stores.  7152 tokens of 8 heads of 128 to f16, pages of 16 (15 MB read, 30
+// written): 17 us with four codes and a load a step and 256 threads, 10.8 here (4.1 TB/s).
 // rest: workgroups from it on, two for each 64 token rows (K and V), set those to zero that no
 // sequence has; 0 where such rows stay as they are.  (A fill of all rows before the call: 6 us more, and
 // as many of the host's.)

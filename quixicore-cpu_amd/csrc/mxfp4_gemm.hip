@@ -50,8 +50,9 @@ __device__ __forceinline__ i32x8 fp4_operand(const i32x4& v) {
 // of barrier, LDS reads and MFMAs, the LDS traffic (a 256 x 256 tile reads its 64 KB stage
 // three times and writes it once, as many cycles as its MFMAs) and MFMA power: M = 4096,
 // 14336 x 4096, quantised normal values, 155 us = 3.1 PFLOP/s, the matrix cores busy half of
-// it. Eight waves of 64 x 128 there: four of 128 x 128 are 6% slower, sixteen of
-// 64 x 64 3%; 128 x 128 tiles (M = 512) take 14 us with eight waves, 24 with four.
+// it (this instruction on operands that stay in registers reaches 6.5 PFLOP/s: 74 us). Eight
+// waves of 64 x 128 there: four of 128 x 128 are 6% slower, sixteen of 64 x 64 3%; 128 x 128
+// tiles (M = 512) take 14 us with eight waves, 24 with four.
 __device__ __forceinline__ void ring_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();

@@ -200,7 +200,7 @@ hipError_t rope_layout(const RopeArgs& a, bool interleaved, bool copy, hipStream
 // to 0.008 only), its cosine and sine times the magnitude rounded once.  A thread
 // takes kRun positions of a pair: the first from sincos, the others turned on by (cos w,
 // sin w), each turn within 2^-52.  131072 positions of 32 pairs: 22 us with a sincos
-// each, 9 so.
+// each, 9 so: 3 for the launch and the two sincos before the first store, then 34 MB at 5.8 TB/s.
 constexpr int kRun = 16;
 __global__ __launch_bounds__(kThreads) void rope_table_kernel(float* __restrict__ cosine,
                                                               float* __restrict__ sine,
