@@ -679,7 +679,7 @@ def test_attention_tiny_value_scales_in_some_ranges(qc, dev, route, dtype, new, 
     rng = np.random.default_rng(new)
     batch = Ragged(rng, [new], [4000], 16)
     cache = _random_cache(qc, dev, rng, batch.pages, 2, 16, 64)
-    pid, _ = batch.places(0, 512, 3072)
+    pid, _ = batch.places(0, 512, 2560)
     cache.tensors[3][np.unique(pid)] = scale
     _attend(qc, dev, rng, [new], [4000], 4, 2, 64, 16, dtype, batch=batch, cache=cache)
 
