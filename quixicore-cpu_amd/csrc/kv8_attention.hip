@@ -273,12 +273,13 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
   const int lane = threadIdx.x & 63, row16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Range fastest, then row block, key head, sequence; ranges past every length after all of these.
-  // With blocks enough to fill the chip the range is slowest: workgroups are dealt to the XCDs in turn, and short
-  // sequences' empty ranges would leave some idle (128 sequences of up to 6000 keys, heads of 64, 141 -> 110 us; with
-  // fewer blocks 32 x 16384 keys 154 -> 162, and row blocks that share keys on several XCDs).
+  // With blocks enough to fill the chip and an even number of ranges the range is slowest: workgroups are dealt to the
+  // 8 XCDs in turn, and short sequences' empty ranges would leave some idle (128 sequences of up to 6000 keys, heads of
+  // 64, 2 ranges, 141 -> 110 us; 3 ranges spread by themselves: 64 x 4 row blocks, 11832 keys, 183 -> 200; with fewer
+  // blocks 32 x 16384 keys 154 -> 162, and row blocks that share keys on several XCDs).
   int used;
   const int chunk = range_keys(a, p, 32 * kWaves, 32, used);
-  const bool slowest = p.want == 1 && p.splits > 1;
+  const bool slowest = p.want == 1 && (p.splits & 1) == 0;
   int id = blockIdx.x / used, split = blockIdx.x - id * used;
   if (slowest || used < p.splits) {
     const int blocks = gridDim.x / p.splits, first = slowest ? 0 : blocks * used;   // of the workgroups in that order
@@ -290,6 +291,10 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
   }
   int seq, kvh, rb;
   if (!block_of(a, p, id, seq, kvh, rb)) return;
+  // Where a unit's row blocks lie side by side, the last ones of an even number, which short sequences lack, would
+  // always be the same XCDs': exchanged from unit to unit, within the power of two that divides the number (64
+  // sequences of 4 to 16 tokens, 8 blocks each, 2000 keys, 129 -> 111 us).
+  if (p.listed == kPadded && (slowest || p.splits == 1)) rb ^= (seq * a.kv_heads + kvh) & ((p.row_blocks & -p.row_blocks) - 1);
   Unit u;
   if (!kv8_sequence(a, seq, u.first, u.rows, u.kv) || u.rows * p.group >= p.rows_to) return;
   const int r0 = rb * RT * 16, r1 = min(r0 + RT * 16, u.rows * p.group);
