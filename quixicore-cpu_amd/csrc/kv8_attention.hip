@@ -559,7 +559,10 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
     if (more) load_v(at0, at1);
   }
 
-  // join the waves: the common maximum, then the sums pairwise in a fixed order
+  // join the waves: the common maximum, then the sums pairwise in a fixed order; unit 2^-15 with half
+  // of its power of two here and the rest with 1 / l, so that neither factor underflows
+  const int half_e = unit_e / 2;
+  const float early = ldexpf(1.0f / 32768.0f, half_e), back = ldexpf(unit_m, unit_e - half_e);
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     l[t] = lanes16_sum(l[t]);
@@ -575,7 +578,7 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) all = fmaxf(all, s_m[w][16 * t + row16]);
     const float ref = all == -INFINITY ? 0.f : all;
-    const float mine = __builtin_amdgcn_exp2f(m[t] - ref);
+    const float mine = __builtin_amdgcn_exp2f(m[t] - ref) * early;
 #pragma unroll
     for (int k = 0; k < VB; ++k)
 #pragma unroll
@@ -604,7 +607,6 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
     if (half > 1) __syncthreads();
   }
   if (wave > 0) return;
-  const float back = unit_m * (1.0f / 32768.0f);  // (times 2^unit_e, last: no factor underflows)
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = r0 + 16 * t + row16;
@@ -626,7 +628,7 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
       if (d >= a.head_dim) continue;
       float v[VB];
 #pragma unroll
-      for (int k = 0; k < VB; ++k) v[k] = ldexpf(acc[t][k][e] * f, unit_e);
+      for (int k = 0; k < VB; ++k) v[k] = acc[t][k][e] * f;
       if (last)
         store_n<TYPE, VB>(p.out, (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim + d,
                           p.vec, v);
