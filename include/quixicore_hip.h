@@ -25,8 +25,8 @@
  *   - Results are deterministic: rerunning a call gives bit-identical output.
  *   - Scratch: entry points whose kernels need device scratch (qc_hip_qgemm
  *     from M = 2, the canonical int8 projections from M = 2, the affine
- *     canonical W8A8 route, qc_hip_kv8_attention of long caches and of long prompts,
- *     qc_hip_mxfp4_gemm of scale arrays that do not begin at a multiple of 4 bytes, or of
+ *     canonical W8A8 route, qc_hip_kv8_attention (and qc_hip_kv8_tree_attention) of long caches and of long prompts,
+ *     qc_hip_mxfp4_moe, qc_hip_mxfp4_gemm of scale arrays that do not begin at a multiple of 4 bytes, or of
  *     many rows of x whose scale rows do not) take it from a per-(device, stream) cache that
  *     only grows; the first call on a stream, or one needing more, allocates
  *     (hipMalloc), later calls do not.  Calls on one stream share its buffers
@@ -466,6 +466,52 @@ int qc_hip_kv8_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, c
                          long long heads, float scale, int causal, long long window,
                          int* dev_status, void* stream);
 
+/* qc_hip_rope and qc_hip_kv8_append in one launch: the batch's keys go into the cache turned, its
+ * queries into q_out.  A token's position is positions[token] ([tokens]), or, with positions NULL, its place
+ * in its sequence (kv_len - n + i).  A turned key's products and sums are rounded to f32 one by one and nothing is
+ * rounded to `type` between: scales and codes are those that qc_hip_kv8_append makes of the turned f32 keys.  q and q_out:
+ * [tokens][heads * head_dim], rows q_stride / out_stride elements apart; q_out may be q (same strides), other
+ * overlaps are not allowed; heads 0: no queries (q and q_out are not looked at).  cosine, sine, max_position,
+ * rotary_dim (even, at most head_dim) and layout as for qc_hip_rope.  Errors as for qc_hip_kv8_append, and
+ * a position outside [0, max_position): that token's queries, and the pages and heads that its key goes to, are left
+ * as they were (its value is not).  Rows of no sequence are neither read nor written.  Status: 1 for sizes out of
+ * range, 2 for an unknown type, 3 for NULL or misaligned pointers or a bad layout. */
+int qc_hip_kv8_rope_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* q,
+                           long long q_stride, void* q_out, long long out_stride, long long heads,
+                           const void* k, long long k_stride, const void* v, long long v_stride,
+                           int type, const float* cosine, const float* sine, const int* positions,
+                           long long max_position, long long rotary_dim, int layout,
+                           int* dev_status, void* stream);
+
+/* qc_hip_kv8_attention for trees of drafted tokens: the new tokens of a sequence are seen by a mask.  With
+ * c = kv_len - n, token i sees the positions j < c, and of the new ones c + b where bit b % 32 of word b / 32 of
+ * mask[token][mask_words] is set (bits from n on are not looked at); itself only if its own bit is.  window > 0:
+ * of the positions below c it sees those j > positions[token] - window, positions[token] (its depth's: c .. kv_len -
+ * 1; [tokens], NULL without a window) being where qc_hip_rope turned it; the mask alone says which new ones.  A
+ * position that is not in c .. kv_len - 1 is an error and counts as the nearest that is.  A row that sees nothing is
+ * zeros.  Everything else as for qc_hip_kv8_attention.  Status: 1 for sizes out of range (mask_words of fewer bits than
+ * the smaller of max_new and tokens), 2 for an unknown type, 3 for NULL or misaligned pointers (positions with a
+ * window) or a scale that is not finite. */
+int qc_hip_kv8_tree_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* q,
+                              long long q_stride, void* out, long long out_stride, int type,
+                              long long heads, float scale, const uint32_t* mask,
+                              long long mask_words, const int* positions, long long window,
+                              int* dev_status, void* stream);
+
+/* The accepted ones of each sequence's new tokens close up behind the others: with c = kv_len - n, new token
+ * kept[s * kept_columns + a] (ascending indexes below n, kept_count[s] of them) moves to position c + a, and
+ * new_len[s] = c + kept_count[s]; kv_len stays as it is.  A page and head that receives tokens of other pages takes
+ * the largest magnitude of its scale and theirs, s'; the codes held below the new ones, and those that come, become
+ * clamp(rint(code * (s / s')), +-127), s the scale they had, each step rounded to f32; other pages move codes as they are.
+ * Slots from the new length on hold anything.  A page written by a call must belong to one sequence; new_len overlaps
+ * nothing that is read.  Errors: a count outside 0 .. min(n, kept_columns), indexes that are not ascending or below n, n
+ * above kv_len, a page id out of range: the sequence and its new_len are left as they were; a page that a token
+ * comes from or goes to whose scale is not finite: that head's keys or values are (new_len is written).  Status: 1 for
+ * sizes out of range, 3 for NULL or misaligned pointers or new_len at kv_len. */
+int qc_hip_kv8_keep(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const int* kept,
+                    long long kept_columns, const int* kept_count, int* new_len, int* dev_status,
+                    void* stream);
+
 /* MXFP4: blocks of 32 values of a row as 4-bit floats (sign, 2 exponent bits, 1
  * mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6) under a power of two.  codes
  * [rows][dim / 2], the even element in a byte's low half; scales [rows][dim / 32],
@@ -493,6 +539,38 @@ int qc_hip_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, void* o
 int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uint8_t* x_codes,
                       const uint8_t* x_scales, void* y, int y_type, long long m, long long n,
                       long long k, void* stream);
+
+/* A mixture-of-experts feed-forward with MXFP4 weights, for a few tokens (more than 512 go in passes of
+ * 512, each of which reads the weights).  gate_up [experts][2 * inter][dim]: an expert's gate rows, then its up
+ * rows; down [experts][dim][inter]; router [experts][dim] of router_type, router_bias f32 [experts] or NULL.  dim and
+ * inter are multiples of 32, codes 16-byte aligned, experts at most 1024, experts * dim and experts * inter at
+ * most 2^27. */
+typedef struct qc_mxfp4_moe {
+  const void* router;
+  const float* router_bias;
+  const uint8_t* gate_up_codes;
+  const uint8_t* gate_up_scales;
+  const uint8_t* down_codes;
+  const uint8_t* down_scales;
+  int router_type;
+  long long experts;
+  long long dim;
+  long long inter;
+} qc_mxfp4_moe;
+
+/* y = residual + sum_s weights[s] down_e (act(gate_e x) * (up_e x)), e = ids[s], for each token's top_k
+ * experts.  Logits are x . router + router_bias, summed in 64 bits; ids [tokens][top_k] are those of the largest, in
+ * falling order (of equal ones the lowest index first; NaN counts as the lowest), weights [tokens][top_k] their
+ * softmax over the chosen (normalize != 0) or over all experts, times weight_scale.  act: SiLU, or GELU-tanh (gelu_tanh != 0).
+ * x, y and residual (NULL: none): [tokens][dim] of `type`, rows that many elements apart; y may be residual (same
+ * strides) or x.  Weights and products are exact, a code times its block's scale as bf16 (a block scale byte of
+ * 255: NaN); x enters with all its bits, the hidden values with 16 (f32: 24), sums are f32, y is rounded once.  A
+ * token that is not finite makes its own row so, no other.  Status: 1 for sizes out of range (top_k above
+ * experts or 64), 2 for an unknown type, 3 for NULL or misaligned pointers or a weight_scale that is not finite. */
+int qc_hip_mxfp4_moe(const qc_mxfp4_moe* layer, const void* x, long long x_stride,
+                     const void* residual, long long residual_stride, void* y, long long y_stride,
+                     int type, long long tokens, long long top_k, int normalize, float weight_scale,
+                     int gelu_tanh, int* ids, float* weights, void* stream);
 
 /* Measurement seam with no reference counterpart: reads `bytes` (a multiple
  * of 16) of device memory with 16-byte loads as fast as the chip allows and
@@ -579,7 +657,7 @@ int qc_hip_set_cint8_dot(int mode);
  * counterpart. */
 int qc_hip_set_qgemm_fold(int mode);
 
-/* Kernels of qc_hip_kv8_attention (process-wide): 0 (default) chooses from the
+/* Kernels of qc_hip_kv8_attention and qc_hip_kv8_tree_attention (process-wide): 0 (default) chooses from the
  * sizes; 1 / 2 read the cache directly for 16 or 32 rows a workgroup (head_dim above
  * 128 with f32: always 16); 3 lays it out for MFMA tiles first.  All stay within
  * the stated precision.  Tuning and test knob with no reference counterpart. */

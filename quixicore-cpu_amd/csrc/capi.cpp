@@ -961,6 +961,124 @@ int qc_hip_kv8_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, c
       [&](int* flag) { return qc::launch_kv8_attention(r, flag, s); });
 }
 
+int qc_hip_kv8_rope_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* q,
+                           long long q_stride, void* q_out, long long out_stride, long long heads,
+                           const void* k, long long k_stride, const void* v, long long v_stride,
+                           int type, const float* cosine, const float* sine, const int* positions,
+                           long long max_position, long long rotary_dim, int layout,
+                           int* dev_status, void* stream) {
+  if (cache == nullptr || batch == nullptr) return QC_INVALID_ARGUMENT;
+  if (!kv8_shapes(*cache, *batch)) return QC_INVALID_SHAPE;
+  const long long row = cache->kv_heads * cache->head_dim, most = LLONG_MAX / 8 / batch->tokens;
+  if (k_stride < row || v_stride < row || k_stride > most || v_stride > most) return QC_INVALID_SHAPE;
+  if (heads < 0 || heads > INT_MAX / 256) return QC_INVALID_SHAPE;
+  if (heads > 0) {
+    const long long q_row = heads * cache->head_dim;
+    if (q_stride < q_row || out_stride < q_row || q_stride > most || out_stride > most) return QC_INVALID_SHAPE;
+    // a token's heads are counted in an int
+    if (q_row > (1LL << 30)) return QC_INVALID_SHAPE;
+  }
+  if (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > cache->head_dim) return QC_INVALID_SHAPE;
+  if (max_position <= 0 || max_position > INT_MAX) return QC_INVALID_SHAPE;
+  if (!known_storage(type)) return QC_UNSUPPORTED_FORMAT;
+  if (layout != QC_ROPE_HALF && layout != QC_ROPE_INTERLEAVED) return QC_INVALID_ARGUMENT;
+  if (!kv8_pointers(*cache, *batch) || k == nullptr || v == nullptr || cosine == nullptr || sine == nullptr)
+    return QC_INVALID_ARGUMENT;
+  if (heads > 0 && (q == nullptr || q_out == nullptr || (q == q_out && q_stride != out_stride)))
+    return QC_INVALID_ARGUMENT;
+  qc::Kv8Turn t;
+  t.cosine = cosine;
+  t.sine = sine;
+  t.positions = positions;
+  t.max_position = max_position;
+  t.rotary = rotary_dim;
+  t.q = q;
+  t.q_out = q_out;
+  t.q_stride = q_stride;
+  t.out_stride = out_stride;
+  t.heads = heads;
+  t.type = type;
+  t.interleaved = layout == QC_ROPE_INTERLEAVED;
+  const hipStream_t s = as_stream(stream);
+  return checked(
+      dev_status, s,
+      [&](int* flag) {
+        hipError_t e = qc::launch_kv8_check(*cache, *batch, qc::Kv8Call::kAppend, 0, flag, s);
+        if (e == hipSuccess) e = qc::launch_kv8_nonfinite(*cache, *batch, k, k_stride, v, v_stride, type, flag, s);
+        if (e == hipSuccess)
+          e = qc::launch_kv8_rope_append(*cache, *batch, t, k, k_stride, v, v_stride, /*check=*/true, flag, s);
+        return e;
+      },
+      [&](int* flag) {
+        return qc::launch_kv8_rope_append(*cache, *batch, t, k, k_stride, v, v_stride, /*check=*/false, flag, s);
+      });
+}
+
+int qc_hip_kv8_tree_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* q,
+                              long long q_stride, void* out, long long out_stride, int type,
+                              long long heads, float scale, const uint32_t* mask,
+                              long long mask_words, const int* positions, long long window,
+                              int* dev_status, void* stream) {
+  if (cache == nullptr || batch == nullptr) return QC_INVALID_ARGUMENT;
+  if (!kv8_shapes(*cache, *batch)) return QC_INVALID_SHAPE;
+  if (heads <= 0 || heads % cache->kv_heads != 0 || heads > INT_MAX / 256 || window < 0)
+    return QC_INVALID_SHAPE;
+  const long long drafted = std::min(batch->max_new, batch->tokens);
+  if (drafted * (heads / cache->kv_heads) > INT_MAX / 2) return QC_INVALID_SHAPE;
+  if (mask_words <= 0 || mask_words > INT_MAX / 32 || 32 * mask_words < drafted) return QC_INVALID_SHAPE;
+  const long long row = heads * cache->head_dim, most = LLONG_MAX / 8 / batch->tokens;
+  if (q_stride < row || out_stride < row || q_stride > most || out_stride > most)
+    return QC_INVALID_SHAPE;
+  if (!known_storage(type)) return QC_UNSUPPORTED_FORMAT;
+  if (!kv8_pointers(*cache, *batch) || q == nullptr || out == nullptr || mask == nullptr) return QC_INVALID_ARGUMENT;
+  if (!std::isfinite(scale) || (window > 0 && positions == nullptr)) return QC_INVALID_ARGUMENT;
+  qc::Kv8Attention r;
+  r.cache = cache;
+  r.batch = batch;
+  r.q = q;
+  r.out = out;
+  r.q_stride = q_stride;
+  r.out_stride = out_stride;
+  r.type = type;
+  r.heads = heads;
+  r.window = std::min<long long>(window, INT_MAX / 2);
+  r.scale = scale;
+  r.causal = 0;
+  r.mask = mask;
+  r.mask_words = mask_words;
+  r.positions = positions;
+  r.route = g_knobs.kv8_route.load(std::memory_order_relaxed);
+  const hipStream_t s = as_stream(stream);
+  return checked(
+      dev_status, s,
+      [&](int* flag) {
+        hipError_t e = qc::launch_kv8_check(*cache, *batch, qc::Kv8Call::kAttention, static_cast<int>(r.window), flag, s);
+        if (e == hipSuccess && window > 0) e = qc::launch_kv8_positions(*cache, *batch, positions, flag, s);
+        return e;
+      },
+      [&](int* flag) { return qc::launch_kv8_attention(r, flag, s); });
+}
+
+int qc_hip_kv8_keep(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const int* kept,
+                    long long kept_columns, const int* kept_count, int* new_len, int* dev_status,
+                    void* stream) {
+  if (cache == nullptr || batch == nullptr) return QC_INVALID_ARGUMENT;
+  if (!kv8_shapes(*cache, *batch)) return QC_INVALID_SHAPE;
+  if (kept_columns <= 0 || kept_columns > INT_MAX) return QC_INVALID_SHAPE;
+  if (!kv8_pointers(*cache, *batch) || kept == nullptr || kept_count == nullptr || new_len == nullptr ||
+      new_len == batch->kv_len)
+    return QC_INVALID_ARGUMENT;
+  const hipStream_t s = as_stream(stream);
+  return checked(
+      dev_status, s,
+      [&](int* flag) {
+        return qc::launch_kv8_keep(*cache, *batch, kept, kept_columns, kept_count, new_len, /*check=*/true, flag, s);
+      },
+      [&](int* flag) {
+        return qc::launch_kv8_keep(*cache, *batch, kept, kept_columns, kept_count, new_len, /*check=*/false, flag, s);
+      });
+}
+
 int qc_hip_quantize_mxfp4(const void* x, int type, long long x_stride, uint8_t* codes,
                           uint8_t* scales, long long rows, long long dim, int* dev_status,
                           void* stream) {
@@ -1004,6 +1122,48 @@ int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uin
                                         g_knobs.mxfp4_route.load(std::memory_order_relaxed),
                                         as_stream(stream)));
   });
+}
+
+int qc_hip_mxfp4_moe(const qc_mxfp4_moe* layer, const void* x, long long x_stride,
+                     const void* residual, long long residual_stride, void* y, long long y_stride,
+                     int type, long long tokens, long long top_k, int normalize, float weight_scale,
+                     int gelu_tanh, int* ids, float* weights, void* stream) {
+  if (layer == nullptr) return QC_INVALID_ARGUMENT;
+  const qc_mxfp4_moe& l = *layer;
+  constexpr long long kMost = 1LL << 27;
+  if (l.experts <= 0 || l.experts > 1024 || l.dim <= 0 || l.inter <= 0 || l.dim % 32 != 0 || l.inter % 32 != 0 ||
+      l.dim > kMost / l.experts || l.inter > kMost / l.experts)
+    return QC_INVALID_SHAPE;
+  if (tokens <= 0 || top_k <= 0 || top_k > l.experts || top_k > 64 || tokens > INT_MAX / 64) return QC_INVALID_SHAPE;
+  const long long most = LLONG_MAX / 8 / tokens;
+  const auto stride_ok = [&](long long st) { return tokens == 1 || (st >= l.dim && st <= most); };
+  if (!stride_ok(x_stride) || !stride_ok(y_stride) || (residual != nullptr && !stride_ok(residual_stride)))
+    return QC_INVALID_SHAPE;
+  if (!known_storage(type) || !known_storage(l.router_type)) return QC_UNSUPPORTED_FORMAT;
+  if (x == nullptr || y == nullptr || ids == nullptr || weights == nullptr || l.router == nullptr ||
+      l.gate_up_codes == nullptr || l.gate_up_scales == nullptr || l.down_codes == nullptr ||
+      l.down_scales == nullptr || !aligned16(l.gate_up_codes) || !aligned16(l.down_codes))
+    return QC_INVALID_ARGUMENT;
+  qc::Moe m;
+  m.layer = layer;
+  m.x = x;
+  m.residual = residual;
+  m.y = y;
+  m.x_stride = tokens > 1 ? x_stride : 0;
+  m.residual_stride = tokens > 1 ? residual_stride : 0;
+  m.y_stride = tokens > 1 ? y_stride : 0;
+  if (y == residual && m.y_stride != m.residual_stride) return QC_INVALID_ARGUMENT;
+  if (y == x && m.y_stride != m.x_stride) return QC_INVALID_ARGUMENT;
+  if (!std::isfinite(weight_scale)) return QC_INVALID_ARGUMENT;
+  m.type = type;
+  m.tokens = tokens;
+  m.top = top_k;
+  m.normalize = normalize != 0;
+  m.gelu_tanh = gelu_tanh != 0;
+  m.scale = weight_scale;
+  m.ids = ids;
+  m.weights = weights;
+  return guarded([&] { return finish(qc::launch_mxfp4_moe(m, as_stream(stream))); });
 }
 
 int qc_hip_set_qgemm_panel(int mode) {

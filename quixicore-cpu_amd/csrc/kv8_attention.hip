@@ -53,6 +53,9 @@ struct AttnArgs {
   int rows_from, rows_to;   // sequences of [rows_from, rows_to) rows a key head are worked on
   int listed;           // what blocks are counted by: kPadded, kBlocks, kSequences
   int route;            // host: 0 by size, 1 / 2 one or two row tiles, 3 tiled
+  const uint32_t* mask; // TREE: [tokens][words], what a row sees of its sequence's new tokens
+  int words;
+  const int* positions; // TREE with a window: rows' positions
 };
 
 // How blocks are counted.  kPadded: every sequence has row_blocks of them.  kBlocks:
@@ -88,10 +91,34 @@ __device__ __forceinline__ bool block_of(const Kv8Args& a, const AttnArgs& p, in
 }
 
 // Keys [lo, hi) that rows of tokens t0..t1 (inclusive) see together.
+template <bool TREE>
 __device__ __forceinline__ void seen_range(const AttnArgs& p, const Unit& u, int t0, int t1, int& lo,
                                            int& hi) {
+  if (TREE) {
+    // no row's position is before the first new token's
+    hi = u.kv;
+    lo = p.window > 0 ? max(0, u.position(0) + 1 - p.window) : 0;
+    return;
+  }
   hi = p.causal ? min(u.kv, u.position(t1) + 1) : u.kv;
   lo = p.window > 0 ? max(0, u.position(t0) + 1 - p.window) : 0;
+}
+
+// TREE: the first context key that a row sees.  A position that is not one of the new tokens' is an error and
+// counts as the nearest that is.
+__device__ __forceinline__ int tree_low(const Kv8Args& a, const AttnArgs& p, const Unit& u, int token) {
+  if (p.window <= 0) return 0;
+  const int at = p.positions[u.first + token];
+  if (at < u.position(0) || at >= u.kv) *a.status = QC_INVALID_ARGUMENT;
+  return min(max(at, u.position(0)), u.kv - 1) + 1 - p.window;
+}
+
+// Bits of a row's mask for keys j .. j + 31, bit b that of key c + b (clear outside the mask).
+__device__ __forceinline__ uint32_t tree_bits(const AttnArgs& p, const uint32_t* row, int b) {
+  const int w = b >> 5, by = b & 31;
+  const uint32_t low = w >= 0 && w < p.words ? row[w] : 0;
+  const uint32_t high = w + 1 >= 0 && w + 1 < p.words ? row[w + 1] : 0;
+  return by == 0 ? low : low >> by | high << (32 - by);
 }
 
 // The most keys of a sequence with rows; for all lanes.
@@ -253,7 +280,7 @@ __device__ __forceinline__ void store_n(void* out, long long at, bool vec, const
 constexpr int kWaves = 4;
 constexpr int kMaxGroups = 1024;   // 16-key groups of a range
 
-template <int DP, int RT, int TYPE>
+template <int DP, int RT, int TYPE, bool TREE>
 __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STORAGE_F32 ? 4 : 1) void attention_direct(Kv8Args a, AttnArgs p) {
   constexpr int KC = DP / 64;                     // 16-byte chunks of a key a lane holds
   constexpr int KS = DP / 32;                     // MFMAs of 32 dimensions
@@ -300,7 +327,7 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
   const int r0 = rb * RT * 16, r1 = min(r0 + RT * 16, u.rows * p.group);
   if (r0 >= r1) return;
   int lo, hi;
-  seen_range(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
+  seen_range<TREE>(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
   const int base = lo & ~31;
   const int from = __builtin_amdgcn_readfirstlane(base + split * chunk);   // a multiple of 32
   const int to = __builtin_amdgcn_readfirstlane(min(hi, from + chunk));
@@ -400,7 +427,8 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
   // q's fragments: row row16 of tile t, dimensions 64 c + 16 g + 8 h + j
   f16x8 qf[RT][KS][NQ];
   float factor[RT];                               // score's scale in log2 units, over q's
-  int row_lo[RT], row_hi[RT];                     // keys the lane's row sees
+  int row_lo[RT], row_hi[RT];                     // keys the lane's row sees (TREE: of the context)
+  const uint32_t* row_mask[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = r0 + 16 * t + row16;
@@ -434,13 +462,23 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
         qf[t][s][0][j] = static_cast<_Float16>(x);
         if constexpr (NQ == 2) qf[t][s][1][j] = static_cast<_Float16>(x - static_cast<float>(qf[t][s][0][j]));
       }
-    row_hi[t] = has ? (p.causal ? min(u.kv, u.position(token) + 1) : u.kv) : 0;
-    row_lo[t] = p.window > 0 ? u.position(token) + 1 - p.window : 0;
+    if constexpr (TREE) {
+      row_hi[t] = u.position(0);
+      row_lo[t] = tree_low(a, p, u, token);
+      row_mask[t] = p.mask + static_cast<long long>(u.first + token) * p.words;
+    } else {
+      row_hi[t] = has ? (p.causal ? min(u.kv, u.position(token) + 1) : u.kv) : 0;
+      row_lo[t] = p.window > 0 ? u.position(token) + 1 - p.window : 0;
+    }
   }
   // keys that every row of the block sees (its rows past r1 count for nothing whatever they see)
   int all_hi = hi, all_lo = lo;
   if (p.causal) all_hi = min(u.kv, u.position(r0 / p.group) + 1);
   if (p.window > 0) all_lo = u.position((r1 - 1) / p.group) + 1 - p.window;
+  if (TREE) {
+    all_hi = u.position(0);
+    if (p.window > 0) all_lo = u.kv - p.window;
+  }
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) unit = fmaxf(unit, s_red[w]);
@@ -505,7 +543,15 @@ __global__ __launch_bounds__(64 * kWaves, RT == 1 && DP <= 128 && TYPE != QC_STO
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[4 * t + e] = s[rt][t][e] * c;
       }
-      if (!whole) {
+      if (TREE && !whole) {
+        const uint32_t bits = tok + 32 > all_hi ? tree_bits(p, row_mask[rt], tok - all_hi) : 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int o = 16 * (e >> 2) + 4 * g + (e & 3), j = tok + o;
+          const bool sees = j < all_hi ? j >= row_lo[rt] : (bits >> o & 1) != 0;
+          if (!sees || j >= u.kv || page[e >> 2] < 0) z[e] = -INFINITY;
+        }
+      } else if (!whole) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = tok + 16 * (e >> 2) + 4 * g + (e & 3);
@@ -778,7 +824,7 @@ template <int DP>
 constexpr int kTiledGroups = DP == 256 ? 1024 : 4096;
 constexpr int kTiledLeast = 1024;   // keys of a range, where there are as many
 
-template <int DP, int NW, int TYPE>
+template <int DP, int NW, int TYPE, bool TREE>
 __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, AttnArgs p, Frags f) {
   constexpr int NF = DP / 16, DT = DP / 32;
   constexpr int NQ = TYPE == QC_STORAGE_F32 ? 2 : 1;
@@ -821,7 +867,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   const int r0 = rb * NW * 32, r1 = min(r0 + NW * 32, u.rows * p.group);
   if (r0 >= r1) return;
   int lo, hi;
-  seen_range(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
+  seen_range<TREE>(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
   int used;
   const int chunk = range_keys(a, p, kTiledLeast, 64, used);
   const int from = __builtin_amdgcn_readfirstlane((lo & ~63) + split * chunk);
@@ -874,7 +920,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   const bool has = r < r1;
   const int token = (has ? r : r0) / p.group, head = kvh * p.group + (has ? r : r0) - token * p.group;
   const int row_hi = has ? (p.causal ? min(u.kv, u.position(token) + 1) : u.kv) : 0;
-  const int row_lo = p.window > 0 ? u.position(token) + 1 - p.window : 0;
+  const int row_lo = TREE ? tree_low(a, p, u, token) : p.window > 0 ? u.position(token) + 1 - p.window : 0;
+  const uint32_t* row_mask = TREE ? p.mask + static_cast<long long>(u.first + token) * p.words : nullptr;
   float factor, broken = 0.f;                     // broken: NaN for a row that is not finite
   {
     const long long at = (u.first + token) * p.q_stride + static_cast<long long>(head) * a.head_dim;
@@ -920,6 +967,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
     any_hi = max(any_hi, __shfl_xor(any_hi, o));
     all_lo = max(all_lo, __shfl_xor(all_lo, o));
   }
+  if (TREE) all_hi = u.position(0);
   all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   any_hi = __builtin_amdgcn_readfirstlane(any_hi);
   all_lo = __builtin_amdgcn_readfirstlane(all_lo);
@@ -1006,7 +1054,18 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
     pin();
     f32x4 c = s_c[step];
     const f32x4 b = s_b[step], inv = s_inv[step];
-    if (any_bad || tok < all_lo || tok + 64 > all_hi) {
+    if (TREE && (any_bad || tok < all_lo || tok + 64 > all_hi)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const uint32_t bits = tree_bits(p, row_mask, tok + 32 * t - all_hi);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int o = 8 * (e >> 2) + 4 * half + (e & 3), j = tok + 32 * t + o;
+          const bool sees = j < all_hi ? j >= row_lo : (bits >> o & 1) != 0;
+          if (!sees || j >= u.kv || c[2 * t + (e >> 3)] < 0.f) s[t][e] = -INFINITY;
+        }
+      }
+    } else if (any_bad || tok < all_lo || tok + 64 > all_hi) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -1258,10 +1317,11 @@ hipError_t run_join(const Kv8Args& a, const AttnArgs& p, long long blocks, hipSt
 // Keys that a block of `rows` rows can see, from a multiple of `align` on.
 long long key_span(const Kv8Args& a, const AttnArgs& p, int rows, int align) {
   if (p.window <= 0) return a.max_kv;
+  if (p.mask != nullptr) return std::min<long long>(a.max_kv, static_cast<long long>(p.window) + a.max_new + align);
   return std::min<long long>(a.max_kv, static_cast<long long>(p.window) + (rows + p.group - 1) / p.group + align);
 }
 
-template <int DP, int RT, int TYPE>
+template <int DP, int RT, int TYPE, bool TREE>
 hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   const long long rows = std::min<long long>(static_cast<long long>(a.max_new) * p.group, p.rows_to - 1);
   p.per = RT * 16;
@@ -1291,7 +1351,7 @@ hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
     hold = std::unique_lock<std::mutex>(ws->call);
     if ((e = part_buffers(a, p, ws, s)) != hipSuccess) return e;
   }
-  attention_direct<DP, RT, TYPE><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a, p);
+  attention_direct<DP, RT, TYPE, TREE><<<static_cast<unsigned>(grid), 64 * kWaves, 0, s>>>(a, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   return run_join<TYPE>(a, p, units, s);
@@ -1326,7 +1386,7 @@ TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per, int max_groups) {
   return {seqs * a.kv_heads, blocks};
 }
 
-template <int DP, int NW, int TYPE>
+template <int DP, int NW, int TYPE, bool TREE>
 hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   const TiledPlan plan = plan_tiled(a, p, 32 * NW, kTiledGroups<DP>);
   const long long units = plan.units, blocks = plan.blocks;
@@ -1358,7 +1418,7 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
     attention_layout<DP><<<static_cast<unsigned>(n) * tiles, 256, 0, s>>>(a, lay, f, tiles);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     const long long grid = (p.listed == kPadded ? n * p.row_blocks : blocks * a.kv_heads) * p.splits;
-    attention_tiled<DP, NW, TYPE><<<static_cast<unsigned>(grid), 64 * NW, 0, s>>>(a, p, f);
+    attention_tiled<DP, NW, TYPE, TREE><<<static_cast<unsigned>(grid), 64 * NW, 0, s>>>(a, p, f);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   return p.splits > 1 ? run_join<TYPE>(a, p, blocks * a.kv_heads, s) : hipSuccess;
@@ -1383,7 +1443,7 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
 // not every sequence can have as many, those that have are laid out and the others
 // read directly: 4096 new tokens beside 63 sequences of one, 4000 to 8000 keys, 2317 us
 // with all laid out, 700 so (the prompt alone 460, the others 170).
-template <int DP, int TYPE>
+template <int DP, int TYPE, bool TREE>
 hipError_t run_rows(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   constexpr int NW = DP == 256 ? 4 : 8;
   const bool brief = a.max_kv <= 1024;
@@ -1399,7 +1459,7 @@ hipError_t run_rows(const Kv8Args& a, AttnArgs p, hipStream_t s) {
     tiled = 4 * groups >= (brief ? 2 : 3) * device_cu_count();
     if (tiled) p.rows_from = q.rows_from;
   }
-  if (tiled && p.rows_from == 0) return run_tiled<DP, NW, TYPE>(a, p, s);
+  if (tiled && p.rows_from == 0) return run_tiled<DP, NW, TYPE, TREE>(a, p, s);
   double keys = a.max_kv;
   if (p.causal) keys -= 0.5 * std::min(a.max_new, a.max_kv);
   if (p.window > 0) keys = std::min<double>(keys, p.window);
@@ -1411,18 +1471,22 @@ hipError_t run_rows(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   if (tiled) few.rows_to = many;
   hipError_t e = hipSuccess;
   if constexpr (DP < 256 || TYPE != QC_STORAGE_F32) {   // (two of f32 256 do not fit the registers)
-    e = two ? run_direct<DP, 2, TYPE>(a, few, s) : run_direct<DP, 1, TYPE>(a, few, s);
+    e = two ? run_direct<DP, 2, TYPE, TREE>(a, few, s) : run_direct<DP, 1, TYPE, TREE>(a, few, s);
   } else {
-    e = run_direct<DP, 1, TYPE>(a, few, s);
+    e = run_direct<DP, 1, TYPE, TREE>(a, few, s);
   }
-  return tiled && e == hipSuccess ? run_tiled<DP, NW, TYPE>(a, p, s) : e;
+  return tiled && e == hipSuccess ? run_tiled<DP, NW, TYPE, TREE>(a, p, s) : e;
 }
 
+template <int TYPE, bool TREE>
+hipError_t run_sized(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
+  if (a.head_dim <= 64) return run_rows<64, TYPE, TREE>(a, p, s);
+  if (a.head_dim <= 128) return run_rows<128, TYPE, TREE>(a, p, s);
+  return run_rows<256, TYPE, TREE>(a, p, s);
+}
 template <int TYPE>
 hipError_t run_typed(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
-  if (a.head_dim <= 64) return run_rows<64, TYPE>(a, p, s);
-  if (a.head_dim <= 128) return run_rows<128, TYPE>(a, p, s);
-  return run_rows<256, TYPE>(a, p, s);
+  return p.mask != nullptr ? run_sized<TYPE, true>(a, p, s) : run_sized<TYPE, false>(a, p, s);
 }
 
 }  // namespace
@@ -1440,6 +1504,9 @@ hipError_t launch_kv8_attention(const Kv8Attention& r, int* status, hipStream_t 
   p.causal = r.causal;
   p.window = static_cast<int>(r.window);
   p.route = r.route;
+  p.mask = r.mask;
+  p.words = static_cast<int>(r.mask_words);
+  p.positions = r.positions;
   const int size = r.type == QC_STORAGE_F32 ? 4 : 2;
   p.vec = ((reinterpret_cast<uintptr_t>(r.q) | reinterpret_cast<uintptr_t>(r.out) |
             static_cast<uintptr_t>(r.q_stride * size) | static_cast<uintptr_t>(r.out_stride * size)) & 15) == 0;

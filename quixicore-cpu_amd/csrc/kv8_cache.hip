@@ -9,6 +9,11 @@
 // 127), ties to even, each step rounded to f32.  So a call's codes are
 // defined bit for bit, and a page that is filled token by token has been rounded
 // at most once for each growth of its scale.
+//
+// Append with rotation.  The same with the keys turned by their tokens' positions on the way:
+// a' = a c - b s, b' = b c + a s, each product and sum rounded to f32, which is what the
+// scale and codes are made of (no rounding to the rows' type between).  The queries are turned by further
+// workgroups of the same launch.
 #include <algorithm>
 
 #include "qc_kv8.h"
@@ -81,6 +86,150 @@ __device__ __forceinline__ int code_of(float v) {
   return static_cast<int>(fminf(fmaxf(rintf(v), -127.f), 127.f));
 }
 
+// What an append turns: the cache's keys, and q into q_out.
+struct Turn {
+  const float* cosine;
+  const float* sine;       // [max_position][rotary / 2]
+  const int* positions;    // of the batch's tokens; null: their places in their sequences
+  int max_position, rotary;
+  const void* q;
+  void* q_out;
+  long long q_stride, out_stride;
+  int heads;               // of q; 0 where there is none
+  unsigned from;           // workgroups from it on turn q
+  int parts;               // of them a token
+};
+enum { kPlain, kHalf, kInterleaved };
+
+// Element d of a head at x, turned by the table row c, s.
+template <int TYPE, int ROT>
+__device__ __forceinline__ float turned(const typename Storage<TYPE>::raw* x, int d, const float* c, const float* s,
+                                        int rotary) {
+  const float u = decode<TYPE>(x[d]);
+  if (d >= rotary) return u;
+  const int half = rotary / 2;
+  const bool second = ROT == kHalf ? d >= half : (d & 1) != 0;
+  const int i = ROT == kHalf ? (second ? d - half : d) : d >> 1;
+  const float v = decode<TYPE>(x[ROT == kHalf ? (second ? d - half : d + half) : d ^ 1]);
+  return second ? u * c[i] + v * s[i] : u * c[i] - v * s[i];
+}
+
+// The same for V elements from d on in 16-byte accesses (V divides rotary / 2, or rotary if
+// interleaved).
+template <int TYPE, int ROT>
+__device__ __forceinline__ void turned16(const typename Storage<TYPE>::raw* x, int d, const float* c, const float* s,
+                                         int rotary, float* f) {
+  constexpr int V = Storage<TYPE>::per16;
+  float u[V];
+  decode16<TYPE>(*reinterpret_cast<const u32x4*>(x + d), u);
+  if (d >= rotary) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = u[j];
+    return;
+  }
+  if constexpr (ROT == kHalf) {
+    const int half = rotary / 2;
+    const bool second = d >= half;
+    const int i = second ? d - half : d;
+    float v[V];
+    decode16<TYPE>(*reinterpret_cast<const u32x4*>(x + (second ? i : i + half)), v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float a = u[j] * c[i + j], b = v[j] * s[i + j];
+      f[j] = second ? a + b : a - b;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float cj = c[(d + j) >> 1], sj = s[(d + j) >> 1];
+      f[j] = u[j] * cj - u[j + 1] * sj;
+      f[j + 1] = u[j + 1] * cj + u[j] * sj;
+    }
+  }
+}
+
+// The sequence that token t belongs to and t's place in it; every lane of the wavefront takes part, with the
+// same t.  False where it is no sequence's, or one's that an append leaves alone.
+__device__ __forceinline__ bool place_of_token(const Kv8Args& a, int t, int& place) {
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < a.seqs; base += 64) {
+    int first = 0, rows = 0, kv = 0;
+    const bool mine = base + lane < a.seqs && kv8_sequence(a, base + lane, first, rows, kv) && t >= first &&
+                      t < first + rows;
+    const uint64_t hit = __ballot(mine);
+    if (hit == 0) continue;
+    const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+    place = __builtin_amdgcn_readlane(kv - rows + t - first, l);
+    return __builtin_amdgcn_readlane(kv - rows, l) >= 0;
+  }
+  return false;
+}
+
+// Workgroup `part` of a token's q heads: a pair of chunks a thread.
+template <int TYPE, int NT, bool VEC, int ROT>
+__device__ __forceinline__ void turn_q(const Kv8Args& a, const Turn& w, int id) {
+  typedef typename Storage<TYPE>::raw raw;
+  constexpr int V = VEC ? Storage<TYPE>::per16 : 4;
+  const int t = id / w.parts, part = id - t * w.parts;
+  int p;
+  if (!place_of_token(a, t, p)) return;
+  if (w.positions != nullptr) p = w.positions[t];
+  if (static_cast<unsigned>(p) >= static_cast<unsigned>(w.max_position)) {
+    if (threadIdx.x == 0) *a.status = QC_INVALID_ARGUMENT;
+    return;
+  }
+  const raw* x = static_cast<const raw*>(w.q) + t * w.q_stride;
+  raw* y = static_cast<raw*>(w.q_out) + t * w.out_stride;
+  const int half = w.rotary / 2;
+  const float* c = w.cosine + static_cast<long long>(p) * half;
+  const float* s = w.sine + static_cast<long long>(p) * half;
+  // chunks of a head: of pairs, then of what is copied (nothing in place)
+  const int turns = ROT == kHalf ? (half + V - 1) / V : (w.rotary + V - 1) / V;
+  const int rest = w.q == w.q_out ? 0 : (a.head_dim - w.rotary + V - 1) / V;
+  const int all = turns + rest, i = part * NT + threadIdx.x;
+  const int head = i / all, chunk = i - head * all;
+  if (head >= w.heads) return;
+  x += static_cast<long long>(head) * a.head_dim;
+  y += static_cast<long long>(head) * a.head_dim;
+  if (chunk >= turns) {
+    const int d = w.rotary + (chunk - turns) * V;
+    if constexpr (VEC) {
+      *reinterpret_cast<u32x4*>(y + d) = *reinterpret_cast<const u32x4*>(x + d);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (d + j < a.head_dim) y[d + j] = x[d + j];
+    }
+    return;
+  }
+  const int d = chunk * V;
+  if constexpr (VEC) {
+    float f[V];
+    turned16<TYPE, ROT>(x, d, c, s, w.rotary, f);
+    if constexpr (ROT == kHalf) {
+      float g[V];
+      turned16<TYPE, ROT>(x, d + half, c, s, w.rotary, g);
+      *reinterpret_cast<u32x4*>(y + d + half) = encode16<TYPE>(g);
+    }
+    *reinterpret_cast<u32x4*>(y + d) = encode16<TYPE>(f);
+  } else {
+    const int n = ROT == kHalf ? half : w.rotary;
+    float f[V], g[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (d + j < n) {
+        f[j] = turned<TYPE, ROT>(x, d + j, c, s, w.rotary);
+        if constexpr (ROT == kHalf) g[j] = turned<TYPE, ROT>(x, d + j + half, c, s, w.rotary);
+      }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (d + j < n) {
+        y[d + j] = encode<TYPE>(f[j]);
+        if constexpr (ROT == kHalf) y[d + j + half] = encode<TYPE>(g[j]);
+      }
+  }
+}
+
 // Chunks of V elements (VEC: 16 bytes of a row, aligned); the first kHeld of a thread
 // stay in registers between the maximum and the codes, the others are read again
 // (from L2).  A page and head is a chain of dependent reads (lengths, page id, rows, scale)
@@ -89,11 +238,13 @@ __device__ __forceinline__ int code_of(float v) {
 // read, 15 of codes written): 39 us with an element a thread, 14.8 here: 3.0 TB/s, 1.7 times what the bytes
 // take at a copy's rate, for that chain and the VALU (busy two thirds of the time).
 constexpr int kHeld = 8;
-template <int TYPE, int NT, bool VEC>
-__global__ __launch_bounds__(NT) void append_kernel(Kv8Args a, Rows k, Rows v, int slots) {
+template <int TYPE, int NT, bool VEC, int ROT>
+__global__ __launch_bounds__(NT) void append_kernel(Kv8Args a, Rows k, Rows v, int slots, Turn turn) {
   typedef typename Storage<TYPE>::raw raw;
   constexpr int V = VEC ? Storage<TYPE>::per16 : 4;
   __shared__ float stop[NT / 64];
+  if constexpr (ROT != kPlain)
+    if (blockIdx.x >= turn.from) return turn_q<TYPE, NT, VEC, ROT>(a, turn, blockIdx.x - turn.from);
   Place w;
   if (!place_of(a, slots, w) || w.unit < 0) return;
   const Rows src = w.which ? v : k;
@@ -106,7 +257,23 @@ __global__ __launch_bounds__(NT) void append_kernel(Kv8Args a, Rows k, Rows v, i
   auto load = [&](int i, float* f) {
     const int t = i / per_row;
     const raw* p = x + t * src.stride + (i - t * per_row) * V;
-    if constexpr (VEC) {
+    if (ROT != kPlain && w.which == 0) {
+      const int at = turn.positions != nullptr ? turn.positions[w.row + t] : w.lo + t;
+      if (static_cast<unsigned>(at) >= static_cast<unsigned>(turn.max_position)) {   // an error, like a NaN
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = __uint_as_float(0x7FC00000u);
+        return;
+      }
+      const float* c = turn.cosine + static_cast<long long>(at) * (turn.rotary / 2);
+      const float* s = turn.sine + static_cast<long long>(at) * (turn.rotary / 2);
+      const int d = (i - t * per_row) * V;
+      if constexpr (VEC) {
+        turned16<TYPE, ROT>(p - d, d, c, s, turn.rotary, f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = turned<TYPE, ROT>(p - d, d + j, c, s, turn.rotary);
+      }
+    } else if constexpr (VEC) {
       decode16<TYPE>(*reinterpret_cast<const u32x4*>(p), f);
     } else {
 #pragma unroll
@@ -301,6 +468,16 @@ __global__ __launch_bounds__(kThreads) void kv8_check(Kv8Args a, Kv8Call call, i
   }
 }
 
+// Positions of a sequence's new tokens that are not its last ones.
+__global__ __launch_bounds__(kThreads) void kv8_positions(Kv8Args a, const int* __restrict__ positions) {
+  int first, rows, kv;
+  if (!kv8_sequence(a, blockIdx.x, first, rows, kv)) return;
+  for (int i = threadIdx.x; i < rows; i += kThreads) {
+    const int p = positions[first + i];
+    if (p < kv - rows || p >= kv) *a.status = QC_INVALID_ARGUMENT;
+  }
+}
+
 // *flag = 3 where a row of the batch's sequences holds NaN or +-inf; `parts` workgroups a
 // sequence for K and V each.
 template <int TYPE>
@@ -315,6 +492,28 @@ __global__ __launch_bounds__(kThreads) void kv8_nonfinite(Kv8Args a, Rows k, Row
     for (int i = threadIdx.x; i < row; i += kThreads)
       if (!isfinite(decode<TYPE>(static_cast<const raw*>(src.p)[(first + t) * src.stride + i])))
         *a.status = QC_INVALID_ARGUMENT;
+}
+
+// *flag = 3 where a token of the batch's sequences has no table row, or a key is not finite once turned: a
+// workgroup a token.
+template <int TYPE, int ROT>
+__global__ __launch_bounds__(64) void turn_check(Kv8Args a, Rows k, Turn w) {
+  typedef typename Storage<TYPE>::raw raw;
+  const int t = blockIdx.x;
+  int p;
+  if (!place_of_token(a, t, p)) return;
+  if (w.positions != nullptr) p = w.positions[t];
+  if (static_cast<unsigned>(p) >= static_cast<unsigned>(w.max_position)) {
+    *a.status = QC_INVALID_ARGUMENT;
+    return;
+  }
+  const raw* x = static_cast<const raw*>(k.p) + t * k.stride;
+  const float* c = w.cosine + static_cast<long long>(p) * (w.rotary / 2);
+  const float* s = w.sine + static_cast<long long>(p) * (w.rotary / 2);
+  for (int i = threadIdx.x; i < a.kv_heads * a.head_dim; i += 64) {
+    const int h = i / a.head_dim, d = i - h * a.head_dim;
+    if (!isfinite(turned<TYPE, ROT>(x + h * a.head_dim, d, c, s, w.rotary))) *a.status = QC_INVALID_ARGUMENT;
+  }
 }
 
 // Pages that max_new tokens in a row can touch.
@@ -363,6 +562,14 @@ hipError_t launch_kv8_check(const qc_kv8_cache& c, const qc_kv8_batch& b, Kv8Cal
   return hipGetLastError();
 }
 
+hipError_t launch_kv8_positions(const qc_kv8_cache& c, const qc_kv8_batch& b, const int* positions, int* flag,
+                                hipStream_t s) {
+  const Kv8Args a = kv8_args(c, b, flag);
+  if (!kv8_grid_fits(a.seqs, kThreads)) return hipErrorInvalidValue;
+  kv8_positions<<<a.seqs, kThreads, 0, s>>>(a, positions);
+  return hipGetLastError();
+}
+
 hipError_t launch_kv8_nonfinite(const qc_kv8_cache& c, const qc_kv8_batch& b, const void* k,
                                 long long k_stride, const void* v, long long v_stride, int type,
                                 int* flag, hipStream_t s) {
@@ -387,18 +594,47 @@ bool wide_rows(const void* p, long long stride, int size) {
   return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * size)) % 16 == 0;
 }
 
-template <int TYPE>
-hipError_t run_append(const Kv8Args& a, const Rows& k, const Rows& v, hipStream_t s) {
-  constexpr int size = TYPE == QC_STORAGE_F32 ? 4 : 2;
+template <int TYPE, int NT, bool VEC, int ROT>
+hipError_t append_with(const Kv8Args& a, const Rows& k, const Rows& v, Turn turn, hipStream_t s) {
   int slots;
-  const unsigned grid = touched_grid(a, slots);
-  const bool vec = wide_rows(k.p, k.stride, size) && wide_rows(v.p, v.stride, size);
-  const bool small = std::min(a.max_new, a.page_tokens) * a.head_dim <= 4096;
-  if (!kv8_grid_fits(grid, vec && small ? 64 : 256)) return hipErrorInvalidValue;
-  if (vec && small) append_kernel<TYPE, 64, true><<<grid, 64, 0, s>>>(a, k, v, slots);
-  else if (vec) append_kernel<TYPE, 256, true><<<grid, 256, 0, s>>>(a, k, v, slots);
-  else append_kernel<TYPE, 256, false><<<grid, 256, 0, s>>>(a, k, v, slots);
+  long long grid = touched_grid(a, slots);
+  if (ROT != kPlain) {
+    constexpr int V = VEC ? Storage<TYPE>::per16 : 4;
+    const int pairs = ROT == kHalf ? turn.rotary / 2 : turn.rotary;
+    const int chunks = (pairs + V - 1) / V + (turn.q == turn.q_out ? 0 : (a.head_dim - turn.rotary + V - 1) / V);
+    turn.from = static_cast<unsigned>(grid);
+    turn.parts = static_cast<int>((static_cast<long long>(turn.heads) * chunks + NT - 1) / NT);
+    grid += static_cast<long long>(a.tokens) * turn.parts;
+  }
+  if (!kv8_grid_fits(grid, NT)) return hipErrorInvalidValue;
+  append_kernel<TYPE, NT, VEC, ROT><<<static_cast<unsigned>(grid), NT, 0, s>>>(a, k, v, slots, turn);
   return hipGetLastError();
+}
+
+template <int TYPE, int ROT>
+hipError_t run_append(const Kv8Args& a, const Rows& k, const Rows& v, const Turn& turn, hipStream_t s) {
+  constexpr int size = TYPE == QC_STORAGE_F32 ? 4 : 2, V = Storage<TYPE>::per16;
+  bool vec = wide_rows(k.p, k.stride, size) && wide_rows(v.p, v.stride, size);
+  if (ROT != kPlain && vec) {
+    vec = (ROT == kHalf ? turn.rotary / 2 : turn.rotary) % V == 0;
+    if (turn.heads > 0) vec = vec && wide_rows(turn.q, turn.q_stride, size) && wide_rows(turn.q_out, turn.out_stride, size);
+  }
+  const bool small = std::min(a.max_new, a.page_tokens) * a.head_dim <= 4096;
+  if (vec && small) return append_with<TYPE, 64, true, ROT>(a, k, v, turn, s);
+  if (vec) return append_with<TYPE, 256, true, ROT>(a, k, v, turn, s);
+  return append_with<TYPE, 256, false, ROT>(a, k, v, turn, s);
+}
+
+template <int TYPE>
+hipError_t run_turn(const Kv8Args& a, const Rows& k, const Rows& v, const Turn& turn, bool interleaved, bool check,
+                    hipStream_t s) {
+  if (check) {
+    if (!kv8_grid_fits(a.tokens, 64)) return hipErrorInvalidValue;
+    if (interleaved) turn_check<TYPE, kInterleaved><<<a.tokens, 64, 0, s>>>(a, k, turn);
+    else turn_check<TYPE, kHalf><<<a.tokens, 64, 0, s>>>(a, k, turn);
+    return hipGetLastError();
+  }
+  return interleaved ? run_append<TYPE, kInterleaved>(a, k, v, turn, s) : run_append<TYPE, kHalf>(a, k, v, turn, s);
 }
 
 template <int TYPE>
@@ -426,9 +662,32 @@ hipError_t launch_kv8_append(const qc_kv8_cache& c, const qc_kv8_batch& b, const
   const Kv8Args a = kv8_args(c, b, status);
   const Rows kr = {k, k_stride}, vr = {v, v_stride};
   switch (type) {
-    case QC_STORAGE_F32: return run_append<QC_STORAGE_F32>(a, kr, vr, s);
-    case QC_STORAGE_F16: return run_append<QC_STORAGE_F16>(a, kr, vr, s);
-    default: return run_append<QC_STORAGE_BF16>(a, kr, vr, s);
+    case QC_STORAGE_F32: return run_append<QC_STORAGE_F32, kPlain>(a, kr, vr, {}, s);
+    case QC_STORAGE_F16: return run_append<QC_STORAGE_F16, kPlain>(a, kr, vr, {}, s);
+    default: return run_append<QC_STORAGE_BF16, kPlain>(a, kr, vr, {}, s);
+  }
+}
+
+hipError_t launch_kv8_rope_append(const qc_kv8_cache& c, const qc_kv8_batch& b, const Kv8Turn& t, const void* k,
+                                  long long k_stride, const void* v, long long v_stride, bool check, int* status,
+                                  hipStream_t s) {
+  const Kv8Args a = kv8_args(c, b, status);
+  const Rows kr = {k, k_stride}, vr = {v, v_stride};
+  Turn w = {};
+  w.cosine = t.cosine;
+  w.sine = t.sine;
+  w.positions = t.positions;
+  w.max_position = static_cast<int>(t.max_position);
+  w.rotary = static_cast<int>(t.rotary);
+  w.q = t.q;
+  w.q_out = t.q_out;
+  w.q_stride = t.q_stride;
+  w.out_stride = t.out_stride;
+  w.heads = static_cast<int>(t.heads);
+  switch (t.type) {
+    case QC_STORAGE_F32: return run_turn<QC_STORAGE_F32>(a, kr, vr, w, t.interleaved, check, s);
+    case QC_STORAGE_F16: return run_turn<QC_STORAGE_F16>(a, kr, vr, w, t.interleaved, check, s);
+    default: return run_turn<QC_STORAGE_BF16>(a, kr, vr, w, t.interleaved, check, s);
   }
 }
 

@@ -291,9 +291,30 @@ hipError_t launch_kv8_nonfinite(const qc_kv8_cache& c, const qc_kv8_batch& b, co
 hipError_t launch_kv8_append(const qc_kv8_cache& c, const qc_kv8_batch& b, const void* k,
                              long long k_stride, const void* v, long long v_stride, int type,
                              int* status, hipStream_t s);
+// qc_hip_kv8_rope_append; check: looks at positions and turned keys only.
+struct Kv8Turn {
+  const float* cosine = nullptr;
+  const float* sine = nullptr;
+  const int* positions = nullptr;
+  long long max_position = 0, rotary = 0;
+  const void* q = nullptr;
+  void* q_out = nullptr;
+  long long q_stride = 0, out_stride = 0, heads = 0;
+  int type = QC_STORAGE_F32;
+  bool interleaved = false;
+};
+hipError_t launch_kv8_rope_append(const qc_kv8_cache& c, const qc_kv8_batch& b, const Kv8Turn& t, const void* k,
+                                  long long k_stride, const void* v, long long v_stride, bool check, int* status,
+                                  hipStream_t s);
+// qc_hip_kv8_keep; check: looks at the paths, pages and scales only.
+hipError_t launch_kv8_keep(const qc_kv8_cache& c, const qc_kv8_batch& b, const int* kept, long long kept_columns,
+                           const int* kept_count, int* new_len, bool check, int* status, hipStream_t s);
 hipError_t launch_kv8_gather(const qc_kv8_cache& c, const qc_kv8_batch& b, void* k,
                              long long k_stride, void* v, long long v_stride, int type, bool zero_rest,
                              int* status, hipStream_t s);
+// *flag = 3 where a new token's position is not one of its sequence's new ones.
+hipError_t launch_kv8_positions(const qc_kv8_cache& c, const qc_kv8_batch& b, const int* positions, int* flag,
+                                hipStream_t s);
 struct Kv8Attention {
   const qc_kv8_cache* cache = nullptr;
   const qc_kv8_batch* batch = nullptr;
@@ -305,6 +326,9 @@ struct Kv8Attention {
   float scale = 1.f;
   int causal = 1;
   int route = 0;        // 0 by size, 1 / 2 straight from the cache, one or two row tiles, 3 tiled
+  const uint32_t* mask = nullptr;   // qc_hip_kv8_tree_attention: what rows see of the new tokens
+  long long mask_words = 0;
+  const int* positions = nullptr;   // with a window
 };
 hipError_t launch_kv8_attention(const Kv8Attention& r, int* status, hipStream_t s);
 
@@ -321,5 +345,21 @@ hipError_t launch_dequantize_mxfp4(const uint8_t* codes, const uint8_t* scales, 
 hipError_t launch_mxfp4_gemm(const uint8_t* w, const uint8_t* ws, const uint8_t* x,
                              const uint8_t* xs, void* y, int type, long long m, long long n,
                              long long k, int route, hipStream_t s);   // route: 0 by size, 1..7 a tile
+
+// qc_hip_mxfp4_moe, all checks done by the caller.
+struct Moe {
+  const qc_mxfp4_moe* layer = nullptr;
+  const void* x = nullptr;
+  const void* residual = nullptr;
+  void* y = nullptr;
+  long long x_stride = 0, residual_stride = 0, y_stride = 0;
+  int type = QC_STORAGE_F32;
+  long long tokens = 0, top = 0;
+  bool normalize = true, gelu_tanh = false;
+  float scale = 1.f;
+  int* ids = nullptr;
+  float* weights = nullptr;
+};
+hipError_t launch_mxfp4_moe(const Moe& m, hipStream_t s);
 
 }  // namespace qc

@@ -78,6 +78,13 @@ _SIGS = {
     "qc_hip_kv8_gather": ([_P, _P, _P, _LL, _P, _LL, _I, _I, _P, _P], _I),
     "qc_hip_kv8_attention": ([_P, _P, _P, _LL, _P, _LL, _I, _LL, ctypes.c_float, _I, _LL, _P, _P],
                              _I),
+    "qc_hip_kv8_rope_append": ([_P, _P, _P, _LL, _P, _LL, _LL, _P, _LL, _P, _LL, _I, _P, _P, _P, _LL,
+                                _LL, _I, _P, _P], _I),
+    "qc_hip_kv8_tree_attention": ([_P, _P, _P, _LL, _P, _LL, _I, _LL, ctypes.c_float, _P, _LL, _P,
+                                   _LL, _P, _P], _I),
+    "qc_hip_kv8_keep": ([_P, _P, _P, _LL, _P, _P, _P, _P], _I),
+    "qc_hip_mxfp4_moe": ([_P, _P, _LL, _P, _LL, _P, _LL, _I, _LL, _LL, _I, ctypes.c_float, _I, _P, _P,
+                          _P], _I),
     "qc_hip_quantize_mxfp4": ([_P, _I, _LL, _P, _P, _LL, _LL, _P, _P], _I),
     "qc_hip_dequantize_mxfp4": ([_P, _P, _P, _I, _LL, _LL, _P], _I),
     "qc_hip_set_kv8_attention_route": ([_I], _I),
@@ -590,6 +597,176 @@ def kv8_attention(cache, batch, q, scale=None, causal=True, window=0, out=None, 
                                     1 if causal else 0, window, _status(dev_status), _stream(None)),
            "kv8_attention")
     return out
+
+
+def kv8_rope_append(cache, batch, q, k, v, cosine, sine, positions=None, interleaved=False, out=None,
+                    dev_status=None):
+    """Writes the batch's new tokens' k and v ([tokens][kv_heads][head_dim] or flat rows) into the
+    cache, k turned by the tokens' positions (None: their places in their sequences), and returns q
+    ([tokens][heads][head_dim], rows may be strided; None: no queries) turned likewise; out may be q.
+    Rows of no sequence are left as they were (zeros in a new tensor)."""
+    st = _storage(k)
+    _kv8_here(cache, batch, k, v)
+    tokens, kv_heads, head_dim = batch.tokens, cache.kv_heads, cache.head_dim
+    if v.dtype is not k.dtype or k.shape[0] != tokens or v.shape[0] != tokens:
+        raise ValueError("kv8_rope_append: k and v of one type, a row for each of the batch's tokens")
+    _flat("rope tables", _types[2], cosine, sine)
+    most, half = table = cosine.shape
+    if sine.shape != table:
+        raise ValueError("kv8_rope_append: tables [max_position][rotary_dim / 2]")
+    at = None
+    if positions is not None:
+        _flat("rope positions", _types[0], positions)
+        if positions.numel() != tokens:
+            raise ValueError("kv8_rope_append: a position for each of the batch's tokens")
+        at = positions.data_ptr()
+    heads = qp = qs = op = os_ = 0
+    if q is not None:
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != tokens or q.dtype is not k.dtype:
+            raise ValueError("kv8_rope_append: q is [tokens][heads][head_dim] of k's type, a row for each "
+                             "of the batch's tokens")
+        heads = shape[1]
+        if out is None:
+            import torch
+            out = torch.zeros(shape, dtype=q.dtype, device=q.device)
+        elif out.shape != shape or out.dtype is not q.dtype:
+            raise ValueError("kv8_rope_append: out is of q's shape and type")
+        _here(q, out)
+        qp, op = q.data_ptr(), out.data_ptr()
+        qs, os_ = _rows("q", q, heads, head_dim), _rows("out", out, heads, head_dim)
+    _check(lib.qc_hip_kv8_rope_append(ctypes.addressof(cache), ctypes.addressof(batch), qp, qs, op, os_,
+                                      heads, k.data_ptr(), _rows("k", k, kv_heads, head_dim),
+                                      v.data_ptr(), _rows("v", v, kv_heads, head_dim), st,
+                                      cosine.data_ptr(), sine.data_ptr(), at, most, 2 * half,
+                                      1 if interleaved else 0, _status(dev_status), _stream(None)),
+           "kv8_rope_append")
+    return out
+
+
+def kv8_tree_attention(cache, batch, q, mask, scale=None, positions=None, window=0, out=None,
+                       dev_status=None):
+    """kv8_attention for trees of drafted tokens: each of a sequence's new tokens sees what was there
+    before them, and of them those whose bits are set in its row of mask (int32 [tokens][words], bit b %
+    32 of word b / 32; itself too only by its bit).  With a window, positions (int32 [tokens]) are the
+    rows' own and the window cuts what was there before."""
+    st = _storage(q)
+    head_dim, shape = cache.head_dim, q.shape
+    if len(shape) != 3 or shape[0] != batch.tokens:
+        raise ValueError("kv8_tree_attention: q is [tokens][heads][head_dim], a row for each of the "
+                         "batch's tokens")
+    heads = shape[1]
+    if out is None:
+        import torch
+        out = torch.zeros(shape, dtype=q.dtype, device=q.device)
+    elif out.shape != shape or out.dtype is not q.dtype:
+        raise ValueError("kv8_tree_attention: out is of q's shape and type")
+    _kv8_here(cache, batch, q, out)
+    _flat("kv8_tree_attention's mask", _types[0], mask)
+    if mask.dim() != 2 or mask.shape[0] != batch.tokens:
+        raise ValueError("kv8_tree_attention: mask is [tokens][words]")
+    at = None
+    if positions is not None:
+        _flat("kv8_tree_attention's positions", _types[0], positions)
+        if positions.numel() != batch.tokens:
+            raise ValueError("kv8_tree_attention: a position for each of the batch's tokens")
+        at = positions.data_ptr()
+    if scale is None:
+        scale = head_dim ** -0.5
+    _check(lib.qc_hip_kv8_tree_attention(ctypes.addressof(cache), ctypes.addressof(batch),
+                                         q.data_ptr(), _rows("q", q, heads, head_dim),
+                                         out.data_ptr(), _rows("out", out, heads, head_dim), st,
+                                         heads, scale, mask.data_ptr(), mask.shape[1], at, window,
+                                         _status(dev_status), _stream(None)), "kv8_tree_attention")
+    return out
+
+
+def kv8_keep(cache, batch, kept, count, out=None, dev_status=None):
+    """The accepted ones of each sequence's new tokens (kept int32 [seqs][columns], count[seqs] ascending
+    indexes of them) close up behind what was there before; returns the new lengths (int32 [seqs]).
+    Sequences in error are left as they were, their lengths in a new tensor too (their kv_len)."""
+    if _device is None:
+        _start()
+    _kv8_here(cache, batch)
+    _flat("kv8_keep", _types[0], kept, count)
+    if kept.dim() != 2 or kept.shape[0] != batch.seqs or count.numel() != batch.seqs:
+        raise ValueError("kv8_keep: kept [seqs][columns], count [seqs]")
+    if out is None:
+        out = batch.tensors[2].clone()
+    else:
+        _flat("kv8_keep's lengths", _types[0], out)
+        if out.numel() != batch.seqs:
+            raise ValueError("kv8_keep: a length for each sequence")
+    _check(lib.qc_hip_kv8_keep(ctypes.addressof(cache), ctypes.addressof(batch), kept.data_ptr(),
+                               kept.shape[1], count.data_ptr(), out.data_ptr(), _status(dev_status),
+                               _stream(None)), "kv8_keep")
+    return out
+
+
+class Mxfp4Moe(ctypes.Structure):
+    """qc_mxfp4_moe over router [experts][dim], bias f32 [experts] or None, and uint8 codes
+    [experts][rows][k / 2] and scales [experts][rows][k / 32] of gate_up (gate rows, then up rows) and
+    down; keeps the tensors alive."""
+    _fields_ = [("router", ctypes.c_void_p), ("router_bias", ctypes.c_void_p),
+                ("gate_up_codes", ctypes.c_void_p), ("gate_up_scales", ctypes.c_void_p),
+                ("down_codes", ctypes.c_void_p), ("down_scales", ctypes.c_void_p),
+                ("router_type", ctypes.c_int), ("experts", ctypes.c_longlong),
+                ("dim", ctypes.c_longlong), ("inter", ctypes.c_longlong)]
+
+    def __init__(self, router, gate_up_codes, gate_up_scales, down_codes, down_scales, bias=None):
+        import torch
+        st = _storage(router)
+        _here(router)
+        _flat("router", router.dtype, router)
+        _flat("expert weights", torch.uint8, gate_up_codes, gate_up_scales, down_codes, down_scales)
+        experts, dim = router.shape
+        inter = 2 * down_codes.shape[-1]
+        for name, t, shape in (("gate_up codes", gate_up_codes, (experts, 2 * inter, dim // 2)),
+                               ("gate_up scales", gate_up_scales, (experts, 2 * inter, dim // 32)),
+                               ("down codes", down_codes, (experts, dim, inter // 2)),
+                               ("down scales", down_scales, (experts, dim, inter // 32))):
+            if t.shape != shape:
+                raise ValueError(f"{name}: {shape} expected, got {tuple(t.shape)}")
+        if bias is not None:
+            _flat("router bias", torch.float32, bias)
+            if bias.numel() != experts:
+                raise ValueError("router bias: one for each expert")
+        self.tensors = (router, bias, gate_up_codes, gate_up_scales, down_codes, down_scales)
+        self.device = router.get_device()
+        super().__init__(*[None if t is None else t.data_ptr() for t in self.tensors], st, experts, dim,
+                         inter)
+
+
+def mxfp4_moe(layer, x, top_k, normalize=True, weight_scale=1.0, gelu_tanh=False, residual=None,
+              out=None):
+    """(y, ids, weights) of a mixture-of-experts feed-forward: y [tokens][dim] = residual + sum_s
+    weights[s] down_e(act(gate_e x) * up_e x), e = ids[s], over each token's top_k experts; x, residual
+    and out: rows may be strided, out may be residual or x."""
+    import torch
+    st = _storage(x)
+    if layer.device != _device():
+        raise ValueError(f"experts on cuda:{layer.device}: the current device is cuda:{_device()}")
+    _here(x)
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != layer.dim or x.stride(1) != 1:
+        raise ValueError("mxfp4_moe: x is [tokens][dim], elements side by side")
+    tokens = shape[0]
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    for t in (out, residual):
+        if t is None:
+            continue
+        _here(t)
+        if t.shape != shape or t.dtype is not x.dtype or t.stride(1) != 1:
+            raise ValueError("mxfp4_moe: out and residual are of x's shape and type, elements side by side")
+    ids = torch.empty((tokens, top_k), dtype=torch.int32, device=x.device)
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=x.device)
+    res, res_stride = (None, 0) if residual is None else (residual.data_ptr(), residual.stride(0))
+    _check(lib.qc_hip_mxfp4_moe(ctypes.addressof(layer), x.data_ptr(), x.stride(0), res, res_stride,
+                                out.data_ptr(), out.stride(0), st, tokens, top_k, 1 if normalize else 0,
+                                weight_scale, 1 if gelu_tanh else 0, ids.data_ptr(), weights.data_ptr(),
+                                _stream(None)), "mxfp4_moe")
+    return out, ids, weights
 
 
 def quantize_mxfp4(x, dev_status=None):
