@@ -563,10 +563,11 @@ typedef struct qc_mxfp4_moe {
  * falling order (of equal ones the lowest index first; NaN counts as the lowest), weights [tokens][top_k] their
  * softmax over the chosen (normalize != 0) or over all experts, times weight_scale.  act: SiLU, or GELU-tanh (gelu_tanh != 0).
  * x, y and residual (NULL: none): [tokens][dim] of `type`, rows that many elements apart; y may be residual (same
- * strides) or x.  Weights and products are exact, a code times its block's scale as bf16 (a block scale byte of
- * 255: NaN); x enters with all its bits, the hidden values with 16 (f32: 24), sums are f32, y is rounded once.  A
- * token that is not finite makes its own row so, no other.  Status: 1 for sizes out of range (top_k above
- * experts or 64), 2 for an unknown type, 3 for NULL or misaligned pointers or a weight_scale that is not finite. */
+ * strides) or x.  Weights enter as they are (a block scale byte of 255: NaN), x with all its bits, the hidden values
+ * with 12 (f16: 16, f32: 24); a value far below the largest, m, of its 32 is held to 2^-14 m (f16: 2^-18 m, f32: 2^-30 m).
+ * Products are exact, sums f32, y is rounded once.  A token that is not finite makes its own row so, no other.
+ * Status: 1 for sizes out of range (top_k above experts or 64), 2 for an unknown type, 3 for NULL or misaligned
+ * pointers or a weight_scale that is not finite. */
 int qc_hip_mxfp4_moe(const qc_mxfp4_moe* layer, const void* x, long long x_stride,
                      const void* residual, long long residual_stride, void* y, long long y_stride,
                      int type, long long tokens, long long top_k, int normalize, float weight_scale,
