@@ -489,7 +489,8 @@ int qc_hip_kv8_rope_append(const qc_kv8_cache* cache, const qc_kv8_batch* batch,
  * of the positions below c it sees those j > positions[token] - window, positions[token] (its depth's: c .. kv_len -
  * 1; [tokens], NULL without a window) being where qc_hip_rope turned it; the mask alone says which new ones.  A
  * position that is not in c .. kv_len - 1 is an error and counts as the nearest that is.  A row that sees nothing is
- * zeros.  Everything else as for qc_hip_kv8_attention.  Status: 1 for sizes out of range (mask_words of fewer bits than
+ * zeros.  Everything else as for qc_hip_kv8_attention (f16 q of many rows a key head: as of prompts).  Status: 1 for sizes
+ * out of range (mask_words of fewer bits than
  * the smaller of max_new and tokens), 2 for an unknown type, 3 for NULL or misaligned pointers (positions with a
  * window) or a scale that is not finite. */
 int qc_hip_kv8_tree_attention(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const void* q,
@@ -660,7 +661,8 @@ int qc_hip_set_qgemm_fold(int mode);
 
 /* Kernels of qc_hip_kv8_attention and qc_hip_kv8_tree_attention (process-wide): 0 (default) chooses from the
  * sizes; 1 / 2 read the cache directly for 16 or 32 rows a workgroup (head_dim above
- * 128 with f32: always 16); 3 lays it out for MFMA tiles first.  All stay within
+ * 128 with f32: always 16); 3 lays it out for MFMA tiles first (trees: turns codes for 128 or 256 rows once; head_dim above
+ * 128 with f32: as 1).  All stay within
  * the stated precision.  Tuning and test knob with no reference counterpart. */
 int qc_hip_set_kv8_attention_route(int route);
 

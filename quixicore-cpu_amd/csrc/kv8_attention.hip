@@ -27,6 +27,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -52,7 +55,7 @@ struct AttnArgs {
   int per, row_blocks;  // rows of a row block, row blocks of a sequence's key head at most
   int rows_from, rows_to;   // sequences of [rows_from, rows_to) rows a key head are worked on
   int listed;           // what blocks are counted by: kPadded, kBlocks, kSequences
-  int route;            // host: 0 by size, 1 / 2 one or two row tiles, 3 tiled
+  int route;            // host: 0 by size, 1 / 2 one or two row tiles, 3 tiled (trees: shared)
   const uint32_t* mask; // TREE: [tokens][words], what a row sees of its sequence's new tokens
   int words;
   const int* positions; // TREE with a window: rows' positions
@@ -120,6 +123,9 @@ __device__ __forceinline__ uint32_t tree_bits(const AttnArgs& p, const uint32_t*
   const uint32_t high = w + 1 >= 0 && w + 1 < p.words ? row[w + 1] : 0;
   return by == 0 ? low : low >> by | high << (32 - by);
 }
+
+// The bits below bit n, of 32.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
 // The most keys of a sequence with rows; for all lanes.
 __device__ __forceinline__ int longest(const Kv8Args& a) {
@@ -824,7 +830,84 @@ template <int DP>
 constexpr int kTiledGroups = DP == 256 ? 1024 : 4096;
 constexpr int kTiledLeast = 1024;   // keys of a range, where there are as many
 
-template <int DP, int NW, int TYPE, bool TREE>
+// A row's fragments of q, NQ f16 terms under a power of two: dimensions 16 s + 8 half + j.  factor: a score's scale in log2
+// units; broken: NaN for a row that is not finite (whose terms are zero), else 0.
+template <int NF, int NQ, int TYPE>
+__device__ __forceinline__ void row_fragments(const Kv8Args& a, const AttnArgs& p, long long at, bool has, int half,
+                                              f16x8 (&qf)[NF][NQ], float& factor, float& broken) {
+  float v[NF][8], top = 0.f;
+  bool nan = false;
+#pragma unroll
+  for (int s = 0; s < NF; ++s) {
+    const int d = 16 * s + 8 * half;
+    load8<TYPE>(p.q, at + d, has && d < a.head_dim, p.vec, v[s]);
+  }
+#pragma unroll
+  for (int s = 0; s < NF; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      top = fmaxf(top, fabsf(v[s][j]));
+      nan = nan || v[s][j] != v[s][j];
+    }
+  if (nan) top = INFINITY;
+  top = fmaxf(top, __shfl_xor(top, 32));
+  float inverse;
+  float up = row_scale(top, inverse);
+  broken = 0.f;
+  if (inverse != inverse) {
+    broken = inverse;
+    inverse = 1.f;
+    up = 0.f;
+  }
+  factor = fabsf(p.scale) * kLog2e * inverse;
+  if (p.scale < 0.f) up = -up;
+#pragma unroll
+  for (int s = 0; s < NF; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = in_f32(broken != broken ? 0.f : v[s][j] * up);
+      qf[s][0][j] = static_cast<_Float16>(x);
+      if constexpr (NQ == 2) qf[s][1][j] = static_cast<_Float16>(x - static_cast<float>(qf[s][0][j]));
+    }
+}
+
+// A row's sums to where they belong: out, or the range's partial sums and statistics.  acc[t][e]: dimension 32 t +
+// 8 (e >> 2) + 4 half + (e & 3) in units of unit 2^-shift.
+template <int DT, int NQ, int TYPE>
+__device__ __forceinline__ void store_row(const Kv8Args& a, const AttnArgs& p, const Unit& u, int token, int head, int split,
+                                          int half, const f32x16 (&acc)[DT], float m, float l, float unit, float broken) {
+  const bool last = p.splits == 1;
+  int unit_e;                                     // its power of two comes last: no factor underflows
+  const float unit_m = split_unit(unit, unit_e);
+  const float back = unit_m * (NQ == 2 ? 1.0f / 32768.0f : 1.0f / 2048.0f) + broken;   // 2^-kShift
+  const float scale = last ? (l == 0.f ? 0.f : back / l) : back;
+  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
+  const long long part = static_cast<long long>(split) * a.tokens * p.heads + row;
+  if (!last) {
+    if (half == 0) {
+      p.stats[2 * part] = l == 0.f ? -INFINITY : m;
+      p.stats[2 * part + 1] = l;
+    }
+    if (l == 0.f) return;
+  }
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int d = 32 * t + 2 * e + 4 * half;
+      if (d >= a.head_dim) continue;
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = l == 0.f ? 0.f : ldexpf(acc[t][e + j] * scale, unit_e);
+      if (last)
+        store_n<TYPE, 4>(p.out, (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim + d,
+                         p.vec, v);
+      else
+        store_n<QC_STORAGE_F32, 4>(p.part, part * a.head_dim + d, true, v);
+    }
+}
+
+template <int DP, int NW, int TYPE>
 __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, AttnArgs p, Frags f) {
   constexpr int NF = DP / 16, DT = DP / 32;
   constexpr int NQ = TYPE == QC_STORAGE_F32 ? 2 : 1;
@@ -867,7 +950,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   const int r0 = rb * NW * 32, r1 = min(r0 + NW * 32, u.rows * p.group);
   if (r0 >= r1) return;
   int lo, hi;
-  seen_range<TREE>(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
+  seen_range<false>(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
   int used;
   const int chunk = range_keys(a, p, kTiledLeast, 64, used);
   const int from = __builtin_amdgcn_readfirstlane((lo & ~63) + split * chunk);
@@ -920,45 +1003,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   const bool has = r < r1;
   const int token = (has ? r : r0) / p.group, head = kvh * p.group + (has ? r : r0) - token * p.group;
   const int row_hi = has ? (p.causal ? min(u.kv, u.position(token) + 1) : u.kv) : 0;
-  const int row_lo = TREE ? tree_low(a, p, u, token) : p.window > 0 ? u.position(token) + 1 - p.window : 0;
-  const uint32_t* row_mask = TREE ? p.mask + static_cast<long long>(u.first + token) * p.words : nullptr;
-  float factor, broken = 0.f;                     // broken: NaN for a row that is not finite
-  {
-    const long long at = (u.first + token) * p.q_stride + static_cast<long long>(head) * a.head_dim;
-    float v[NF][8], top = 0.f;
-    bool nan = false;
-#pragma unroll
-    for (int s = 0; s < NF; ++s) {
-      const int d = 16 * s + 8 * half;
-      load8<TYPE>(p.q, at + d, has && d < a.head_dim, p.vec, v[s]);
-    }
-#pragma unroll
-    for (int s = 0; s < NF; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        top = fmaxf(top, fabsf(v[s][j]));
-        nan = nan || v[s][j] != v[s][j];
-      }
-    if (nan) top = INFINITY;
-    top = fmaxf(top, __shfl_xor(top, 32));
-    float inverse;
-    float up = row_scale(top, inverse);
-    if (inverse != inverse) {
-      broken = inverse;
-      inverse = 1.f;
-      up = 0.f;
-    }
-    factor = fabsf(p.scale) * kLog2e * inverse;
-    if (p.scale < 0.f) up = -up;
-#pragma unroll
-    for (int s = 0; s < NF; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = in_f32(broken != broken ? 0.f : v[s][j] * up);
-        qf[s][0][j] = static_cast<_Float16>(x);
-        if constexpr (NQ == 2) qf[s][1][j] = static_cast<_Float16>(x - static_cast<float>(qf[s][0][j]));
-      }
-  }
+  const int row_lo = p.window > 0 ? u.position(token) + 1 - p.window : 0;
+  float factor, broken;
+  row_fragments<NF, NQ, TYPE>(a, p, (u.first + token) * p.q_stride + static_cast<long long>(head) * a.head_dim, has, half,
+                              qf, factor, broken);
   // keys every row of the wave sees, and any of them
   int all_hi = row_hi, any_hi = row_hi, all_lo = row_lo;
 #pragma unroll
@@ -967,7 +1015,6 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
     any_hi = max(any_hi, __shfl_xor(any_hi, o));
     all_lo = max(all_lo, __shfl_xor(all_lo, o));
   }
-  if (TREE) all_hi = u.position(0);
   all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   any_hi = __builtin_amdgcn_readfirstlane(any_hi);
   all_lo = __builtin_amdgcn_readfirstlane(all_lo);
@@ -1054,18 +1101,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
     pin();
     f32x4 c = s_c[step];
     const f32x4 b = s_b[step], inv = s_inv[step];
-    if (TREE && (any_bad || tok < all_lo || tok + 64 > all_hi)) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint32_t bits = tree_bits(p, row_mask, tok + 32 * t - all_hi);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int o = 8 * (e >> 2) + 4 * half + (e & 3), j = tok + 32 * t + o;
-          const bool sees = j < all_hi ? j >= row_lo : (bits >> o & 1) != 0;
-          if (!sees || j >= u.kv || c[2 * t + (e >> 3)] < 0.f) s[t][e] = -INFINITY;
-        }
-      }
-    } else if (any_bad || tok < all_lo || tok + 64 > all_hi) {
+    if (any_bad || tok < all_lo || tok + 64 > all_hi) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -1132,35 +1168,383 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   wait_vmcnt<0>();   // no load may land in LDS that is no longer this workgroup's
   l += __shfl_xor(l, 32);
   if (!has) return;
-  const bool last = p.splits == 1;
-  int unit_e;                                     // its power of two comes last: no factor underflows
-  const float unit_m = split_unit(unit, unit_e);
-  const float back = unit_m * (NQ == 2 ? 1.0f / 32768.0f : 1.0f / 2048.0f) + broken;   // 2^-kShift
-  const float scale = last ? (l == 0.f ? 0.f : back / l) : back;
-  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
-  const long long part = static_cast<long long>(split) * a.tokens * p.heads + row;
-  if (!last) {
-    if (half == 0) {
-      p.stats[2 * part] = l == 0.f ? -INFINITY : m;
-      p.stats[2 * part + 1] = l;
+  store_row<DT, NQ, TYPE>(a, p, u, token, head, split, half, acc, m, l, unit, broken);
+}
+
+// ---- Trees of more rows a key head than the direct form's -----------------------
+//
+// Masks as above; scores, probabilities and sums as in the tiled form, but the codes become f16 operands on their way into
+// LDS: a workgroup's waves, 32 rows each, share them, and no launch lays the cache out first.  A lane loads 16 codes
+// of a key two steps of 64 keys ahead and turns them one step ahead, between a wave's other work.  Tiles of 32 keys: K is
+// one ahead of V, in rings of four tiles each, so a step of two meets one barrier.
+//
+// K's tile: fragments of the tiled form, 16-byte places exchanged by dimension, so that the eight lanes that write a
+// key's codes meet different banks.  V's: keys' rows of f16, 32-byte places exchanged by key, read by ds_read_b64_tr_b16:
+// of 16 lanes' 8 bytes each, lanes 4 r .. 4 r + 3 holding 16 dimensions of key r, lane i receives dimension i of four keys.
+//
+// One sequence of 64 tokens on 131072 keys, 32 / 8 heads of 128, bf16 (137 GFLOP): 170 us, 2.4 a step of 64 keys for 256 rows
+// beside 16 of start, partial sums and end; reads of LDS, turned codes, MFMAs and exponentials each take a quarter of a step
+// and overlap little with two waves a SIMD, for which the registers suffice.  Value products of a half tile issued beside the
+// next one's exponentials change nothing (170); ranges cut from the batch's lengths so that no more have keys than run at once
+// are slower than equal ones (16 sequences to 16384 keys, 6 to 24 tokens: 186 against 160).
+
+// Eight codes as f16 times `times`, twice 1, -1 or 0 there; plus: what the bytes' bias makes of it.
+__device__ __forceinline__ u32x4 codes_to_f16(uint32_t w0, uint32_t w1, f16x2 times, f16x2 plus) {
+  const uint32_t u0 = w0 ^ 0x80808080u, u1 = w1 ^ 0x80808080u;
+  auto turned = [&](uint32_t u, uint32_t pick) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, pick)),
+                                                                  times, plus));
+  };
+  return u32x4{turned(u0, 0x04010400u), turned(u0, 0x04030402u), turned(u1, 0x04010400u), turned(u1, 0x04030402u)};
+}
+
+// 16-key groups of a range: what LDS holds beside the rings, of two workgroups of four waves a CU.
+template <int DP, int NW>
+constexpr int kTreeGroups = DP == 256 ? 1024 : NW == 4 ? 512 : 2048;
+constexpr int kTreeLeast = 512;     // keys of a range, where there are as many
+
+template <int DP, int NW, int TYPE>
+__global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attention_tree(Kv8Args a, AttnArgs p) {
+  constexpr int NF = DP / 16, DT = DP / 32;
+  constexpr int NQ = TYPE == QC_STORAGE_F32 ? 2 : 1;
+  constexpr int kTile = 64 * DP;                  // bytes of 32 keys of K, or of V
+  constexpr int kGroups = kTreeGroups<DP, NW>;
+  constexpr int CPK = DP / 16, CL = 4 * DP / (64 * NW), KW = 64 / CPK;   // pieces of a key, of a lane; keys of a wave
+  static_assert(CL > 0 && 16 % KW == 0, "a wave's keys are one group's");
+  __shared__ __attribute__((aligned(1024))) uint8_t s_k[4 * kTile], s_v[4 * kTile];
+  __shared__ f32x2 s_c[kGroups / 2], s_b[kGroups / 2], s_inv[kGroups / 2];
+  __shared__ u32x2 s_at[kGroups];                 // where a group's codes are
+  __shared__ u32x2 s_times[kGroups];              // what K's and V's are turned by, twice in f16
+  __shared__ float s_unit[NW];
+  __shared__ int s_bad[NW];
+
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // range slowest, so that a sequence's key heads, which end alike, and its row blocks, which share keys, are neighbours
+  int used;
+  const int chunk = range_keys(a, p, kTreeLeast, 64, used);
+  const int blocks = gridDim.x / p.splits, split = blockIdx.x / blocks;
+  int seq, kvh, rb;
+  if (!block_of(a, p, blockIdx.x - split * blocks, seq, kvh, rb)) return;
+  Unit u;
+  if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return;
+  const int r0 = rb * NW * 32, r1 = min(r0 + NW * 32, u.rows * p.group);
+  if (r0 >= r1) return;
+  int lo, hi;
+  seen_range<true>(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
+  const int from = __builtin_amdgcn_readfirstlane((lo & ~63) + split * chunk);
+  const int to = __builtin_amdgcn_readfirstlane(min(hi, from + chunk));
+  if (from >= to && p.splits > 1) {               // a range without keys
+    for (int r = r0 + threadIdx.x; r < r1; r += 64 * NW) {
+      const int token = r / p.group, head = kvh * p.group + r - token * p.group;
+      float* st = p.stats + 2 * ((static_cast<long long>(split) * a.tokens + u.first + token) * p.heads + head);
+      st[0] = -INFINITY;
+      st[1] = 0.f;
     }
-    if (l == 0.f) return;
+    return;
   }
+  const int steps = to > from ? (to - from + 63) >> 6 : 0;
+  const int* table = a.table + static_cast<long long>(seq) * a.columns;
+  auto listed_page = [&](int group) {
+    const int tok = from + 16 * group;
+    return tok < to && tok + 15 >= lo ? table[tok >> a.page_shift] : -1;
+  };
+
+  // Pieces of the wave's keys key .. key + KW - 1 of the range; before it and past it, of keys at its ends.  A group
+  // without a page reads page 0 and counts for nothing, pieces past head_dim are dimension 0's: q is zero there, and
+  // sums there are not stored.
+  const int piece = lane % CPK;
+  const int piece_at = ((wave * KW & 15) + lane / CPK) * a.head_dim + (16 * piece < a.head_dim ? 16 * piece : 0);
+  auto group_of = [&](int key) { return min(max(key, 0) >> 4, 4 * steps - 1); };
+  auto place_of = [&](int page, int group) {
+    const int at = static_cast<unsigned>(page) < static_cast<unsigned>(a.pages) ? page : 0;
+    return ((static_cast<long long>(at) * a.kv_heads + kvh) * a.page_tokens + ((from + 16 * group) & (a.page_tokens - 1))) * a.head_dim;
+  };
+  auto fetch = [&](const int8_t* codes, u32x2 at) {
+    const uint64_t low = __builtin_amdgcn_readfirstlane(at[0]), high = __builtin_amdgcn_readfirstlane(at[1]);
+    return *reinterpret_cast<const u32x4*>(codes + (high << 32 | low) + piece_at);
+  };
+  auto k_place = [](int s) { return DP == 64 ? 2 * s : s & 7; };
+  auto v_place = [](int key) { return DP == 64 ? key & 2 : 2 * (key & 3); };
+  // the wave's n-th pieces of a step begin at key (n NW + wave) KW: in tile n NW KW / 32, or either
+  const int second = NW * KW == 64 ? wave * KW >> 5 : 0;
+  const int mine = (wave * KW & 31) + lane / CPK;  // of a tile's keys, before n's
+  auto put = [&](uint8_t* at, int gap, const u32x4& r, uint32_t turn) {
+    const f16x2 times = __builtin_bit_cast(f16x2, turn), bias = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+    const f16x2 plus = times * bias;
+    *reinterpret_cast<u32x4*>(at) = codes_to_f16(r[0], r[1], times, plus);
+    *reinterpret_cast<u32x4*>(at + gap) = codes_to_f16(r[2], r[3], times, plus);
+  };
+  // odd: of the step
+  auto put_k = [&](int n, int odd, uint32_t turn, const u32x4& r) {
+    const int tile = (2 * odd + 1 + n * NW * KW / 32 + second) & 3, key = mine + (n * NW * KW & 31);
+    put(s_k + (tile * NF + piece) * 1024 + 16 * (key ^ k_place(piece)), 512, r, turn);
+  };
+  auto put_v = [&](int n, int odd, uint32_t turn, const u32x4& r) {
+    const int tile = 2 * odd + n * NW * KW / 32 + second, key = mine + (n * NW * KW & 31);
+    put(s_v + tile * kTile + key * 2 * DP + 32 * (piece ^ v_place(key)), 16, r, turn);
+  };
+  // of the wave's n-th pieces of a step: V's of tiles 2 step and 2 step + 1, K's of the tiles one later
+  auto v_key = [&](int step, int n) { return 64 * step + (n * NW + wave) * KW; };
+  auto k_key = [&](int step, int n) { return 64 * step + 32 + (n * NW + wave) * KW; };
+  u32x4 kr[CL], vr[CL], k0[CL], k1[CL], v0[CL];
+  if (steps > 0) {
+#pragma unroll
+    for (int n = 0; n < CL; ++n) {
+      auto early = [&](const int8_t* codes, int key) {
+        const int group = group_of(key);
+        const uint64_t at = place_of(listed_page(group), group);
+        return fetch(codes, u32x2{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32)});
+      };
+      k0[n] = early(a.k_codes, k_key(-1, n));
+      k1[n] = early(a.k_codes, k_key(0, n));
+      v0[n] = early(a.v_codes, v_key(0, n));
+      vr[n] = early(a.v_codes, v_key(1, n));
+      kr[n] = early(a.k_codes, k_key(1, n));
+    }
+  }
+
+  // the range's pages and scales
+  constexpr float kLow = -3.0e38f;                // below every score
+  constexpr float kShift = NQ == 2 ? 15.f : 11.f, kSlack = 15.f - kShift;
+  float* const cs = reinterpret_cast<float*>(s_c);
+  float* const bs = reinterpret_cast<float*>(s_b);
+  float unit = 0.f;
+  bool bad = false;
+  for (int i = threadIdx.x; i < 4 * steps; i += 64 * NW) {
+    const int page = listed_page(i);
+    float sk = -1.f, sv = 0.f;
+    bool ok = false;
+    if (static_cast<unsigned>(page) < static_cast<unsigned>(a.pages)) {
+      const long long head = static_cast<long long>(page) * a.kv_heads + kvh;
+      sk = a.k_scales[head];
+      sv = a.v_scales[head];
+      ok = isfinite(sk) && isfinite(sv);
+    }
+    if (!ok && from + 16 * i < to && from + 16 * i + 15 >= lo) {
+      *a.status = QC_INVALID_ARGUMENT;
+      bad = true;
+    }
+    const uint64_t at = place_of(page, i);
+    s_at[i] = u32x2{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32)};
+    s_times[i] = u32x2{ok && sk < 0.f ? 0xBC00BC00u : 0x3C003C00u, ok && sv < 0.f ? 0xBC00BC00u : ok && sv == 0.f ? 0u : 0x3C003C00u};
+    cs[i] = ok ? fabsf(sk) : -1.f;                // marks keys without a page
+    bs[i] = ok ? fabsf(sv) : 0.f;
+    unit = fmaxf(unit, bs[i]);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) unit = fmaxf(unit, __shfl_xor(unit, o));
+  bad = __any(bad);
+  if (lane == 0) {
+    s_unit[wave] = unit;
+    s_bad[wave] = bad;
+  }
+
+  // q: row lane & 31, dimensions 16 s + 8 half + j
+  f16x8 qf[NF][NQ];
+  const int r = r0 + 32 * wave + (lane & 31);
+  const bool has = r < r1;
+  const int token = (has ? r : r0) / p.group, head = kvh * p.group + (has ? r : r0) - token * p.group;
+  const int row_lo = tree_low(a, p, u, token);
+  const uint32_t* row_mask = p.mask + static_cast<long long>(u.first + token) * p.words;
+  float factor, broken;
+  row_fragments<NF, NQ, TYPE>(a, p, (u.first + token) * p.q_stride + static_cast<long long>(head) * a.head_dim, has, half,
+                              qf, factor, broken);
+  int all_lo = row_lo;                            // keys every row of the wave sees
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) all_lo = max(all_lo, __shfl_xor(all_lo, o));
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  const int all_hi = __builtin_amdgcn_readfirstlane(u.position(0));
+  __syncthreads();
+  int any_bad = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    unit = fmaxf(unit, s_unit[w]);
+    any_bad |= s_bad[w];
+  }
+  any_bad = __builtin_amdgcn_readfirstlane(any_bad);
+  for (int i = threadIdx.x; i < 4 * steps; i += 64 * NW) {
+    // a scale of 0 has codes of 0, so any b will do for it
+    const float b = kShift + (bs[i] > 0.f ? fmaxf(__log2f(bs[i] / unit), -100.f) : 0.f);
+    bs[i] = b;
+    reinterpret_cast<float*>(s_inv)[i] = __builtin_amdgcn_exp2f(-b);
+  }
+  if (steps > 0) {
+#pragma unroll
+    for (int n = 0; n < CL; ++n) {
+      put_k(n, 1, s_times[group_of(k_key(-1, n))][0], k0[n]);
+      put_k(n, 0, s_times[group_of(k_key(0, n))][0], k1[n]);
+      put_v(n, 0, s_times[group_of(v_key(0, n))][1], v0[n]);
+    }
+  }
+  // Piece j of a step's 2 CL, V's and K's in turn: its codes of the next step go to LDS, those a step later on their
+  // way; ahead: what that takes, read before.
+  auto read_ahead = [&](int step, int j, u32x2& at, uint32_t& turn) {
+    const int key = j % 2 == 0 ? v_key(step + 1, j / 2) : k_key(step + 1, j / 2);
+    at = s_at[group_of(key + 64)];
+    turn = s_times[group_of(key)][j % 2 == 0 ? 1 : 0];
+  };
+  auto turn_codes = [&](int odd, int j, u32x2 at, uint32_t turn) {
+    if (j % 2 == 0) {
+      put_v(j / 2, !odd, turn, vr[j / 2]);
+      vr[j / 2] = fetch(a.v_codes, at);
+    } else {
+      put_k(j / 2, !odd, turn, kr[j / 2]);
+      kr[j / 2] = fetch(a.k_codes, at);
+    }
+  };
+  __syncthreads();
+  if (DP < 256 && r0 + 32 * wave >= r1) {         // a wave without rows only turns codes
+    for (int step = 0; step < steps; ++step) {
+      u32x2 at[2 * CL];
+      uint32_t turn[2 * CL];
+#pragma unroll
+      for (int j = 0; j < 2 * CL; ++j) read_ahead(step, j, at[j], turn[j]);
+      ring_sync();
+#pragma unroll
+      for (int j = 0; j < 2 * CL; ++j) turn_codes(step & 1, j, at[j], turn[j]);
+    }
+    return;
+  }
+
+  float m = kLow, l = 0.f;
+  f32x16 acc[DT], s, sn;
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const int d = 32 * t + 2 * e + 4 * half;
-      if (d >= a.head_dim) continue;
-      float v[4];
+    for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
+  // half i of the dimensions of a ring's tile
+  auto load_k = [&](int slot, int i, f16x8 (&k)[NF / 2]) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = l == 0.f ? 0.f : ldexpf(acc[t][e + j] * scale, unit_e);
-      if (last)
-        store_n<TYPE, 4>(p.out, (u.first + token) * p.out_stride + static_cast<long long>(head) * a.head_dim + d,
-                         p.vec, v);
-      else
-        store_n<QC_STORAGE_F32, 4>(p.part, part * a.head_dim + d, true, v);
+    for (int d = 0; d < NF / 2; ++d) {
+      const int f = i * (NF / 2) + d;
+      k[d] = *reinterpret_cast<const f16x8*>(s_k + slot * kTile + f * 1024 + 512 * half + 16 * ((lane & 31) ^ k_place(f)));
     }
+  };
+  auto scores = [&](const f16x8 (&k)[NF / 2], int i, f32x16& o) {
+    if (i == 0) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] = 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < NF / 2; ++d)
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) o = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[d], qf[i * (NF / 2) + d][q], o, 0, 0, 0);
+  };
+  // keys 16 i + 8 (j >> 2) + 4 half + (j & 3) of a ring's tile
+  const int v_key4 = 4 * half + (lane >> 2 & 3);
+  const int v_lane = v_key4 * 2 * DP + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
+  auto load_v = [&](int slot, int i, f16x8 (&v)[DT]) {
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      const uint8_t* at = s_v + slot * kTile + 32 * i * DP + v_lane + 32 * ((2 * t) ^ v_place(v_key4));
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(at));
+      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(at + 16 * DP));
+      v[t] = __builtin_bit_cast(f16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
+  auto pin = [] {
+    if constexpr (NQ == 1) __builtin_amdgcn_sched_barrier(0);
+  };
+  if (steps > 0) {
+    f16x8 kq[NF / 2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      load_k(0, i, kq);
+      scores(kq, i, s);
+    }
+  }
+
+  // s: the tile's scores; sn: receives the next one's; slot: the tile's in the rings
+  auto run = [&](int tile, auto slot_of, f32x16& s, f32x16& sn) {
+    constexpr int slot = decltype(slot_of)::value, next = (slot + 1) & 3;
+    const int tok = from + 32 * tile, step = tile >> 1;
+    if (slot % 2 == 0) ring_sync();               // the step's codes are there, the step before's free
+    f16x8 kq[NF / 2], vq[DT];
+    constexpr int first = slot % 2 * CL;          // the tile's pieces
+    u32x2 at[CL];
+    uint32_t turn[CL];
+    f32x2 c = s_c[tile];
+    const f32x2 b = s_b[tile], inv = s_inv[tile];
+    load_k(next, 0, kq);
+#pragma unroll
+    for (int j = 0; j < CL; ++j) read_ahead(step, first + j, at[j], turn[j]);
+    pin();
+    if (any_bad || tok < all_lo || tok + 32 > all_hi) {
+      // bit o: key tok + o is seen
+      uint32_t seen = tree_bits(p, row_mask, tok - all_hi) | (below(all_hi - tok) & ~below(row_lo - tok));
+      seen &= below(u.kv - tok) & ((c[0] < 0.f ? 0u : 0xFFFFu) | (c[1] < 0.f ? 0u : 0xFFFF0000u));
+      seen >>= 4 * half;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if ((seen & 1u << (8 * (e >> 2) + (e & 3))) == 0) s[e] = -INFINITY;
+    }
+    float top = kLow;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      c[i] = fmaxf(c[i] * factor, 1e-37f);        // above 0: masked scores stay -inf
+      const int o = 8 * i;
+      top = fmaxf(top, c[i] * max3(max3(s[o], s[o + 1], s[o + 2]), max3(s[o + 3], s[o + 4], s[o + 5]),
+                                   max3(s[o + 6], s[o + 7], s[o + 7])));
+    }
+    {
+      auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    }
+    if (__any(top > m + kSlack)) {
+      const float mn = fmaxf(m, top);
+      const float alpha = __builtin_amdgcn_exp2f(m - mn);
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[t][e] *= alpha;
+      m = mn;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      load_v(slot, i, vq);
+      pin();
+      scores(kq, i, sn);                          // past the last tile: of no use, and not used
+#pragma unroll
+      for (int j = 0; j < CL; ++j)
+        if (j * 2 / CL == i) turn_codes(slot / 2, first + j, at[j], turn[j]);
+      const float off = b[i] - m;
+      float e8[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e8[j] = __builtin_amdgcn_exp2f(fmaf(s[8 * i + j], c[i], off));
+      f16x8 pf[NQ];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        pf[0][j] = static_cast<_Float16>(e8[j]);
+        if constexpr (NQ == 2) pf[1][j] = static_cast<_Float16>(e8[j] - static_cast<float>(pf[0][j]));
+      }
+      const float sum = ((e8[0] + e8[1]) + (e8[2] + e8[3])) + ((e8[4] + e8[5]) + (e8[6] + e8[7]));
+      l = fmaf(sum, inv[i], l);
+      if (i == 0) load_k(next, 1, kq);
+      pin();
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vq[t], pf[q], acc[t], 0, 0, 0);
+    }
+  };
+  // (one loop left in its middle would hold the sums twice: 64 moves a tile, and spills)
+  int tile = 0;
+  for (; tile + 2 < 2 * steps; tile += 4) {
+    run(tile, std::integral_constant<int, 0>{}, s, sn);
+    run(tile + 1, std::integral_constant<int, 1>{}, sn, s);
+    run(tile + 2, std::integral_constant<int, 2>{}, s, sn);
+    run(tile + 3, std::integral_constant<int, 3>{}, sn, s);
+  }
+  if (tile < 2 * steps) {
+    run(tile, std::integral_constant<int, 0>{}, s, sn);
+    run(tile + 1, std::integral_constant<int, 1>{}, sn, s);
+  }
+  l += __shfl_xor(l, 32);
+  if (!has) return;
+  store_row<DT, NQ, TYPE>(a, p, u, token, head, split, half, acc, m, l, unit, broken);
 }
 
 // Row `item` of a join's grid: `per` rows of each row block.
@@ -1365,7 +1749,7 @@ constexpr long long kFragPass = 1LL << 30;
 struct TiledPlan {
   long long units, blocks;
 };
-TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per, int max_groups) {
+TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per, int max_groups, int least = kTiledLeast, int fill = 1) {
   const long long rows = static_cast<long long>(a.max_new) * p.group;
   p.per = per;
   p.row_blocks = static_cast<int>((rows + per - 1) / per);
@@ -1375,9 +1759,9 @@ TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per, int max_groups) {
   const long long padded = seqs * p.row_blocks, there = all / per + seqs;   // at most
   p.listed = p.rows_from > 0 || padded > there ? kBlocks : kPadded;
   const long long blocks = std::min(padded, p.listed == kBlocks ? there : padded);
-  const long long want = std::max<long long>(1, device_cu_count() / (blocks * a.kv_heads));
+  const long long want = std::max<long long>(1, static_cast<long long>(fill) * device_cu_count() / (blocks * a.kv_heads));
   long long chunk = ((span + want - 1) / want + 63) / 64 * 64;
-  chunk = std::max<long long>(chunk, kTiledLeast);
+  chunk = std::max<long long>(chunk, least);
   chunk = std::min<long long>(chunk, 16 * max_groups);
   p.chunk = static_cast<int>(chunk);
   p.splits = static_cast<int>((span + chunk - 1) / chunk);
@@ -1386,7 +1770,7 @@ TiledPlan plan_tiled(const Kv8Args& a, AttnArgs& p, int per, int max_groups) {
   return {seqs * a.kv_heads, blocks};
 }
 
-template <int DP, int NW, int TYPE, bool TREE>
+template <int DP, int NW, int TYPE>
 hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   const TiledPlan plan = plan_tiled(a, p, 32 * NW, kTiledGroups<DP>);
   const long long units = plan.units, blocks = plan.blocks;
@@ -1418,7 +1802,7 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
     attention_layout<DP><<<static_cast<unsigned>(n) * tiles, 256, 0, s>>>(a, lay, f, tiles);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     const long long grid = (p.listed == kPadded ? n * p.row_blocks : blocks * a.kv_heads) * p.splits;
-    attention_tiled<DP, NW, TYPE, TREE><<<static_cast<unsigned>(grid), 64 * NW, 0, s>>>(a, p, f);
+    attention_tiled<DP, NW, TYPE><<<static_cast<unsigned>(grid), 64 * NW, 0, s>>>(a, p, f);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   return p.splits > 1 ? run_join<TYPE>(a, p, blocks * a.kv_heads, s) : hipSuccess;
@@ -1443,7 +1827,7 @@ hipError_t run_tiled(const Kv8Args& a, AttnArgs p, hipStream_t s) {
 // not every sequence can have as many, those that have are laid out and the others
 // read directly: 4096 new tokens beside 63 sequences of one, 4000 to 8000 keys, 2317 us
 // with all laid out, 700 so (the prompt alone 460, the others 170).
-template <int DP, int TYPE, bool TREE>
+template <int DP, int TYPE>
 hipError_t run_rows(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   constexpr int NW = DP == 256 ? 4 : 8;
   const bool brief = a.max_kv <= 1024;
@@ -1459,7 +1843,7 @@ hipError_t run_rows(const Kv8Args& a, AttnArgs p, hipStream_t s) {
     tiled = 4 * groups >= (brief ? 2 : 3) * device_cu_count();
     if (tiled) p.rows_from = q.rows_from;
   }
-  if (tiled && p.rows_from == 0) return run_tiled<DP, NW, TYPE, TREE>(a, p, s);
+  if (tiled && p.rows_from == 0) return run_tiled<DP, NW, TYPE>(a, p, s);
   double keys = a.max_kv;
   if (p.causal) keys -= 0.5 * std::min(a.max_new, a.max_kv);
   if (p.window > 0) keys = std::min<double>(keys, p.window);
@@ -1471,22 +1855,74 @@ hipError_t run_rows(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   if (tiled) few.rows_to = many;
   hipError_t e = hipSuccess;
   if constexpr (DP < 256 || TYPE != QC_STORAGE_F32) {   // (two of f32 256 do not fit the registers)
-    e = two ? run_direct<DP, 2, TYPE, TREE>(a, few, s) : run_direct<DP, 1, TYPE, TREE>(a, few, s);
+    e = two ? run_direct<DP, 2, TYPE, false>(a, few, s) : run_direct<DP, 1, TYPE, false>(a, few, s);
   } else {
-    e = run_direct<DP, 1, TYPE, TREE>(a, few, s);
+    e = run_direct<DP, 1, TYPE, false>(a, few, s);
   }
-  return tiled && e == hipSuccess ? run_tiled<DP, NW, TYPE, TREE>(a, p, s) : e;
+  return tiled && e == hipSuccess ? run_tiled<DP, NW, TYPE>(a, p, s) : e;
 }
 
-template <int TYPE, bool TREE>
-hipError_t run_sized(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
-  if (a.head_dim <= 64) return run_rows<64, TYPE, TREE>(a, p, s);
-  if (a.head_dim <= 128) return run_rows<128, TYPE, TREE>(a, p, s);
-  return run_rows<256, TYPE, TREE>(a, p, s);
+template <int DP, int NW, int TYPE>
+hipError_t run_shared(const Kv8Args& a, AttnArgs p, hipStream_t s) {
+  const TiledPlan plan = plan_tiled(a, p, 32 * NW, kTreeGroups<DP, NW>, kTreeLeast, NW == 4 && DP < 256 ? 2 : 1);
+  const long long grid = plan.blocks * a.kv_heads * p.splits;
+  if (!kv8_grid_fits(grid, 64 * NW)) return hipErrorInvalidValue;
+  std::unique_lock<std::mutex> hold;
+  hipError_t e = hipSuccess;
+  if (p.splits > 1) {
+    StreamWorkspace* ws = nullptr;
+    if ((e = stream_workspace(s, &ws)) != hipSuccess) return e;
+    hold = std::unique_lock<std::mutex>(ws->call);
+    if ((e = part_buffers(a, p, ws, s)) != hipSuccess) return e;
+  }
+  attention_tree<DP, NW, TYPE><<<static_cast<unsigned>(grid), 64 * NW, 0, s>>>(a, p);
+  if ((e = hipGetLastError()) != hipSuccess || p.splits == 1) return e;
+  return run_join<TYPE>(a, p, plan.blocks * a.kv_heads, s);
+}
+
+// Trees: the direct form, of one tile of 16 rows or two by the rule above, up to a key head's 32 rows (64 of f32, or of
+// heads above 128) and for little work, where the shared form's longer start decides; then that one.  Of heads up to 128 it takes
+// 256 rows a workgroup where those are few, so that a CU's eight waves are one workgroup's, or 128, two to a CU.  us, one /
+// two / 128 rows / 256 rows, 8 key heads, sequences x rows x keys:
+//                1 x 64 x 4000      1 x 128 x 32768     16 x 128 x 4000      64 x 128 x 1000      64 x 512 x 1000
+//   bf16, 128    19 / 23 / 26 / 23  67 / 55 / 47 / 43   107 / 77 / 57 / 58   81 / 92 / 48 / 63    216 / 245 / 129 / 152
+//   f32, 128     21 / 26 / 31 / 28  80 / 66 / 65 / 55   99 / 96 / 86 / 78    100 / 109 / 73 / 83  274 / 289 / 204 / 222
+//   bf16, 64     15 / 17 / 19       48 / 42 / 33        65 / 56 / 38         52 / 56 / 33         142 / 137 / 75
+//   bf16, 256    28 / 45 / 43       105 / 111 / 81      167 / 153 / 119      167 / 227 / 132      499 / 736 / 364
+// and, bf16, 128, 1 x 32 x 32768 30 / 31 / 36 / 36, 1 x 64 x 32768 43 / 38 / 41 / 39, 8 x 256 x 1000 30 / 30 / 33 / 37.
+template <int DP, int TYPE>
+hipError_t run_tree(const Kv8Args& a, AttnArgs p, hipStream_t s) {
+  const long long rows = static_cast<long long>(a.max_new) * p.group;
+  const long long all = std::min(a.seqs * rows, static_cast<long long>(a.tokens) * p.group);
+  p.rows_to = INT_MAX;
+  double keys = a.max_kv;
+  if (p.window > 0) keys = std::min<double>(keys, p.window);
+  const double pairs = static_cast<double>(all) * a.kv_heads / 16 * keys;
+  if constexpr (DP < 256 || TYPE != QC_STORAGE_F32) {   // (of f32 256 neither two tiles nor the shared form fit the registers)
+    constexpr int few = DP == 256 || TYPE == QC_STORAGE_F32 ? 64 : 32;
+    if (p.route == 3 || (p.route == 0 && rows > few && pairs >= (keys >= 8192 ? 0x1.4p19 : 0x1.8p20))) {
+      if constexpr (DP == 128) {
+        const long long wide = (rows + 255) / 256 * a.seqs * a.kv_heads;
+        if (wide <= (rows > 128 ? 2 * device_cu_count() : device_cu_count() / 4)) return run_shared<DP, 8, TYPE>(a, p, s);
+      }
+      return run_shared<DP, 4, TYPE>(a, p, s);
+    }
+    const bool two = p.route == 0 ? rows > 16 && (DP <= 128 ? pairs >= 0x1p19 : keys >= 600 && pairs >= 0x1p20)
+                                  : p.route == 2;
+    if (two) return run_direct<DP, 2, TYPE, true>(a, p, s);
+  }
+  return run_direct<DP, 1, TYPE, true>(a, p, s);
+}
+
+template <int DP, int TYPE>
+hipError_t run_form(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
+  return p.mask != nullptr ? run_tree<DP, TYPE>(a, p, s) : run_rows<DP, TYPE>(a, p, s);
 }
 template <int TYPE>
 hipError_t run_typed(const Kv8Args& a, const AttnArgs& p, hipStream_t s) {
-  return p.mask != nullptr ? run_sized<TYPE, true>(a, p, s) : run_sized<TYPE, false>(a, p, s);
+  if (a.head_dim <= 64) return run_form<64, TYPE>(a, p, s);
+  if (a.head_dim <= 128) return run_form<128, TYPE>(a, p, s);
+  return run_form<256, TYPE>(a, p, s);
 }
 
 }  // namespace

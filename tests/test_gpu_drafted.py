@@ -355,6 +355,70 @@ def test_tree_rows_that_see_nothing(qc, dev, route, dtype, new, kv):
     _attend(qc, dev, rng, new, kv, 8, 2, 64, 16, dtype, empty=0.5)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new,kv,heads,kvh,hd,page", [
+    ([64], [20600], 32, 8, 128, 64), ([33] * 65, [401] * 64 + [33], 32, 8, 128, 16), ([40, 24, 7], [9000, 8200, 7], 32, 8, 64, 32),
+    ([70, 30], [9001, 5000], 8, 2, 256, 128)])
+def test_tree_by_size(qc, dev, dtype, new, kv, heads, kvh, hd, page):
+    """As a call of its size is worked on: one sequence's 256 rows a workgroup, 128 of many sequences', ..."""
+    print(f"tree by size {dtype} {len(new)} x {max(new)} x {max(kv)}", flush=True)
+    _attend(qc, dev, np.random.default_rng(hd), new, kv, heads, kvh, hd, page, dtype)
+
+
+@pytest.mark.parametrize("pages", ["negative", "nan", "missing"])
+def test_tree_shared_scales(qc, dev, route, pages):
+    """Scales of either sign and of zero; a page that is not there, or whose scale is not finite: its keys count for
+    nothing, and the status says so."""
+    import torch
+    rng = np.random.default_rng(17)
+    new, kv, kvh, page, hd = [40, 21], [400, 333], 2, 32, 128
+    batch = Ragged(rng, new, kv, page)
+    cache = _random_cache(qc, dev, rng, batch.pages, kvh, page, hd)
+    g = torch.Generator(device=dev).manual_seed(3)
+    for s in cache.tensors[2:]:
+        sign = torch.randint(-1, 2, s.shape, generator=g, device=dev).float()
+        s.copy_(s * torch.where(sign == 0, torch.zeros_like(sign) if s is cache.tensors[3] else torch.ones_like(sign), sign))
+    if pages == "negative":
+        _attend(qc, dev, rng, new, kv, 8, kvh, hd, page, "bfloat16", cache=cache, batch=batch)
+        return
+    lost = int(batch.table[0][2])
+    trees = [_tree(rng, n) for n in new]
+    mask = torch.from_numpy(_bits(rng, batch, trees, 2)).to(dev)
+    q = torch.from_numpy(rng.standard_normal((batch.tokens, 8, hd))).to(torch.bfloat16).to(dev)
+    b = batch.device(qc, dev)
+    if pages == "nan":
+        cache.tensors[3][lost, 1] = float("nan")
+    else:
+        b.tensors[0][0, 2] = batch.pages + 5
+    st = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = qc.kv8_tree_attention(cache, b, q, mask, dev_status=st)
+    assert st.item() == 3
+    # the same with the page's keys out of sight: a context without them
+    kc, vc, ks, vs = _host(cache)
+    for s, (n, length) in enumerate(zip(new, kv)):
+        for h in range(8):
+            j = np.arange(length)
+            pid = batch.table[s][j // page]
+            seen = np.zeros((n, length), bool)
+            seen[:, :length - n] = True
+            seen[:, length - n:] = trees[s][0]
+            if s == 0 and (pages == "missing" or h // 4 == 1):
+                seen[:, 2 * page:3 * page] = False
+            K = kc[pid, h // 4, j % page] * ks[pid, h // 4][:, None].astype(np.float64)
+            V = np.nan_to_num(vc[pid, h // 4, j % page] * vs[pid, h // 4][:, None].astype(np.float64))
+            K, V = np.nan_to_num(K), np.nan_to_num(V)
+            rows, scale = slice(batch.start[s], batch.start[s + 1]), float(np.float32(hd ** -0.5))
+            Q = q[rows, h].double().cpu().numpy()
+            z = np.where(seen, scale * (Q @ K.T), -np.inf)
+            p = np.exp(z - z.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            # as _tree_reference: what scores, probabilities, sums and the output's rounding are off by
+            size = scale * (np.abs(Q) @ np.abs(K).T).max(1, keepdims=True)
+            ds = size * ((hd + 8) * 2.0 ** -24 + 2.0 ** -40) + 2 * size * 2.0 ** -22 + size * hd * 2.0 ** -38
+            tol = p @ np.abs(V) * (2.0 ** -11 + 2 * ds + (length / 16 + 16) * 2.0 ** -23) + np.abs(V).sum() * 2.0 ** -36
+            assert np.all(np.abs(out[rows, h].double().cpu().numpy() - p @ V) <= tol + 2.0 ** -8 * 1.001 * np.abs(p @ V))
+
+
 def test_tree_wide_masks_and_strides(qc, dev, route):
     """Mask rows wider than the batch needs; q and out rows of a wider array."""
     import torch
