@@ -132,12 +132,15 @@ __device__ __forceinline__ void e4m3_terms(float (&v)[4], uint32_t scale, uint32
   }
 }
 
-// A wavefront: one expert's logits of LT tokens.  The first expert's also write x's terms.
+// A wavefront: one expert's logits of LT tokens.  The first eight experts' share the writing of x's terms (one wavefront
+// alone took 11.5 us for 17 f32 tokens of 2752).
 template <int TYPE, int RTYPE, int NX, int LT>
 __global__ __launch_bounds__(64) void moe_logits(MoeArgs a) {
   constexpr int XV = Storage<TYPE>::per16, RV = Storage<RTYPE>::per16, V = XV > RV ? XV : RV;
   const int lane = threadIdx.x, e = blockIdx.x % a.experts, t0 = blockIdx.x / a.experts * LT;
   double acc[LT][2] = {};
+  const int share = min(a.experts, 8);
+  int turn = 0;
 #pragma unroll 2
   for (int d = lane * V; d < a.dim; d += 64 * V) {
     float r[V], x[LT][V];
@@ -152,7 +155,9 @@ __global__ __launch_bounds__(64) void moe_logits(MoeArgs a) {
     for (int t = 0; t < LT; ++t)
 #pragma unroll
       for (int j = 0; j < V; ++j) acc[t][j & 1] = fma(static_cast<double>(x[t][j]), static_cast<double>(r[j]), acc[t][j & 1]);
-    if (e != 0) continue;
+    const bool mine = turn == e;
+    turn = turn + 1 < share ? turn + 1 : 0;
+    if (!mine) continue;
 #pragma unroll
     for (int t = 0; t < LT; ++t) {
       if (t0 + t >= a.tokens) break;
@@ -304,10 +309,12 @@ __global__ __launch_bounds__(1024) void moe_plan(MoeArgs a) {
   make_plan<1024>(a, n, s_wave);
 }
 
-// Both in one workgroup, for kSelect logits at most: a thread takes logits of any token.
-constexpr int kSelect = 8192;
+// Both in one workgroup: a thread takes logits of any token.  For few comparisons, tokens * experts^2: one launch of 7.6 us
+// (8 tokens, 64 experts) in place of two of 4.3 and 3.1 and the gap between; 64 tokens, 64 experts: 28 us.  Of a pass of 512
+// tokens and kCompare comparisons there are (512 kCompare)^1/2 logits at most.
+constexpr int kCompare = 1 << 16, kSelect = 6 * 1024;
+static_assert(1LL * kSelect * kSelect >= 1LL * kPass * kCompare, "room for the logits");
 __global__ __launch_bounds__(1024) void moe_select_few(MoeArgs a) {
-  typedef double f64x2 __attribute__((ext_vector_type(2)));
   __shared__ __attribute__((aligned(16))) double l[kSelect + 2];
   __shared__ double first[kPass];
   __shared__ int n[kMaxExperts], s_wave[32];
@@ -941,7 +948,7 @@ hipError_t run_pass(const MoeArgs& a, hipStream_t s) {
     moe_small_down<TYPE, NH><<<a.dim / 16, 1024, 0, s>>>(a, shift);
     return hipGetLastError();
   }
-  if (a.tokens * a.experts <= kSelect) {
+  if (static_cast<long long>(a.tokens) * a.experts * a.experts <= kCompare) {
     moe_select_few<<<1, 1024, 0, s>>>(a);
   } else {
     moe_select<<<a.tokens, 256, 0, s>>>(a);
