@@ -138,39 +138,36 @@ template <int TYPE, int RTYPE, int NX, int LT>
 __global__ __launch_bounds__(64) void moe_logits(MoeArgs a) {
   constexpr int XV = Storage<TYPE>::per16, RV = Storage<RTYPE>::per16, V = XV > RV ? XV : RV;
   const int lane = threadIdx.x, e = blockIdx.x % a.experts, t0 = blockIdx.x / a.experts * LT;
+  auto load_x = [&](int t, int d, float* x) {
+#pragma unroll
+    for (int j = 0; j < V; j += XV) load_n<TYPE>(a.x, min(t0 + t, a.tokens - 1) * a.x_stride + d + j, a.vec, x + j);
+  };
   double acc[LT][2] = {};
-  const int share = min(a.experts, 8);
-  int turn = 0;
-#pragma unroll 2
+#pragma unroll 4
   for (int d = lane * V; d < a.dim; d += 64 * V) {
     float r[V], x[LT][V];
 #pragma unroll
     for (int j = 0; j < V; j += RV) load_n<RTYPE>(a.router, static_cast<long long>(e) * a.dim + d + j, a.vec, r + j);
-#pragma unroll
-    for (int t = 0; t < LT; ++t)
-#pragma unroll
-      for (int j = 0; j < V; j += XV)
-        load_n<TYPE>(a.x, min(t0 + t, a.tokens - 1) * a.x_stride + d + j, a.vec, x[t] + j);
+    for (int t = 0; t < LT; ++t) load_x(t, d, x[t]);
 #pragma unroll
     for (int t = 0; t < LT; ++t)
 #pragma unroll
       for (int j = 0; j < V; ++j) acc[t][j & 1] = fma(static_cast<double>(x[t][j]), static_cast<double>(r[j]), acc[t][j & 1]);
-    const bool mine = turn == e;
-    turn = turn + 1 < share ? turn + 1 : 0;
-    if (!mine) continue;
+  }
+  const int share = min(a.experts, 8);
+  for (int d = (64 * e + lane) * V; e < share && d < a.dim; d += 64 * share * V) {
+    for (int t = 0; t < LT && t0 + t < a.tokens; ++t) {
+      float x[V], top = 0.f;
+      load_x(t, d, x);
 #pragma unroll
-    for (int t = 0; t < LT; ++t) {
-      if (t0 + t >= a.tokens) break;
-      float top = 0.f;
-#pragma unroll
-      for (int j = 0; j < V; ++j) top = x[t][j] == x[t][j] ? fmaxf(top, fabsf(x[t][j])) : INFINITY;
+      for (int j = 0; j < V; ++j) top = x[j] == x[j] ? fmaxf(top, fabsf(x[j])) : INFINITY;
       top = fmaxf(top, dpp_f32<0xB1>(top));                // a block: 4 lanes, or 8
       top = fmaxf(top, dpp_f32<0x4E>(top));
       if (V == 4) top = fmaxf(top, dpp_f32<0x141>(top));
       const uint32_t scale = block_scale<NX>(top);
 #pragma unroll
       for (int j = 0; j < V; j += 4) {
-        float v[4] = {x[t][j], x[t][j + 1], x[t][j + 2], x[t][j + 3]};
+        float v[4] = {x[j], x[j + 1], x[j + 2], x[j + 3]};
         uint32_t w[NX];
         e4m3_terms<NX>(v, scale, w);
 #pragma unroll
@@ -705,7 +702,7 @@ struct Chunk {
   static constexpr int Q = 2;
   static constexpr int kRow = 128 * Q;                                   // bytes of a column and term
   static constexpr int PER = CT * 16 * NX * kRow / 16 / 256;             // 16-byte pieces a thread
-  static constexpr int WAVES = CT == 1 && NX < 6 ? 3 : 2;                // a SIMD: what holds without spills
+  static constexpr int WAVES = CT * NX >= 12 ? 1 : CT == 1 && NX < 6 ? 3 : 2;   // a SIMD: what LDS, then registers hold
 };
 
 template <bool UP, int CT, int NX, int NH>
