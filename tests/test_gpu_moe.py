@@ -124,6 +124,27 @@ def test_moe_precision(qc, dev, tokens, dtype, most):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [2, 30])
+def test_moe_outliers(qc, dev, tokens, dtype):
+    """Single values far above their block's others, and blocks of very different sizes."""
+    import torch
+    layer, values = _layer(qc, dev, 6, 192, 160, 7)
+    rng = np.random.default_rng(7)
+    x = rng.standard_normal((tokens, 192)) * np.repeat(2.0 ** rng.integers(-12, 4, (tokens, 6)), 32, 1)
+    x[np.arange(tokens), rng.integers(0, 192, tokens)] *= 1000
+    x = torch.from_numpy(x).to(getattr(torch, dtype))
+    y, ids, _ = qc.mxfp4_moe(layer, x.to(dev), 2)
+    want, wid, _, tol = _reference(values, x.double().numpy(), 2, True, False, None, 1.0, HALF[dtype])
+    assert np.array_equal(ids.cpu().numpy(), wid)
+    got = y.double().cpu().numpy()
+    # f16 ends at 65504, the values that round up from 65520 on are infinite
+    past = (np.abs(want) - tol >= 65520) & (dtype == "float16")
+    near = (np.abs(want) + tol >= 65520) & (dtype == "float16")
+    ok = np.where(past | (near & np.isinf(got)), got == np.sign(want) * np.inf, np.abs(got - want) <= tol)
+    assert ok.all(), np.argwhere(~ok)[:4].tolist()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("normalize", [True, False])
 @pytest.mark.parametrize("gelu", [False, True])
 @pytest.mark.parametrize("residual,router,bias,scale", [(True, "float32", False, 1.0), (False, "bfloat16", True, 2.5),
