@@ -1883,13 +1883,15 @@ hipError_t run_shared(const Kv8Args& a, AttnArgs p, hipStream_t s) {
 // Trees: the direct form, of one tile of 16 rows or two by the rule above, up to a key head's 32 rows (64 of f32, or of
 // heads above 128) and for little work, where the shared form's longer start decides; then that one.  Of heads up to 128 it takes
 // 256 rows a workgroup where those are few, so that a CU's eight waves are one workgroup's, or 128, two to a CU.  us, one /
-// two / 128 rows / 256 rows, 8 key heads, sequences x rows x keys:
+// two / 128 rows / 256 rows, 8 key heads, sequences x rows x keys, rows and keys being the longest sequence's of lengths from
+// a quarter of that on:
 //                1 x 64 x 4000      1 x 128 x 32768     16 x 128 x 4000      64 x 128 x 1000      64 x 512 x 1000
 //   bf16, 128    19 / 23 / 26 / 23  67 / 55 / 47 / 43   107 / 77 / 57 / 58   81 / 92 / 48 / 63    216 / 245 / 129 / 152
 //   f32, 128     21 / 26 / 31 / 28  80 / 66 / 65 / 55   99 / 96 / 86 / 78    100 / 109 / 73 / 83  274 / 289 / 204 / 222
 //   bf16, 64     15 / 17 / 19       48 / 42 / 33        65 / 56 / 38         52 / 56 / 33         142 / 137 / 75
 //   bf16, 256    28 / 45 / 43       105 / 111 / 81      167 / 153 / 119      167 / 227 / 132      499 / 736 / 364
-// and, bf16, 128, 1 x 32 x 32768 30 / 31 / 36 / 36, 1 x 64 x 32768 43 / 38 / 41 / 39, 8 x 256 x 1000 30 / 30 / 33 / 37.
+// and, bf16, 128, 1 x 32 x 32768 30 / 31 / 36 / 36, 1 x 64 x 32768 43 / 38 / 41 / 39, 8 x 256 x 1000 30 / 30 / 33 / 37,
+// 8 x 256 x 2000 - / 47 / - / 39.
 template <int DP, int TYPE>
 hipError_t run_tree(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   const long long rows = static_cast<long long>(a.max_new) * p.group;
@@ -1900,7 +1902,8 @@ hipError_t run_tree(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   const double pairs = static_cast<double>(all) * a.kv_heads / 16 * keys;
   if constexpr (DP < 256 || TYPE != QC_STORAGE_F32) {   // (of f32 256 neither two tiles nor the shared form fit the registers)
     constexpr int few = DP == 256 || TYPE == QC_STORAGE_F32 ? 64 : 32;
-    if (p.route == 3 || (p.route == 0 && rows > few && pairs >= (keys >= 8192 ? 0x1.4p19 : 0x1.8p20))) {
+    constexpr double least = TYPE == QC_STORAGE_F32 ? 0x1.8p20 : 0x1p20;
+    if (p.route == 3 || (p.route == 0 && rows > few && pairs >= (keys >= 8192 ? 0x1.4p19 : least))) {
       if constexpr (DP == 128) {
         const long long wide = (rows + 255) / 256 * a.seqs * a.kv_heads;
         if (wide <= (rows > 128 ? 2 * device_cu_count() : device_cu_count() / 4)) return run_shared<DP, 8, TYPE>(a, p, s);
