@@ -33,7 +33,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kPass = 512;              // tokens of a pass
 constexpr int kMaxExperts = 1024;       // (and 64 of a token)
-constexpr int kSmall = 16;              // pairs of a token and an expert that are worked on one by one
+constexpr int kSmall = 16;              // pairs of a token and an expert that are worked on one by one (see pair_by_pair)
 
 struct MoeArgs {
   const void* router;
@@ -609,6 +609,8 @@ __global__ __launch_bounds__(256) void moe_small_up(MoeArgs a, int tiles) {
 // Outputs: workgroup 16 rows of all pairs' experts, its sixteen waves shared among the pairs; the sums over K and
 // over the pairs of a token in order.
 constexpr int kDownLds = 49152;      // bytes of the hidden values in LDS
+// Whether a pass is worked on pair by pair: not where rows are so long that this launch's work-items, 64 of dim, pass 32 bits.
+bool pair_by_pair(long long pairs, long long dim) { return pairs <= kSmall && dim / 16 <= static_cast<long long>(UINT32_MAX) / 1024; }
 template <int TYPE, int NH>
 __global__ __launch_bounds__(1024) void moe_small_down(MoeArgs a, int shift) {   // 2^shift waves a pair
   typedef typename Storage<TYPE>::raw raw;
@@ -938,7 +940,7 @@ hipError_t run_pass(const MoeArgs& a, hipStream_t s) {
   hipError_t e = many ? run_logits<TYPE, NX, 4>(a, s) : run_logits<TYPE, NX, 1>(a, s);
   if (e != hipSuccess) return e;
   const int pairs = a.tokens * a.top, hits = std::min(a.experts, pairs);
-  if (pairs <= kSmall) {
+  if (pair_by_pair(pairs, a.dim)) {
     const int tiles = a.inter / 32;
     moe_small_up<NX, NH><<<static_cast<unsigned>(pairs) * tiles, 256, 0, s>>>(a, tiles);
     if ((e = hipGetLastError()) != hipSuccess) return e;
@@ -999,7 +1001,7 @@ hipError_t launch_mxfp4_moe(const Moe& m, hipStream_t s) {
   const auto whole = [](long long n) { return (n + 255) / 256 * 256; };
   const long long parts[7] = {whole(t * a.experts * 8), whole(nx * t * a.dim), whole(t * scale_row(a.dim)),
                               whole(nh * pairs * a.inter), whole(pairs * scale_row(a.inter)),
-                              pairs > kSmall ? whole(a.parts * pairs * a.dim * 4) : 0, whole((2 + 2 * a.experts + pairs) * 4)};
+                              pair_by_pair(pairs, a.dim) ? 0 : whole(a.parts * pairs * a.dim * 4), whole((2 + 2 * a.experts + pairs) * 4)};
   long long bytes = 0;
   for (long long n : parts) bytes += n;
   StreamWorkspace* ws = nullptr;

@@ -457,3 +457,40 @@ def test_a_verification_step(qc, dev, captured):
                 assert float((got - want).abs().max()) <= 0.5 * (rep + 3) * float(scale.max())
             assert bool(torch.isfinite(out).all())
     assert st.item() == 0
+
+
+def test_moe_longest_rows(qc, dev):
+    """Rows of 2^26 values through one expert: 64 work-items of the pair form's last launch a value would pass 32 bits.
+    x is zero but for twelve blocks, so that the sums are those of 384 values."""
+    import torch
+    dim, inter, blocks = 1 << 26, 32, 12
+    g = torch.Generator(device=dev)
+    g.manual_seed(26)
+    rng = np.random.default_rng(26)
+    at = np.unique(np.concatenate([[0, 1, dim // 32 - 1, dim // 64], rng.choice(dim // 32, blocks - 4, replace=False)]))
+    columns = torch.from_numpy((32 * at[:, None] + np.arange(32)).ravel()).to(dev)
+    guc = torch.randint(0, 256, (1, 2 * inter, dim // 2), generator=g, device=dev, dtype=torch.uint8)
+    gus = torch.full((1, 2 * inter, dim // 32), 127 - 6, dtype=torch.uint8, device=dev)
+    dc = torch.randint(0, 256, (1, dim, inter // 2), generator=g, device=dev, dtype=torch.uint8)
+    ds = torch.full((1, dim, inter // 32), 127 - 6, dtype=torch.uint8, device=dev)
+    layer = qc.Mxfp4Moe(torch.zeros(1, dim, dtype=torch.bfloat16, device=dev), guc, gus, dc, ds)
+    short = torch.from_numpy(rng.standard_normal((1, columns.numel()))).to(torch.bfloat16)
+    x = torch.zeros(1, dim, dtype=torch.bfloat16, device=dev)
+    x[:, columns] = short.to(dev)
+    y, ids, weights = qc.mxfp4_moe(layer, x, 1)
+    assert ids.tolist() == [[0]] and weights.tolist() == [[1.0]]
+    # the columns that are not zero, and some rows of the result: its ends, its middle and what lies between
+    pick = lambda t: t[0].unflatten(1, (dim // 32, -1))[:, torch.from_numpy(at).to(dev)].flatten(1).contiguous()
+    gu = qc.dequantize_mxfp4(pick(guc), pick(gus)).double().cpu().numpy()[None]
+    rows = np.unique(np.concatenate([np.arange(512), dim // 2 + np.arange(-512, 512), dim - 512 + np.arange(512),
+                                     rng.integers(0, dim, 2048)]))
+    R = torch.from_numpy(rows).to(dev)
+    dn = qc.dequantize_mxfp4(dc[0, R].contiguous(), ds[0, R].contiguous()).double().cpu().numpy()[None]
+    values = (np.zeros((1, columns.numel())), np.zeros(1), gu, dn)
+    want, _, _, tol = _reference(values, short.double().numpy(), 1, True, False, np.zeros((1, len(rows))), 1.0, HALF["bfloat16"])
+    assert np.all(np.abs(y[:, R].double().cpu().numpy() - want) <= tol)
+    # and every row: a hidden value is at most `most`, so no sum of 32 of weights up to 6 / 64 is more
+    x64 = short.double().numpy()[0]
+    z = np.abs(gu[0]) @ np.abs(x64)
+    assert bool(torch.isfinite(y).all()) and float(y.abs().max()) <= 32 * 6 / 64 * (z[:inter] * z[inter:]).max() * 1.01
+    assert float((y == 0).float().mean()) < 0.01
