@@ -59,6 +59,8 @@ struct AttnArgs {
   const uint32_t* mask; // TREE: [tokens][words], what a row sees of its sequence's new tokens
   int words;
   const int* positions; // TREE with a window: rows' positions
+  int block0;           // shared form: the first block of a pass
+  long long pass_rows;  // rows of a pass, `per` of each block, where partial sums are theirs; 0: all tokens' and heads'
 };
 
 // How blocks are counted.  kPadded: every sequence has row_blocks of them.  kBlocks:
@@ -871,18 +873,23 @@ __device__ __forceinline__ void row_fragments(const Kv8Args& a, const AttnArgs& 
     }
 }
 
-// A row's sums to where they belong: out, or the range's partial sums and statistics.  acc[t][e]: dimension 32 t +
+// A row's place among the partial sums and statistics, range after range.
+__device__ __forceinline__ long long part_of(const Kv8Args& a, const AttnArgs& p, const Unit& u, int token, int head, int split) {
+  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
+  return static_cast<long long>(split) * a.tokens * p.heads + row;
+}
+
+// A row's sums to where they belong: out, or place place() of the partial sums and statistics.  acc[t][e]: dimension 32 t +
 // 8 (e >> 2) + 4 half + (e & 3) in units of unit 2^-shift.
-template <int DT, int NQ, int TYPE>
-__device__ __forceinline__ void store_row(const Kv8Args& a, const AttnArgs& p, const Unit& u, int token, int head, int split,
+template <int DT, int NQ, int TYPE, class Place>
+__device__ __forceinline__ void store_row(const Kv8Args& a, const AttnArgs& p, const Unit& u, int token, int head, Place&& place,
                                           int half, const f32x16 (&acc)[DT], float m, float l, float unit, float broken) {
   const bool last = p.splits == 1;
   int unit_e;                                     // its power of two comes last: no factor underflows
   const float unit_m = split_unit(unit, unit_e);
   const float back = unit_m * (NQ == 2 ? 1.0f / 32768.0f : 1.0f / 2048.0f) + broken;   // 2^-kShift
   const float scale = last ? (l == 0.f ? 0.f : back / l) : back;
-  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
-  const long long part = static_cast<long long>(split) * a.tokens * p.heads + row;
+  const long long part = place();
   if (!last) {
     if (half == 0) {
       p.stats[2 * part] = l == 0.f ? -INFINITY : m;
@@ -1168,7 +1175,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   wait_vmcnt<0>();   // no load may land in LDS that is no longer this workgroup's
   l += __shfl_xor(l, 32);
   if (!has) return;
-  store_row<DT, NQ, TYPE>(a, p, u, token, head, split, half, acc, m, l, unit, broken);
+  store_row<DT, NQ, TYPE>(a, p, u, token, head, [&] { return part_of(a, p, u, token, head, split); }, half, acc, m, l, unit,
+                          broken);
 }
 
 // ---- Trees of more rows a key head than the direct form's -----------------------
@@ -1223,13 +1231,17 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attention_tree(Kv8
   // range slowest, so that a sequence's key heads, which end alike, and its row blocks, which share keys, are neighbours
   int used;
   const int chunk = range_keys(a, p, kTreeLeast, 64, used);
-  const int blocks = gridDim.x / p.splits, split = blockIdx.x / blocks;
+  const int blocks = gridDim.x / p.splits, split = blockIdx.x / blocks, block = blockIdx.x - split * blocks;
   int seq, kvh, rb;
-  if (!block_of(a, p, blockIdx.x - split * blocks, seq, kvh, rb)) return;
+  if (!block_of(a, p, p.block0 + block, seq, kvh, rb)) return;
   Unit u;
   if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return;
   const int r0 = rb * NW * 32, r1 = min(r0 + NW * 32, u.rows * p.group);
   if (r0 >= r1) return;
+  auto part_at = [&](int row, int token, int head) {   // row: of the block
+    return p.pass_rows > 0 ? split * p.pass_rows + static_cast<long long>(block) * (32 * NW) + row
+                           : part_of(a, p, u, token, head, split);
+  };
   int lo, hi;
   seen_range<true>(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
   const int from = __builtin_amdgcn_readfirstlane((lo & ~63) + split * chunk);
@@ -1237,7 +1249,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attention_tree(Kv8
   if (from >= to && p.splits > 1) {               // a range without keys
     for (int r = r0 + threadIdx.x; r < r1; r += 64 * NW) {
       const int token = r / p.group, head = kvh * p.group + r - token * p.group;
-      float* st = p.stats + 2 * ((static_cast<long long>(split) * a.tokens + u.first + token) * p.heads + head);
+      float* st = p.stats + 2 * part_at(r - r0, token, head);
       st[0] = -INFINITY;
       st[1] = 0.f;
     }
@@ -1544,19 +1556,23 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attention_tree(Kv8
   }
   l += __shfl_xor(l, 32);
   if (!has) return;
-  store_row<DT, NQ, TYPE>(a, p, u, token, head, split, half, acc, m, l, unit, broken);
+  store_row<DT, NQ, TYPE>(a, p, u, token, head, [&] { return part_at(32 * wave + (lane & 31), token, head); }, half, acc, m,
+                          l, unit, broken);
 }
 
-// Row `item` of a join's grid: `per` rows of each row block.
+// Row `item` of a join's grid: `per` rows of each row block; row: its place among a range's partial sums, of `rows`.
 __device__ __forceinline__ bool join_row(const Kv8Args& a, const AttnArgs& p, int item, int per, Unit& u, int& token,
-                                         int& head) {
+                                         int& head, long long& row, long long& rows) {
   int seq, kvh, rb;
-  if (!block_of(a, p, item / per, seq, kvh, rb) || seq >= a.seqs) return false;
+  const int block = item / per, at = item - block * per;
+  if (!block_of(a, p, p.block0 + block, seq, kvh, rb) || seq >= a.seqs) return false;
   if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return false;
-  const int r = rb * p.per + item % per, all = u.rows * p.group;
+  const int r = rb * p.per + at, all = u.rows * p.group;
   if (r >= all || all < p.rows_from || all >= p.rows_to) return false;
   token = r / p.group;
   head = kvh * p.group + r - token * p.group;
+  row = p.pass_rows > 0 ? static_cast<long long>(block) * p.per + at : part_of(a, p, u, token, head, 0);
+  rows = p.pass_rows > 0 ? p.pass_rows : static_cast<long long>(a.tokens) * p.heads;
   return true;
 }
 
@@ -1572,9 +1588,8 @@ __global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p, int
   const int tid = threadIdx.x;
   Unit u;
   int token, head;
-  if (!join_row(a, p, blockIdx.x, per, u, token, head)) return;
-  const long long rows = static_cast<long long>(a.tokens) * p.heads;
-  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
+  long long row, rows;
+  if (!join_row(a, p, blockIdx.x, per, u, token, head, row, rows)) return;
   const float* stats = p.stats + 2 * row;
   float m = -INFINITY;
   for (int s = tid; s < p.splits; s += 256) m = fmaxf(m, stats[2 * s * rows]);
@@ -1635,9 +1650,9 @@ __global__ __launch_bounds__(256) void attention_join_few(Kv8Args a, AttnArgs p,
   Unit u;
   int token, head;
   // (a wavefront's rows, 16 at most, are one block's where blocks are listed)
-  if (!join_row(a, p, blockIdx.x * (256 >> shift) + (threadIdx.x >> shift), per, u, token, head) || d >= a.head_dim) return;
-  const long long rows = static_cast<long long>(a.tokens) * p.heads;
-  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
+  long long row, rows;
+  if (!join_row(a, p, blockIdx.x * (256 >> shift) + (threadIdx.x >> shift), per, u, token, head, row, rows) || d >= a.head_dim)
+    return;
   float ms[kFewSplits], ls[kFewSplits], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) {
@@ -1671,7 +1686,7 @@ __global__ __launch_bounds__(256) void attention_join_few(Kv8Args a, AttnArgs p,
 
 // A call's partial sums where its keys are split.
 hipError_t part_buffers(const Kv8Args& a, AttnArgs& p, StreamWorkspace* ws, hipStream_t s) {
-  const size_t outs = static_cast<size_t>(p.splits) * a.tokens * p.heads;
+  const size_t outs = p.splits * (p.pass_rows > 0 ? static_cast<size_t>(p.pass_rows) : static_cast<size_t>(a.tokens) * p.heads);
   void* buf = nullptr;
   const hipError_t e = stream_buffer(ws, s, outs * (a.head_dim + 2) * sizeof(float), 0, &buf);
   p.part = static_cast<float*>(buf);
@@ -1741,8 +1756,9 @@ hipError_t run_direct(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   return run_join<TYPE>(a, p, units, s);
 }
 
-// Bytes of fragments laid out at a time; a call with more goes in passes of whole units.
-constexpr long long kFragPass = 1LL << 30;
+// Bytes of fragments laid out at a time, and of a tree's partial sums; a call with more goes in passes of whole units, or
+// blocks.
+constexpr long long kFragPass = 1LL << 30, kPartPass = 1LL << 30;
 
 // The tiled form's grid for sequences of p.rows_from rows or more: units laid out at most, row
 // blocks of a key head, ranges of keys.
@@ -1865,8 +1881,18 @@ hipError_t run_rows(const Kv8Args& a, AttnArgs p, hipStream_t s) {
 template <int DP, int NW, int TYPE>
 hipError_t run_shared(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   const TiledPlan plan = plan_tiled(a, p, 32 * NW, kTreeGroups<DP, NW>, kTreeLeast, NW == 4 && DP < 256 ? 2 : 1);
-  const long long grid = plan.blocks * a.kv_heads * p.splits;
-  if (!kv8_grid_fits(grid, 64 * NW)) return hipErrorInvalidValue;
+  const long long blocks = plan.blocks * a.kv_heads;
+  if (blocks > INT_MAX) return hipErrorInvalidValue;
+  // LDS ends a range however many rows there are: partial sums of more than 1 GB go in passes of blocks, which still fill
+  // the chip (64 sequences of 128 tokens, 64 / 8 heads of 128, a bound of 131072 keys: 4.4 GB in one, 1.0 so; of 16000 keys 6.5 ms
+  // in one, 6.1 so, of 1000 1.54 and 1.57, the most that was lost 11%: 16 sequences of 1000 under 2^20)
+  const long long row_bytes = static_cast<long long>(p.splits) * (a.head_dim + 2) * sizeof(float);
+  long long pass = blocks;
+  if (p.splits > 1 && row_bytes * a.tokens * p.heads > kPartPass) {
+    pass = std::min(blocks, std::max<long long>(1, kPartPass / (row_bytes * p.per)));
+    p.pass_rows = pass * p.per;
+  }
+  if (!kv8_grid_fits(pass * p.splits, 64 * NW)) return hipErrorInvalidValue;
   std::unique_lock<std::mutex> hold;
   hipError_t e = hipSuccess;
   if (p.splits > 1) {
@@ -1875,9 +1901,14 @@ hipError_t run_shared(const Kv8Args& a, AttnArgs p, hipStream_t s) {
     hold = std::unique_lock<std::mutex>(ws->call);
     if ((e = part_buffers(a, p, ws, s)) != hipSuccess) return e;
   }
-  attention_tree<DP, NW, TYPE><<<static_cast<unsigned>(grid), 64 * NW, 0, s>>>(a, p);
-  if ((e = hipGetLastError()) != hipSuccess || p.splits == 1) return e;
-  return run_join<TYPE>(a, p, plan.blocks * a.kv_heads, s);
+  for (long long b0 = 0; b0 < blocks; b0 += pass) {
+    const long long n = std::min(pass, blocks - b0);
+    p.block0 = static_cast<int>(b0);
+    attention_tree<DP, NW, TYPE><<<static_cast<unsigned>(n * p.splits), 64 * NW, 0, s>>>(a, p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (p.splits > 1 && (e = run_join<TYPE>(a, p, n, s)) != hipSuccess) return e;
+  }
+  return e;
 }
 
 // Trees: the direct form, of one tile of 16 rows or two by the rule above, up to a key head's 32 rows (64 of f32, or of

@@ -782,3 +782,34 @@ def test_keep_graph(qc, dev):
             assert out.tolist() == want
             _same_kept(cache, host, batch, want)
     assert st.item() == 0
+
+
+@pytest.mark.parametrize("dtype,hd,seqs,bound,most,longest", [
+    ("bfloat16", 64, 64, 1 << 17, 128, 20000), ("float32", 64, 64, 1 << 17, 128, 9000),
+    ("float16", 128, 16, 1 << 20, 128, 40000), ("bfloat16", 128, 70, 1 << 17, 60, 17000),
+    ("bfloat16", 256, 4, 1 << 20, 128, 20000)])
+def test_tree_partial_sums_of_a_loose_bound(qc, dev, dtype, hd, seqs, bound, most, longest):
+    """Partial sums that would pass 1 GB go in passes: the scratch of many rows under a bound far above the lengths
+    stays near that, and results are what they were."""
+    import torch
+    print(f"tree under {bound} keys, {seqs} x {most}, {dtype} heads of {hd}", flush=True)
+    rng = np.random.default_rng(hd + seqs)
+    new = [most] + rng.integers(1, 40, seqs - 1).tolist()
+    new[seqs // 2], new[seqs - 2] = 10, 0
+    kv = [n + int(k) for n, k in zip(new, rng.integers(0, 150, seqs))]
+    kv[seqs // 2] = longest
+    batch = Ragged(rng, new, kv, 256, spare=seqs * most - sum(new), columns=bound // 256)
+    batch.max_kv = bound
+    cache = _random_cache(qc, dev, rng, batch.pages, 8, 256, hd)
+    q = torch.from_numpy(rng.standard_normal((batch.tokens, 64, hd)).astype(np.float32)).to(getattr(torch, dtype)).to(dev)
+    out, b = torch.zeros_like(q), batch.device(qc, dev)
+    mask = torch.zeros(batch.tokens, -(-most // 32), dtype=torch.int32, device=dev)
+    st = torch.zeros(1, dtype=torch.int32, device=dev)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        before = torch.cuda.mem_get_info()[0]
+        qc.kv8_tree_attention(cache, b, q, mask, out=out, dev_status=st)
+        stream.synchronize()
+        assert before - torch.cuda.mem_get_info()[0] <= 1.05 * (1 << 30) and st.item() == 0
+        _attend(qc, dev, rng, new, kv, 64, 8, hd, 256, dtype, spare=batch.tokens - sum(new), cache=cache, batch=batch, q=q.cpu())
