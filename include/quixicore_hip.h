@@ -542,7 +542,7 @@ int qc_hip_mxfp4_gemm(const uint8_t* w_codes, const uint8_t* w_scales, const uin
                       long long k, void* stream);
 
 /* A mixture-of-experts feed-forward with MXFP4 weights, for a few tokens (more than 512 go in passes of
- * 512, each of which reads the weights).  gate_up [experts][2 * inter][dim]: an expert's gate rows, then its up
+ * 512, or of fewer where rows are very long, each of which reads the weights).  gate_up [experts][2 * inter][dim]: an expert's gate rows, then its up
  * rows; down [experts][dim][inter]; router [experts][dim] of router_type, router_bias f32 [experts] or NULL.  dim and
  * inter are multiples of 32, codes 16-byte aligned, experts at most 1024, experts * dim and experts * inter at
  * most 2^27. */

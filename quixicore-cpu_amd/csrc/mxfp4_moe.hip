@@ -993,7 +993,9 @@ hipError_t launch_mxfp4_moe(const Moe& m, hipStream_t s) {
   const int nh = m.type == QC_STORAGE_F32 ? 6 : m.type == QC_STORAGE_F16 ? 4 : 3;
   // tokens of a pass: so that offsets into its terms fit 32 bits, and a grid over pairs and 32 rows of inter 2^32 threads
   const long long term_bytes = std::max<long long>(nx * l.dim, nh * static_cast<long long>(a.top) * l.inter);
-  const long long pass = std::max<long long>(1, std::min<long long>({kPass, (1LL << 32) / term_bytes - 1, (1LL << 28) / (a.top * l.inter)}));
+  // (and so that the pairs' outputs, whose parts are one where rows are long, take 1 GB)
+  const long long pass = std::max<long long>(1, std::min<long long>({kPass, (1LL << 32) / term_bytes - 1, (1LL << 28) / (a.top * l.inter),
+                                                                    (1LL << 28) / (a.top * l.dim)}));
   const long long t = std::min(m.tokens, pass), pairs = t * a.top;
   // parts of K in the second product: workgroups for the chip twice, steps enough for each
   const long long down = std::min<long long>(a.experts, pairs) * ((a.dim + 255) / 256);

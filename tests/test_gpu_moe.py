@@ -459,38 +459,56 @@ def test_a_verification_step(qc, dev, captured):
     assert st.item() == 0
 
 
-def test_moe_longest_rows(qc, dev):
-    """Rows of 2^26 values through one expert: 64 work-items of the pair form's last launch a value would pass 32 bits.
-    x is zero but for twelve blocks, so that the sums are those of 384 values."""
+
+def _long_rows(qc, dev, tokens, experts, top, dim, inter=32, blocks=12):
+    """A layer of long rows, run and compared at its result's ends, middle and some rows between: x is zero but for
+    some blocks, so that the sums are those of 32 * blocks values.  (layer, x, y)"""
     import torch
-    dim, inter, blocks = 1 << 26, 32, 12
     g = torch.Generator(device=dev)
     g.manual_seed(26)
     rng = np.random.default_rng(26)
     at = np.unique(np.concatenate([[0, 1, dim // 32 - 1, dim // 64], rng.choice(dim // 32, blocks - 4, replace=False)]))
-    columns = torch.from_numpy((32 * at[:, None] + np.arange(32)).ravel()).to(dev)
-    guc = torch.randint(0, 256, (1, 2 * inter, dim // 2), generator=g, device=dev, dtype=torch.uint8)
-    gus = torch.full((1, 2 * inter, dim // 32), 127 - 6, dtype=torch.uint8, device=dev)
-    dc = torch.randint(0, 256, (1, dim, inter // 2), generator=g, device=dev, dtype=torch.uint8)
-    ds = torch.full((1, dim, inter // 32), 127 - 6, dtype=torch.uint8, device=dev)
-    layer = qc.Mxfp4Moe(torch.zeros(1, dim, dtype=torch.bfloat16, device=dev), guc, gus, dc, ds)
-    short = torch.from_numpy(rng.standard_normal((1, columns.numel()))).to(torch.bfloat16)
-    x = torch.zeros(1, dim, dtype=torch.bfloat16, device=dev)
+    A = torch.from_numpy(at).to(dev)
+    columns = (32 * A[:, None] + torch.arange(32, device=dev)).flatten()
+    codes = lambda *shape: torch.randint(0, 256, shape, generator=g, device=dev, dtype=torch.uint8)
+    guc, dc = codes(experts, 2 * inter, dim // 2), codes(experts, dim, inter // 2)
+    gus, ds = (torch.full(c.shape[:2] + (c.shape[2] // 16,), 127 - 6, dtype=torch.uint8, device=dev) for c in (guc, dc))
+    router = torch.zeros(experts, dim, dtype=torch.bfloat16, device=dev)
+    router[:, columns] = (torch.randn(experts, columns.numel(), generator=g, device=dev) / 8).to(torch.bfloat16)
+    layer = qc.Mxfp4Moe(router, guc, gus, dc, ds)
+    short = torch.from_numpy(rng.standard_normal((tokens, columns.numel()))).to(torch.bfloat16)
+    x = torch.zeros(tokens, dim, dtype=torch.bfloat16, device=dev)
     x[:, columns] = short.to(dev)
-    y, ids, weights = qc.mxfp4_moe(layer, x, 1)
-    assert ids.tolist() == [[0]] and weights.tolist() == [[1.0]]
-    # the columns that are not zero, and some rows of the result: its ends, its middle and what lies between
-    pick = lambda t: t[0].unflatten(1, (dim // 32, -1))[:, torch.from_numpy(at).to(dev)].flatten(1).contiguous()
-    gu = qc.dequantize_mxfp4(pick(guc), pick(gus)).double().cpu().numpy()[None]
+    out = torch.zeros_like(x)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        free = torch.cuda.mem_get_info()[0]
+        y, ids, weights = qc.mxfp4_moe(layer, x, top, out=out)
+        stream.synchronize()
+        scratch = free - torch.cuda.mem_get_info()[0]
     rows = np.unique(np.concatenate([np.arange(512), dim // 2 + np.arange(-512, 512), dim - 512 + np.arange(512),
                                      rng.integers(0, dim, 2048)]))
     R = torch.from_numpy(rows).to(dev)
-    dn = qc.dequantize_mxfp4(dc[0, R].contiguous(), ds[0, R].contiguous()).double().cpu().numpy()[None]
-    values = (np.zeros((1, columns.numel())), np.zeros(1), gu, dn)
-    want, _, _, tol = _reference(values, short.double().numpy(), 1, True, False, np.zeros((1, len(rows))), 1.0, HALF["bfloat16"])
-    assert np.all(np.abs(y[:, R].double().cpu().numpy() - want) <= tol)
-    # and every row: a hidden value is at most `most`, so no sum of 32 of weights up to 6 / 64 is more
-    x64 = short.double().numpy()[0]
-    z = np.abs(gu[0]) @ np.abs(x64)
-    assert bool(torch.isfinite(y).all()) and float(y.abs().max()) <= 32 * 6 / 64 * (z[:inter] * z[inter:]).max() * 1.01
-    assert float((y == 0).float().mean()) < 0.01
+    f64 = lambda c, sc: qc.dequantize_mxfp4(c.flatten(0, 1).contiguous(), sc.flatten(0, 1).contiguous()).double().cpu().numpy()
+    gu = f64(guc.unflatten(2, (dim // 32, 16))[:, :, A].flatten(2), gus[:, :, A]).reshape(experts, 2 * inter, -1)
+    dn = f64(dc[:, R], ds[:, R]).reshape(experts, len(rows), inter)
+    some = sorted({0, tokens // 3, tokens // 2, tokens - 1})
+    values = (router[:, columns].double().cpu().numpy(), np.zeros(experts), gu, dn)
+    want, wid, wp, tol = _reference(values, short[some].double().numpy(), top, True, False, np.zeros((len(some), len(rows))), 1.0,
+                                    HALF["bfloat16"])
+    assert np.array_equal(ids[some].cpu().numpy(), wid)
+    assert np.all(np.abs(weights[some].double().cpu().numpy() - wp) <= 2.0 ** -23 * np.abs(wp))
+    assert np.all(np.abs(y[some][:, R].double().cpu().numpy() - want) <= tol)
+    assert bool(torch.isfinite(y).all()) and float((y == 0).float().mean()) < 0.01   # every row is written
+    return scratch
+
+
+def test_moe_longest_rows(qc, dev):
+    """Rows of 2^26 values through one expert: 64 work-items of the pair form's last launch a value would pass 32 bits."""
+    _long_rows(qc, dev, 1, 1, 1, 1 << 26)
+
+
+def test_moe_scratch_of_long_rows(qc, dev):
+    """200 tokens through all of 64 experts of 2^17: their pairs' outputs would be 6.7 GB, and go in passes."""
+    assert _long_rows(qc, dev, 200, 64, 64, 1 << 17) <= 1.2 * (1 << 30)
