@@ -512,3 +512,115 @@ def test_moe_longest_rows(qc, dev):
 def test_moe_scratch_of_long_rows(qc, dev):
     """200 tokens through all of 64 experts of 2^17: their pairs' outputs would be 6.7 GB, and go in passes."""
     assert _long_rows(qc, dev, 200, 64, 64, 1 << 17) <= 1.2 * (1 << 30)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,experts,top,dim,inter", [
+    # the second product's K in two, four and eight parts, some beginning at odd steps, for one to four tiles of columns
+    (20, 2, 1, 96, 2080), (20, 2, 1, 96, 4128), (17, 1, 1, 32, 8224), (40, 2, 1, 64, 3104), (70, 2, 1, 288, 2080),
+    # pair by pair: hidden values that LDS holds in two or more parts, with and without idle waves, ...
+    (5, 3, 3, 64, 1056), (10, 2, 1, 32, 1632), (1, 2, 1, 64, 16416), (3, 2, 2, 96, 5152),
+    # ... and x
+    (1, 2, 1, 8224, 64), (2, 3, 3, 8192 + 96, 32), (1, 4, 2, 16416, 32)])
+def test_moe_wide_experts(qc, dev, dtype, tokens, experts, top, dim, inter):
+    print(f"moe {dtype} {tokens} tokens, {top} of {experts}, {dim} x {inter}", flush=True)
+    _run(qc, dev, tokens, experts, top, dim, inter, dtype, seed=inter + tokens)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,top,inter", [(5, 3, 96), (4, 2, 2080), (40, 1, 2080)])
+def test_moe_nonfinite_tokens_alone(qc, dev, dtype, tokens, top, inter):
+    """As above of few pairs, and of K in parts: the other rows keep their bits."""
+    import torch
+    layer, x, r, y, ids, weights = _run(qc, dev, tokens, 6, top, 64, inter, dtype, seed=5)
+    X, R = x.to(dev), r.to(dev)
+    X[0, 3], X[2, 63] = float("nan"), float("-inf")
+    got, gid, gw = qc.mxfp4_moe(layer, X, top, residual=R)
+    rest = [t for t in range(tokens) if t not in (0, 2)]
+    assert torch.equal(got[rest], y[rest]) and torch.equal(gid[rest], ids[rest]) and torch.equal(gw[rest], weights[rest])
+    assert bool((~torch.isfinite(got[[0, 2]])).any(1).all())
+    assert bool(((gid >= 0) & (gid < 6)).all())
+
+
+@pytest.mark.parametrize("where", ["gate", "up", "down"])
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_moe_marked_blocks(qc, dev, tokens, where):
+    """One block's scale byte 255: NaN in the output row that holds it (down), or in whatever goes through its expert
+    (gate, up), and the same bits everywhere else."""
+    import torch
+    dim, inter, experts = 96, 64, 3
+    layer, _ = _layer(qc, dev, experts, dim, inter, seed=11)
+    x = torch.randn(tokens, dim, generator=torch.Generator(device=dev).manual_seed(3), device=dev)
+    y, ids, weights = qc.mxfp4_moe(layer, x, 1)
+    assert bool(torch.isfinite(y).all()) and len(ids.unique()) > 1
+    e = int(ids[0, 0])
+    scales = layer.tensors[5 if where == "down" else 3]
+    row = {"gate": 37, "up": inter + 37, "down": 50}[where]
+    scales[e, row, 1] = 255
+    got, gid, gw = qc.mxfp4_moe(layer, x, 1)
+    assert torch.equal(gid, ids) and torch.equal(gw, weights)
+    marked = torch.zeros_like(y, dtype=torch.bool)
+    if where == "down":
+        marked[ids[:, 0] == e, row] = True
+    else:
+        marked[ids[:, 0] == e] = True
+    assert torch.equal(torch.isnan(got), marked) and torch.equal(got[~marked], y[~marked])
+
+
+def _kept(v, n):
+    """What n terms of e4m3 hold of blocks of 32: the stated steps in f64."""
+    top = np.repeat(np.abs(v).reshape(*v.shape[:-1], -1, 32).max(-1), 32, -1)
+    scale = 2.0 ** (np.frexp(top)[1] - 8)
+    left, sum_ = v.copy(), np.zeros_like(v)
+    for i in range(n):
+        t = left / scale
+        if i < n - 1:
+            t = np.rint(t * 4) / 4
+        step = 2.0 ** np.maximum(np.frexp(t)[1] - 4, -9)     # three bits after the first
+        t = np.rint(t / step) * step * scale
+        sum_, left, scale = sum_ + t, left - t, scale / 16
+    return sum_
+
+
+def _one_value_rows(x, dtype, keep):
+    """(h, what x's and h's terms may be off by, what h's n terms hold of it) of rows with one value each."""
+    fits = {"float32": 6, "float16": 3, "bfloat16": 2}[dtype]
+    shifted = lambda v: v[:, (np.arange(v.shape[1]) + 7) % v.shape[1]]
+    tops = lambda v: np.repeat(np.abs(v).reshape(*v.shape[:-1], -1, 32).max(-1), 32, -1)
+    small = lambda v, n: 1.1 * 2.0 ** (-4 * n - 6) * tops(v)
+    h, ex = 32.0 * x * shifted(x), small(x, fits)
+    of_x = 32.0 * (ex * shifted(x) + x * shifted(ex) + ex * shifted(ex))
+    return h, of_x + 2.0 ** (-4 * keep) * h + small(h, keep)
+
+
+@pytest.mark.parametrize("dtype,terms,outlier,more", [
+    ("float32", 6, 1, 0.0), ("float32", 6, 4096, 0.1), ("float16", 4, 1, 0.08), ("float16", 4, 64, 0.0),
+    ("bfloat16", 3, 1, 0.4), ("bfloat16", 3, 256, 0.0)])
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_moe_terms(qc, dev, tokens, dtype, terms, outlier, more):
+    """The bits that x and the hidden values are held with, where no sum hides them: every row of the weights has one
+    value, act(v) = v for gates above 32, and -y as residual leaves what y's rounding lost.
+
+    n terms hold a value within 2^-4n of itself and 1.1 2^(-4n - 6) of its block's largest (x: all of its bits, but for
+    the latter); the gate's, the up's and their product's roundings, and those of six terms' sums, are 2^-24 each; y is
+    rounded once.  `more`: the share of values for which hidden values of one term fewer would be further off (0: what
+    x's terms, or f32 sums, may be off by hides it)."""
+    import torch
+    K, half = 64, HALF[dtype]
+    one = lambda value, shift: torch.from_numpy(np.float32(value * np.eye(K)[(np.arange(K) + shift) % K])).to(dev)
+    guc, gus = qc.quantize_mxfp4(torch.cat([one(32.0, 0), one(1.0, 7)]))
+    dc, ds = qc.quantize_mxfp4(one(1.0, 0))
+    layer = qc.Mxfp4Moe(torch.zeros(1, K, device=dev), guc[None], gus[None], dc[None], ds[None])
+    x = np.random.default_rng(tokens).uniform(1, 2 - 2.0 ** -8, (tokens, K))
+    x[:, [5, 40]] *= outlier
+    x = torch.from_numpy(x).to(getattr(torch, dtype))
+    want, held = _one_value_rows(x.double().numpy(), dtype, terms)
+    tol = held + 10 * 2.0 ** -24 * want
+    # the oracle's terms are within that, and one fewer are not
+    assert np.all(np.abs(_kept(want, terms) - want) <= held)
+    assert np.mean(np.abs(_kept(want, terms - 1) - want) > tol) >= more
+    y = qc.mxfp4_moe(layer, x.to(dev), 1)[0]
+    got = y.double().cpu().numpy()
+    assert np.all(np.abs(got - want) <= tol + half * want * 1.001)
+    rest = qc.mxfp4_moe(layer, x.to(dev), 1, residual=-y)[0].double().cpu().numpy()
+    assert np.all(np.abs(rest - (want - got)) <= tol + half * 1.001 * (np.abs(want - got) + tol))
