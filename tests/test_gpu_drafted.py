@@ -813,3 +813,11 @@ def test_tree_partial_sums_of_a_loose_bound(qc, dev, dtype, hd, seqs, bound, mos
         stream.synchronize()
         assert before - torch.cuda.mem_get_info()[0] <= 1.05 * (1 << 30) and st.item() == 0
         _attend(qc, dev, rng, new, kv, 64, 8, hd, 256, dtype, spare=batch.tokens - sum(new), cache=cache, batch=batch, q=q.cpu())
+
+
+@pytest.mark.parametrize("dtype,hd", [("bfloat16", 128), ("float16", 96), ("float32", 128), ("float16", 256), ("float32", 256)])
+@pytest.mark.parametrize("window", [1, 40, 300])
+def test_tree_windows_of_wide_heads(qc, dev, route, dtype, hd, window):
+    """Windows that begin in the context, at its end and before it, for the other sizes of heads."""
+    rng = np.random.default_rng(window + hd)
+    _attend(qc, dev, rng, [33, 9, 40, 1, 0], [700, 9, 300, 257, 5], 8, 2, hd, 32, dtype, window=window, spare=3, empty=0.2)
