@@ -566,7 +566,8 @@ typedef struct qc_mxfp4_moe {
  * x, y and residual (NULL: none): [tokens][dim] of `type`, rows that many elements apart; y may be residual (same
  * strides) or x.  Weights enter as they are (a block scale byte of 255: NaN), x with all its bits, the hidden values
  * with 12 (f16: 16, f32: 24); a value far below the largest, m, of its 32 is held to 2^-14 m (f16: 2^-18 m, f32: 2^-30 m).
- * Products are exact, sums f32, y is rounded once.  A token that is not finite makes its own row so, no other.
+ * Products are exact, sums f32, y is rounded once.  Experts have no biases of their own, their activation no clamp and no
+ * factor, and gate rows are not interleaved with up rows.  A token that is not finite makes its own row so, no other.
  * Status: 1 for sizes out of range (top_k above experts or 64), 2 for an unknown type, 3 for NULL or misaligned
  * pointers or a weight_scale that is not finite. */
 int qc_hip_mxfp4_moe(const qc_mxfp4_moe* layer, const void* x, long long x_stride,

@@ -31,9 +31,9 @@ __device__ __forceinline__ u32x4 turned_codes(u32x4 w, float ratio) {
   return w;
 }
 
-// A workgroup takes a sequence's keys or values of a head, page after page: the token that comes to
-// position c + a was behind it, so what a page or a later one gives is read before it is
-// written over.  CHECK: looks only.
+// A workgroup takes a sequence's keys or values of a head and moves codes in place, page after page: the token that comes to
+// position c + a was behind it, so what a page or a later one gives is read before it is written over.  (A path staged whole
+// in LDS would need no order of pages; not built.)  CHECK: looks only.
 //
 // Bound by dependent reads and barriers, a page after the other, not by its bytes: 64 sequences, up to 59 tokens of 8
 // heads of 128 over pages of 16 (5.1 MB) 12.3 us, 16 sequences of up to 3 tokens 5.1.  Path and page ids kept in LDS from the

@@ -699,7 +699,8 @@ __global__ __launch_bounds__(1024) void moe_small_down(MoeArgs a, int shift) {  
 //
 // What bounds it is what a wave has to do beside the MFMAs, as few of them fit a SIMD: a barrier and new addresses each step
 // (140 VALU instructions beside 16 MFMAs, all operands through an LDS ring) took 172 + 91 us for 64 tokens through 8 experts
-// of 4096 x 14336, a byte of scales a lane and step 207 + 131; so 140 to 146 + 73 to 75: 500 and 250 MB, 3.4 TB/s.  Codes or
+// of 4096 x 14336, a byte of scales a lane and step 207 + 131; so 140 + 73 by
+// the same clock, the first passes of a process, and 125 + 65 later: 500 and 250 MB, 4.0 and 3.8 TB/s.  Codes or
 // scales two chunks ahead change nothing (17 f32 tokens through 25 of 2752 x 1376: 37.4 us, 38.0 and 38.2).
 template <int CT, int NX>
 struct Chunk {
