@@ -504,11 +504,10 @@ int qc_hip_kv8_tree_attention(const qc_kv8_cache* cache, const qc_kv8_batch* bat
  * new_len[s] = c + kept_count[s]; kv_len stays as it is.  A page and head that receives tokens of other pages takes
  * the largest magnitude of its scale and theirs, s'; the codes held below the new ones, and those that come, become
  * clamp(rint(code * (s / s')), +-127), s the scale they had, each step rounded to f32; other pages move codes as they are.
- * Slots from the new length on hold anything.  A page written by a call must belong to one sequence; new_len overlaps
- * nothing that is read.  Errors: a count outside 0 .. min(n, kept_columns), indexes that are not ascending or below n, n
+ * Slots from the new length on hold anything.  A page written by a call must belong to one sequence.  Errors: a count outside 0 .. min(n, kept_columns), indexes that are not ascending or below n, n
  * above kv_len, a page id out of range: the sequence and its new_len are left as they were; a page that a token
  * comes from or goes to whose scale is not finite: that head's keys or values are (new_len is written).  Status: 1 for
- * sizes out of range, 3 for NULL or misaligned pointers or new_len at kv_len. */
+ * sizes out of range, 3 for NULL or misaligned pointers or new_len over kept, kept_count or the batch's arrays. */
 int qc_hip_kv8_keep(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const int* kept,
                     long long kept_columns, const int* kept_count, int* new_len, int* dev_status,
                     void* stream);

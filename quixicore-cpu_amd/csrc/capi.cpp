@@ -178,6 +178,11 @@ bool known_storage(int type) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+bool ints_overlap(const int* a, long long n, const int* b, long long m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + 4 * static_cast<uintptr_t>(m) && y < x + 4 * static_cast<uintptr_t>(n);
+}
+
 // No exception leaves a C entry.
 template <class F>
 int guarded(F&& f) {
@@ -1065,8 +1070,11 @@ int qc_hip_kv8_keep(const qc_kv8_cache* cache, const qc_kv8_batch* batch, const 
   if (cache == nullptr || batch == nullptr) return QC_INVALID_ARGUMENT;
   if (!kv8_shapes(*cache, *batch)) return QC_INVALID_SHAPE;
   if (kept_columns <= 0 || kept_columns > INT_MAX) return QC_INVALID_SHAPE;
-  if (!kv8_pointers(*cache, *batch) || kept == nullptr || kept_count == nullptr || new_len == nullptr ||
-      new_len == batch->kv_len)
+  if (!kv8_pointers(*cache, *batch) || kept == nullptr || kept_count == nullptr || new_len == nullptr)
+    return QC_INVALID_ARGUMENT;
+  const auto over = [&](const int* p, long long n) { return ints_overlap(new_len, batch->seqs, p, n); };
+  if (over(batch->kv_len, batch->seqs) || over(batch->seq_start, batch->seqs + 1) || over(kept_count, batch->seqs) ||
+      over(batch->block_table, batch->seqs * batch->columns) || over(kept, batch->seqs * kept_columns))
     return QC_INVALID_ARGUMENT;
   const hipStream_t s = as_stream(stream);
   return checked(

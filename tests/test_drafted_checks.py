@@ -107,3 +107,16 @@ def test_moe_refusals(q):  # noqa: F811
     for kw in (dict(x=None), dict(y=None), dict(ids=None), dict(weights=None), dict(scale=NAN), dict(scale=INF),
                dict(r=2 * P, rs=65), dict(x=2 * P, xs=65)):
         assert call(ref(good), **kw) == 3, kw
+
+
+def test_keep_refuses_lengths_over_what_it_reads(q):  # noqa: F811
+    """A head's workgroups read the paths, lengths and tables that another's would write new lengths over."""
+    far = {"block_table": 2 * P, "seq_start": 3 * P, "kv_len": 4 * P}     # of 3 sequences and 4 columns
+    cache, batch = _cache(q), _batch(q, **far)
+
+    def call(out):
+        return q.lib.qc_hip_kv8_keep(ref(cache), ref(batch), 5 * P, 3, 6 * P, out, P, None)
+
+    for at, size in ((2 * P, 48), (3 * P, 16), (4 * P, 12), (5 * P, 36), (6 * P, 12)):
+        for out in (at, at - 8, at + size - 4):
+            assert call(out) == 3, (at, out - at)
