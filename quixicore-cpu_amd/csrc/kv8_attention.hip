@@ -59,8 +59,13 @@ struct AttnArgs {
   const uint32_t* mask; // TREE: [tokens][words], what a row sees of its sequence's new tokens
   int words;
   const int* positions; // TREE with a window: rows' positions
-  int block0;           // shared form: the first block of a pass
-  long long pass_rows;  // rows of a pass, `per` of each block, where partial sums are theirs; 0: all tokens' and heads'
+};
+
+// Blocks of a call from `block` on, `per` rows of each having their places among the partial sums, `rows` in all.  (Kernels of
+// its own, PASS: where one kernel did both, every call with a join took 0.3 to 0.4 us more, of 10.)
+struct Pass {
+  int block;
+  long long rows;
 };
 
 // How blocks are counted.  kPadded: every sequence has row_blocks of them.  kBlocks:
@@ -873,23 +878,20 @@ __device__ __forceinline__ void row_fragments(const Kv8Args& a, const AttnArgs& 
     }
 }
 
-// A row's place among the partial sums and statistics, range after range.
-__device__ __forceinline__ long long part_of(const Kv8Args& a, const AttnArgs& p, const Unit& u, int token, int head, int split) {
-  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
-  return static_cast<long long>(split) * a.tokens * p.heads + row;
-}
-
-// A row's sums to where they belong: out, or place place() of the partial sums and statistics.  acc[t][e]: dimension 32 t +
-// 8 (e >> 2) + 4 half + (e & 3) in units of unit 2^-shift.
-template <int DT, int NQ, int TYPE, class Place>
-__device__ __forceinline__ void store_row(const Kv8Args& a, const AttnArgs& p, const Unit& u, int token, int head, Place&& place,
-                                          int half, const f32x16 (&acc)[DT], float m, float l, float unit, float broken) {
+// A row's sums to where they belong: out, or the range's partial sums and statistics (at `place`, where one is given).
+// acc[t][e]: dimension 32 t + 8 (e >> 2) + 4 half + (e & 3) in units of unit 2^-shift.
+template <int DT, int NQ, int TYPE, class... Place>
+__device__ __forceinline__ void store_row(const Kv8Args& a, const AttnArgs& p, const Unit& u, int token, int head, int split,
+                                          int half, const f32x16 (&acc)[DT], float m, float l, float unit, float broken,
+                                          Place... place) {
   const bool last = p.splits == 1;
   int unit_e;                                     // its power of two comes last: no factor underflows
   const float unit_m = split_unit(unit, unit_e);
   const float back = unit_m * (NQ == 2 ? 1.0f / 32768.0f : 1.0f / 2048.0f) + broken;   // 2^-kShift
   const float scale = last ? (l == 0.f ? 0.f : back / l) : back;
-  const long long part = place();
+  const long long row = static_cast<long long>(u.first + token) * p.heads + head;
+  long long part = static_cast<long long>(split) * a.tokens * p.heads + row;
+  ((part = place), ...);
   if (!last) {
     if (half == 0) {
       p.stats[2 * part] = l == 0.f ? -INFINITY : m;
@@ -1175,8 +1177,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void attention_tiled(Kv8Args a, At
   wait_vmcnt<0>();   // no load may land in LDS that is no longer this workgroup's
   l += __shfl_xor(l, 32);
   if (!has) return;
-  store_row<DT, NQ, TYPE>(a, p, u, token, head, [&] { return part_of(a, p, u, token, head, split); }, half, acc, m, l, unit,
-                          broken);
+  store_row<DT, NQ, TYPE>(a, p, u, token, head, split, half, acc, m, l, unit, broken);
 }
 
 // ---- Trees of more rows a key head than the direct form's -----------------------
@@ -1213,8 +1214,8 @@ template <int DP, int NW>
 constexpr int kTreeGroups = DP == 256 ? 1024 : NW == 4 ? 512 : 2048;
 constexpr int kTreeLeast = 512;     // keys of a range, where there are as many
 
-template <int DP, int NW, int TYPE>
-__global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attention_tree(Kv8Args a, AttnArgs p) {
+template <int DP, int NW, int TYPE, bool PASS>
+__global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attention_tree(Kv8Args a, AttnArgs p, Pass pass) {
   constexpr int NF = DP / 16, DT = DP / 32;
   constexpr int NQ = TYPE == QC_STORAGE_F32 ? 2 : 1;
   constexpr int kTile = 64 * DP;                  // bytes of 32 keys of K, or of V
@@ -1235,14 +1236,13 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attention_tree(Kv8
   const int chunk = range_keys(a, p, kTreeLeast, 64, used);
   const int blocks = gridDim.x / p.splits, split = blockIdx.x / blocks, block = blockIdx.x - split * blocks;
   int seq, kvh, rb;
-  if (!block_of(a, p, p.block0 + block, seq, kvh, rb)) return;
+  if (!block_of(a, p, PASS ? pass.block + block : block, seq, kvh, rb)) return;
   Unit u;
   if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return;
   const int r0 = rb * NW * 32, r1 = min(r0 + NW * 32, u.rows * p.group);
   if (r0 >= r1) return;
-  auto part_at = [&](int row, int token, int head) {   // row: of the block
-    return p.pass_rows > 0 ? split * p.pass_rows + static_cast<long long>(block) * (32 * NW) + row
-                           : part_of(a, p, u, token, head, split);
+  auto place = [&](int row) {                     // of a row of the block, PASS
+    return split * pass.rows + static_cast<long long>(block) * (32 * NW) + row;
   };
   int lo, hi;
   seen_range<true>(p, u, r0 / p.group, (r1 - 1) / p.group, lo, hi);
@@ -1251,7 +1251,7 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attention_tree(Kv8
   if (from >= to && p.splits > 1) {               // a range without keys
     for (int r = r0 + threadIdx.x; r < r1; r += 64 * NW) {
       const int token = r / p.group, head = kvh * p.group + r - token * p.group;
-      float* st = p.stats + 2 * part_at(r - r0, token, head);
+      float* st = p.stats + 2 * (PASS ? place(r - r0) : (static_cast<long long>(split) * a.tokens + u.first + token) * p.heads + head);
       st[0] = -INFINITY;
       st[1] = 0.f;
     }
@@ -1558,24 +1558,28 @@ __global__ __launch_bounds__(64 * NW, DP == 256 ? 1 : 2) void attention_tree(Kv8
   }
   l += __shfl_xor(l, 32);
   if (!has) return;
-  store_row<DT, NQ, TYPE>(a, p, u, token, head, [&] { return part_at(32 * wave + (lane & 31), token, head); }, half, acc, m,
-                          l, unit, broken);
+  if constexpr (PASS)
+    store_row<DT, NQ, TYPE>(a, p, u, token, head, split, half, acc, m, l, unit, broken, place(32 * wave + (lane & 31)));
+  else
+    store_row<DT, NQ, TYPE>(a, p, u, token, head, split, half, acc, m, l, unit, broken);
 }
 
-// Row `item` of a join's grid: `per` rows of each row block; row: its place among a range's partial sums, of `rows`.
-__device__ __forceinline__ bool join_row(const Kv8Args& a, const AttnArgs& p, int item, int per, Unit& u, int& token,
-                                         int& head, long long& row, long long& rows) {
+// Row `item` of a join's grid: `per` rows of each row block, from block0 on.
+__device__ __forceinline__ bool join_row(const Kv8Args& a, const AttnArgs& p, int item, int per, int block0, Unit& u, int& token,
+                                         int& head) {
   int seq, kvh, rb;
-  const int block = item / per, at = item - block * per;
-  if (!block_of(a, p, p.block0 + block, seq, kvh, rb) || seq >= a.seqs) return false;
+  if (!block_of(a, p, block0 + item / per, seq, kvh, rb) || seq >= a.seqs) return false;
   if (!kv8_sequence(a, seq, u.first, u.rows, u.kv)) return false;
-  const int r = rb * p.per + at, all = u.rows * p.group;
+  const int r = rb * p.per + item % per, all = u.rows * p.group;
   if (r >= all || all < p.rows_from || all >= p.rows_to) return false;
   token = r / p.group;
   head = kvh * p.group + r - token * p.group;
-  row = p.pass_rows > 0 ? static_cast<long long>(block) * p.per + at : part_of(a, p, u, token, head, 0);
-  rows = p.pass_rows > 0 ? p.pass_rows : static_cast<long long>(a.tokens) * p.heads;
   return true;
+}
+
+// Its place among the partial sums of a pass.
+__device__ __forceinline__ long long pass_row(const AttnArgs& p, int item, int per) {
+  return static_cast<long long>(item / per) * p.per + item % per;
 }
 
 // out = sum over the ranges of 2^(m_s - m) O_s over that of 2^(m_s - m) l_s: a
@@ -1583,15 +1587,16 @@ __device__ __forceinline__ bool join_row(const Kv8Args& a, const AttnArgs& p, in
 // ranges in turn, four loads ahead, and meet in LDS in a fixed order.  (A wavefront a
 // row, its ranges one after the other: 128 ranges of 32 rows 30 us, 5 so.)  `per`: rows of
 // a block that are launched.
-template <int TYPE>
-__global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p, int per, int shift) {
+template <int TYPE, bool PASS>
+__global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p, int per, int shift, Pass pass) {
   __shared__ float s_w[256], s_red[8];
   __shared__ f32x4 s_o[256];
   const int tid = threadIdx.x;
   Unit u;
   int token, head;
-  long long row, rows;
-  if (!join_row(a, p, blockIdx.x, per, u, token, head, row, rows)) return;
+  if (!join_row(a, p, blockIdx.x, per, PASS ? pass.block : 0, u, token, head)) return;
+  const long long rows = PASS ? pass.rows : static_cast<long long>(a.tokens) * p.heads;
+  const long long row = PASS ? pass_row(p, blockIdx.x, per) : static_cast<long long>(u.first + token) * p.heads + head;
   const float* stats = p.stats + 2 * row;
   float m = -INFINITY;
   for (int s = tid; s < p.splits; s += 256) m = fmaxf(m, stats[2 * s * rows]);
@@ -1646,15 +1651,16 @@ __global__ __launch_bounds__(256) void attention_join(Kv8Args a, AttnArgs p, int
 // The same for a few ranges: L threads a row, each through all of them.  Prompts split in
 // two or four have thousands of rows, and a workgroup for each is mostly its own start.
 constexpr int kFewSplits = 8;
-template <int TYPE>
-__global__ __launch_bounds__(256) void attention_join_few(Kv8Args a, AttnArgs p, int per, int shift) {
+template <int TYPE, bool PASS>
+__global__ __launch_bounds__(256) void attention_join_few(Kv8Args a, AttnArgs p, int per, int shift, Pass pass) {
   const int d = 4 * (threadIdx.x & ((1 << shift) - 1));
   Unit u;
   int token, head;
   // (a wavefront's rows, 16 at most, are one block's where blocks are listed)
-  long long row, rows;
-  if (!join_row(a, p, blockIdx.x * (256 >> shift) + (threadIdx.x >> shift), per, u, token, head, row, rows) || d >= a.head_dim)
-    return;
+  const int item = blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
+  if (!join_row(a, p, item, per, PASS ? pass.block : 0, u, token, head) || d >= a.head_dim) return;
+  const long long rows = PASS ? pass.rows : static_cast<long long>(a.tokens) * p.heads;
+  const long long row = PASS ? pass_row(p, item, per) : static_cast<long long>(u.first + token) * p.heads + head;
   float ms[kFewSplits], ls[kFewSplits], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) {
@@ -1687,8 +1693,8 @@ __global__ __launch_bounds__(256) void attention_join_few(Kv8Args a, AttnArgs p,
 }
 
 // A call's partial sums where its keys are split.
-hipError_t part_buffers(const Kv8Args& a, AttnArgs& p, StreamWorkspace* ws, hipStream_t s) {
-  const size_t outs = p.splits * (p.pass_rows > 0 ? static_cast<size_t>(p.pass_rows) : static_cast<size_t>(a.tokens) * p.heads);
+hipError_t part_buffers(const Kv8Args& a, AttnArgs& p, StreamWorkspace* ws, hipStream_t s, long long pass_rows = 0) {
+  const size_t outs = p.splits * (pass_rows > 0 ? static_cast<size_t>(pass_rows) : static_cast<size_t>(a.tokens) * p.heads);
   void* buf = nullptr;
   const hipError_t e = stream_buffer(ws, s, outs * (a.head_dim + 2) * sizeof(float), 0, &buf);
   p.part = static_cast<float*>(buf);
@@ -1696,9 +1702,9 @@ hipError_t part_buffers(const Kv8Args& a, AttnArgs& p, StreamWorkspace* ws, hipS
   return e;
 }
 
-// blocks: row blocks of all key heads (what block_of takes).
-template <int TYPE>
-hipError_t run_join(const Kv8Args& a, const AttnArgs& p, long long blocks, hipStream_t s) {
+// blocks: row blocks of all key heads (what block_of takes), or of a pass.
+template <int TYPE, bool PASS = false>
+hipError_t run_join(const Kv8Args& a, const AttnArgs& p, long long blocks, hipStream_t s, const Pass& pass = {}) {
   int shift = 2;
   while ((4 << shift) < a.head_dim) ++shift;
   const bool one = p.listed != kBlocks && p.row_blocks == 1;
@@ -1708,10 +1714,10 @@ hipError_t run_join(const Kv8Args& a, const AttnArgs& p, long long blocks, hipSt
   const int rows = p.splits <= kFewSplits ? 256 >> shift : 1;   // of a workgroup
   if (!kv8_grid_fits((items + rows - 1) / rows, 256)) return hipErrorInvalidValue;
   if (p.splits <= kFewSplits) {
-    attention_join_few<TYPE><<<static_cast<unsigned>((items + rows - 1) / rows), 256, 0, s>>>(a, p, per, shift);
+    attention_join_few<TYPE, PASS><<<static_cast<unsigned>((items + rows - 1) / rows), 256, 0, s>>>(a, p, per, shift, pass);
     return hipGetLastError();
   }
-  attention_join<TYPE><<<static_cast<unsigned>(items), 256, 0, s>>>(a, p, per, shift);
+  attention_join<TYPE, PASS><<<static_cast<unsigned>(items), 256, 0, s>>>(a, p, per, shift, pass);
   return hipGetLastError();
 }
 
@@ -1889,26 +1895,27 @@ hipError_t run_shared(const Kv8Args& a, AttnArgs p, hipStream_t s) {
   // the chip (64 sequences of 128 tokens, 64 / 8 heads of 128, a bound of 131072 keys: 4.4 GB in one, 1.0 so; of 16000 keys 6.5 ms
   // in one, 6.1 so, of 1000 1.54 and 1.57, the most that was lost 11%: 16 sequences of 1000 under 2^20)
   const long long row_bytes = static_cast<long long>(p.splits) * (a.head_dim + 2) * sizeof(float);
-  long long pass = blocks;
-  if (p.splits > 1 && row_bytes * a.tokens * p.heads > kPartPass) {
-    pass = std::min(blocks, std::max<long long>(1, kPartPass / (row_bytes * p.per)));
-    p.pass_rows = pass * p.per;
-  }
-  if (!kv8_grid_fits(pass * p.splits, 64 * NW)) return hipErrorInvalidValue;
+  const bool passes = p.splits > 1 && row_bytes * a.tokens * p.heads > kPartPass;
+  const long long most = passes ? std::min(blocks, std::max<long long>(1, kPartPass / (row_bytes * p.per))) : blocks;
+  if (!kv8_grid_fits(most * p.splits, 64 * NW)) return hipErrorInvalidValue;
   std::unique_lock<std::mutex> hold;
   hipError_t e = hipSuccess;
   if (p.splits > 1) {
     StreamWorkspace* ws = nullptr;
     if ((e = stream_workspace(s, &ws)) != hipSuccess) return e;
     hold = std::unique_lock<std::mutex>(ws->call);
-    if ((e = part_buffers(a, p, ws, s)) != hipSuccess) return e;
+    if ((e = part_buffers(a, p, ws, s, passes ? most * p.per : 0)) != hipSuccess) return e;
   }
-  for (long long b0 = 0; b0 < blocks; b0 += pass) {
-    const long long n = std::min(pass, blocks - b0);
-    p.block0 = static_cast<int>(b0);
-    attention_tree<DP, NW, TYPE><<<static_cast<unsigned>(n * p.splits), 64 * NW, 0, s>>>(a, p);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    if (p.splits > 1 && (e = run_join<TYPE>(a, p, n, s)) != hipSuccess) return e;
+  if (!passes) {
+    attention_tree<DP, NW, TYPE, false><<<static_cast<unsigned>(blocks * p.splits), 64 * NW, 0, s>>>(a, p, {});
+    if ((e = hipGetLastError()) != hipSuccess || p.splits == 1) return e;
+    return run_join<TYPE>(a, p, blocks, s);
+  }
+  for (long long b0 = 0; b0 < blocks && e == hipSuccess; b0 += most) {
+    const long long n = std::min(most, blocks - b0);
+    const Pass pass = {static_cast<int>(b0), most * p.per};
+    attention_tree<DP, NW, TYPE, true><<<static_cast<unsigned>(n * p.splits), 64 * NW, 0, s>>>(a, p, pass);
+    if ((e = hipGetLastError()) == hipSuccess) e = run_join<TYPE, true>(a, p, n, s, pass);
   }
   return e;
 }
